@@ -6,8 +6,10 @@ Tensors cross the boundary as raw device pointers; the stream is torch's
 current HIP stream.
 """
 
+import contextlib
 import ctypes
 import os
+from ctypes import byref
 
 import torch
 
@@ -116,6 +118,32 @@ class dm_stack_bwd_layer(ctypes.Structure):
                 ("mlp_workspace_bytes", ctypes.c_size_t)]
 
 
+DM_TOP_MAX = 32           # include/dm_abi.h: most likely tokens per row
+DM_ADAMW_BLOCK = 256      # elements per block of the optimizer's states
+DM_ADAMW_WORKSPACE = 16384
+
+
+class dm_logprob_args(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("rows", c_i32), ("cols", c_i32), ("top", c_i32), ("logits", c_vp),
+                ("ld", ctypes.c_int64), ("target", c_vp), ("logp", c_vp), ("lse", c_vp), ("entropy", c_vp),
+                ("stats", c_vp), ("top_logp", c_vp), ("top_ids", c_vp), ("g_logp", c_vp), ("g_entropy", c_vp), ("dlogits", c_vp),
+                ("ld_d", ctypes.c_int64)]
+
+
+class dm_adamw_tensor(ctypes.Structure):
+    _fields_ = [("p", c_vp), ("g", c_vp), ("n", ctypes.c_int64), ("block0", ctypes.c_int64),
+                ("weight_decay", ctypes.c_float), ("lr_scale", ctypes.c_float), ("g_dtype", c_i32), ("reserved", c_i32)]
+
+
+class dm_adamw_args(ctypes.Structure):
+    _fields_ = [("plan", c_vp), ("n_chunks", ctypes.c_int64), ("n_tensors", c_i32), ("state_bits", c_i32),
+                ("exp_avg", c_vp), ("exp_avg_sq", c_vp), ("exp_avg_exponent", c_vp), ("exp_avg_sq_exponent", c_vp),
+                ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("max_norm", ctypes.c_double), ("skip_nonfinite", c_i32), ("seed", ctypes.c_uint32), ("lr", c_vp),
+                ("steps", c_vp), ("norm", c_vp), ("skipped", c_vp), ("workspace", c_vp),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 P = ctypes.POINTER
 
 # name -> (restype, argtypes); every symbol include/dm_abi.h declares
@@ -165,6 +193,13 @@ SIGNATURES = {
     "dm_ce_mean": (ctypes.c_int, [c_vp, c_i32, c_vp, c_vp, c_vp]),
     "dm_rms_wgrad_workspace_bytes": (ctypes.c_size_t, [c_i32]),
     "dm_rms_wgrad": (ctypes.c_int, [c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, ctypes.c_size_t, c_vp]),
+    "dm_logprob_rows": (ctypes.c_int, [P(dm_logprob_args), c_vp]),
+    "dm_logprob_rows_bwd": (ctypes.c_int, [P(dm_logprob_args), c_vp]),
+    "dm_adamw_plan_bytes": (ctypes.c_size_t, [P(dm_adamw_tensor), c_i32]),
+    "dm_adamw_plan": (ctypes.c_int, [P(dm_adamw_tensor), c_i32, c_vp, ctypes.c_size_t, P(ctypes.c_int64)]),
+    "dm_adamw_step": (ctypes.c_int, [P(dm_adamw_args), c_vp]),
+    "dm_grad_norm": (ctypes.c_int, [P(dm_adamw_args), c_vp]),
+    "dm_adamw_values": (ctypes.c_int, [c_vp, c_vp, ctypes.c_int64, c_i32, c_vp, c_vp]),
     "dm_argmax_rows": (ctypes.c_int, [c_i32, c_vp, c_i32, c_i32, ctypes.c_int64, c_vp, c_vp]),
     "dm_stack_fwd_plan_bytes": (ctypes.c_size_t, [P(dm_config), c_i32, P(dm_stack_layer), P(c_i32), c_i32, c_i32]),
     "dm_stack_fwd": (ctypes.c_int, [P(dm_config), c_i32, P(dm_stack_layer), c_fp, c_fp, P(c_i32), c_i32, c_i32,
@@ -275,6 +310,13 @@ def ptr(t):
 
 def stream_ptr():
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device(device):
+    """A context in which ``device`` is the current one (stream_ptr() then gives its current stream)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def dtype_code(dt):

@@ -1,18 +1,15 @@
 // Host-side helpers shared by the translation units of libdm_hip.so:
-// error reporting, argument checks, launch helpers, workspace carving.
+// argument checks, launch helpers, workspace carving.
 #pragma once
 
 #include <algorithm>
-#include <cstdarg>
-#include <cstdio>
 #include <cstdint>
 #include <cstring>
 #include <map>
 #include <mutex>
-#include <string>
 #include <vector>
 
-#include "../../include/dm_abi.h"
+#include "dm_error.h"
 #include "dm_kernels.h"
 #include "dm_prof.h"
 
@@ -57,39 +54,6 @@ namespace dm {
 #endif
 constexpr int SW1_STAGES = DM_SW1_STAGES, SW2_STAGES = DM_SW2_STAGES, DU_STAGES = DM_DU_STAGES;
 constexpr int BIG_BM = DM_BIG_BM, BIG_BN = DM_BIG_BN, BIG_STAGES = DM_BIG_STAGES, KK_STAGES = DM_KK_STAGES;
-
-inline std::string& last_error() {
-  static thread_local std::string e;
-  return e;
-}
-
-inline int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-inline int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  last_error() = buf;
-  return code;
-}
-
-#define DM_REQUIRE(cond, code, ...)                  \
-  do {                                               \
-    if (!(cond)) return ::dm::fail(code, __VA_ARGS__); \
-  } while (0)
-
-#define DM_HIP(call)                                                                             \
-  do {                                                                                           \
-    hipError_t e_ = (call);                                                                      \
-    if (e_ != hipSuccess) return ::dm::fail(DM_ERR_HIP, "%s: %s", #call, hipGetErrorString(e_)); \
-  } while (0)
-
-inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
-inline size_t esz(int dtype) { return dtype == DM_BF16 ? 2 : 4; }
-inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-inline int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 constexpr int COMM_SPLIT_MIN = 256;   // committed keys per split (lower bound)
 constexpr int DEC_SPLIT = 512;        // tape keys per decode split

@@ -1,0 +1,169 @@
+"""Log probabilities of given tokens, entropies and the most likely tokens of logit rows, with the logits' gradient
+(dm_logprob_rows, dm_logprob_rows_bwd).
+
+For rows x of ``logits`` [..., V] (bf16 or fp32; rows may be padded, a slice ``[..., :V]`` of wider ones) and a target
+per row: lse = logsumexp(x), logp = x[target] - lse, entropy = -sum p log p with p = exp(x - lse), in fp32.
+
+  row_logprobs       the values alone (scoring, evaluation, a decode step's tokens)
+  row_logprobs_grad  the values and the gradient of sum(g_logp logp + g_entropy entropy) in one pass, for
+                     coefficients known beforehand (weights, advantages): what HipTrunk's weighted head runs
+  row_logprobs_bwd   the gradient after row_logprobs
+  token_logprobs     (logp, entropy) under torch's autograd
+
+A target < 0 is ignored (logp 0, no gradient from it), one >= V gives NaN. Columns of -inf have no probability; a row
+of nothing else gives every token -inf, entropy 0 and a zero gradient. A NaN makes its row's values NaN.
+"""
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib as L
+
+
+class RowLogprobs(NamedTuple):
+    logp: Optional[torch.Tensor]      # [...] fp32; None without targets
+    entropy: torch.Tensor             # [...] fp32
+    lse: torch.Tensor                 # [...] fp32
+    stats: torch.Tensor               # [..., 2] fp32: the maximum and lse less it, for row_logprobs_bwd
+    top_logp: Optional[torch.Tensor]  # [..., top] fp32, descending; None without top
+    top_ids: Optional[torch.Tensor]   # [..., top] int64, the lower id first among equals
+
+
+def _rows(t, what):
+    """(rows, row stride) of [..., V] with unit stride along V and one stride over all rows."""
+    V = t.shape[-1]
+    if t.numel() == 0:
+        if V == 0:
+            raise ValueError(f"{what}: no columns")
+        return 0, V
+    if t.is_contiguous():
+        return t.numel() // V, V
+    try:
+        t2 = t.view(-1, V)
+    except RuntimeError:
+        raise ValueError(f"{what}: rows of shape {tuple(t.shape)} and strides {t.stride()} have no single stride; pass "
+                         "a contiguous tensor") from None
+    rows, ld = t2.shape[0], t2.stride(0)
+    if V > 1 and t2.stride(1) != 1:
+        raise ValueError(f"{what}: stride {t2.stride(1)} along the columns (1)")
+    if rows == 1:
+        ld = V
+    if ld < V:
+        raise ValueError(f"{what}: row stride {ld} < {V} columns (expanded rows overlap; pass a contiguous tensor)")
+    return rows, ld
+
+
+def _per_row(t, logits, what, dtype):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != logits.shape[:-1] or t.device != logits.device or not t.is_contiguous():
+        raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}; contiguous {dtype} "
+                         f"{tuple(logits.shape[:-1])} on {logits.device} is needed")
+    return t.data_ptr()
+
+
+def _args(logits, targets):
+    if not logits.is_cuda or logits.dim() < 1:
+        raise ValueError(f"logits: shape {tuple(logits.shape)} on {logits.device}; rows [..., V] on a GPU are needed")
+    a = L.dm_logprob_args()
+    a.dtype = L.dtype_code(logits.dtype)
+    a.rows, a.ld = _rows(logits, "logits")
+    a.cols = logits.shape[-1]
+    a.logits, a.target = logits.data_ptr(), _per_row(targets, logits, "targets", torch.int64)
+    return a
+
+
+def _grad_args(a, logits, targets, g_logp, g_entropy, dlogits):
+    if g_logp is None and g_entropy is None:
+        raise ValueError("a gradient needs g_logp or g_entropy")
+    if g_logp is not None and targets is None:
+        raise ValueError("g_logp needs targets")
+    if dlogits is None:
+        dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    elif dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
+        raise ValueError(f"dlogits: {dlogits.dtype} {tuple(dlogits.shape)} on {dlogits.device} for logits {logits.dtype} "
+                         f"{tuple(logits.shape)} on {logits.device}")
+    a.g_logp = _per_row(g_logp, logits, "g_logp", torch.float32)
+    a.g_entropy = _per_row(g_entropy, logits, "g_entropy", torch.float32)
+    a.dlogits, a.ld_d = dlogits.data_ptr(), _rows(dlogits, "dlogits")[1]
+    return dlogits
+
+
+def _call(fn, a, device):
+    with L.on_device(device):
+        L.check(fn(L.byref(a), L.stream_ptr()))
+
+
+def _forward(a, logits, targets, top):
+    kw = dict(device=logits.device, dtype=torch.float32)
+    lead = logits.shape[:-1]
+    if not 0 <= top <= min(L.DM_TOP_MAX, a.cols):
+        raise ValueError(f"top={top} of {a.cols} columns (at most {L.DM_TOP_MAX})")
+    logp, entropy, lse = (torch.empty(lead, **kw) for _ in range(3))
+    stats = torch.empty(lead + (2,), **kw)
+    a.entropy, a.lse, a.stats = entropy.data_ptr(), lse.data_ptr(), stats.data_ptr()
+    if targets is None:
+        logp = None
+    else:
+        a.logp = logp.data_ptr()
+    top_logp = top_ids = None
+    if top:
+        a.top = top
+        top_logp = torch.empty(lead + (top,), **kw)
+        top_ids = torch.empty(lead + (top,), device=logits.device, dtype=torch.int64)
+        a.top_logp, a.top_ids = top_logp.data_ptr(), top_ids.data_ptr()
+    _call(L.lib().dm_logprob_rows, a, logits.device)
+    return RowLogprobs(logp, entropy, lse, stats, top_logp, top_ids)
+
+
+def row_logprobs(logits, targets=None, top=0):
+    """The values of logits [..., V]: logp of ``targets`` (int64 [...], optional), entropy, lse and the ``top`` most
+    likely tokens of each row (at most 32). No gradient."""
+    return _forward(_args(logits, targets), logits, targets, top)
+
+
+def row_logprobs_grad(logits, targets, g_logp, g_entropy=None, top=0, dlogits=None):
+    """row_logprobs, and the gradient of sum(g_logp logp + g_entropy entropy) to the logits (fp32 coefficients [...],
+    either may be None) in the same pass: (RowLogprobs, dlogits). dlogits: a tensor for the gradient, the logits
+    themselves too (in place); by default a new one."""
+    a = _args(logits, targets)
+    dlogits = _grad_args(a, logits, targets, g_logp, g_entropy, dlogits)
+    return _forward(a, logits, targets, top), dlogits
+
+
+def row_logprobs_bwd(logits, targets, r, g_logp, g_entropy=None, dlogits=None):
+    """The gradient of row_logprobs_grad after row_logprobs, from its result ``r`` (stats and, with g_entropy, entropy)."""
+    a = _args(logits, targets)
+    dlogits = _grad_args(a, logits, targets, g_logp, g_entropy, dlogits)
+    a.entropy = _per_row(r.entropy, logits, "entropy", torch.float32)
+    if r.stats.shape != logits.shape[:-1] + (2,) or r.stats.device != logits.device or not r.stats.is_contiguous():
+        raise ValueError(f"stats: {tuple(r.stats.shape)} on {r.stats.device} for logits {tuple(logits.shape)} on {logits.device}")
+    a.stats = r.stats.data_ptr()
+    _call(L.lib().dm_logprob_rows_bwd, a, logits.device)
+    return dlogits
+
+
+class TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets):
+        r = row_logprobs(logits, targets)
+        ctx.save_for_backward(logits, targets, r.stats, r.entropy)
+        ctx.set_materialize_grads(False)
+        return r.logp, r.entropy
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy):
+        if g_logp is None and g_entropy is None:
+            return None, None
+        logits, targets, stats, entropy = ctx.saved_tensors
+        g_logp, g_entropy = (None if g is None else g.contiguous() for g in (g_logp, g_entropy))
+        r = RowLogprobs(None, entropy, None, stats, None, None)
+        return row_logprobs_bwd(logits, targets, r, g_logp, g_entropy), None
+
+
+def token_logprobs(logits, targets):
+    """(logp, entropy) of logits [..., V] and targets [...], differentiable in the logits."""
+    rows_ok = logits.stride(-1) == 1 and (logits.dim() < 2 or logits.is_contiguous())
+    return TokenLogprobsFn.apply(logits if rows_ok else logits.contiguous(), targets.contiguous())

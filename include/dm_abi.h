@@ -521,6 +521,94 @@ int dm_ce_rows(int32_t dtype, void* logits, const int64_t* target, const float* 
 int dm_ce_count(const int64_t* target, int32_t M, float* nvalid, void* stream);
 int dm_ce_mean(const float* loss, int32_t M, const float* nvalid, float* out, void* stream);
 
+/* ---- log probabilities of given tokens ---------------------------------------------------
+ * Rows x of logits [rows, cols] (storage dtype bf16 or fp32, row stride ld >= cols elements), with
+ *   lse = logsumexp(x), logp(v) = x[v] - lse, p = exp(logp), entropy = -sum p logp (0 log 0 = 0),
+ * all in fp32, one pass over a row's logits.
+ * dm_logprob_rows: logp[r] = logp(target[r]) (0 for a target < 0, NaN for one >= cols), lse[r], entropy[r], and
+ *   the `top` most likely tokens of each row, ids and log probabilities [rows, top] in descending order, the
+ *   lower id first among equals, a NaN before every number (as dm_argmax_rows). With dlogits, also the gradient of
+ *   sum_r (g_logp[r] logp[r] + g_entropy[r] entropy[r]),
+ *     dlogits[v] = g_logp (1[v = target] - p) - g_entropy p (logp(v) + entropy),
+ *   for coefficients that are known beforehand.
+ * dm_logprob_rows_bwd: the same gradient after the forward, whose stats and (with g_entropy) entropy it reads;
+ *   the fields logp, lse, top_logp and top_ids are not used.
+ * A row of -inf gives every token -inf: lse -inf, logp -inf, entropy 0, a zero gradient. A row with a NaN: lse,
+ * log probabilities and entropy NaN. With +inf and no NaN: lse +inf, logp -inf for finite logits and NaN for the
+ * infinite ones, entropy NaN. The gradient of those two is NaN. A row whose coefficients are both 0 (g_logp counts
+ * as 0 where the target is < 0) gets zeros whatever its logits; one with a target >= cols and g_logp != 0 NaN.
+ * dlogits (storage dtype, stride ld_d >= cols) may be the logits themselves (same pointer and stride), and may not
+ * overlap them otherwise. Pointers need their element's alignment only. rows may be 0. No workspace; rows are
+ * independent, a row's results do not depend on the others. */
+#define DM_TOP_MAX 32
+typedef struct dm_logprob_args {
+  int32_t dtype, rows, cols;
+  int32_t top;                       /* 0..min(DM_TOP_MAX, cols); dm_logprob_rows only */
+  const void* logits; int64_t ld;
+  const int64_t* target;             /* [rows]; NULL: no logp and no g_logp */
+  float* logp; float* lse; float* entropy;   /* [rows]; outputs of dm_logprob_rows (each may be NULL) */
+  float* stats;                      /* [rows, 2] output (may be NULL) and input of dm_logprob_rows_bwd: the row's
+                                        maximum and lse less it, both infinite or NaN where lse is */
+  float* top_logp; int64_t* top_ids; /* [rows, top] */
+  const float* g_logp; const float* g_entropy;   /* [rows]; with dlogits, at least one */
+  void* dlogits; int64_t ld_d;       /* NULL: no gradient */
+} dm_logprob_args;
+int dm_logprob_rows(const dm_logprob_args* a, void* stream);
+int dm_logprob_rows_bwd(const dm_logprob_args* a, void* stream);
+
+/* ---- AdamW over many tensors --------------------------------------------------------------
+ * One step of AdamW over n tensors (fp32 parameters, fp32 or bf16 gradients, contiguous) in one launch over all
+ * of them, with t the step's number from 1 on:
+ *   g' = c g,  c = min(1, max_norm / (norm + 1e-6)) or 1,  norm = sqrt(sum of g^2 over all tensors)
+ *   m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr' weight_decay) - lr' / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps),  lr' = lr lr_scale
+ * (fp32; the norm, the powers and 1 - lr' weight_decay in 64 bits, summed in a fixed order).
+ * The states live in flat buffers of whole blocks of DM_ADAMW_BLOCK elements, tensor i's from block block0 on.
+ * state_bits 32: fp32 exp_avg / exp_avg_sq. state_bits 8: a byte per element and per block the exponent field e of
+ * the block's largest magnitude (1..253; 255 = a NaN or a magnitude of 2^127 or more: the whole block reads as NaN), with x a code
+ * for a = |x| 2^(125 - e) < 1/2:
+ *   exp_avg     sign, 4 exponent and 3 mantissa bits: (1 + M / 8) 2^(E - 16), M 2^-18 for E = 0
+ *   exp_avg_sq  5 exponent and 3 mantissa bits: (1 + M / 8) 2^(E - 32), M 2^-34 for E = 0; not 0 for v > 0
+ * Rounding to codes is stochastic, by 16 bits each of a 32-bit hash of (seed, t, element): a step moves v by less
+ * than a thousandth, a code is an eighth, and rounding to nearest would leave v where it is.
+ * The parameters are updated from the unrounded states.
+ *
+ * dm_adamw_plan writes the launch plan (host memory, *plan_bytes from dm_adamw_plan_bytes) of the tensors, which the
+ * caller copies to the device; *n_chunks is the number of blocks to launch. Tensors of 0 elements are left out.
+ * The plan holds the tensors' addresses: it is written again when one moves. No parameter may overlap another.
+ * lr (fp32), steps (int64, the number of steps taken, incremented), norm (fp32, written where the norm is computed:
+ * max_norm > 0 or skip_nonfinite) and skipped (int32) are device scalars, so a captured step can be replayed.
+ * skip_nonfinite: a step whose norm is not finite changes nothing but *skipped, which is incremented.
+ * Workspace: DM_ADAMW_WORKSPACE bytes, 16-byte aligned, not shared by steps that may overlap. */
+#define DM_ADAMW_BLOCK 256
+#define DM_ADAMW_WORKSPACE 16384
+typedef struct dm_adamw_tensor {
+  float* p; const void* g;           /* device pointers, n elements each */
+  int64_t n, block0;                 /* elements; first block of the states */
+  float weight_decay, lr_scale;
+  int32_t g_dtype, reserved;         /* dm_dtype of g */
+} dm_adamw_tensor;
+typedef struct dm_adamw_args {
+  const void* plan; int64_t n_chunks;        /* device copy of dm_adamw_plan's output */
+  int32_t n_tensors, state_bits;
+  void* exp_avg; void* exp_avg_sq;           /* [n_blocks * DM_ADAMW_BLOCK] fp32 or codes, 16-byte aligned */
+  uint8_t* exp_avg_exponent; uint8_t* exp_avg_sq_exponent;   /* [n_blocks], state_bits 8 */
+  double beta1, beta2, eps;
+  double max_norm;                           /* <= 0: no clipping */
+  int32_t skip_nonfinite; uint32_t seed;
+  const float* lr; int64_t* steps; float* norm; int32_t* skipped;
+  void* workspace; size_t workspace_bytes;
+} dm_adamw_args;
+size_t dm_adamw_plan_bytes(const dm_adamw_tensor* t, int32_t n_tensors);
+int dm_adamw_plan(const dm_adamw_tensor* t, int32_t n_tensors, void* plan, size_t plan_bytes, int64_t* n_chunks);
+int dm_adamw_step(const dm_adamw_args* a, void* stream);
+/* norm = the gradients' global norm alone (fields plan, n_chunks, n_tensors, norm, workspace). */
+int dm_grad_norm(const dm_adamw_args* a, void* stream);
+/* The numbers that n_blocks blocks of codes stand for, as bf16 (exact: four significant bits; magnitudes below
+ * 2^-133 round): out [n_blocks * DM_ADAMW_BLOCK]. second: 0 exp_avg's codes, 1 exp_avg_sq's. */
+int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_blocks, int32_t second, void* out,
+                    void* stream);
+
 /* ---- RMSNorm weight gradient -----------------------------------------------------------
  * dw [d] fp32 += sum over the M rows of dy x r (dy, x [M, d] storage dtype, r [M] fp32 the rows' scales
  * rsqrt(mean x^2 + eps)): attention.py:74-83's weight, summed in a fixed order over 64 chunks of rows.
