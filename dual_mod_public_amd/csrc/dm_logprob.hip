@@ -9,8 +9,9 @@ using namespace dm;
 
 namespace {
 
-constexpr float INF = __builtin_inff();
+constexpr float INF = __builtin_inff(), NAN_ = __builtin_nanf(""), LEAST = -3.402823466e38f;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int CANDIDATES = 1024;   // of a row's most likely tokens, in LDS
 
 template <typename T> struct LpArgs {
   const T* x;
@@ -23,7 +24,7 @@ template <typename T> struct LpArgs {
   int rows, cols, top;
 };
 
-// The statistics of a row: lse = M + log_z where the maximum M is finite.
+// The statistics of a row: lse = M + log_z, M its maximum.
 struct RowStats {
   float M, log_z, lse, entropy;
   DM_DEV float logp(float x) const {
@@ -36,15 +37,20 @@ struct RowStats {
 DM_DEV float exp_of(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 
 // The order of the most likely tokens as one number per column: by value (NaN first, -0 as 0), then the lower id.
-DM_DEV uint64_t order_of(float x, int id) {
+DM_DEV uint32_t order_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
-  const uint32_t o = x != x ? 0xffffffffu : (b >> 31 ? ~b : b | 0x80000000u);
-  return (uint64_t)o << 32 | (uint32_t)~id;
+  return x != x ? 0xffffffffu : (b >> 31 ? ~b : b | 0x80000000u);
 }
+DM_DEV uint64_t order_of(float x, int id) { return (uint64_t)order_of(x) << 32 | (uint32_t)~id; }
+DM_DEV float value_of(uint32_t order) { return __uint_as_float(order >> 31 ? order & 0x7fffffffu : ~order); }
+constexpr uint32_t ORDER_OF_MINUS_INF = 0x007fffffu;
 
 template <int NT> struct Shared {
-  float f[3][NT / 64];
+  float m[NT / 64], z[NT / 64], q[NT / 64];
   uint64_t key[NT / 64];
+  float largest[NT];            // each thread's largest logit
+  int count;                    // candidates found
+  uint64_t cand[CANDIDATES];
 };
 
 DM_DEV uint64_t wave_max_u64(uint64_t k) {
@@ -62,79 +68,113 @@ struct RowGrad {
   float g, gh;
   bool zero, nan;   // a row of zeros, of NaN
 };
-template <typename T> DM_DEV RowGrad row_grad(const LpArgs<T>& a, long r, float lse) {
+template <typename T> DM_DEV RowGrad row_grad(const LpArgs<T>& a, long r, long t, float lse) {
   RowGrad w;
-  const long t = a.target ? a.target[r] : -1;
   w.g = a.g_logp && t >= 0 ? a.g_logp[r] : 0.f;
   w.gh = a.g_entropy ? a.g_entropy[r] : 0.f;
   w.zero = (w.g == 0.f && w.gh == 0.f) || lse == -INF;
   w.nan = !w.zero && (!(fabsf(lse) < INF) || (w.g != 0.f && t >= a.cols));
   return w;
 }
-template <typename T> DM_DEV float grad_of(const RowStats& s, const RowGrad& w, float x) {
-  const float lp = s.logp(x), p = exp_of(lp);
+DM_DEV float grad_of(const RowStats& s, const RowGrad& w, float x) {
+  const float lp = (x - s.M) - s.log_z, p = exp_of(lp);
   return -p * (w.g + w.gh * (fmaxf(lp, -1e30f) + s.entropy));   // p = 0 at -inf
 }
 
-// One row by one block, element by element: every case.
-template <typename T, int NT>
-DM_DEV void any_row(const LpArgs<T>& a, long r, Shared<NT>& sh) {
-  const T* x = a.x + r * a.ld;
-  const int n = a.cols, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long t = a.target ? a.target[r] : -1;
-  const float xt = t >= 0 && t < n ? to_f(x[t]) : 0.f;
-  float m = -INF;
-  int bad = 0;
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const float v = to_f(x[i]);
-    bad |= v != v;
-    m = fmaxf(m, v);
+// A row in 16-byte vectors: the columns before the first and behind the last whole aligned vector (at most
+// 2 (V - 1), one per thread) and the vectors between them.
+template <typename T> struct RowSpan {
+  static constexpr int V = 16 / (int)sizeof(T);
+  const T* x;
+  int n, c0, nvec;
+  DM_DEV RowSpan(const T* row, int cols) : x(row), n(cols) {
+    c0 = min(n, (int)(-(long)(reinterpret_cast<uintptr_t>(row) / sizeof(T)) & (V - 1)));
+    nvec = (n - c0) / V;
   }
-  bad = __syncthreads_or(bad);
-  m = wave_max(m);
-  if (lane == 0) sh.f[0][wave] = m;
-  __syncthreads();
-  RowStats s;
-  s.M = sh.f[0][0];
-  for (int w = 1; w < NT / 64; ++w) s.M = fmaxf(s.M, sh.f[0][w]);
-  if (bad) {
-    s.M = s.lse = s.entropy = s.log_z = __builtin_nanf("");
-  } else if (fabsf(s.M) == INF) {
-    s.lse = s.log_z = s.M;
-    s.entropy = s.M > 0 ? __builtin_nanf("") : 0.f;
-  } else {
-    float z = 0.f, q = 0.f;
-    for (int i = threadIdx.x; i < n; i += NT) {
-      const float d = to_f(x[i]) - s.M, e = exp_of(d);
-      z += e;
-      q += e * fmaxf(d, -1e30f);
+  DM_DEV int edge_col(int e) const {   // the e-th single column, -1: there is none
+    const int c = e < c0 ? e : c0 + nvec * V + (e - c0);
+    return c < n ? c : -1;
+  }
+  DM_DEV int col(int q) const { return c0 + q * V; }
+  // vector q0 + lane, q0 the same in every lane: a scalar base and one 32-bit lane offset for all of a thread's loads
+  DM_DEV u32x4 vec(int q0, int lane) const {
+    return ld_global<u32x4>(reinterpret_cast<const char*>(x + c0 + (long)q0 * V) + 16u * lane);
+  }
+};
+template <typename T> DM_DEV void unpack(const u32x4& r, float* v) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
-    z = wave_sum(z);
-    q = wave_sum(q);
-    if (lane == 0) sh.f[1][wave] = z, sh.f[2][wave] = q;
-    __syncthreads();
-    z = q = 0.f;
-    for (int w = 0; w < NT / 64; ++w) z += sh.f[1][w], q += sh.f[2][w];
-    s.log_z = logf(z);
-    s.lse = s.M + s.log_z;
-    s.entropy = s.log_z - q / z;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
   }
-  if (threadIdx.x == 0) {
-    if (a.logp) a.logp[r] = t < 0 ? 0.f : t < n ? s.logp(xt) : __builtin_nanf("");
-    if (a.lse) a.lse[r] = s.lse;
-    if (a.entropy) a.entropy[r] = s.entropy;
-    if (a.stats) a.stats[2 * r] = s.M, a.stats[2 * r + 1] = s.log_z;
+}
+
+// x is computed here, not where it is used (all of a tile's summands would wait in registers until then)
+DM_DEV void here(float& x) { asm volatile("" : "+v"(x)); }
+
+// A thread's part of one tile of a row: NV vectors and (first tile) one single column, -inf where there is none.
+template <typename T, int NT, int NV> struct Tile {
+  static constexpr int V = RowSpan<T>::V;
+  u32x4 raw[NV];
+  float edge;
+  DM_DEV void load(const RowSpan<T>& row, int tile) {
+    const uint32_t fill = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int q0 = (tile * NV + i) * NT;
+      raw[i] = u32x4{fill, fill, fill, fill};
+      if (q0 + (int)threadIdx.x < row.nvec) raw[i] = row.vec(q0, threadIdx.x);
+    }
+    const int c = tile == 0 ? row.edge_col(threadIdx.x) : -1;
+    edge = c >= 0 ? to_f(row.x[c]) : -INF;
   }
+  // vector i's logits, converted where they are used: kept from pass to pass the converted ones would take twice the
+  // registers of the row (the statement hides from the compiler that it has converted them before)
+  DM_DEV void get(int i, float (&v)[V]) {
+    asm volatile("" : "+v"(raw[i]));
+    unpack<T>(raw[i], v);
+  }
+};
+
+// The NT threads' (maximum m, z = sum of e^(x - m), q = sum of e^(x - m) (x - m)) as one.
+template <int NT> DM_DEV void combine(float& m, float& z, float& q, Shared<NT>& sh) {
+  auto rescale = [&](float M) {
+    const float d = fmaxf(m - M, -1e30f), f = exp_of(d);   // z = q = 0 where m is LEAST
+    q = f * (q + z * d);
+    z *= f;
+    m = M;
+  };
+  rescale(wave_max(m));
+  z = wave_sum(z);
+  q = wave_sum(q);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) sh.m[wave] = m, sh.z[wave] = z, sh.q[wave] = q;
+  __syncthreads();
+  const int w = threadIdx.x % (NT / 64);   // each wave's lanes combine all waves' values
+  m = sh.m[w], z = sh.z[w], q = sh.q[w];
+  rescale(lanes_max<1, NT / 128>(m));
+  z = lanes_sum<1, NT / 128>(z);
+  q = lanes_sum<1, NT / 128>(q);
+}
+
+// The row's `top` largest in order, found one after the other: any row, any values.
+template <typename T, int NT> DM_DEV void slow_top(const LpArgs<T>& a, long r, const RowStats& s, Shared<NT>& sh) {
+  const T* x = a.x + r * a.ld;
   uint64_t last = ~0ull;
-  for (int j = 0; j < a.top; ++j) {   // the next one in order after `last`
+  for (int j = 0; j < a.top; ++j) {
     uint64_t best = 0;
-    for (int i = threadIdx.x; i < n; i += NT) {
+    for (int i = threadIdx.x; i < a.cols; i += NT) {
       const uint64_t k = order_of(to_f(x[i]), i);
       if (k < last && k > best) best = k;
     }
     best = wave_max_u64(best);
     __syncthreads();
-    if (lane == 0) sh.key[wave] = best;
+    if ((threadIdx.x & 63) == 0) sh.key[threadIdx.x >> 6] = best;
     __syncthreads();
     for (int w = 0; w < NT / 64; ++w) best = max(best, sh.key[w]);
     last = best;
@@ -144,47 +184,268 @@ DM_DEV void any_row(const LpArgs<T>& a, long r, Shared<NT>& sh) {
       a.top_logp[r * a.top + j] = s.logp(to_f(x[id]));
     }
   }
-  __syncthreads();   // the row is read; its buffers are free again
-  if (!a.dx) return;
-  const RowGrad w = row_grad(a, r, s.lse);
-  T* dx = a.dx + r * a.ld_d;
-  for (int i = threadIdx.x; i < n; i += NT)
-    dx[i] = from_f<T>(w.zero ? 0.f : w.nan ? __builtin_nanf("") : grad_of<T>(s, w, to_f(x[i])) + (i == t ? w.g : 0.f));
+  __syncthreads();   // the row has been read
 }
 
-template <typename T> __global__ __launch_bounds__(256) void k_logprob_rows(LpArgs<T> a) {
-  __shared__ Shared<256> sh;
-  for (long r = blockIdx.x; r < a.rows; r += gridDim.x) any_row<T, 256>(a, r, sh);
+// A bound that at least `top` of the row's logits reach, -inf at least: of the 64 lanes' largest logits the top-th.
+template <typename T, int NT> DM_DEV float top_bound(int top, const Shared<NT>& sh) {
+  float g = -INF;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) g = fmaxf(g, sh.largest[w * 64 + (threadIdx.x & 63)]);
+  const uint32_t o = order_of(g);
+  uint32_t bound = 0;   // its upper bits: rounded down it lets a few more pass
+#pragma unroll
+  for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 13); --bit) {
+    const uint32_t b = bound | 1u << bit;
+    if (__popcll(__ballot(o >= b)) >= top) bound = b;
+  }
+  return bound <= ORDER_OF_MINUS_INF ? -INF : value_of(bound);
+}
+template <int NT> DM_DEV void take(float x, int col, Shared<NT>& sh) {
+  const int at = atomicAdd(&sh.count, 1);
+  if (at < CANDIDATES) sh.cand[at] = order_of(x, col);
+}
+// this tile's logits of at least `bound` into the list
+template <typename T, int NT, int NV> DM_DEV void take_tile(const RowSpan<T>& row, Tile<T, NT, NV>& t, int tile, float bound, Shared<NT>& sh) {
+  constexpr int V = RowSpan<T>::V;
+  if (t.edge >= bound && t.edge > -INF) take(t.edge, row.edge_col(threadIdx.x), sh);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float v[V];
+    t.get(i, v);
+    uint32_t hit = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) hit |= (v[j] >= bound && v[j] > -INF) << j;
+    while (hit) {
+      const int j = __ffs(hit) - 1;
+      hit &= hit - 1;
+      float x = v[0];
+#pragma unroll
+      for (int k = 1; k < V; ++k) x = j == k ? v[k] : x;
+      take(x, row.col(tile * NT * NV + i * NT + threadIdx.x) + j, sh);
+    }
+  }
+}
+// the c candidates in order; behind them, where they are fewer, the lowest ids of probability 0
+template <typename T, int NT> DM_DEV void write_top(const LpArgs<T>& a, long r, const RowStats& s, int c, const Shared<NT>& sh) {
+  float* lp = a.top_logp + r * a.top;
+  int64_t* ids = a.top_ids + r * a.top;
+  for (int i = threadIdx.x; i < c; i += NT) {
+    const uint64_t k = sh.cand[i];
+    int rank = 0;
+    for (int j = 0; j < c; ++j) rank += sh.cand[j] > k;
+    if (rank >= a.top) continue;
+    ids[rank] = (uint32_t)~(uint32_t)k;
+    lp[rank] = s.logp(value_of(k >> 32));
+  }
+  if (c < a.top && (int)threadIdx.x < a.top) {   // the first `top` columns hold enough of them
+    int before = 0;
+    bool taken = false;
+    for (int j = 0; j < c; ++j) {
+      const uint32_t id = ~(uint32_t)sh.cand[j];
+      before += id < threadIdx.x;
+      taken |= id == threadIdx.x;
+    }
+    const int at = c + threadIdx.x - before;
+    if (!taken && at < a.top) {
+      ids[at] = threadIdx.x;
+      lp[at] = -INF;
+    }
+  }
 }
 
-template <typename T> __global__ __launch_bounds__(256) void k_logprob_bwd(LpArgs<T> a) {
-  for (long r = blockIdx.y; r < a.rows; r += gridDim.y) {
+// One vector of the gradient into dx's aligned vectors, or element by element where dx lies otherwise than x.
+template <typename T> DM_DEV void store_grad(T* p, const float* v, bool aligned) {
+  constexpr int V = RowSpan<T>::V;
+  if (aligned) {
+    store_vec<T, V>(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) p[j] = from_f<T>(v[j]);
+  }
+}
+template <typename T, int NT, int NV>
+DM_DEV void store_tile(const RowSpan<T>& row, Tile<T, NT, NV>& t, int tile, const RowStats& s, const RowGrad& w, long target, T* dx) {
+  constexpr int V = RowSpan<T>::V;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
+  const float all = w.nan ? NAN_ : 0.f;
+  const bool plain = w.nan || w.zero;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int q = tile * NT * NV + i * NT + threadIdx.x;
+    if (q >= row.nvec) continue;
+    float v[V];
+    t.get(i, v);
+    const long at = target - row.col(q);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = plain ? all : grad_of(s, w, v[j]) + (at == j ? w.g : 0.f);
+    store_grad(dx + row.col(q), v, aligned);
+  }
+  const int c = tile == 0 ? row.edge_col(threadIdx.x) : -1;
+  if (c >= 0) dx[c] = from_f<T>(plain ? all : grad_of(s, w, t.edge) + (c == target ? w.g : 0.f));
+}
+
+// A block per row, the row in tiles of NT NV vectors held in registers.
+template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT, 4) void k_logprob_rows(LpArgs<T> a) {
+  __shared__ Shared<NT> sh;
+  for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const RowSpan<T> row(a.x + r * a.ld, a.cols);
+    const int tiles = max(1, (row.nvec + NT * NV - 1) / (NT * NV));
+    const long t = a.target ? a.target[r] : -1;
+    const float xt = t >= 0 && t < a.cols ? to_f(row.x[t]) : 0.f;
+    float m = LEAST, z = 0.f, q = 0.f;
+    Tile<T, NT, NV> tile;
+    if (a.top && threadIdx.x == 0) sh.count = 0;
+    for (int i = 0; i < tiles; ++i) {
+      tile.load(row, i);
+      float m1 = fmaxf(m, tile.edge);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float v[RowSpan<T>::V];
+        tile.get(k, v);
+#pragma unroll
+        for (int j = 0; j < RowSpan<T>::V; ++j) m1 = fmaxf(m1, v[j]);
+        here(m1);
+      }
+      const float d0 = fmaxf(m - m1, -1e30f), f = exp_of(d0);
+      q = f * (q + z * d0);
+      z *= f;
+      m = m1;
+      auto add = [&](float x) {
+        const float d = x - m, e = exp_of(d);
+        z += e;
+        q += e * fmaxf(d, -1e30f);
+      };
+      add(tile.edge);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float v[RowSpan<T>::V];
+        tile.get(k, v);
+#pragma unroll
+        for (int j = 0; j < RowSpan<T>::V; ++j) add(v[j]);
+        here(z);
+        here(q);
+      }
+      if (a.top) {   // the bound only rises from tile to tile
+        sh.largest[threadIdx.x] = z > 0.f ? m : -INF;
+        __syncthreads();
+        take_tile(row, tile, i, top_bound<T>(a.top, sh), sh);
+        if (i + 1 < tiles) __syncthreads();
+      }
+    }
+    combine(m, z, q, sh);
+    RowStats s;
+    const bool bad = !(z < INF);   // a NaN or +inf in the row
+    if (bad) {
+      int nan = 0;
+      for (int i = threadIdx.x; i < a.cols; i += NT) {
+        const float v = to_f(row.x[i]);
+        nan |= v != v;
+      }
+      s.M = s.log_z = s.lse = __syncthreads_or(nan) ? NAN_ : INF;
+      s.entropy = NAN_;
+    } else if (z == 0.f) {
+      s.M = s.log_z = s.lse = -INF;
+      s.entropy = 0.f;
+    } else {
+      s.M = m;
+      s.log_z = logf(z);
+      s.lse = m + s.log_z;
+      s.entropy = s.log_z - q / z;
+    }
+    if (threadIdx.x == 0) {
+      if (a.logp) a.logp[r] = t < 0 ? 0.f : t < a.cols ? s.logp(xt) : NAN_;
+      if (a.lse) a.lse[r] = s.lse;
+      if (a.entropy) a.entropy[r] = s.entropy;
+      if (a.stats) a.stats[2 * r] = s.M, a.stats[2 * r + 1] = s.log_z;
+    }
+    if (a.top) {
+      const int c = sh.count;
+      if (bad || c > CANDIDATES) slow_top<T, NT>(a, r, s, sh);
+      else write_top<T, NT>(a, r, s, c, sh);
+    }
+    if constexpr (GRAD) {
+      const RowGrad w = row_grad(a, r, t, s.lse);
+      T* dx = a.dx + r * a.ld_d;
+      for (int i = 0; i < tiles; ++i) {
+        if (tiles > 1) tile.load(row, i);
+        store_tile(row, tile, i, s, w, t, dx);
+      }
+    }
+    __syncthreads();   // sh is free again
+  }
+}
+
+// NT threads per row part of NV vectors each, 256 / NT rows per block.
+template <typename T, int NT, int NV> __global__ __launch_bounds__(256) void k_logprob_bwd(LpArgs<T> a, int parts) {
+  const long items = (long)a.rows * parts;
+  for (long it = blockIdx.x * (256L / NT) + threadIdx.x / NT; it < items; it += gridDim.x * (256L / NT)) {
+    const long r = it / parts;
+    const int q0 = (int)(it % parts) * NT * NV + threadIdx.x % NT;
     RowStats s;
     s.M = a.stats[2 * r];
     s.log_z = a.stats[2 * r + 1];
     s.lse = s.M + s.log_z;
     s.entropy = a.g_entropy ? a.entropy[r] : 0.f;
-    const RowGrad w = row_grad(a, r, s.lse);
     const long t = a.target ? a.target[r] : -1;
-    const T* x = a.x + r * a.ld;
+    const RowGrad w = row_grad(a, r, t, s.lse);
+    const RowSpan<T> row(a.x + r * a.ld, a.cols);
     T* dx = a.dx + r * a.ld_d;
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < a.cols; i += gridDim.x * 256)
-      dx[i] = from_f<T>(w.zero ? 0.f : w.nan ? __builtin_nanf("") : grad_of<T>(s, w, to_f(x[i])) + (i == t ? w.g : 0.f));
+    const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
+    const float all = w.nan ? NAN_ : 0.f;
+    const bool plain = w.nan || w.zero;
+    u32x4 raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      raw[i] = u32x4{0, 0, 0, 0};
+      if (!plain && q0 + i * NT < row.nvec) raw[i] = row.vec(0, q0 + i * NT);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int q = q0 + i * NT;
+      if (q >= row.nvec) continue;
+      float v[RowSpan<T>::V];
+      unpack<T>(raw[i], v);
+      const long at = t - row.col(q);
+#pragma unroll
+      for (int j = 0; j < RowSpan<T>::V; ++j) v[j] = plain ? all : grad_of(s, w, v[j]) + (at == j ? w.g : 0.f);
+      store_grad(dx + row.col(q), v, aligned);
+    }
+    const int c = it % parts == 0 ? row.edge_col(q0) : -1;
+    if (c >= 0) dx[c] = from_f<T>(plain ? all : grad_of(s, w, to_f(row.x[c])) + (c == t ? w.g : 0.f));
   }
 }
 
-constexpr int MAX_BLOCKS = 1 << 20;   // a grid's blocks per dimension; further rows by the same blocks
+constexpr int MAX_BLOCKS = 1 << 20;   // of a grid; further rows by the same blocks
 
 template <typename T> LpArgs<T> typed(const dm_logprob_args* a) {
   return {(const T*)a->logits, (T*)a->dlogits, a->target, a->logp, a->lse, a->entropy, a->stats, a->top_logp,
           a->top_ids, a->g_logp, a->g_entropy, a->ld, a->ld_d, a->rows, a->cols, a->top};
 }
 
+template <typename T, int NT, int NV> void launch_rows(const LpArgs<T>& a, hipStream_t s) {
+  const dim3 grid(std::min(a.rows, MAX_BLOCKS));
+  if (a.dx) hipLaunchKernelGGL((k_logprob_rows<T, NT, NV, true>), grid, dim3(NT), 0, s, a);
+  else hipLaunchKernelGGL((k_logprob_rows<T, NT, NV, false>), grid, dim3(NT), 0, s, a);
+}
 template <typename T> void run_rows(const LpArgs<T>& a, hipStream_t s) {
-  hipLaunchKernelGGL(k_logprob_rows<T>, dim3(std::min(a.rows, MAX_BLOCKS)), dim3(256), 0, s, a);
+  const int nvec = cdiv(a.cols, RowSpan<T>::V);
+  if (nvec <= 64 * 4) launch_rows<T, 64, 4>(a, s);
+  else if (nvec <= 256 * 4) launch_rows<T, 256, 4>(a, s);
+  else if (a.rows <= 512 && nvec <= 1024 * 4) launch_rows<T, 1024, 4>(a, s);
+  else if (nvec <= 256 * 16) launch_rows<T, 256, 16>(a, s);
+  else if (a.rows > 512 && nvec <= 512 * 16) launch_rows<T, 512, 16>(a, s);
+  else launch_rows<T, 1024, 16>(a, s);
 }
 template <typename T> void run_bwd(const LpArgs<T>& a, hipStream_t s) {
-  hipLaunchKernelGGL(k_logprob_bwd<T>, dim3(cdiv(a.cols, 4096), std::min(a.rows, 65535)), dim3(256), 0, s, a);
+  const int nvec = cdiv(a.cols, RowSpan<T>::V);
+  auto go = [&](auto kernel, int nt, int nv) {
+    const int parts = cdiv(nvec, nt * nv);
+    const long items = (long)a.rows * parts;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<long>((items + 256 / nt - 1) / (256 / nt), MAX_BLOCKS)), dim3(256), 0, s, a, parts);
+  };
+  if (nvec <= 64 * 4) go(k_logprob_bwd<T, 64, 4>, 64, 4);
+  else go(k_logprob_bwd<T, 256, 4>, 256, 4);
 }
 
 bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
