@@ -9,8 +9,9 @@ using namespace dm;
 
 namespace {
 
-constexpr float INF = __builtin_inff(), NAN_ = __builtin_nanf(""), LEAST = -3.402823466e38f;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float INF = __builtin_inff(), NAN_ = __builtin_nanf("");
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float FLOOR = -0x1p100f;   // fills the places of a tile without a logit; no reference of a sum is lower
 constexpr int CANDIDATES = 1024;   // of a row's most likely tokens, in LDS
 
 template <typename T> struct LpArgs {
@@ -117,21 +118,31 @@ template <typename T> DM_DEV void unpack(const u32x4& r, float* v) {
 // x is computed here, not where it is used (all of a tile's summands would wait in registers until then)
 DM_DEV void here(float& x) { asm volatile("" : "+v"(x)); }
 
-// A thread's part of one tile of a row: NV vectors and (first tile) one single column, -inf where there is none.
+// The larger of two pairs of bf16 numbers. Both formats order by sign and magnitude, so fp16's maximum serves; it passes
+// over what reads as a NaN there, magnitudes of 2^121 and more, infinities and NaN among them.
+DM_DEV uint32_t pair_max(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("v_pk_max_f16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
+// A thread's part of one tile of a row: NV vectors and (first tile) one single column, FLOOR where there is none.
 template <typename T, int NT, int NV> struct Tile {
   static constexpr int V = RowSpan<T>::V;
+  static constexpr uint32_t FILL = sizeof(T) == 2 ? 0xf180f180u : 0xf1800000u;
   u32x4 raw[NV];
   float edge;
+  int nv;   // vectors that any of the block's threads has
   DM_DEV void load(const RowSpan<T>& row, int tile) {
-    const uint32_t fill = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+    nv = (row.nvec + NT - 1) / NT - tile * NV;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int q0 = (tile * NV + i) * NT;
-      raw[i] = u32x4{fill, fill, fill, fill};
+      raw[i] = u32x4{FILL, FILL, FILL, FILL};
       if (q0 + (int)threadIdx.x < row.nvec) raw[i] = row.vec(q0, threadIdx.x);
     }
     const int c = tile == 0 ? row.edge_col(threadIdx.x) : -1;
-    edge = c >= 0 ? to_f(row.x[c]) : -INF;
+    edge = c >= 0 ? to_f(row.x[c]) : FLOOR;
   }
   // vector i's logits, converted where they are used: kept from pass to pass the converted ones would take twice the
   // registers of the row (the statement hides from the compiler that it has converted them before)
@@ -139,27 +150,128 @@ template <typename T, int NT, int NV> struct Tile {
     asm volatile("" : "+v"(raw[i]));
     unpack<T>(raw[i], v);
   }
+  // the largest logit of a vector, FLOOR at least (bf16: magnitudes of 2^121 left out)
+  DM_DEV float largest_of(int i) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t p = pair_max(pair_max(raw[i][0], raw[i][1]), pair_max(raw[i][2], pair_max(raw[i][3], FILL)));
+      return fmaxf(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+    } else {
+      return fmaxf(fmaxf(fmaxf(__uint_as_float(raw[i][0]), __uint_as_float(raw[i][1])),
+                         fmaxf(__uint_as_float(raw[i][2]), __uint_as_float(raw[i][3]))), FLOOR);
+    }
+  }
+  DM_DEV float largest() {
+    float m = fmaxf(edge, FLOOR);
+    uint32_t p = FILL;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (i >= nv) continue;
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p = pair_max(p, raw[i][j]);
+      } else {
+        m = fmaxf(m, largest_of(i));
+      }
+    }
+    if constexpr (sizeof(T) == 2) m = fmaxf(m, fmaxf(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)));
+    return m;
+  }
 };
 
-// The NT threads' (maximum m, z = sum of e^(x - m), q = sum of e^(x - m) (x - m)) as one.
-template <int NT> DM_DEV void combine(float& m, float& z, float& q, Shared<NT>& sh) {
-  auto rescale = [&](float M) {
-    const float d = fmaxf(m - M, -1e30f), f = exp_of(d);   // z = q = 0 where m is LEAST
-    q = f * (q + z * d);
+// A thread's sums over its logits relative to a reference m: with y = x log2 e + c and c = -m log2 e (rounded: it is c
+// that counts, so far rows lose nothing), z = sum of 2^y and q = sum of 2^y y.
+struct Sums {
+  float m, c, z, q;
+  DM_DEV Sums() : m(FLOOR), c(-FLOOR * LOG2E), z(0.f), q(0.f) {}
+  DM_DEV void refer(float to) {
+    const float c1 = -to * LOG2E, d = c1 - c, f = __builtin_amdgcn_exp2f(d);
+    q = f > 0.f ? f * (q + z * d) : 0.f;
     z *= f;
-    m = M;
-  };
-  rescale(wave_max(m));
+    m = to;
+    c = c1;
+  }
+  template <typename T, int NT, int NV> DM_DEV void add(Tile<T, NT, NV>& t) {
+    float zt = 0.f, qt = 0.f;
+    pass<false>(t, zt, qt);
+    if (__any(qt != qt)) {   // -inf among them: 0 times -inf
+      zt = qt = 0.f;
+      pass<true>(t, zt, qt);
+    }
+    z += zt;
+    q += qt;
+  }
+  template <bool CLAMP, typename T, int NT, int NV> DM_DEV void pass(Tile<T, NT, NV>& t, float& zt, float& qt) {
+    auto one = [&](float x) {
+      const float y = fmaf(x, LOG2E, c), e = __builtin_amdgcn_exp2f(y);
+      zt += e;
+      qt = fmaf(e, CLAMP ? fmaxf(y, -1e30f) : y, qt);
+    };
+    one(t.edge);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (i >= t.nv) continue;
+      float v[Tile<T, NT, NV>::V];
+      t.get(i, v);
+#pragma unroll
+      for (int j = 0; j < Tile<T, NT, NV>::V; ++j) one(v[j]);
+      here(zt);
+      here(qt);
+    }
+  }
+  // the block's sums in every thread
+  template <int NT> DM_DEV void join(Shared<NT>& sh) {
+    refer(wave_max(m));
+    z = wave_sum(z);
+    q = wave_sum(q);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) sh.m[wave] = m, sh.z[wave] = z, sh.q[wave] = q;
+    __syncthreads();
+    const int w = threadIdx.x % (NT / 64);   // each wave's lanes join all waves' sums
+    m = sh.m[w], z = sh.z[w], q = sh.q[w];
+    c = -m * LOG2E;
+    refer(lanes_max<1, NT / 128>(m));
+    z = lanes_sum<1, NT / 128>(z);
+    q = lanes_sum<1, NT / 128>(q);
+  }
+};
+
+// A row's statistics element by element: rows with a NaN, +inf, or nothing above FLOOR.
+template <typename T, int NT> DM_DEV RowStats slow_stats(const T* x, int n, Shared<NT>& sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float m = -INF;
+  int nan = 0;
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const float v = to_f(x[i]);
+    nan |= v != v;
+    m = fmaxf(m, v);
+  }
+  m = wave_max(m);
+  __syncthreads();   // the sums in sh have been read
+  if (lane == 0) sh.m[wave] = m;
+  nan = __syncthreads_or(nan);
+  RowStats s;
+  s.M = sh.m[0];
+  for (int w = 1; w < NT / 64; ++w) s.M = fmaxf(s.M, sh.m[w]);
+  if (nan) s.M = NAN_;
+  s.lse = s.log_z = s.M;
+  s.entropy = s.M == -INF ? 0.f : NAN_;
+  if (nan || fabsf(s.M) == INF) return s;
+  float z = 0.f, q = 0.f;
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const float d = to_f(x[i]) - s.M, e = exp_of(d);
+    z += e;
+    q += e * fmaxf(d, -1e30f);
+  }
   z = wave_sum(z);
   q = wave_sum(q);
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) sh.m[wave] = m, sh.z[wave] = z, sh.q[wave] = q;
+  if (lane == 0) sh.z[wave] = z, sh.q[wave] = q;
   __syncthreads();
-  const int w = threadIdx.x % (NT / 64);   // each wave's lanes combine all waves' values
-  m = sh.m[w], z = sh.z[w], q = sh.q[w];
-  rescale(lanes_max<1, NT / 128>(m));
-  z = lanes_sum<1, NT / 128>(z);
-  q = lanes_sum<1, NT / 128>(q);
+  z = q = 0.f;
+  for (int w = 0; w < NT / 64; ++w) z += sh.z[w], q += sh.q[w];
+  s.log_z = logf(z);
+  s.lse = s.M + s.log_z;
+  s.entropy = s.log_z - q / z;
+  return s;
 }
 
 // The row's `top` largest in order, found one after the other: any row, any values.
@@ -187,7 +299,7 @@ template <typename T, int NT> DM_DEV void slow_top(const LpArgs<T>& a, long r, c
   __syncthreads();   // the row has been read
 }
 
-// A bound that at least `top` of the row's logits reach, -inf at least: of the 64 lanes' largest logits the top-th.
+// A bound that at least `top` of the row's logits reach, or the least number: of the 64 lanes' largest logits the top-th.
 template <typename T, int NT> DM_DEV float top_bound(int top, const Shared<NT>& sh) {
   float g = -INF;
 #pragma unroll
@@ -199,30 +311,29 @@ template <typename T, int NT> DM_DEV float top_bound(int top, const Shared<NT>& 
     const uint32_t b = bound | 1u << bit;
     if (__popcll(__ballot(o >= b)) >= top) bound = b;
   }
-  return bound <= ORDER_OF_MINUS_INF ? -INF : value_of(bound);
+  return bound <= ORDER_OF_MINUS_INF ? -3.402823466e38f : value_of(bound);
 }
 template <int NT> DM_DEV void take(float x, int col, Shared<NT>& sh) {
   const int at = atomicAdd(&sh.count, 1);
   if (at < CANDIDATES) sh.cand[at] = order_of(x, col);
 }
-// this tile's logits of at least `bound` into the list
+// this tile's logits of at least `bound` (a number) into the list
 template <typename T, int NT, int NV> DM_DEV void take_tile(const RowSpan<T>& row, Tile<T, NT, NV>& t, int tile, float bound, Shared<NT>& sh) {
   constexpr int V = RowSpan<T>::V;
-  if (t.edge >= bound && t.edge > -INF) take(t.edge, row.edge_col(threadIdx.x), sh);
+  const int c = tile == 0 ? row.edge_col(threadIdx.x) : -1;
+  if (c >= 0 && t.edge >= bound) take(t.edge, c, sh);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    if (i >= t.nv) continue;
+    const int q = (tile * NV + i) * NT + threadIdx.x;
+    if (fmaxf(t.largest_of(i), FLOOR) < bound || q >= row.nvec) continue;
     float v[V];
     t.get(i, v);
-    uint32_t hit = 0;
-#pragma unroll
-    for (int j = 0; j < V; ++j) hit |= (v[j] >= bound && v[j] > -INF) << j;
-    while (hit) {
-      const int j = __ffs(hit) - 1;
-      hit &= hit - 1;
+    for (int j = 0; j < V; ++j) {
       float x = v[0];
 #pragma unroll
       for (int k = 1; k < V; ++k) x = j == k ? v[k] : x;
-      take(x, row.col(tile * NT * NV + i * NT + threadIdx.x) + j, sh);
+      if (x >= bound) take(x, row.col(q) + j, sh);
     }
   }
 }
@@ -272,7 +383,8 @@ DM_DEV void store_tile(const RowSpan<T>& row, Tile<T, NT, NV>& t, int tile, cons
   const bool plain = w.nan || w.zero;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int q = tile * NT * NV + i * NT + threadIdx.x;
+    if (i >= t.nv) continue;
+    const int q = (tile * NV + i) * NT + threadIdx.x;
     if (q >= row.nvec) continue;
     float v[V];
     t.get(i, v);
@@ -293,65 +405,31 @@ template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT
     const int tiles = max(1, (row.nvec + NT * NV - 1) / (NT * NV));
     const long t = a.target ? a.target[r] : -1;
     const float xt = t >= 0 && t < a.cols ? to_f(row.x[t]) : 0.f;
-    float m = LEAST, z = 0.f, q = 0.f;
+    Sums u;
     Tile<T, NT, NV> tile;
     if (a.top && threadIdx.x == 0) sh.count = 0;
     for (int i = 0; i < tiles; ++i) {
       tile.load(row, i);
-      float m1 = fmaxf(m, tile.edge);
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        float v[RowSpan<T>::V];
-        tile.get(k, v);
-#pragma unroll
-        for (int j = 0; j < RowSpan<T>::V; ++j) m1 = fmaxf(m1, v[j]);
-        here(m1);
-      }
-      const float d0 = fmaxf(m - m1, -1e30f), f = exp_of(d0);
-      q = f * (q + z * d0);
-      z *= f;
-      m = m1;
-      auto add = [&](float x) {
-        const float d = x - m, e = exp_of(d);
-        z += e;
-        q += e * fmaxf(d, -1e30f);
-      };
-      add(tile.edge);
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        float v[RowSpan<T>::V];
-        tile.get(k, v);
-#pragma unroll
-        for (int j = 0; j < RowSpan<T>::V; ++j) add(v[j]);
-        here(z);
-        here(q);
-      }
+      u.refer(fmaxf(u.m, tile.largest()));
+      u.add(tile);
       if (a.top) {   // the bound only rises from tile to tile
-        sh.largest[threadIdx.x] = z > 0.f ? m : -INF;
+        sh.largest[threadIdx.x] = u.m > FLOOR ? u.m : -INF;
         __syncthreads();
         take_tile(row, tile, i, top_bound<T>(a.top, sh), sh);
         if (i + 1 < tiles) __syncthreads();
       }
     }
-    combine(m, z, q, sh);
+    u.join(sh);
     RowStats s;
-    const bool bad = !(z < INF);   // a NaN or +inf in the row
-    if (bad) {
-      int nan = 0;
-      for (int i = threadIdx.x; i < a.cols; i += NT) {
-        const float v = to_f(row.x[i]);
-        nan |= v != v;
-      }
-      s.M = s.log_z = s.lse = __syncthreads_or(nan) ? NAN_ : INF;
-      s.entropy = NAN_;
-    } else if (z == 0.f) {
-      s.M = s.log_z = s.lse = -INF;
-      s.entropy = 0.f;
+    const bool slow = !(u.z < INF) || u.m <= FLOOR;
+    if (slow) {
+      s = slow_stats<T, NT>(row.x, a.cols, sh);
     } else {
-      s.M = m;
-      s.log_z = logf(z);
-      s.lse = m + s.log_z;
-      s.entropy = s.log_z - q / z;
+      s.M = u.m;
+      const float l2 = __builtin_amdgcn_logf(u.z), shift = fmaf(u.m, LOG2E, u.c);   // what c's rounding left
+      s.log_z = (l2 - shift) * LN2;
+      s.lse = s.M + s.log_z;
+      s.entropy = (l2 - u.q / u.z) * LN2;
     }
     if (threadIdx.x == 0) {
       if (a.logp) a.logp[r] = t < 0 ? 0.f : t < a.cols ? s.logp(xt) : NAN_;
@@ -361,7 +439,7 @@ template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT
     }
     if (a.top) {
       const int c = sh.count;
-      if (bad || c > CANDIDATES) slow_top<T, NT>(a, r, s, sh);
+      if (slow || c > CANDIDATES) slow_top<T, NT>(a, r, s, sh);
       else write_top<T, NT>(a, r, s, c, sh);
     }
     if constexpr (GRAD) {
