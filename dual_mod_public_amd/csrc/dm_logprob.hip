@@ -64,22 +64,29 @@ DM_DEV uint64_t wave_max_u64(uint64_t k) {
   return k;
 }
 
-// What a row's gradient is made of: dx[v] = -p (g + gh (logp(v) + H)), + g at the target.
+// What a row's gradient is made of: dx[v] = -p (g + gh (logp(v) + H)), + g at the target, as p (a + b y) with
+// y = logp(v) log2 e, p = 2^y.
 struct RowGrad {
-  float g, gh;
-  bool zero, nan;   // a row of zeros, of NaN
+  float M, l2z, a, b, g;
+  bool fill;      // every element the same:
+  float value;    // 0 or NaN
+  DM_DEV float of(float x) const {
+    const float y = fmaf(x - M, LOG2E, -l2z), p = __builtin_amdgcn_exp2f(y);
+    return p * fmaf(b, fmaxf(y, -1e30f), a);   // p = 0 at -inf
+  }
 };
-template <typename T> DM_DEV RowGrad row_grad(const LpArgs<T>& a, long r, long t, float lse) {
+template <typename T> DM_DEV RowGrad row_grad(const LpArgs<T>& a, long r, long t, const RowStats& s) {
   RowGrad w;
+  const float gh = a.g_entropy ? a.g_entropy[r] : 0.f;
   w.g = a.g_logp && t >= 0 ? a.g_logp[r] : 0.f;
-  w.gh = a.g_entropy ? a.g_entropy[r] : 0.f;
-  w.zero = (w.g == 0.f && w.gh == 0.f) || lse == -INF;
-  w.nan = !w.zero && (!(fabsf(lse) < INF) || (w.g != 0.f && t >= a.cols));
+  w.M = s.M;
+  w.l2z = s.log_z * LOG2E;
+  w.a = -w.g - (gh == 0.f ? 0.f : gh * s.entropy);
+  w.b = -gh * LN2;
+  const bool zero = (w.g == 0.f && gh == 0.f) || s.lse == -INF;
+  w.fill = zero || !(fabsf(s.lse) < INF) || (w.g != 0.f && t >= a.cols);
+  w.value = zero ? 0.f : NAN_;
   return w;
-}
-DM_DEV float grad_of(const RowStats& s, const RowGrad& w, float x) {
-  const float lp = (x - s.M) - s.log_z, p = exp_of(lp);
-  return -p * (w.g + w.gh * (fmaxf(lp, -1e30f) + s.entropy));   // p = 0 at -inf
 }
 
 // A row in 16-byte vectors: the columns before the first and behind the last whole aligned vector (at most
@@ -365,36 +372,49 @@ template <typename T, int NT> DM_DEV void write_top(const LpArgs<T>& a, long r, 
   }
 }
 
-// One vector of the gradient into dx's aligned vectors, or element by element where dx lies otherwise than x.
-template <typename T> DM_DEV void store_grad(T* p, const float* v, bool aligned) {
+// Vector q0 + lane of a row's gradient dx (RowSpan::vec's addressing), element by element where dx lies otherwise in its
+// 16 bytes than x.
+template <typename T> DM_DEV void store_grad(T* dx, const RowSpan<T>& row, int q0, int lane, const float* v, bool aligned) {
   constexpr int V = RowSpan<T>::V;
+  T* p = reinterpret_cast<T*>(reinterpret_cast<char*>(dx + row.c0 + (long)q0 * V) + 16u * lane);
   if (aligned) {
-    store_vec<T, V>(p, v);
+    store_vec_nt<T, V>(p, v);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) p[j] = from_f<T>(v[j]);
   }
 }
-template <typename T, int NT, int NV>
-DM_DEV void store_tile(const RowSpan<T>& row, Tile<T, NT, NV>& t, int tile, const RowStats& s, const RowGrad& w, long target, T* dx) {
+template <typename T> DM_DEV bool same_alignment(const T* dx, const RowSpan<T>& row) {
+  return ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
+}
+// the gradient of vector q0 + lane from its logits v
+template <typename T>
+DM_DEV void grad_vec(T* dx, const RowSpan<T>& row, int q0, int lane, float* v, const RowGrad& w, int target, bool aligned) {
   constexpr int V = RowSpan<T>::V;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
-  const float all = w.nan ? NAN_ : 0.f;
-  const bool plain = w.nan || w.zero;
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = w.of(v[j]);
+  const int at = target - row.col(q0 + lane);
+  if ((unsigned)at < (unsigned)V) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += at == j ? w.g : 0.f;
+  }
+  store_grad(dx, row, q0, lane, v, aligned);
+}
+template <typename T> DM_DEV void grad_edge(T* dx, int c, float x, const RowGrad& w, int target) {
+  if (c >= 0) dx[c] = from_f<T>(w.of(x) + (c == target ? w.g : 0.f));
+}
+template <typename T, int NT, int NV>
+DM_DEV void store_tile(const RowSpan<T>& row, Tile<T, NT, NV>& t, int tile, const RowGrad& w, int target, T* dx) {
+  const bool aligned = same_alignment(dx, row);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (i >= t.nv) continue;
-    const int q = (tile * NV + i) * NT + threadIdx.x;
-    if (q >= row.nvec) continue;
-    float v[V];
+    const int q0 = (tile * NV + i) * NT;
+    if (i >= t.nv || q0 + (int)threadIdx.x >= row.nvec) continue;
+    float v[RowSpan<T>::V];
     t.get(i, v);
-    const long at = target - row.col(q);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = plain ? all : grad_of(s, w, v[j]) + (at == j ? w.g : 0.f);
-    store_grad(dx + row.col(q), v, aligned);
+    grad_vec(dx, row, q0, threadIdx.x, v, w, target, aligned);
   }
-  const int c = tile == 0 ? row.edge_col(threadIdx.x) : -1;
-  if (c >= 0) dx[c] = from_f<T>(plain ? all : grad_of(s, w, t.edge) + (c == target ? w.g : 0.f));
+  if (tile == 0) grad_edge(dx, row.edge_col(threadIdx.x), t.edge, w, target);
 }
 
 // A block per row, the row in tiles of NT NV vectors held in registers.
@@ -443,11 +463,16 @@ template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT
       else write_top<T, NT>(a, r, s, c, sh);
     }
     if constexpr (GRAD) {
-      const RowGrad w = row_grad(a, r, t, s.lse);
+      const RowGrad w = row_grad(a, r, t, s);
+      const int target = t < a.cols ? (int)t : -1;
       T* dx = a.dx + r * a.ld_d;
-      for (int i = 0; i < tiles; ++i) {
-        if (tiles > 1) tile.load(row, i);
-        store_tile(row, tile, i, s, w, t, dx);
+      if (w.fill) {
+        for (int i = threadIdx.x; i < a.cols; i += NT) dx[i] = from_f<T>(w.value);
+      } else {
+        for (int i = 0; i < tiles; ++i) {
+          if (tiles > 1) tile.load(row, i);
+          store_tile(row, tile, i, w, target, dx);
+        }
       }
     }
     __syncthreads();   // sh is free again
@@ -466,17 +491,16 @@ template <typename T, int NT, int NV> __global__ __launch_bounds__(256) void k_l
     s.lse = s.M + s.log_z;
     s.entropy = a.g_entropy ? a.entropy[r] : 0.f;
     const long t = a.target ? a.target[r] : -1;
-    const RowGrad w = row_grad(a, r, t, s.lse);
+    const RowGrad w = row_grad(a, r, t, s);
+    const int target = t < a.cols ? (int)t : -1;
     const RowSpan<T> row(a.x + r * a.ld, a.cols);
     T* dx = a.dx + r * a.ld_d;
-    const bool aligned = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(row.x)) & 15) == 0;
-    const float all = w.nan ? NAN_ : 0.f;
-    const bool plain = w.nan || w.zero;
+    const bool aligned = same_alignment(dx, row);
     u32x4 raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       raw[i] = u32x4{0, 0, 0, 0};
-      if (!plain && q0 + i * NT < row.nvec) raw[i] = row.vec(0, q0 + i * NT);
+      if (!w.fill && q0 + i * NT < row.nvec) raw[i] = row.vec(0, q0 + i * NT);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -484,13 +508,17 @@ template <typename T, int NT, int NV> __global__ __launch_bounds__(256) void k_l
       if (q >= row.nvec) continue;
       float v[RowSpan<T>::V];
       unpack<T>(raw[i], v);
-      const long at = t - row.col(q);
+      if (w.fill) {
 #pragma unroll
-      for (int j = 0; j < RowSpan<T>::V; ++j) v[j] = plain ? all : grad_of(s, w, v[j]) + (at == j ? w.g : 0.f);
-      store_grad(dx + row.col(q), v, aligned);
+        for (int j = 0; j < RowSpan<T>::V; ++j) v[j] = w.value;
+        store_grad(dx, row, 0, q, v, aligned);
+      } else {
+        grad_vec(dx, row, 0, q, v, w, target, aligned);
+      }
     }
     const int c = it % parts == 0 ? row.edge_col(q0) : -1;
-    if (c >= 0) dx[c] = from_f<T>(plain ? all : grad_of(s, w, to_f(row.x[c])) + (c == t ? w.g : 0.f));
+    if (c >= 0 && w.fill) dx[c] = from_f<T>(w.value);
+    else if (c >= 0) grad_edge(dx, c, to_f(row.x[c]), w, target);
   }
 }
 
@@ -501,19 +529,34 @@ template <typename T> LpArgs<T> typed(const dm_logprob_args* a) {
           a->top_ids, a->g_logp, a->g_entropy, a->ld, a->ld_d, a->rows, a->cols, a->top};
 }
 
-template <typename T, int NT, int NV> void launch_rows(const LpArgs<T>& a, hipStream_t s) {
-  const dim3 grid(std::min(a.rows, MAX_BLOCKS));
-  if (a.dx) hipLaunchKernelGGL((k_logprob_rows<T, NT, NV, true>), grid, dim3(NT), 0, s, a);
-  else hipLaunchKernelGGL((k_logprob_rows<T, NT, NV, false>), grid, dim3(NT), 0, s, a);
+template <bool GRAD, typename T, int NT, int NV> void launch_rows(const LpArgs<T>& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_logprob_rows<T, NT, NV, GRAD>), dim3(std::min(a.rows, MAX_BLOCKS)), dim3(NT), 0, s, a);
 }
+// The threads of a row and their vectors per tile, by the row's 16-byte vectors (bf16: 8 logits, fp32: 4).
+// Fewer rows than CUs: as many threads as a block has, since nothing else hides a row's latencies (one row of 32000 bf16
+// 6.7 us, at 256 threads 8.4).
+// Otherwise the smallest blocks that fill a CU's memory pipes while others of the CU wait at their barriers (4096 rows of
+// 32000 bf16: 64 threads 51 us, 256 48, 1024 80). With the gradient a row is best read once and held until it is
+// written (the same rows: 256 threads of 16 vectors, all of a row, 106 us; of 8 vectors, read twice, 121); rows past
+// 65536 fp32 or 131072 bf16 are read twice (2000 rows of 100003 bf16: 188 us held, 193 read twice).
 template <typename T> void run_rows(const LpArgs<T>& a, hipStream_t s) {
   const int nvec = cdiv(a.cols, RowSpan<T>::V);
-  if (nvec <= 64 * 4) launch_rows<T, 64, 4>(a, s);
-  else if (nvec <= 256 * 4) launch_rows<T, 256, 4>(a, s);
-  else if (a.rows <= 512 && nvec <= 1024 * 4) launch_rows<T, 1024, 4>(a, s);
-  else if (nvec <= 256 * 16) launch_rows<T, 256, 16>(a, s);
-  else if (a.rows > 512 && nvec <= 512 * 16) launch_rows<T, 512, 16>(a, s);
-  else launch_rows<T, 1024, 16>(a, s);
+  const bool few = a.rows < 256 && nvec > 256 * 4;
+  if (!a.dx) {
+    if (nvec <= 64 * 4) launch_rows<false, T, 64, 4>(a, s);
+    else if (nvec <= 256 * 4) launch_rows<false, T, 256, 4>(a, s);
+    else if (!few) launch_rows<false, T, 256, 8>(a, s);
+    else if (nvec <= 1024 * 4) launch_rows<false, T, 1024, 4>(a, s);
+    else launch_rows<false, T, 1024, 16>(a, s);
+  } else {
+    if (nvec <= 64 * 4) launch_rows<true, T, 64, 4>(a, s);
+    else if (nvec <= 64 * 8) launch_rows<true, T, 64, 8>(a, s);
+    else if (nvec <= 256 * 4) launch_rows<true, T, 256, 4>(a, s);
+    else if (few && nvec <= 1024 * 4) launch_rows<true, T, 1024, 4>(a, s);
+    else if (nvec <= 256 * 16) launch_rows<true, T, 256, 16>(a, s);
+    else if (!few && nvec <= 512 * 16) launch_rows<true, T, 512, 16>(a, s);
+    else launch_rows<true, T, 1024, 16>(a, s);
+  }
 }
 template <typename T> void run_bwd(const LpArgs<T>& a, hipStream_t s) {
   const int nvec = cdiv(a.cols, RowSpan<T>::V);
