@@ -24,7 +24,6 @@ struct PlanTensor {
 };
 // what the step's kernels share: written by k_adamw_begin
 struct Control {
-  double norm;
   float coef, rate, v_scale, lr;   // c, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
   uint32_t key;                    // the step's hash
   int skip;
@@ -46,7 +45,22 @@ struct AdamArgs {
 };
 
 DM_DEV float grad_at(const PlanTensor& t, long i) {
-  return t.g_bf16 ? to_f(((const bf16*)t.g)[i]) : ((const float*)t.g)[i];
+  return t.g_bf16 ? __uint_as_float((uint32_t)ld_global<uint16_t>((const bf16*)t.g + i) << 16) : ld_global<float>((const float*)t.g + i);
+}
+// Four elements from i on. Parameters and gradients may be views at any element of a buffer: their vectors are aligned
+// to their elements only.
+template <bool BF16> DM_DEV floatx4 grads4(const PlanTensor& t, long i) {
+  if constexpr (BF16) {
+    const u32x2 r = ld_global_a<u32x2, 2>((const bf16*)t.g + i);
+    return floatx4{__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xffff0000u), __uint_as_float(r[1] << 16),
+                   __uint_as_float(r[1] & 0xffff0000u)};
+  } else {
+    return ld_global_a<floatx4, 4>((const float*)t.g + i);
+  }
+}
+DM_DEV void store4(float* p, const floatx4& v) {   // global, as ld_global_a
+  typedef floatx4 V __attribute__((aligned(4)));
+  *(__attribute__((address_space(1))) V*)p = v;
 }
 
 DM_DEV double block_sum(double x, double* red) {
@@ -60,21 +74,40 @@ DM_DEV double block_sum(double x, double* red) {
   return x;
 }
 
-// part[b] = sum of g^2 over chunks b, b + NORM_PARTS, ...
+template <bool BF16> DM_DEV void add_squares(const PlanTensor& t, long i, long end, double (&s)[4]) {
+  constexpr int STEP = 256 * 4, IN_FLIGHT = 4;
+  i += 4 * threadIdx.x;
+  for (; i + (IN_FLIGHT - 1) * STEP + 3 < end; i += IN_FLIGHT * STEP) {
+    floatx4 g[IN_FLIGHT];
+#pragma unroll
+    for (int k = 0; k < IN_FLIGHT; ++k) g[k] = grads4<BF16>(t, i + k * STEP);
+#pragma unroll
+    for (int k = 0; k < IN_FLIGHT; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] += (double)g[k][j] * g[k][j];
+  }
+  for (; i < end; i += STEP)
+    for (int j = 0; j < 4 && i + j < end; ++j) {
+      const double g = grad_at(t, i + j);
+      s[j] += g * g;
+    }
+}
+// part[b] = sum of g^2 over the b-th run of chunks. The squares of fp32 are exact in 64 bits, so the norm is the same for
+// any order of the sum but for its last bits. Bound by reading the gradients.
 __global__ __launch_bounds__(256) void k_grad_sumsq(const PlanTensor* tensors, const int* chunk_tensor, long n_chunks,
                                                     double* part) {
   __shared__ double red[4];
-  double s = 0.;
-  for (long c = blockIdx.x; c < n_chunks; c += gridDim.x) {
+  double s[4] = {0., 0., 0., 0.};
+  const long end = (blockIdx.x + 1) * n_chunks / gridDim.x;
+  for (long c = blockIdx.x * n_chunks / gridDim.x; c < end;) {
     const PlanTensor t = tensors[chunk_tensor[c]];
-    const long i0 = (c - t.chunk0) * CHUNK;
-    for (long i = i0 + threadIdx.x; i < min(i0 + CHUNK, t.n); i += 256) {
-      const double g = grad_at(t, i);
-      s += g * g;
-    }
+    const long first = (c - t.chunk0) * CHUNK, last = min((end - t.chunk0) * CHUNK, t.n);   // this run's part of the tensor
+    if (t.g_bf16) add_squares<true>(t, first, last, s);
+    else add_squares<false>(t, first, last, s);
+    c = t.chunk0 + (last + CHUNK - 1) / CHUNK;
   }
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) part[blockIdx.x] = s;
+  const double x = block_sum((s[0] + s[1]) + (s[2] + s[3]), red);
+  if (threadIdx.x == 0) part[blockIdx.x] = x;
 }
 
 // A 32-bit hash: two odd multipliers and three shifts.
@@ -90,7 +123,7 @@ struct BeginArgs {
   Control* c;
   const double* part;
   int parts;   // 0: no norm
-  double beta1, beta2, max_norm;
+  double log2_beta1, log2_beta2, max_norm;
   int skip_nonfinite;
   uint32_t seed;
   const float* lr;
@@ -103,20 +136,20 @@ __global__ __launch_bounds__(256) void k_adamw_begin(BeginArgs a) {
   __shared__ double red[4];
   double s = 0.;
   for (int i = threadIdx.x; i < a.parts; i += 256) s += a.part[i];
+  const int64_t t = a.steps ? *a.steps + 1 : 0;
+  const double power1 = exp2(t * a.log2_beta1), power2 = exp2(t * a.log2_beta2);
   s = block_sum(s, red);
   if (threadIdx.x > 0) return;
   const double norm = sqrt(s);
   if (a.parts > 0 && a.norm) *a.norm = (float)norm;
   if (!a.steps) return;   // the norm alone
-  Control c;
-  c.norm = norm;
+  Control c{};
   c.skip = a.skip_nonfinite && !(norm < __builtin_inf());
   if (c.skip) {
     *a.skipped += 1;
     *a.c = c;
     return;
   }
-  const int64_t t = *a.steps + 1;
   *a.steps = t;
   c.coef = 1.f;
   if (a.max_norm > 0.) {
@@ -124,25 +157,71 @@ __global__ __launch_bounds__(256) void k_adamw_begin(BeginArgs a) {
     c.coef = k < 1. || k != k ? (float)k : 1.f;
   }
   c.lr = *a.lr;
-  c.rate = (float)(c.lr / (1. - pow(a.beta1, (double)t)));
-  c.v_scale = (float)(1. / sqrt(1. - pow(a.beta2, (double)t)));
+  c.rate = (float)(c.lr / (1. - power1));
+  c.v_scale = (float)(1. / sqrt(1. - power2));
   c.key = mix(a.seed + (uint32_t)t * 0x9E3779B1u);
   *a.c = c;
 }
 
 // m and v of one element from its gradient; each product and sum rounded by itself, so that the codes made from them
 // do not depend on how a compiler contracts them
-DM_DEV void moments(const AdamArgs& a, float g, float& m, float& v) {
+DM_DEV void moments(const AdamArgs& a, float b1, float b2, float g, float& m, float& v) {
 #pragma clang fp contract(off)
-  const float m0 = a.b1 * m, m1 = a.c1 * g, v0 = a.b2 * v, v1 = a.c2 * (g * g);
+  const float m0 = b1 * m, m1 = a.c1 * g, v0 = b2 * v, v1 = a.c2 * (g * g);
   m = m0 + m1;
   v = v0 + v1;
 }
-DM_DEV float updated(const AdamArgs& a, const Control& c, const PlanTensor& t, float p, float m, float v) {
-  const float keep = (float)(1. - (double)c.lr * t.lr_scale * t.weight_decay);
-  return p * keep - c.rate * t.lr_scale * (m / (sqrtf(v) * c.v_scale + a.eps));
-}
+// The parameters' part of a step, per tensor.
+struct Update {
+  float keep, rate, v_scale, eps;
+  DM_DEV Update(const AdamArgs& a, const Control& c, const PlanTensor& t)
+      : keep((float)(1. - (double)c.lr * t.lr_scale * t.weight_decay)), rate(c.rate * t.lr_scale), v_scale(c.v_scale), eps(a.eps) {}
+  DM_DEV float of(float p, float m, float v) const {   // a square root and a reciprocal of one ulp each
+    const float denom = fmaf(__builtin_amdgcn_sqrtf(v), v_scale, eps);
+    return p * keep - rate * (m * __builtin_amdgcn_rcpf(denom));
+  }
+};
 
+// A block per chunk; bound by its 28 bytes per element.
+template <bool BF16> DM_DEV void step32(const AdamArgs& a, const Control& c, const PlanTensor& t, long i0, float* ms, float* vs) {
+  const Update u(a, c, t);
+  constexpr int STEP = 256 * 4, N = CHUNK / STEP;
+  if (i0 + CHUNK <= t.n) {
+    i0 += 4 * threadIdx.x;
+    floatx4 p[N], g[N], m[N], v[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const long i = i0 + k * STEP;
+      g[k] = grads4<BF16>(t, i);
+      m[k] = ld_global<floatx4>(ms + i);
+      v[k] = ld_global<floatx4>(vs + i);
+      p[k] = ld_global_a<floatx4, 4>(t.p + i);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const long i = i0 + k * STEP;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float m1 = m[k][j], v1 = v[k][j];
+        moments(a, a.b1, a.b2, g[k][j] * c.coef, m1, v1);
+        m[k][j] = m1;
+        v[k][j] = v1;
+        p[k][j] = u.of(p[k][j], m1, v1);
+      }
+      store4(ms + i, m[k]);
+      store4(vs + i, v[k]);
+      store4(t.p + i, p[k]);
+    }
+    return;
+  }
+  for (long i = i0 + threadIdx.x; i < t.n; i += 256) {
+    float m = ms[i], v = vs[i];
+    moments(a, a.b1, a.b2, grad_at(t, i) * c.coef, m, v);
+    ms[i] = m;
+    vs[i] = v;
+    t.p[i] = u.of(t.p[i], m, v);
+  }
+}
 __global__ __launch_bounds__(256) void k_adamw32(AdamArgs a) {
   const Control c = *a.c;
   if (c.skip) return;
@@ -150,32 +229,22 @@ __global__ __launch_bounds__(256) void k_adamw32(AdamArgs a) {
   const long i0 = (blockIdx.x - t.chunk0) * CHUNK;
   float* ms = (float*)a.m + t.block0 * BLOCK;
   float* vs = (float*)a.v + t.block0 * BLOCK;
-  for (long i = i0 + threadIdx.x; i < min(i0 + CHUNK, t.n); i += 256) {
-    float m = ms[i], v = vs[i];
-    moments(a, grad_at(t, i) * c.coef, m, v);
-    ms[i] = m;
-    vs[i] = v;
-    t.p[i] = updated(a, c, t, t.p[i], m, v);
-  }
+  if (t.g_bf16) step32<true>(a, c, t, i0, ms, vs);
+  else step32<false>(a, c, t, i0, ms, vs);
 }
 
-// The two code formats: a normal code is the exponent and the three upper mantissa bits of a, less (EXP - 1) << 3,
-// EXP the exponent field of the smallest normal a; below it the grid is 2^-GRID.
+// The two code formats. Shifted to the place of an fp32 number's exponent and upper mantissa bits, a code is one, its
+// smallest binade fp32's subnormal numbers; the value is that number times 2^(e - BIAS), e the block's exponent.
 struct First {
-  static constexpr int EXP = 112, GRID = 18;
+  static constexpr int BIAS = 14;
 };
 struct Second {
-  static constexpr int EXP = 96, GRID = 34;
+  static constexpr int BIAS = 30;
 };
-template <typename F> DM_DEV float decoded(uint32_t code, int e) {   // code without sign
-  const float a = code >= 8 ? __uint_as_float((code + ((F::EXP - 1) << 3)) << 20) : ldexpf((float)code, -F::GRID);
-  return e == 255 ? __builtin_nanf("") : ldexpf(a, e - 125);
-}
-// x >= 0 rounded by the 20 random bits r20; e: its block's exponent
+template <typename F> DM_DEV float decoded(uint32_t code, int e) { return ldexpf(__uint_as_float(code << 20), e - F::BIAS); }
+// x >= 0 rounded by the 20 random bits r20
 template <typename F> DM_DEV uint32_t encoded(float x, int e, uint32_t r20) {
-  const float a = ldexpf(x, 125 - e);
-  if (a >= ldexpf(1.f, 3 - F::GRID)) return ((__float_as_uint(a) + r20) >> 20) - ((F::EXP - 1) << 3);
-  return (uint32_t)(ldexpf(a, F::GRID) + ldexpf((float)r20, -20));
+  return (__float_as_uint(ldexpf(x, F::BIAS - e)) + r20) >> 20;
 }
 // the exponent field of a block's largest magnitude, 255 where one is not below 2^127; every lane of the wave
 DM_DEV int block_exponent(float largest, bool bad) {
@@ -184,34 +253,52 @@ DM_DEV int block_exponent(float largest, bool bad) {
 }
 DM_DEV bool too_large(float x) { return !(fabsf(x) < 0x1p127f); }
 
-// a wave per 256-element block, four elements per lane
-__global__ __launch_bounds__(256) void k_adamw8(AdamArgs a) {
-  const Control c = *a.c;
-  if (c.skip) return;
-  const PlanTensor t = a.tensors[a.chunk_tensor[blockIdx.x]];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int b = wave; b < CHUNK / BLOCK; b += 4) {
-    const long i0 = (blockIdx.x - t.chunk0) * CHUNK + b * BLOCK;
-    if (i0 >= t.n) return;
-    const long blk = t.block0 + i0 / BLOCK, at = blk * BLOCK + 4 * lane;
-    const int me = a.me[blk], ve = a.ve[blk];
-    const uint32_t mc = *(const uint32_t*)((const uint8_t*)a.m + at), vc = *(const uint32_t*)((const uint8_t*)a.v + at);
-    const uint32_t key = mix(c.key + (uint32_t)blk * 0x9E3779B1u);
+// A wave per run of four 256-element blocks, four elements per lane and block. Bound by its 16 bytes per element
+// (fp32 gradients) and the hash, two 32-bit products per element, about equally.
+template <bool BF16> DM_DEV void step8(const AdamArgs& a, const Control& c, const PlanTensor& t, long i0) {
+  constexpr int N = CHUNK / BLOCK / 4;
+  const Update u(a, c, t);
+  const int lane = threadIdx.x & 63;
+  const long blk0 = t.block0 + i0 / BLOCK;
+  floatx4 p[N], g[N];
+  uint32_t mc[N], vc[N];
+  int me[N], ve[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const long i = i0 + k * BLOCK + 4 * lane;
+    g[k] = p[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+    mc[k] = vc[k] = me[k] = ve[k] = 0;
+    if (i0 + k * BLOCK >= t.n) continue;
+    if (i + 3 < t.n) {
+      g[k] = grads4<BF16>(t, i);
+      p[k] = ld_global_a<floatx4, 4>(t.p + i);
+    } else {
+      for (int j = 0; j < 3; ++j)
+        if (i + j < t.n) g[k][j] = grad_at(t, i + j), p[k][j] = t.p[i + j];
+    }
+    mc[k] = ld_global<uint32_t>((const uint8_t*)a.m + (blk0 + k) * BLOCK + 4 * lane);
+    vc[k] = ld_global<uint32_t>((const uint8_t*)a.v + (blk0 + k) * BLOCK + 4 * lane);
+    me[k] = a.me[blk0 + k];
+    ve[k] = a.ve[blk0 + k];
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const long i = i0 + k * BLOCK + 4 * lane;
+    if (i0 + k * BLOCK >= t.n) return;
+    // a block of NaN stays one
+    const float b1 = me[k] == 255 ? __builtin_nanf("") : a.b1, b2 = ve[k] == 255 ? __builtin_nanf("") : a.b2;
+    const uint32_t key = mix(c.key + (uint32_t)(blk0 + k) * 0x9E3779B1u) + lane * (4 * 0x9E3779B1u);
     float m[4], v[4], mmax = 0.f, vmax = 0.f;
     bool mbad = false, vbad = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const long i = i0 + 4 * lane + j;
-      const uint32_t cm = mc >> 8 * j & 255, cv = vc >> 8 * j & 255;
-      m[j] = decoded<First>(cm & 127, me);
+      const uint32_t cm = mc[k] >> 8 * j & 255;
+      m[j] = decoded<First>(cm & 127, me[k]);
       m[j] = cm & 128 ? -m[j] : m[j];
-      v[j] = decoded<Second>(cv, ve);
-      if (i < t.n) {
-        moments(a, grad_at(t, i) * c.coef, m[j], v[j]);
-        t.p[i] = updated(a, c, t, t.p[i], m[j], v[j]);
-      } else {
-        m[j] = v[j] = 0.f;
-      }
+      v[j] = decoded<Second>(vc[k] >> 8 * j & 255, ve[k]);
+      moments(a, b1, b2, g[k][j] * c.coef, m[j], v[j]);
+      p[k][j] = u.of(p[k][j], m[j], v[j]);
+      if (i + j >= t.n) m[j] = v[j] = 0.f;   // behind the tensor's end
       mmax = fmaxf(mmax, fabsf(m[j]));
       vmax = fmaxf(vmax, v[j]);
       mbad |= too_large(m[j]);
@@ -221,35 +308,53 @@ __global__ __launch_bounds__(256) void k_adamw8(AdamArgs a) {
     uint32_t mo = 0, vo = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t r = mix(key + (4 * lane + j) * 0x9E3779B1u);
-      uint32_t cm = me1 == 255 ? 0 : encoded<First>(fabsf(m[j]), me1, (r & 0xffff) << 4 | 8);
-      cm |= m[j] < 0.f && cm ? 128 : 0;
-      uint32_t cv = ve1 == 255 ? 0 : encoded<Second>(v[j], ve1, r >> 16 << 4 | 8);
-      if (v[j] > 0.f && cv == 0) cv = 1;
+      const uint32_t r = mix(key + j * 0x9E3779B1u);
+      uint32_t cm = encoded<First>(fabsf(m[j]), me1, (r & 0xffff) << 4 | 8);
+      cm |= cm ? __float_as_uint(m[j]) >> 24 & 128 : 0;
+      const uint32_t cv = max(encoded<Second>(v[j], ve1, r >> 16 << 4 | 8), v[j] > 0.f ? 1u : 0u);
       mo |= cm << 8 * j;
       vo |= cv << 8 * j;
     }
-    *(uint32_t*)((uint8_t*)a.m + at) = mo;
-    *(uint32_t*)((uint8_t*)a.v + at) = vo;
+    *(uint32_t*)((uint8_t*)a.m + (blk0 + k) * BLOCK + 4 * lane) = me1 == 255 ? 0 : mo;
+    *(uint32_t*)((uint8_t*)a.v + (blk0 + k) * BLOCK + 4 * lane) = ve1 == 255 ? 0 : vo;
     if (lane == 0) {
-      a.me[blk] = me1;
-      a.ve[blk] = ve1;
+      a.me[blk0 + k] = me1;
+      a.ve[blk0 + k] = ve1;
+    }
+    if (i + 3 < t.n) {
+      store4(t.p + i, p[k]);
+    } else {
+      for (int j = 0; j < 3; ++j)
+        if (i + j < t.n) t.p[i + j] = p[k][j];
     }
   }
 }
+__global__ __launch_bounds__(256) void k_adamw8(AdamArgs a) {
+  const Control c = *a.c;
+  if (c.skip) return;
+  const PlanTensor t = a.tensors[a.chunk_tensor[blockIdx.x]];
+  const long i0 = (blockIdx.x - t.chunk0) * CHUNK + (threadIdx.x >> 6) * (CHUNK / 4);
+  if (i0 >= t.n) return;
+  if (t.g_bf16) step8<true>(a, c, t, i0);
+  else step8<false>(a, c, t, i0);
+}
 
+// Sixteen codes per lane.
 template <typename F> __global__ __launch_bounds__(256) void k_adamw_values(const uint8_t* codes, const uint8_t* exps, long n_blocks, bf16* out) {
-  const int lane = threadIdx.x & 63;
-  for (long b = blockIdx.x * 4L + (threadIdx.x >> 6); b < n_blocks; b += gridDim.x * 4L) {
-    const uint32_t c = *(const uint32_t*)(codes + b * BLOCK + 4 * lane);
-    const int e = exps[b];
+  constexpr bool SIGNED = F::BIAS == First::BIAS;
+  const long n = n_blocks * (BLOCK / 16);
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) {
+    const u32x4 c = ld_global<u32x4>(codes + 16 * i);
+    const int e = exps[i / (BLOCK / 16)];
+    float v[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t q = c >> 8 * j & 255;
-      const bool neg = F::GRID == First::GRID && q & 128;
-      const float x = decoded<F>(F::GRID == First::GRID ? q & 127 : q, e);
-      out[b * BLOCK + 4 * lane + j] = from_f<bf16>(neg ? -x : x);
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t q = c[j / 4] >> 8 * (j % 4) & 255;
+      v[j] = decoded<F>(SIGNED ? q & 127 : q, e);
+      if (SIGNED && q & 128) v[j] = -v[j];
+      if (e == 255) v[j] = __builtin_nanf("");
     }
+    store_vec<bf16, 16>(out + 16 * i, v);
   }
 }
 
@@ -330,7 +435,7 @@ int dm_adamw_step(const dm_adamw_args* a, void* stream) {
   const Workspace w = carve(a->workspace);
   const int parts = norm ? run_sumsq(a, w.part, s) : 0;
   hipLaunchKernelGGL(k_adamw_begin, dim3(1), dim3(256), 0, s,
-                     BeginArgs{w.c, w.part, parts, a->beta1, a->beta2, a->max_norm, a->skip_nonfinite, a->seed, a->lr, a->steps,
+                     BeginArgs{w.c, w.part, parts, std::log2(a->beta1), std::log2(a->beta2), a->max_norm, a->skip_nonfinite, a->seed, a->lr, a->steps,
                                a->norm, a->skipped});
   const AdamArgs k{(const PlanTensor*)a->plan, chunk_map(a), a->exp_avg, a->exp_avg_sq, a->exp_avg_exponent,
                    a->exp_avg_sq_exponent, (float)a->beta1, (float)(1. - a->beta1), (float)a->beta2, (float)(1. - a->beta2),
@@ -359,7 +464,7 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
   DM_REQUIRE(n_blocks >= 0 && n_blocks < (1L << 40), DM_ERR_INVALID, "n_blocks=%lld", (long long)n_blocks);
   if (n_blocks == 0) return DM_OK;
   DM_REQUIRE(codes && exponents && out && aligned16(codes) && aligned16(out), DM_ERR_INVALID, "null or unaligned operand");
-  const dim3 grid((unsigned)std::min<long>((n_blocks + 3) / 4, 1 << 16));
+  const dim3 grid((unsigned)std::min<long>((n_blocks + 15) / 16, 1 << 16));
   if (second) hipLaunchKernelGGL(k_adamw_values<Second>, grid, dim3(256), 0, S(stream), codes, exponents, (long)n_blocks, (bf16*)out);
   else hipLaunchKernelGGL(k_adamw_values<First>, grid, dim3(256), 0, S(stream), codes, exponents, (long)n_blocks, (bf16*)out);
   DM_HIP(hipGetLastError());
