@@ -6,7 +6,6 @@ Tensors cross the boundary as raw device pointers; the stream is torch's
 current HIP stream.
 """
 
-import contextlib
 import ctypes
 import os
 from ctypes import byref
@@ -312,11 +311,15 @@ def stream_ptr():
     return torch.cuda.current_stream().cuda_stream
 
 
-def on_device(device):
-    """A context in which ``device`` is the current one (stream_ptr() then gives its current stream)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def call_on(device, fn, args):
+    """fn(args, stream) of the library with ``device`` current, on its current stream (by the raw handles: the stream
+    and device objects of torch.cuda cost more than the rest of a small call)."""
+    i = device.index
+    if i == torch._C._cuda_getDevice():
+        check(fn(args, torch._C._cuda_getCurrentRawStream(i)))
+        return
+    with torch.cuda.device(i):
+        check(fn(args, torch._C._cuda_getCurrentRawStream(i)))
 
 
 def dtype_code(dt):

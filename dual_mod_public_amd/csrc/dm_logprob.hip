@@ -455,7 +455,7 @@ template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT
       if (a.logp) a.logp[r] = t < 0 ? 0.f : t < a.cols ? s.logp(xt) : NAN_;
       if (a.lse) a.lse[r] = s.lse;
       if (a.entropy) a.entropy[r] = s.entropy;
-      if (a.stats) a.stats[2 * r] = s.M, a.stats[2 * r + 1] = s.log_z;
+      if (a.stats) a.stats[3 * r] = s.M, a.stats[3 * r + 1] = s.log_z, a.stats[3 * r + 2] = s.entropy;
     }
     if (a.top) {
       const int c = sh.count;
@@ -486,10 +486,10 @@ template <typename T, int NT, int NV> __global__ __launch_bounds__(256) void k_l
     const long r = it / parts;
     const int q0 = (int)(it % parts) * NT * NV + threadIdx.x % NT;
     RowStats s;
-    s.M = a.stats[2 * r];
-    s.log_z = a.stats[2 * r + 1];
+    s.M = a.stats[3 * r];
+    s.log_z = a.stats[3 * r + 1];
+    s.entropy = a.stats[3 * r + 2];
     s.lse = s.M + s.log_z;
-    s.entropy = a.g_entropy ? a.entropy[r] : 0.f;
     const long t = a.target ? a.target[r] : -1;
     const RowGrad w = row_grad(a, r, t, s);
     const int target = t < a.cols ? (int)t : -1;
@@ -591,7 +591,7 @@ int check_logprob(const dm_logprob_args* a, bool bwd) {
              (long long)a->ld_d);
   DM_REQUIRE(a->g_logp || a->g_entropy, DM_ERR_INVALID, "a gradient without coefficients");
   DM_REQUIRE(!a->g_logp || a->target, DM_ERR_INVALID, "g_logp without targets");
-  DM_REQUIRE(!bwd || (a->stats && (a->entropy || !a->g_entropy)), DM_ERR_INVALID, "the forward's stats (and entropy) are needed");
+  DM_REQUIRE(!bwd || a->stats, DM_ERR_INVALID, "the forward's stats are needed");
   const uintptr_t x = reinterpret_cast<uintptr_t>(a->logits), d = reinterpret_cast<uintptr_t>(a->dlogits);
   const size_t xe = ((size_t)(a->rows - 1) * a->ld + a->cols) * e, de = ((size_t)(a->rows - 1) * a->ld_d + a->cols) * e;
   DM_REQUIRE((x == d && a->ld == a->ld_d) || x + xe <= d || d + de <= x, DM_ERR_INVALID, "dlogits overlaps the logits in part");

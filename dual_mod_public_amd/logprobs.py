@@ -25,7 +25,7 @@ class RowLogprobs(NamedTuple):
     logp: Optional[torch.Tensor]      # [...] fp32; None without targets
     entropy: torch.Tensor             # [...] fp32
     lse: torch.Tensor                 # [...] fp32
-    stats: torch.Tensor               # [..., 2] fp32: the maximum and lse less it, for row_logprobs_bwd
+    stats: torch.Tensor               # [..., 3] fp32: maximum, lse less it, entropy, for row_logprobs_bwd
     top_logp: Optional[torch.Tensor]  # [..., top] fp32, descending; None without top
     top_ids: Optional[torch.Tensor]   # [..., top] int64, the lower id first among equals
 
@@ -63,18 +63,14 @@ def _per_row(t, logits, what, dtype):
     return t.data_ptr()
 
 
-def _args(logits, targets):
+def _logits(logits):
     if not logits.is_cuda or logits.dim() < 1:
         raise ValueError(f"logits: shape {tuple(logits.shape)} on {logits.device}; rows [..., V] on a GPU are needed")
-    a = L.dm_logprob_args()
-    a.dtype = L.dtype_code(logits.dtype)
-    a.rows, a.ld = _rows(logits, "logits")
-    a.cols = logits.shape[-1]
-    a.logits, a.target = logits.data_ptr(), _per_row(targets, logits, "targets", torch.int64)
-    return a
+    return _rows(logits, "logits")
 
 
-def _grad_args(a, logits, targets, g_logp, g_entropy, dlogits):
+def _gradient(logits, targets, g_logp, g_entropy, dlogits):
+    """(dlogits, the arguments that say where the gradient comes from and goes to)."""
     if g_logp is None and g_entropy is None:
         raise ValueError("a gradient needs g_logp or g_entropy")
     if g_logp is not None and targets is None:
@@ -84,63 +80,55 @@ def _grad_args(a, logits, targets, g_logp, g_entropy, dlogits):
     elif dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
         raise ValueError(f"dlogits: {dlogits.dtype} {tuple(dlogits.shape)} on {dlogits.device} for logits {logits.dtype} "
                          f"{tuple(logits.shape)} on {logits.device}")
-    a.g_logp = _per_row(g_logp, logits, "g_logp", torch.float32)
-    a.g_entropy = _per_row(g_entropy, logits, "g_entropy", torch.float32)
-    a.dlogits, a.ld_d = dlogits.data_ptr(), _rows(dlogits, "dlogits")[1]
-    return dlogits
+    return dlogits, (_per_row(g_logp, logits, "g_logp", torch.float32), _per_row(g_entropy, logits, "g_entropy", torch.float32),
+                     dlogits.data_ptr(), _rows(dlogits, "dlogits")[1])
 
 
-def _call(fn, a, device):
-    with L.on_device(device):
-        L.check(fn(L.byref(a), L.stream_ptr()))
-
-
-def _forward(a, logits, targets, top):
-    kw = dict(device=logits.device, dtype=torch.float32)
-    lead = logits.shape[:-1]
-    if not 0 <= top <= min(L.DM_TOP_MAX, a.cols):
-        raise ValueError(f"top={top} of {a.cols} columns (at most {L.DM_TOP_MAX})")
-    logp, entropy, lse = (torch.empty(lead, **kw) for _ in range(3))
-    stats = torch.empty(lead + (2,), **kw)
-    a.entropy, a.lse, a.stats = entropy.data_ptr(), lse.data_ptr(), stats.data_ptr()
-    if targets is None:
-        logp = None
-    else:
-        a.logp = logp.data_ptr()
+def _forward(logits, targets, top, rows, ld, gradient=(None, None, None, 0)):
+    V, dev, lead = logits.shape[-1], logits.device, logits.shape[:-1]
+    if not 0 <= top <= min(L.DM_TOP_MAX, V):
+        raise ValueError(f"top={top} of {V} columns (at most {L.DM_TOP_MAX})")
+    t = _per_row(targets, logits, "targets", torch.int64)
+    logp = None if targets is None else torch.empty(lead, device=dev, dtype=torch.float32)
+    entropy = torch.empty(lead, device=dev, dtype=torch.float32)
+    lse = torch.empty(lead, device=dev, dtype=torch.float32)
+    stats = torch.empty((*lead, 3), device=dev, dtype=torch.float32)
     top_logp = top_ids = None
     if top:
-        a.top = top
-        top_logp = torch.empty(lead + (top,), **kw)
-        top_ids = torch.empty(lead + (top,), device=logits.device, dtype=torch.int64)
-        a.top_logp, a.top_ids = top_logp.data_ptr(), top_ids.data_ptr()
-    _call(L.lib().dm_logprob_rows, a, logits.device)
+        top_logp = torch.empty((*lead, top), device=dev, dtype=torch.float32)
+        top_ids = torch.empty((*lead, top), device=dev, dtype=torch.int64)
+    a = L.dm_logprob_args(L.dtype_code(logits.dtype), rows, V, top, logits.data_ptr(), ld, t, L.ptr(logp), lse.data_ptr(),
+                          entropy.data_ptr(), stats.data_ptr(), L.ptr(top_logp), L.ptr(top_ids), *gradient)
+    L.call_on(dev, L.lib().dm_logprob_rows, L.byref(a))
     return RowLogprobs(logp, entropy, lse, stats, top_logp, top_ids)
 
 
 def row_logprobs(logits, targets=None, top=0):
     """The values of logits [..., V]: logp of ``targets`` (int64 [...], optional), entropy, lse and the ``top`` most
     likely tokens of each row (at most 32). No gradient."""
-    return _forward(_args(logits, targets), logits, targets, top)
+    return _forward(logits, targets, top, *_logits(logits))
 
 
 def row_logprobs_grad(logits, targets, g_logp, g_entropy=None, top=0, dlogits=None):
     """row_logprobs, and the gradient of sum(g_logp logp + g_entropy entropy) to the logits (fp32 coefficients [...],
     either may be None) in the same pass: (RowLogprobs, dlogits). dlogits: a tensor for the gradient, the logits
     themselves too (in place); by default a new one."""
-    a = _args(logits, targets)
-    dlogits = _grad_args(a, logits, targets, g_logp, g_entropy, dlogits)
-    return _forward(a, logits, targets, top), dlogits
+    rows, ld = _logits(logits)
+    dlogits, gradient = _gradient(logits, targets, g_logp, g_entropy, dlogits)
+    return _forward(logits, targets, top, rows, ld, gradient), dlogits
 
 
-def row_logprobs_bwd(logits, targets, r, g_logp, g_entropy=None, dlogits=None):
-    """The gradient of row_logprobs_grad after row_logprobs, from its result ``r`` (stats and, with g_entropy, entropy)."""
-    a = _args(logits, targets)
-    dlogits = _grad_args(a, logits, targets, g_logp, g_entropy, dlogits)
-    a.entropy = _per_row(r.entropy, logits, "entropy", torch.float32)
-    if r.stats.shape != logits.shape[:-1] + (2,) or r.stats.device != logits.device or not r.stats.is_contiguous():
-        raise ValueError(f"stats: {tuple(r.stats.shape)} on {r.stats.device} for logits {tuple(logits.shape)} on {logits.device}")
-    a.stats = r.stats.data_ptr()
-    _call(L.lib().dm_logprob_rows_bwd, a, logits.device)
+def row_logprobs_bwd(logits, targets, stats, g_logp, g_entropy=None, dlogits=None):
+    """The gradient of row_logprobs_grad after row_logprobs, from the ``stats`` of its result."""
+    rows, ld = _logits(logits)
+    dlogits, gradient = _gradient(logits, targets, g_logp, g_entropy, dlogits)
+    if (stats.shape != logits.shape[:-1] + (3,) or stats.dtype != torch.float32 or stats.device != logits.device
+            or not stats.is_contiguous()):
+        raise ValueError(f"stats: {stats.dtype} {tuple(stats.shape)} on {stats.device} for logits {tuple(logits.shape)} on {logits.device}")
+    a = L.dm_logprob_args(L.dtype_code(logits.dtype), rows, logits.shape[-1], 0, logits.data_ptr(), ld,
+                          _per_row(targets, logits, "targets", torch.int64), None, None, None, stats.data_ptr(), None, None,
+                          *gradient)
+    L.call_on(logits.device, L.lib().dm_logprob_rows_bwd, L.byref(a))
     return dlogits
 
 
@@ -148,19 +136,20 @@ class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets):
         r = row_logprobs(logits, targets)
-        ctx.save_for_backward(logits, targets, r.stats, r.entropy)
+        ctx.save_for_backward(logits, targets)
+        ctx.stats = r.stats
         ctx.set_materialize_grads(False)
         return r.logp, r.entropy
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy):
+        if torch.is_grad_enabled():
+            raise NotImplementedError("token_logprobs is differentiable once (create_graph)")
         if g_logp is None and g_entropy is None:
             return None, None
-        logits, targets, stats, entropy = ctx.saved_tensors
+        logits, targets = ctx.saved_tensors
         g_logp, g_entropy = (None if g is None else g.contiguous() for g in (g_logp, g_entropy))
-        r = RowLogprobs(None, entropy, None, stats, None, None)
-        return row_logprobs_bwd(logits, targets, r, g_logp, g_entropy), None
+        return row_logprobs_bwd(logits, targets, ctx.stats, g_logp, g_entropy), None
 
 
 def token_logprobs(logits, targets):

@@ -18,6 +18,7 @@ bit for bit. A NaN or infinity in a state makes its block NaN; ``skip_nonfinite`
 """
 
 import ctypes
+from itertools import chain
 
 import torch
 
@@ -80,7 +81,7 @@ class AdamW:
         self.norm = torch.zeros((), dtype=torch.float32, **kw)       # the last step's gradient norm (before clipping)
         self.skipped = torch.zeros((), dtype=torch.int32, **kw)      # steps left out by skip_nonfinite
         self._ws = torch.empty(L.DM_ADAMW_WORKSPACE, dtype=torch.uint8, **kw)
-        self._key = self._plan = None
+        self._key = self._plan = self._a = None
         self._in_graphs = []    # plans that captured steps read
         torch.cuda.current_stream(self.device).synchronize()   # the buffers are ready on every stream
 
@@ -92,27 +93,18 @@ class AdamW:
     def _args(self):
         """dm_adamw_args of a step now; the plan is written again where a tensor has moved."""
         grads = self.grads if self.grads is not None else [p.grad for p in self.params]
-        key = [(p.data_ptr(), 0, None) if g is None else (p.data_ptr(), g.data_ptr(), g.dtype)
-               for p, g in zip(self.params, grads)]
+        key = [None if t is None else t.data_ptr() for t in chain(self.params, grads)]
         if key != self._key:
             self._write_plan(grads)
             self._key = key
         if torch.cuda.is_current_stream_capturing() and not any(self._plan is t for t in self._in_graphs):
             self._in_graphs.append(self._plan)
-        a = L.dm_adamw_args()
-        a.plan, a.n_chunks, a.n_tensors, a.state_bits = self._plan.data_ptr(), self._n_chunks, self._n_tensors, self.state_bits
-        a.exp_avg, a.exp_avg_sq = self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr()
-        a.exp_avg_exponent, a.exp_avg_sq_exponent = L.ptr(self.exp_avg_exponent), L.ptr(self.exp_avg_sq_exponent)
-        a.beta1, a.beta2, a.eps = self.betas[0], self.betas[1], self.eps
-        a.max_norm, a.skip_nonfinite, a.seed = self.max_norm or 0.0, int(self.skip_nonfinite), self.seed
-        a.lr, a.steps = self.lr.data_ptr(), self.steps.data_ptr()
-        a.norm, a.skipped = self.norm.data_ptr(), self.skipped.data_ptr()
-        a.workspace, a.workspace_bytes = self._ws.data_ptr(), self._ws.numel()
-        return a
+        return self._a
 
     def _write_plan(self, grads):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a tensor has moved since the last step; take one step before capturing")
+        self._key = None
         rows = []
         for i, (p, g) in enumerate(zip(self.params, grads)):
             if g is None or p.numel() == 0:
@@ -131,24 +123,34 @@ class AdamW:
         host, n = torch.empty(nb, dtype=torch.uint8), ctypes.c_int64()
         L.check(L.lib().dm_adamw_plan(arr, len(rows), host.data_ptr(), nb, ctypes.byref(n)))
         torch.cuda.synchronize(self.device)   # no step still reads the plan that this one replaces
-        self._plan, self._n_chunks, self._n_tensors = host.to(self.device), n.value, len(rows)
+        self._plan = host.to(self.device)
         torch.cuda.current_stream(self.device).synchronize()
+        a = self._a = L.dm_adamw_args()
+        a.plan, a.n_chunks, a.n_tensors, a.state_bits = self._plan.data_ptr(), n.value, len(rows), self.state_bits
+        a.exp_avg, a.exp_avg_sq = self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr()
+        a.exp_avg_exponent, a.exp_avg_sq_exponent = L.ptr(self.exp_avg_exponent), L.ptr(self.exp_avg_sq_exponent)
+        a.beta1, a.beta2, a.eps = self.betas[0], self.betas[1], self.eps
+        a.max_norm, a.skip_nonfinite, a.seed = self.max_norm or 0.0, int(self.skip_nonfinite), self.seed
+        a.lr, a.steps = self.lr.data_ptr(), self.steps.data_ptr()
+        a.norm, a.skipped = self.norm.data_ptr(), self.skipped.data_ptr()
+        a.workspace, a.workspace_bytes = self._ws.data_ptr(), self._ws.numel()
 
-    @torch.no_grad()
+    def _call(self, fn):
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self._call(fn)
+        L.call_on(self.device, fn, L.byref(self._args()))
+
     def step(self):
         """One step. Returns the gradients' global norm before clipping (a device scalar, overwritten by the next
         step) where it is computed: with max_norm or skip_nonfinite; else None."""
-        with L.on_device(self.device):
-            a = self._args()
-            L.check(L.lib().dm_adamw_step(L.byref(a), L.stream_ptr()))
+        self._call(L.lib().dm_adamw_step)
         self.mark_updated()
-        return self.norm if a.max_norm > 0 or a.skip_nonfinite else None
+        return self.norm if self.max_norm is not None or self.skip_nonfinite else None
 
     def grad_norm(self):
         """The gradients' global norm alone (a device scalar, overwritten by the next call or step)."""
-        with L.on_device(self.device):
-            a = self._args()
-            L.check(L.lib().dm_grad_norm(L.byref(a), L.stream_ptr()))
+        self._call(L.lib().dm_grad_norm)
         return self.norm
 
     def mark_updated(self):
@@ -170,7 +172,7 @@ class AdamW:
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
         out = [torch.empty(self.exp_avg.numel(), device=self.device, dtype=torch.bfloat16) for _ in range(2)]
-        with L.on_device(self.device):
+        with torch.cuda.device(self.device):
             for second, (c, e) in enumerate(((self.exp_avg, self.exp_avg_exponent), (self.exp_avg_sq, self.exp_avg_sq_exponent))):
                 L.check(L.lib().dm_adamw_values(c.data_ptr(), e.data_ptr(), self.n_blocks, second, out[second].data_ptr(),
                                                 L.stream_ptr()))

@@ -531,8 +531,8 @@ int dm_ce_mean(const float* loss, int32_t M, const float* nvalid, float* out, vo
  *   sum_r (g_logp[r] logp[r] + g_entropy[r] entropy[r]),
  *     dlogits[v] = g_logp (1[v = target] - p) - g_entropy p (logp(v) + entropy),
  *   for coefficients that are known beforehand.
- * dm_logprob_rows_bwd: the same gradient after the forward, whose stats and (with g_entropy) entropy it reads;
- *   the fields logp, lse, top_logp and top_ids are not used.
+ * dm_logprob_rows_bwd: the same gradient after the forward, whose stats it reads; the fields logp, lse, entropy,
+ *   top_logp and top_ids are not used.
  * A row of -inf gives every token -inf: lse -inf, logp -inf, entropy 0, a zero gradient. A row with a NaN: lse,
  * log probabilities and entropy NaN. With +inf and no NaN: lse +inf, logp -inf for finite logits and NaN for the
  * infinite ones, entropy NaN. The gradient of those two is NaN. A row whose coefficients are both 0 (g_logp counts
@@ -547,8 +547,8 @@ typedef struct dm_logprob_args {
   const void* logits; int64_t ld;
   const int64_t* target;             /* [rows]; NULL: no logp and no g_logp */
   float* logp; float* lse; float* entropy;   /* [rows]; outputs of dm_logprob_rows (each may be NULL) */
-  float* stats;                      /* [rows, 2] output (may be NULL) and input of dm_logprob_rows_bwd: the row's
-                                        maximum and lse less it, both infinite or NaN where lse is */
+  float* stats;                      /* [rows, 3] output (may be NULL) and input of dm_logprob_rows_bwd: the row's
+                                        maximum and lse less it (both infinite or NaN where lse is), the entropy */
   float* top_logp; int64_t* top_ids; /* [rows, top] */
   const float* g_logp; const float* g_entropy;   /* [rows]; with dlogits, at least one */
   void* dlogits; int64_t ld_d;       /* NULL: no gradient */

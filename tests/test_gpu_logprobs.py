@@ -137,17 +137,17 @@ def test_values_and_gradient(M, V, dtype):
         r2, dx = lp.row_logprobs_grad(x, t, w, gh, top=top)
         assert all(torch.equal(a, b) for a, b in zip(r, r2) if a is not None)
         check_grad(x, t, w, gh, dx, f"case {case} fused")
-        dx2 = lp.row_logprobs_bwd(x, t, r, w, gh)
+        dx2 = lp.row_logprobs_bwd(x, t, r.stats, w, gh)
         check_grad(x, t, w, gh, dx2, f"case {case} backward")
         assert torch.equal(buf, before)
         # one coefficient alone; the gradient in place, its surroundings as they were
-        check_grad(x, t, w, None, lp.row_logprobs_bwd(x, t, r, w), f"case {case} logp only")
+        check_grad(x, t, w, None, lp.row_logprobs_bwd(x, t, r.stats, w), f"case {case} logp only")
         check_grad(x, t, None, gh, lp.row_logprobs_grad(x, t, None, gh)[1], f"case {case} entropy only")
         clean = x.clone()
         _, dx3 = lp.row_logprobs_grad(x, t, w, gh, dlogits=x)
         assert dx3.data_ptr() == x.data_ptr() and torch.equal(x, dx)
         x.copy_(clean)
-        lp.row_logprobs_bwd(x, t, r, w, gh, dlogits=x)
+        lp.row_logprobs_bwd(x, t, r.stats, w, gh, dlogits=x)
         assert torch.equal(x, dx2)
         x.copy_(clean)
         assert torch.equal(buf, before)
@@ -168,7 +168,7 @@ def test_gradient_stride_of_its_own(dtype):
         assert torch.equal(buf, around)
         d.zero_()
         r = lp.row_logprobs(x, t)
-        lp.row_logprobs_bwd(x, t, r, w, dlogits=d)
+        lp.row_logprobs_bwd(x, t, r.stats, w, dlogits=d)
         check_grad(x, t, w, None, d)
         assert torch.equal(buf[:base], around[:base]) and torch.equal(buf[base + M * ld:], around[base + M * ld:])
 
@@ -219,7 +219,7 @@ def test_special_rows(V, dtype):
             s = slice(i, i + 1)
             check_values(x[s], t[s], top, lp.RowLogprobs(*[None if v is None else v[s] for v in r]), f"{name} top={top}")
             check_grad(x[s], t[s], w[s], gh[s], dx[s], f"{name} top={top}")
-    dx = lp.row_logprobs_bwd(x, t, r, w, gh)
+    dx = lp.row_logprobs_bwd(x, t, r.stats, w, gh)
     for i, (name, _, _) in enumerate(rows):
         check_grad(x[i:i + 1], t[i:i + 1], w[i:i + 1], gh[i:i + 1], dx[i:i + 1], name)
 
@@ -244,7 +244,7 @@ def test_nan_and_infinity(V, dtype):
     assert torch.isnan(r.lse[[1, 4, 6]]).all() and r.lse[3] == INF
     assert torch.isnan(r.entropy[[1, 3, 4, 6]]).all() and torch.isfinite(r.entropy[5])
     assert torch.isnan(dx[[1, 3, 4, 5, 6]]).all()
-    assert torch.isnan(lp.row_logprobs_bwd(x, t, r, ones, 0.5 * ones)[[1, 3, 4, 5, 6]]).all()
+    assert torch.isnan(lp.row_logprobs_bwd(x, t, r.stats, ones, 0.5 * ones)[[1, 3, 4, 5, 6]]).all()
     # NaN before every number, then infinities, the lower id first; finite tokens beside an infinite one
     assert r.top_ids[1, 0] == V // 2 and r.top_ids[3, :2].tolist() == [4, 20] and r.top_ids[4, :2].tolist() == [9, 4]
     assert torch.isnan(r.top_logp[1]).all() and torch.isnan(r.top_logp[3, :2]).all() and (r.top_logp[3, 2:] == -INF).all()
@@ -253,7 +253,7 @@ def test_nan_and_infinity(V, dtype):
     # rows whose coefficients are 0 are zeros, whatever they hold
     zero = lp.row_logprobs_grad(x, t, 0 * ones)[1]
     assert (zero == 0).all()
-    assert (lp.row_logprobs_bwd(x, t, r, 0 * ones, 0 * ones) == 0).all()
+    assert (lp.row_logprobs_bwd(x, t, r.stats, 0 * ones, 0 * ones) == 0).all()
     assert (lp.row_logprobs_grad(x, t, ones)[1][6] == 0).all()          # ignored
 
 
@@ -298,7 +298,10 @@ def test_autograd(dtype):
     # four stored gradients, each rounded once, and their sum's roundings
     tol = (4 * torch.finfo(dtype).eps) * (p * 4 + (want + 4 * p)) + 1e-6
     assert ((d.double().cpu() - want).abs() <= tol).all()
-    # nothing written into what autograd keeps
+    # differentiable once; nothing written into what autograd keeps
+    logp, _ = lp.token_logprobs(wide[..., :100], t)
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(logp.sum(), wide, create_graph=True)
     logp, _ = lp.token_logprobs(wide[..., :100].contiguous(), t)
     assert logp.grad_fn is not None and not lp.row_logprobs(wide.detach()[..., :100], t).logp.requires_grad
 
@@ -314,7 +317,7 @@ def test_rows_past_32_bits():
     check_values(x[-1:], t[-1:], 1, lp.RowLogprobs(*[v[-1:] for v in r]))
     check_grad(x[-1:], t[-1:], torch.ones(1, device=DEV), None, dx[-1:])
     check_values(x[-2:-1], t[-2:-1], 1, lp.RowLogprobs(*[v[-2:-1] for v in r]))
-    want = lp.row_logprobs_bwd(x, t, r, torch.ones(M, device=DEV), dlogits=x)
+    want = lp.row_logprobs_bwd(x, t, r.stats, torch.ones(M, device=DEV), dlogits=x)
     check_grad(torch.zeros(1, V), t[:1], torch.ones(1, device=DEV), None, want[:1])
     assert torch.equal(want[-1], dx[-1]) or (want[-1].float() - dx[-1].float()).abs().max() <= 2.0 ** -8 * dx[-1].float().abs().max()
 
@@ -327,7 +330,7 @@ def test_many_short_rows():
     r, dx = lp.row_logprobs_grad(x, t, w, top=2)
     check_values(x, t, 2, r)
     check_grad(x, t, w, None, dx)
-    check_grad(x, t, w, None, lp.row_logprobs_bwd(x, t, r, w))
+    check_grad(x, t, w, None, lp.row_logprobs_bwd(x, t, r.stats, w))
 
 
 def test_rows_do_not_depend_on_the_batch():
@@ -360,12 +363,12 @@ def test_streams_and_graph(M, V):
     torch.cuda.synchronize()
     with torch.cuda.graph(graph, stream=s):
         r, dx = lp.row_logprobs_grad(x, t, w, gh, top=6)
-        dx2 = lp.row_logprobs_bwd(x, t, r, w, gh)
+        dx2 = lp.row_logprobs_bwd(x, t, r.stats, w, gh)
     for k in range(4):
         x.copy_(torch.randn(M, V, generator=g, device=DEV).to(x.dtype))
         graph.replay()
         want = lp.row_logprobs_grad(x, t, w, gh, top=6)
-        want2 = lp.row_logprobs_bwd(x, t, want[0], w, gh)
+        want2 = lp.row_logprobs_bwd(x, t, want[0].stats, w, gh)
         torch.cuda.synchronize()
         assert torch.equal(dx, want[1]) and torch.equal(dx2, want2)
         assert all(torch.equal(a, b) for a, b in zip(r, want[0]))
@@ -392,7 +395,7 @@ def test_refusals():
            lambda: lp.row_logprobs(x.half(), t), lambda: lp.row_logprobs_grad(x, t, None), lambda: lp.row_logprobs_grad(x, None, w),
            lambda: lp.row_logprobs_grad(x, t, w.double()), lambda: lp.row_logprobs_grad(x, t, w, dlogits=x.bfloat16()),
            lambda: lp.row_logprobs_grad(x, t, w, dlogits=torch.empty(4, 101, device=DEV)),
-           lambda: lp.row_logprobs_bwd(x, t, lp.row_logprobs(x[:3], t[:3]), w),
+           lambda: lp.row_logprobs_bwd(x, t, lp.row_logprobs(x[:3], t[:3]).stats, w), lambda: lp.row_logprobs_bwd(x, t, w, w),
            lambda: lp.row_logprobs(torch.zeros(2, 3, 8, device=DEV).transpose(0, 1), torch.zeros(3, 2, dtype=torch.int64, device=DEV))]
     for i, f in enumerate(bad):
         with pytest.raises((ValueError, NotImplementedError)):
