@@ -20,11 +20,19 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from .decode import StaticTape
+from .logprobs import row_logprobs
 
 
 class GraphDecoder:
-    def __init__(self, model, B, P_max, dtype=None):
+    """top: with a number (0..32) every step also gives the picked token's log probability, the distribution's
+    entropy (``logp``, ``entropy`` [B, 1]) and its ``top`` most likely tokens (``top_logp``, ``top_ids`` [B, 1, top]);
+    ``generate`` keeps the former in ``gen_logp`` [B, k]. No reference counterpart."""
+
+    def __init__(self, model, B, P_max, dtype=None, top=None):
         self.m = model
+        if top is not None and not 0 <= top <= L.DM_TOP_MAX:
+            raise ValueError(f"top={top} (0..{L.DM_TOP_MAX})")
+        self.top = top
         cfg = model.cfg
         self.dev = next(model.parameters()).device
         if P_max > cfg.max_seq_len:
@@ -39,6 +47,11 @@ class GraphDecoder:
         self.pos = torch.zeros(1, dtype=torch.int32, device=self.dev)          # absolute position
         self.logits = torch.zeros(B, 1, self.vocab, device=self.dev)          # fp32 out
         self.next = torch.zeros(B, 1, dtype=torch.long, device=self.dev)       # argmax out
+        self.gen_logp = None
+        if top is not None:
+            self.logp, self.entropy = (torch.zeros(B, 1, device=self.dev) for _ in range(2))
+            self.top_logp = torch.zeros(B, 1, top, device=self.dev)
+            self.top_ids = torch.zeros(B, 1, top, dtype=torch.long, device=self.dev)
         self.cos = model.rope_cos.to(self.dev, torch.float32).contiguous()
         self.sin = model.rope_sin.to(self.dev, torch.float32).contiguous()
         # compute-dtype weight copies at fixed addresses (the autocast casts, done once per version)
@@ -87,6 +100,13 @@ class GraphDecoder:
         self.logits.copy_(lg)                                           # exact bf16 -> fp32 in one copy
         L.check(L.lib().dm_argmax_rows(L.dtype_code(self.dt), L.ptr(lg), B, self.vocab, self.vocab,
                                        L.ptr(self.next), L.stream_ptr()))
+        if self.top is not None:
+            r = row_logprobs(lg, self.next, top=self.top)
+            self.logp.copy_(r.logp)
+            self.entropy.copy_(r.entropy)
+            if self.top:
+                self.top_logp.copy_(r.top_logp)
+                self.top_ids.copy_(r.top_ids)
         self.pos += 1
 
     def _run_step(self):
@@ -148,10 +168,13 @@ class GraphDecoder:
             self.tok.copy_(prompt[:, p:p + 1])
             self.step()
         gen = torch.zeros(B, max_new, dtype=torch.long, device=self.dev)
+        logp = torch.zeros(B, max_new, device=self.dev) if self.top is not None else None
         done = torch.zeros(B, dtype=torch.bool)
         k = 0
         while k < max_new:
             gen[:, k].copy_(self.next[:, 0])
+            if logp is not None:
+                logp[:, k].copy_(self.logp[:, 0])
             k += 1
             if k % check_every == 0 or k == max_new:
                 g_cpu = gen[:, :k].cpu()
@@ -164,4 +187,6 @@ class GraphDecoder:
             if k < max_new:
                 self.tok.copy_(self.next)
                 self.step()
+        if logp is not None:
+            self.gen_logp = logp[:, :k].cpu()
         return gen[:, :k].cpu(), k

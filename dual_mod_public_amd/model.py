@@ -16,6 +16,7 @@ import torch.nn.functional as F
 from . import _lib as L
 from .attention import DualModAttention, RMSNorm
 from .config import DualModConfig
+from .logprobs import token_logprobs
 from .rope import build_rope_cache
 
 
@@ -115,6 +116,11 @@ class DualModLM(nn.Module):
         if targets is not None:
             loss = F.cross_entropy(logits.float().view(-1, logits.shape[-1]), targets.reshape(-1), ignore_index=-1)
         return logits, loss
+
+    def token_logprobs(self, idx, targets):
+        """(log probabilities of targets [B, T] after idx [B, T], entropies), fp32, differentiable in the parameters; a
+        target of -1 is ignored (log probability 0). No reference counterpart."""
+        return token_logprobs(self(idx)[0], targets)
 
     # ---- incremental decode (model.py:285-313) --------------------------------------
     def decode_init(self):

@@ -39,6 +39,8 @@ import torch
 
 from . import _lib as L
 from .engine import HipSweepCell, LayerGrads, _sched, check_supported, uniform_chunks
+from .logprobs import RowLogprobs, row_logprobs, row_logprobs_grad
+from .optim import AdamW
 
 
 def _rms(x, w, eps):
@@ -113,12 +115,22 @@ class HipTrunk:
     if all fit, else none; None: every layer; "auto": the device memory still free once everything
     else is allocated, less TAPE_RESERVE). ``refresh()`` re-reads the parameters (packs the
     attention and MLP weights, casts the embedding / head weight) and must follow every parameter
-    update; ``capture()`` records one step as a HIP graph."""
+    update; ``capture()`` records one step as a HIP graph.
+
+    objective "ce": the mean cross entropy over the targets >= 0. "weighted": the mean over them of
+    -weight logp(target) - entropy_coef entropy, with a weight per token given to each step (masked or
+    reweighted fine-tuning, policy gradients: the weights are the advantages); the step's token log
+    probabilities and entropies are then in ``logp`` and ``entropy`` [B, T]. No reference counterpart."""
 
     TAPE_RESERVE = 24e9   # bytes left free by tape_budget="auto" (the head's chunks, the graph pool)
 
-    def __init__(self, model, B, T, schedule=None, tape_budget=None, loss_chunk=4096, wavefront=False):
+    def __init__(self, model, B, T, schedule=None, tape_budget=None, loss_chunk=4096, wavefront=False,
+                 objective="ce", entropy_coef=0.0):
         cfg = model.cfg
+        if objective not in ("ce", "weighted"):
+            raise ValueError(f"objective={objective!r} (\"ce\" or \"weighted\")")
+        if objective == "ce" and entropy_coef:
+            raise ValueError("entropy_coef belongs to objective=\"weighted\"")
         check_supported(cfg)
         if cfg.gate_rank or cfg.ctx_rank:
             raise NotImplementedError("the trunk step takes dense attention parameters (gate_rank = ctx_rank = 0)")
@@ -210,6 +222,9 @@ class HipTrunk:
         self.tapes = [self.cells[l].new_tape(self.schedule) if l < n_tape else None for l in range(nl)]
         self.n_tape = n_tape
         self.loss = torch.zeros((), device=self.dev, dtype=torch.float32)
+        self.objective, self.entropy_coef = objective, float(entropy_coef)
+        if objective == "weighted":
+            self.weights, self.logp, self.entropy = (torch.ones(B, T, device=self.dev) for _ in range(3))
         self.cos = model.rope_cos[:T].to(self.dev, torch.float32).contiguous()
         self.sin = model.rope_sin[:T].to(self.dev, torch.float32).contiguous()
         self.w_emb = torch.zeros(V, d, **kw)   # the embedding / head weight in the compute dtype
@@ -314,12 +329,17 @@ class HipTrunk:
                                      L.stream_ptr()))
 
     # ---- the head, the loss and the embedding ---------------------------------------------------
+    def _chunks(self):
+        M = self.B * self.T
+        return [(r, min(r + self.loss_chunk, M)) for r in range(0, M, self.loss_chunk)]
+
     def _head(self):
         """norm_f, the tied head and the mean cross entropy (ignore_index -1, model.py:279-281), with
         its gradient: the loss's softmax gradient needs nothing but the logits, so the head's VJP runs
         with its forward, chunk by chunk of rows (the reference's loss_chunk, graphs.py:322-341). The sums
         over rows run in libdm_hip.so: torch's split a long column over blocks and clear their counters
-        with memsets, which a captured step would hold as nodes."""
+        with memsets, which a captured step would hold as nodes. The weighted objective's coefficients of a
+        token's log probability and entropy are known beforehand too."""
         m = self.m
         M, d = self.B * self.T, self.cfg.d_model
         x = self.xs[-1].view(M, d)
@@ -329,24 +349,41 @@ class HipTrunk:
         gnf = self.grad["norm_f.weight"]
         loss = torch.empty(M, device=self.dev, dtype=torch.float32)
         dxl = self.dxs[-1].view(M, d)
-        for r0 in range(0, M, self.loss_chunk):
-            r1 = min(r0 + self.loss_chunk, M)
+        weighted = self.objective == "weighted"
+        if weighted:
+            valid = tg >= 0
+            logp, entropy = self.logp.view(M), self.entropy.view(M)
+            g_logp = -self.weights.view(M) / nvalid
+            g_entropy = torch.where(valid, -self.entropy_coef / nvalid, 0.0) if self.entropy_coef else None
+        for r0, r1 in self._chunks():
             xc, t = x[r0:r1], tg[r0:r1]
             hf, r = _rms(xc, m.norm_f.weight, m.norm_f.eps)
-            dl = hf @ self.w_emb.t()
-            L.ce_rows(dl, t, nvalid, loss[r0:r1])   # dl: the logits, then their gradient
+            dl = hf @ self.w_emb.t()   # the logits, then their gradient
+            if weighted:
+                v, _ = row_logprobs_grad(dl, t, g_logp[r0:r1], None if g_entropy is None else g_entropy[r0:r1], dlogits=dl)
+                logp[r0:r1].copy_(v.logp)
+                entropy[r0:r1].copy_(v.entropy)
+            else:
+                L.ce_rows(dl, t, nvalid, loss[r0:r1])
             gw.add_(_mm32(dl.t(), hf))
             dhf = dl @ self.w_emb
             dxl[r0:r1].copy_(_rms_vjp(dhf, xc, r, m.norm_f.weight, gnf))
+        if weighted:
+            loss = torch.where(valid, -self.weights.view(M) * logp, 0.0)
+            if self.entropy_coef:
+                loss = loss - self.entropy_coef * torch.where(valid, entropy, 0.0)
         L.ce_mean(loss, nvalid, self.loss)
 
     def _embed_bwd(self):
         M, d = self.B * self.T, self.cfg.d_model
         L.embed_bwd(self.dxs[0].view(M, d), self.idx.view(M), self.grad["tok_emb.weight"])
 
+    def _embed(self):
+        torch.index_select(self.w_emb, 0, self.idx.view(-1), out=self.xs[0].view(-1, self.cfg.d_model))
+
     def _run(self):
         with torch.no_grad():
-            torch.index_select(self.w_emb, 0, self.idx.view(-1), out=self.xs[0].view(-1, self.cfg.d_model))
+            self._embed()
             if self.wavefront:
                 self._stack_fwd()
                 self.flat.zero_()
@@ -388,19 +425,59 @@ class HipTrunk:
         torch.cuda.synchronize(self.dev)
         return self
 
-    def train_step(self, idx, targets):
+    def train_step(self, idx, targets, weights=None):
         """Forward + backward of the batch (idx [B, T] token ids of the table; targets [B, T], of which
-        -1 is ignored and one >= vocab_size makes the loss NaN).
+        -1 is ignored and one >= vocab_size makes the loss NaN; weights [B, T] of the weighted objective,
+        by default 1).
         Returns the loss (a static device scalar, overwritten by the next step); the gradients are
         the views ``grad[name]`` of the flat buffer ``flat`` (``to_param_grads`` copies them into
         the parameters' .grad)."""
+        if weights is not None and self.objective != "weighted":
+            raise ValueError("weights belong to objective=\"weighted\"")
         self.idx.copy_(idx)
         self.targets.copy_(targets)
+        if self.objective == "weighted":
+            if weights is None:
+                self.weights.fill_(1.0)
+            else:
+                self.weights.copy_(weights)
         if self.graph is not None:
             self.graph.replay()
         else:
             self._run()
         return self.loss
+
+    @torch.no_grad()
+    def score(self, idx, targets, top=0):
+        """The forward alone: RowLogprobs of targets [B, T] (logprobs.row_logprobs: a target of -1 is ignored) after
+        idx [B, T], with the ``top`` most likely tokens of each position. Overwrites the activations of the last
+        step, none of its gradients."""
+        self.idx.copy_(idx)
+        self._embed()
+        if self.wavefront:
+            self._stack_fwd()
+        else:
+            for l in range(self.cfg.n_layers):
+                self._attn_fwd(l)
+                self._mlp_fwd(l)
+        m, x = self.m, self.xs[-1].view(self.B * self.T, self.cfg.d_model)
+        tg = targets.to(device=self.dev, dtype=torch.int64).reshape(-1)
+        parts = []
+        for r0, r1 in self._chunks():
+            hf, _ = _rms(x[r0:r1], m.norm_f.weight, m.norm_f.eps)
+            parts.append(row_logprobs(hf @ self.w_emb.t(), tg[r0:r1], top=top))
+        return RowLogprobs(*(None if f[0] is None else torch.cat(f).view(self.B, self.T, *f[0].shape[1:])
+                             for f in zip(*parts)))
+
+    def optimizer(self, lr=1e-3, weight_decay=0.1, **kw):
+        """optim.AdamW over the model's parameters and this trunk's gradients: the matrices decayed, the vectors (norm
+        weights, biases, gains) not. A step of training: ``train_step``, the optimizer's ``step()``, ``refresh()``."""
+        params = dict(self.m.named_parameters())
+        names = sorted(self.names, key=lambda n: params[n].dim() < 2)    # stable: the matrices first
+        mats = [n for n in names if params[n].dim() >= 2]
+        groups = [dict(params=[params[n] for n in mats], weight_decay=weight_decay),
+                  dict(params=[params[n] for n in names[len(mats):]], weight_decay=0.0)]
+        return AdamW(groups, grads=[self.grad[n] for n in names], lr=lr, **kw)
 
     def to_param_grads(self):
         """param.grad = the flat buffer's view of it (GradBuffers.to_param_grads, backward.py:52-61)."""
