@@ -125,13 +125,13 @@ template <typename T> DM_DEV void unpack(const u32x4& r, float* v) {
 // x is computed here, not where it is used (all of a tile's summands would wait in registers until then)
 DM_DEV void here(float& x) { asm volatile("" : "+v"(x)); }
 
-// The larger of two pairs of bf16 numbers. Both formats order by sign and magnitude, so fp16's maximum serves; it passes
-// over what reads as a NaN there, magnitudes of 2^121 and more, infinities and NaN among them.
-DM_DEV uint32_t pair_max(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("v_pk_max_f16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-  return r;
-}
+// bf16 numbers as 16-bit integers: those >= 0 order as signed ones, above all others; the negative ones as unsigned ones
+// the other way round.
+typedef short shortx2 __attribute__((ext_vector_type(2)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+DM_DEV shortx2 signed_pair(uint32_t x) { return __builtin_bit_cast(shortx2, x); }
+DM_DEV ushortx2 unsigned_pair(uint32_t x) { return __builtin_bit_cast(ushortx2, x); }
+DM_DEV float bf16_value(int bits) { return __uint_as_float((uint32_t)bits << 16); }
 
 // A thread's part of one tile of a row: NV vectors and (first tile) one single column, FLOOR where there is none.
 template <typename T, int NT, int NV> struct Tile {
@@ -157,31 +157,54 @@ template <typename T, int NT, int NV> struct Tile {
     asm volatile("" : "+v"(raw[i]));
     unpack<T>(raw[i], v);
   }
-  // the largest logit of a vector, FLOOR at least (bf16: magnitudes of 2^121 left out)
-  DM_DEV float largest_of(int i) {
-    if constexpr (sizeof(T) == 2) {
-      const uint32_t p = pair_max(pair_max(raw[i][0], raw[i][1]), pair_max(raw[i][2], pair_max(raw[i][3], FILL)));
-      return fmaxf(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
-    } else {
-      return fmaxf(fmaxf(fmaxf(__uint_as_float(raw[i][0]), __uint_as_float(raw[i][1])),
-                         fmaxf(__uint_as_float(raw[i][2]), __uint_as_float(raw[i][3]))), FLOOR);
-    }
-  }
+  // the thread's largest logit, FLOOR at least; NaN is passed over or taken
   DM_DEV float largest() {
     float m = fmaxf(edge, FLOOR);
-    uint32_t p = FILL;
+    if constexpr (sizeof(T) == 2) {
+      shortx2 p = signed_pair(FILL);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (i >= nv) continue;
-      if constexpr (sizeof(T) == 2) {
+      for (int i = 0; i < NV; ++i) {
+        if (i >= nv) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p = pair_max(p, raw[i][j]);
-      } else {
-        m = fmaxf(m, largest_of(i));
+        for (int j = 0; j < 4; ++j) p = __builtin_elementwise_max(p, signed_pair(raw[i][j]));
+      }
+      int best = max((int)p[0], (int)p[1]);
+      if (__any(best < 0)) {   // somebody has negative ones only
+        ushortx2 u = unsigned_pair(FILL);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (i >= nv) continue;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) u = __builtin_elementwise_min(u, unsigned_pair(raw[i][j]));
+        }
+        if (best < 0) best = min((int)u[0], (int)u[1]);
+      }
+      m = fmaxf(m, bf16_value(best));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (i >= nv) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, __uint_as_float(raw[i][j]));
       }
     }
-    if constexpr (sizeof(T) == 2) m = fmaxf(m, fmaxf(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)));
     return m;
+  }
+  // whether one of a vector's logits may reach `bound`
+  DM_DEV bool reaches(int i, float bound) {
+    if constexpr (sizeof(T) == 2) {
+      if (bound > 0.f) {
+        const shortx2 p = __builtin_elementwise_max(__builtin_elementwise_max(signed_pair(raw[i][0]), signed_pair(raw[i][1])),
+                                                    __builtin_elementwise_max(signed_pair(raw[i][2]), signed_pair(raw[i][3])));
+        return max((int)p[0], (int)p[1]) >= (int)(__float_as_uint(bound) >> 16);   // bound: rounded down to bf16's bits
+      }
+    }
+    float v[V];
+    unpack<T>(raw[i], v);
+    float m = v[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) m = fmaxf(m, v[j]);
+    return m >= bound;
   }
 };
 
@@ -333,7 +356,7 @@ template <typename T, int NT, int NV> DM_DEV void take_tile(const RowSpan<T>& ro
   for (int i = 0; i < NV; ++i) {
     if (i >= t.nv) continue;
     const int q = (tile * NV + i) * NT + threadIdx.x;
-    if (fmaxf(t.largest_of(i), FLOOR) < bound || q >= row.nvec) continue;
+    if (!t.reaches(i, bound) || q >= row.nvec) continue;
     float v[V];
     t.get(i, v);
     for (int j = 0; j < V; ++j) {
@@ -441,7 +464,7 @@ template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT
     }
     u.join(sh);
     RowStats s;
-    const bool slow = !(u.z < INF) || u.m <= FLOOR;
+    const bool slow = !(u.z > 0.f && u.z < INF) || u.m <= FLOOR;
     if (slow) {
       s = slow_stats<T, NT>(row.x, a.cols, sh);
     } else {
@@ -522,6 +545,7 @@ template <typename T, int NT, int NV> __global__ __launch_bounds__(256) void k_l
   }
 }
 
+constexpr int MAX_COLS = 1 << 27;     // a row's bytes in 32 bits
 constexpr int MAX_BLOCKS = 1 << 20;   // of a grid; further rows by the same blocks
 
 template <typename T> LpArgs<T> typed(const dm_logprob_args* a) {
@@ -575,8 +599,8 @@ bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p)
 int check_logprob(const dm_logprob_args* a, bool bwd) {
   DM_REQUIRE(a != nullptr, DM_ERR_INVALID, "null arguments");
   DM_REQUIRE(a->dtype == DM_BF16 || a->dtype == DM_F32, DM_ERR_INVALID, "dtype %d", a->dtype);
-  DM_REQUIRE(a->rows >= 0 && a->cols > 0 && a->ld >= a->cols, DM_ERR_INVALID, "rows=%d cols=%d ld=%lld", a->rows, a->cols,
-             (long long)a->ld);
+  DM_REQUIRE(a->rows >= 0 && a->cols > 0 && a->cols <= MAX_COLS && a->ld >= a->cols, DM_ERR_INVALID,
+             "rows=%d cols=%d ld=%lld (at most %d columns)", a->rows, a->cols, (long long)a->ld, MAX_COLS);
   if (a->rows == 0) return DM_OK;
   const size_t e = esz(a->dtype);
   DM_REQUIRE(a->logits && aligned_to(a->logits, e), DM_ERR_INVALID, "null or unaligned logits");

@@ -18,6 +18,7 @@ bit for bit. A NaN or infinity in a state makes its block NaN; ``skip_nonfinite`
 """
 
 import ctypes
+from bisect import bisect_left
 from itertools import chain
 
 import torch
@@ -54,6 +55,7 @@ class AdamW:
         spans = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in self.params if p.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("two parameters share memory")
+        starts = [a for a, _ in spans]
         self.grads = None
         if grads is not None:
             self.grads = list(grads)
@@ -61,6 +63,9 @@ class AdamW:
                 raise ValueError(f"{len(self.grads)} gradients for {len(self.params)} parameters")
             for i, (p, g) in enumerate(zip(self.params, self.grads)):
                 self._check_grad(i, p, g)
+                k = bisect_left(starts, g.data_ptr() + g.numel() * g.element_size())   # parameters that start before its end
+                if k and g.numel() and spans[k - 1][1] > g.data_ptr():
+                    raise ValueError(f"gradient {i} shares memory with a parameter")
         self.betas, self.eps, self.max_norm = (float(betas[0]), float(betas[1])), float(eps), max_norm
         self.skip_nonfinite, self.state_bits, self.seed = bool(skip_nonfinite), state_bits, int(seed) & 0xffffffff
 
@@ -122,6 +127,7 @@ class AdamW:
             raise L.DMError("dm_adamw_plan_bytes: " + L.lib().dm_last_error().decode())
         host, n = torch.empty(nb, dtype=torch.uint8), ctypes.c_int64()
         L.check(L.lib().dm_adamw_plan(arr, len(rows), host.data_ptr(), nb, ctypes.byref(n)))
+        self._held = [p.detach() for p in self.params]   # what the plan writes stays allocated
         torch.cuda.synchronize(self.device)   # no step still reads the plan that this one replaces
         self._plan = host.to(self.device)
         torch.cuda.current_stream(self.device).synchronize()

@@ -182,7 +182,8 @@ def special_rows(V, dtype):
            ("zero signs", torch.zeros(V), 1), ("descending", torch.arange(V, 0, -1) / 64.0, 0), ("ascending", torch.arange(V) / 64.0, 0),
            ("lowest", torch.full((V,), low), 2), ("three allowed", torch.full((V,), low), 3), ("masked target", n.clone(), 5),
            ("huge", n * 1e30, 0), ("peaked", n.clone(), 7), ("one lane", n.clone(), 4), ("far", n + 30000.0, 4), ("ignored", n.clone(), -1),
-           ("contiguous few", torch.full((V,), -INF), V - 1)]
+           ("contiguous few", torch.full((V,), -INF), V - 1), ("negative", -5 - n.abs(), 6), ("beside -1e37", n - 3, 2),
+           ("all far below", -1e37 * (1 + n.abs()), 2), ("largest number", n.clone(), 3), ("two largest", n.clone(), 3)]
     rows = []
     for name, row, t in out:
         row = row.to(DEV).float()
@@ -199,6 +200,13 @@ def special_rows(V, dtype):
             row[7] = 200.0
         if name == "one lane":
             row[8 * 64 * 4::8 * 64 * 4] += 50.0       # the largest far apart at one stride
+        if name == "beside -1e37":
+            row[5::7] = -1e37
+            row[torch.arange(V, device=DEV) % 8 != 2] = -1e37
+        if name in ("largest number", "two largest"):
+            row[3] = 3e38
+        if name == "two largest":
+            row[V // 2] = 3e38
         if name == "contiguous few":
             row[V - 9:] = n[:9]
         rows.append((name, row.to(dtype), t))

@@ -393,6 +393,29 @@ def test_state_dict_continues(bits):
         AdamW(ps[:1], grads=gs[:1], state_bits=bits).load_state_dict(saved)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_elements_past_32_bits(bits):
+    """A tensor of more than 2^31 elements: its first and last ones are updated as a short tensor's."""
+    n = (1 << 31) + 777
+    p, g = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV, dtype=torch.bfloat16)
+    ends = [slice(0, 300), slice(n - 300, n)]
+    for s in ends:
+        p[s] = torch.linspace(-1, 1, 300, device=DEV)
+        g[s] = torch.linspace(-2, 1, 300, device=DEV).bfloat16()
+    small = p[ends[1]].clone()
+    opt = AdamW([p], grads=[g], lr=LR, max_norm=1.0, state_bits=bits)
+    other = AdamW([small], grads=[g[ends[1]].clone()], lr=LR)
+    norm = math.sqrt(sum(float(g[s].double().square().sum()) for s in ends))
+    got = opt.step()
+    assert abs(float(got) - norm) <= U * norm * 1.001
+    other.step()
+    # the first step moves by lr g / (|g| + eps / c): the clipping cancels but for eps, below 1e-6 of it
+    for s in ends:
+        assert ((p[s] - small).abs() <= LR * 1e-4 + 4 * U).all()
+    m, v = opt.state_values()
+    assert (m[n - 100:n] != 0).all() and (v[n - 100:n] != 0).any() and float(p[300:n - 300].abs().max()) == 0
+
+
 def test_other_stream():
     ps, gs, groups, P, _ = make([5000, 3])
     ps2, gs2, groups2, P2, _ = make([5000, 3])
@@ -417,4 +440,10 @@ def test_refusals():
         with pytest.raises((ValueError, NotImplementedError)):
             f()
             pytest.fail(f"call {i} was not refused")
-    AdamW([p[:5], p[5:]], grads=[p[:5], p[5:]])       # neighbours are not overlaps
+    q = torch.zeros(10, device=DEV)
+    AdamW([p[:5], p[5:]], grads=[q[:5], q[:5]])       # neighbours are not overlaps, and gradients may be shared
+    both = torch.zeros(20, device=DEV)
+    AdamW([both[:10]], grads=[both[10:]])
+    for g in (both[:10], both[9:19]):
+        with pytest.raises(ValueError, match="shares memory"):
+            AdamW([both[:10]], grads=[g])

@@ -19,7 +19,7 @@ def rows_args(**kw):
     return a
 
 
-@pytest.mark.parametrize("kw", [dict(dtype=2), dict(rows=-1), dict(cols=0), dict(ld=9), dict(logits=None), dict(logits=0x10002),
+@pytest.mark.parametrize("kw", [dict(dtype=2), dict(rows=-1), dict(cols=0), dict(cols=(1 << 27) + 1, ld=1 << 40), dict(ld=9), dict(logits=None), dict(logits=0x10002),
                                 dict(target=None), dict(top=33), dict(top=-1), dict(top=3), dict(cols=2, top=3, top_logp=1, top_ids=1),
                                 dict(dlogits=0x40000, ld_d=10), dict(dlogits=0x40000, ld_d=9, g_logp=0x50000),
                                 dict(dlogits=0x40001, ld_d=10, g_logp=0x50000),
