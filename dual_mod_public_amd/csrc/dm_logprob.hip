@@ -104,9 +104,13 @@ template <typename T> struct RowSpan {
     return c < n ? c : -1;
   }
   DM_DEV int col(int q) const { return c0 + q * V; }
-  // vector q0 + lane, q0 the same in every lane: a scalar base and one 32-bit lane offset for all of a thread's loads
-  DM_DEV u32x4 vec(int q0, int lane) const {
-    return ld_global<u32x4>(reinterpret_cast<const char*>(x + c0 + (long)q0 * V) + 16u * lane);
+  // vector q0 + lane, q0 the same in every lane: a scalar base and one 32-bit lane offset for all of a thread's loads.
+  // ONCE: no kernel of the call reads it again, and it goes past the caches (4096 rows of 32000 bf16: 44 us, kept 49;
+  // with the gradient 98 and 107; but 2000 rows of 100003 read twice 236, kept 197)
+  template <bool ONCE> DM_DEV u32x4 vec(int q0, int lane) const {
+    const auto* p = (const __attribute__((address_space(1))) u32x4*)(reinterpret_cast<const char*>(x + c0 + (long)q0 * V) + 16u * lane);
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return *p;
   }
 };
 template <typename T> DM_DEV void unpack(const u32x4& r, float* v) {
@@ -140,13 +144,13 @@ template <typename T, int NT, int NV> struct Tile {
   u32x4 raw[NV];
   float edge;
   int nv;   // vectors that any of the block's threads has
-  DM_DEV void load(const RowSpan<T>& row, int tile) {
+  template <bool ONCE> DM_DEV void load(const RowSpan<T>& row, int tile) {
     nv = (row.nvec + NT - 1) / NT - tile * NV;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int q0 = (tile * NV + i) * NT;
       raw[i] = u32x4{FILL, FILL, FILL, FILL};
-      if (q0 + (int)threadIdx.x < row.nvec) raw[i] = row.vec(q0, threadIdx.x);
+      if (q0 + (int)threadIdx.x < row.nvec) raw[i] = row.template vec<ONCE>(q0, threadIdx.x);
     }
     const int c = tile == 0 ? row.edge_col(threadIdx.x) : -1;
     edge = c >= 0 ? to_f(row.x[c]) : FLOOR;
@@ -359,11 +363,18 @@ template <typename T, int NT, int NV> DM_DEV void take_tile(const RowSpan<T>& ro
     if (!t.reaches(i, bound) || q >= row.nvec) continue;
     float v[V];
     t.get(i, v);
-    for (int j = 0; j < V; ++j) {
-      float x = v[0];
+    uint32_t hit = 0;
 #pragma unroll
-      for (int k = 1; k < V; ++k) x = j == k ? v[k] : x;
-      if (x >= bound) take(x, row.col(q) + j, sh);
+    for (int j = 0; j < V; ++j) hit |= v[j] >= bound ? 1u << j : 0u;
+    while (hit) {   // one, as a rule
+      const int j = __builtin_ctz(hit), k = j * (int)sizeof(T) / 4;
+      hit &= hit - 1;
+      uint32_t w = t.raw[i][0];
+      w = k == 1 ? t.raw[i][1] : w;
+      w = k == 2 ? t.raw[i][2] : w;
+      w = k == 3 ? t.raw[i][3] : w;
+      if constexpr (sizeof(T) == 2) w = j & 1 ? w & 0xffff0000u : w << 16;
+      take(__uint_as_float(w), row.col(q) + j, sh);
     }
   }
 }
@@ -440,11 +451,12 @@ DM_DEV void store_tile(const RowSpan<T>& row, Tile<T, NT, NV>& t, int tile, cons
   if (tile == 0) grad_edge(dx, row.edge_col(threadIdx.x), t.edge, w, target);
 }
 
-// A block per row, the row in tiles of NT NV vectors held in registers.
-template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT, 4) void k_logprob_rows(LpArgs<T> a) {
+// A block per row, the row in tiles of NT NV vectors held in registers. ONCE: the gradient's rows are one tile.
+template <typename T, int NT, int NV, bool GRAD, bool ONCE> __global__ __launch_bounds__(NT, 4) void k_logprob_rows(LpArgs<T> a) {
   __shared__ Shared<NT> sh;
   for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const RowSpan<T> row(a.x + r * a.ld, a.cols);
+    // (also where it is 1: known to be, the row's values would be kept converted between the passes, and spilled)
     const int tiles = max(1, (row.nvec + NT * NV - 1) / (NT * NV));
     const long t = a.target ? a.target[r] : -1;
     const float xt = t >= 0 && t < a.cols ? to_f(row.x[t]) : 0.f;
@@ -452,7 +464,7 @@ template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT
     Tile<T, NT, NV> tile;
     if (a.top && threadIdx.x == 0) sh.count = 0;
     for (int i = 0; i < tiles; ++i) {
-      tile.load(row, i);
+      tile.template load<ONCE>(row, i);
       u.refer(fmaxf(u.m, tile.largest()));
       u.add(tile);
       if (a.top) {   // the bound only rises from tile to tile
@@ -493,7 +505,7 @@ template <typename T, int NT, int NV, bool GRAD> __global__ __launch_bounds__(NT
         for (int i = threadIdx.x; i < a.cols; i += NT) dx[i] = from_f<T>(w.value);
       } else {
         for (int i = 0; i < tiles; ++i) {
-          if (tiles > 1) tile.load(row, i);
+          if (!ONCE) tile.template load<true>(row, i);
           store_tile(row, tile, i, w, target, dx);
         }
       }
@@ -523,7 +535,7 @@ template <typename T, int NT, int NV> __global__ __launch_bounds__(256) void k_l
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       raw[i] = u32x4{0, 0, 0, 0};
-      if (!w.fill && q0 + i * NT < row.nvec) raw[i] = row.vec(0, q0 + i * NT);
+      if (!w.fill && q0 + i * NT < row.nvec) raw[i] = row.template vec<true>(0, q0 + i * NT);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -553,16 +565,17 @@ template <typename T> LpArgs<T> typed(const dm_logprob_args* a) {
           a->top_ids, a->g_logp, a->g_entropy, a->ld, a->ld_d, a->rows, a->cols, a->top};
 }
 
-template <bool GRAD, typename T, int NT, int NV> void launch_rows(const LpArgs<T>& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_logprob_rows<T, NT, NV, GRAD>), dim3(std::min(a.rows, MAX_BLOCKS)), dim3(NT), 0, s, a);
+template <bool GRAD, typename T, int NT, int NV, bool ONCE = true> void launch_rows(const LpArgs<T>& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_logprob_rows<T, NT, NV, GRAD, ONCE>), dim3(std::min(a.rows, MAX_BLOCKS)), dim3(NT), 0, s, a);
 }
 // The threads of a row and their vectors per tile, by the row's 16-byte vectors (bf16: 8 logits, fp32: 4).
 // Fewer rows than CUs: as many threads as a block has, since nothing else hides a row's latencies (one row of 32000 bf16
-// 6.7 us, at 256 threads 8.4).
+// with 5 alternatives 7.0 us, at 256 threads 9.6; without them 4.9, where a block of so many threads takes 3.8 for a row
+// of 8). Several blocks per row with a second launch to join them would cost that launch.
 // Otherwise the smallest blocks that fill a CU's memory pipes while others of the CU wait at their barriers (4096 rows of
-// 32000 bf16: 64 threads 51 us, 256 48, 1024 80). With the gradient a row is best read once and held until it is
-// written (the same rows: 256 threads of 16 vectors, all of a row, 106 us; of 8 vectors, read twice, 121); rows past
-// 65536 fp32 or 131072 bf16 are read twice (2000 rows of 100003 bf16: 188 us held, 193 read twice).
+// 32000 bf16: 64 threads of 4 vectors 47 us, 256 of 8 44, 1024 of 4 72). With the gradient a row is best read once and
+// held until it is written (the same rows: 256 threads of 16 vectors, all of a row, 98 us; of 8 vectors, read twice,
+// 114); rows past 65536 fp32 or 131072 bf16 are read twice (2000 rows of 100003 bf16: 186 us held, 197 read twice).
 template <typename T> void run_rows(const LpArgs<T>& a, hipStream_t s) {
   const int nvec = cdiv(a.cols, RowSpan<T>::V);
   const bool few = a.rows < 256 && nvec > 256 * 4;
@@ -579,7 +592,8 @@ template <typename T> void run_rows(const LpArgs<T>& a, hipStream_t s) {
     else if (few && nvec <= 1024 * 4) launch_rows<true, T, 1024, 4>(a, s);
     else if (nvec <= 256 * 16) launch_rows<true, T, 256, 16>(a, s);
     else if (!few && nvec <= 512 * 16) launch_rows<true, T, 512, 16>(a, s);
-    else launch_rows<true, T, 1024, 16>(a, s);
+    else if (nvec <= 1024 * 16) launch_rows<true, T, 1024, 16>(a, s);
+    else launch_rows<true, T, 1024, 16, false>(a, s);
   }
 }
 template <typename T> void run_bwd(const LpArgs<T>& a, hipStream_t s) {

@@ -47,21 +47,38 @@ struct AdamArgs {
 DM_DEV float grad_at(const PlanTensor& t, long i) {
   return t.g_bf16 ? __uint_as_float((uint32_t)ld_global<uint16_t>((const bf16*)t.g + i) << 16) : ld_global<float>((const float*)t.g + i);
 }
-// Four elements from i on. Parameters and gradients may be views at any element of a buffer: their vectors are aligned
+// Vectors in global memory, aligned to A bytes. PAST: with the non-temporal hint, for what is larger than the caches
+// keep from one kernel to the next (see Stream).
+template <typename V, int A, bool PAST, typename P> DM_DEV V load(const P* p) {
+  typedef V VA __attribute__((aligned(A)));
+  const auto* q = (const __attribute__((address_space(1))) VA*)p;
+  if constexpr (PAST) return __builtin_nontemporal_load(q);
+  else return *q;
+}
+template <int A, bool PAST, typename V, typename P> DM_DEV void store(P* p, const V& v) {
+  typedef V VA __attribute__((aligned(A)));
+  auto* q = (__attribute__((address_space(1))) VA*)p;
+  if constexpr (PAST) __builtin_nontemporal_store(v, q);
+  else *q = v;
+}
+// Four gradients from i on. Parameters and gradients may be views at any element of a buffer: their vectors are aligned
 // to their elements only.
-template <bool BF16> DM_DEV floatx4 grads4(const PlanTensor& t, long i) {
+template <bool BF16, bool PAST> DM_DEV floatx4 grads4(const PlanTensor& t, long i) {
   if constexpr (BF16) {
-    const u32x2 r = ld_global_a<u32x2, 2>((const bf16*)t.g + i);
+    const u32x2 r = load<u32x2, 2, PAST>((const bf16*)t.g + i);
     return floatx4{__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xffff0000u), __uint_as_float(r[1] << 16),
                    __uint_as_float(r[1] & 0xffff0000u)};
   } else {
-    return ld_global_a<floatx4, 4>((const float*)t.g + i);
+    return load<floatx4, 4, PAST>((const float*)t.g + i);
   }
 }
-DM_DEV void store4(float* p, const floatx4& v) {   // global, as ld_global_a
-  typedef floatx4 V __attribute__((aligned(4)));
-  *(__attribute__((address_space(1))) V*)p = v;
-}
+// What goes past the caches. A small model's step finds its data in the last one, of 256 MB (2.9M parameters, 80 MB: 20.1 us
+// kept, 22.6 past). A larger step's parameters and states, read and written, only push one another out: past the caches 15M
+// parameters take 78 us (93), with 8-bit states 63 (70), 47M 236 (283). The gradients stay as long as they fit by
+// themselves, since the norm has read them just before (past as well: 85, 250); beyond, they go past too (543M: 2.98 ms;
+// 3.07 with the gradients kept, 3.26 with everything; with 8-bit states 1.84 ms, 2.07 with everything).
+enum class Stream { KEPT, STATES, ALL };
+constexpr double CACHE_BYTES = 256 << 20;
 
 DM_DEV double block_sum(double x, double* red) {
 #pragma unroll
@@ -74,13 +91,13 @@ DM_DEV double block_sum(double x, double* red) {
   return x;
 }
 
-template <bool BF16> DM_DEV void add_squares(const PlanTensor& t, long i, long end, double (&s)[4]) {
+template <bool BF16, bool PAST> DM_DEV void add_squares(const PlanTensor& t, long i, long end, double (&s)[4]) {
   constexpr int STEP = 256 * 4, IN_FLIGHT = 4;
   i += 4 * threadIdx.x;
   for (; i + (IN_FLIGHT - 1) * STEP + 3 < end; i += IN_FLIGHT * STEP) {
     floatx4 g[IN_FLIGHT];
 #pragma unroll
-    for (int k = 0; k < IN_FLIGHT; ++k) g[k] = grads4<BF16>(t, i + k * STEP);
+    for (int k = 0; k < IN_FLIGHT; ++k) g[k] = grads4<BF16, PAST>(t, i + k * STEP);
 #pragma unroll
     for (int k = 0; k < IN_FLIGHT; ++k)
 #pragma unroll
@@ -94,7 +111,7 @@ template <bool BF16> DM_DEV void add_squares(const PlanTensor& t, long i, long e
 }
 // part[b] = sum of g^2 over the b-th run of chunks. The squares of fp32 are exact in 64 bits, so the norm is the same for
 // any order of the sum but for its last bits. Bound by reading the gradients.
-__global__ __launch_bounds__(256) void k_grad_sumsq(const PlanTensor* tensors, const int* chunk_tensor, long n_chunks,
+template <bool PAST> __global__ __launch_bounds__(256) void k_grad_sumsq(const PlanTensor* tensors, const int* chunk_tensor, long n_chunks,
                                                     double* part) {
   __shared__ double red[4];
   double s[4] = {0., 0., 0., 0.};
@@ -102,8 +119,8 @@ __global__ __launch_bounds__(256) void k_grad_sumsq(const PlanTensor* tensors, c
   for (long c = blockIdx.x * n_chunks / gridDim.x; c < end;) {
     const PlanTensor t = tensors[chunk_tensor[c]];
     const long first = (c - t.chunk0) * CHUNK, last = min((end - t.chunk0) * CHUNK, t.n);   // this run's part of the tensor
-    if (t.g_bf16) add_squares<true>(t, first, last, s);
-    else add_squares<false>(t, first, last, s);
+    if (t.g_bf16) add_squares<true, PAST>(t, first, last, s);
+    else add_squares<false, PAST>(t, first, last, s);
     c = t.chunk0 + (last + CHUNK - 1) / CHUNK;
   }
   const double x = block_sum((s[0] + s[1]) + (s[2] + s[3]), red);
@@ -183,19 +200,20 @@ struct Update {
 };
 
 // A block per chunk; bound by its 28 bytes per element.
-template <bool BF16> DM_DEV void step32(const AdamArgs& a, const Control& c, const PlanTensor& t, long i0, float* ms, float* vs) {
+template <bool BF16, Stream S> DM_DEV void step32(const AdamArgs& a, const Control& c, const PlanTensor& t, long i0, float* ms, float* vs) {
   const Update u(a, c, t);
   constexpr int STEP = 256 * 4, N = CHUNK / STEP;
+  constexpr bool PAST = S != Stream::KEPT;
   if (i0 + CHUNK <= t.n) {
     i0 += 4 * threadIdx.x;
     floatx4 p[N], g[N], m[N], v[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const long i = i0 + k * STEP;
-      g[k] = grads4<BF16>(t, i);
-      m[k] = ld_global<floatx4>(ms + i);
-      v[k] = ld_global<floatx4>(vs + i);
-      p[k] = ld_global_a<floatx4, 4>(t.p + i);
+      g[k] = grads4<BF16, S == Stream::ALL>(t, i);
+      m[k] = load<floatx4, 16, PAST>(ms + i);
+      v[k] = load<floatx4, 16, PAST>(vs + i);
+      p[k] = load<floatx4, 4, PAST>(t.p + i);
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -208,9 +226,9 @@ template <bool BF16> DM_DEV void step32(const AdamArgs& a, const Control& c, con
         v[k][j] = v1;
         p[k][j] = u.of(p[k][j], m1, v1);
       }
-      store4(ms + i, m[k]);
-      store4(vs + i, v[k]);
-      store4(t.p + i, p[k]);
+      store<16, PAST>(ms + i, m[k]);
+      store<16, PAST>(vs + i, v[k]);
+      store<4, PAST>(t.p + i, p[k]);
     }
     return;
   }
@@ -222,15 +240,15 @@ template <bool BF16> DM_DEV void step32(const AdamArgs& a, const Control& c, con
     t.p[i] = u.of(t.p[i], m, v);
   }
 }
-__global__ __launch_bounds__(256) void k_adamw32(AdamArgs a) {
+template <Stream S> __global__ __launch_bounds__(256) void k_adamw32(AdamArgs a) {
   const Control c = *a.c;
   if (c.skip) return;
   const PlanTensor t = a.tensors[a.chunk_tensor[blockIdx.x]];
   const long i0 = (blockIdx.x - t.chunk0) * CHUNK;
   float* ms = (float*)a.m + t.block0 * BLOCK;
   float* vs = (float*)a.v + t.block0 * BLOCK;
-  if (t.g_bf16) step32<true>(a, c, t, i0, ms, vs);
-  else step32<false>(a, c, t, i0, ms, vs);
+  if (t.g_bf16) step32<true, S>(a, c, t, i0, ms, vs);
+  else step32<false, S>(a, c, t, i0, ms, vs);
 }
 
 // The two code formats. Shifted to the place of an fp32 number's exponent and upper mantissa bits, a code is one, its
@@ -255,8 +273,9 @@ DM_DEV bool too_large(float x) { return !(fabsf(x) < 0x1p127f); }
 
 // A wave per run of four 256-element blocks, four elements per lane and block. Bound by its 16 bytes per element
 // (fp32 gradients) and the hash, two 32-bit products per element, about equally.
-template <bool BF16> DM_DEV void step8(const AdamArgs& a, const Control& c, const PlanTensor& t, long i0) {
+template <bool BF16, Stream S> DM_DEV void step8(const AdamArgs& a, const Control& c, const PlanTensor& t, long i0) {
   constexpr int N = CHUNK / BLOCK / 4;
+  constexpr bool PAST = S != Stream::KEPT;
   const Update u(a, c, t);
   const int lane = threadIdx.x & 63;
   const long blk0 = t.block0 + i0 / BLOCK;
@@ -270,14 +289,14 @@ template <bool BF16> DM_DEV void step8(const AdamArgs& a, const Control& c, cons
     mc[k] = vc[k] = me[k] = ve[k] = 0;
     if (i0 + k * BLOCK >= t.n) continue;
     if (i + 3 < t.n) {
-      g[k] = grads4<BF16>(t, i);
-      p[k] = ld_global_a<floatx4, 4>(t.p + i);
+      g[k] = grads4<BF16, S == Stream::ALL>(t, i);
+      p[k] = load<floatx4, 4, PAST>(t.p + i);
     } else {
       for (int j = 0; j < 3; ++j)
         if (i + j < t.n) g[k][j] = grad_at(t, i + j), p[k][j] = t.p[i + j];
     }
-    mc[k] = ld_global<uint32_t>((const uint8_t*)a.m + (blk0 + k) * BLOCK + 4 * lane);
-    vc[k] = ld_global<uint32_t>((const uint8_t*)a.v + (blk0 + k) * BLOCK + 4 * lane);
+    mc[k] = load<uint32_t, 4, PAST>((const uint8_t*)a.m + (blk0 + k) * BLOCK + 4 * lane);
+    vc[k] = load<uint32_t, 4, PAST>((const uint8_t*)a.v + (blk0 + k) * BLOCK + 4 * lane);
     me[k] = a.me[blk0 + k];
     ve[k] = a.ve[blk0 + k];
   }
@@ -315,28 +334,28 @@ template <bool BF16> DM_DEV void step8(const AdamArgs& a, const Control& c, cons
       mo |= cm << 8 * j;
       vo |= cv << 8 * j;
     }
-    *(uint32_t*)((uint8_t*)a.m + (blk0 + k) * BLOCK + 4 * lane) = me1 == 255 ? 0 : mo;
-    *(uint32_t*)((uint8_t*)a.v + (blk0 + k) * BLOCK + 4 * lane) = ve1 == 255 ? 0 : vo;
+    store<4, PAST>((uint8_t*)a.m + (blk0 + k) * BLOCK + 4 * lane, me1 == 255 ? 0 : mo);
+    store<4, PAST>((uint8_t*)a.v + (blk0 + k) * BLOCK + 4 * lane, ve1 == 255 ? 0 : vo);
     if (lane == 0) {
       a.me[blk0 + k] = me1;
       a.ve[blk0 + k] = ve1;
     }
     if (i + 3 < t.n) {
-      store4(t.p + i, p[k]);
+      store<4, PAST>(t.p + i, p[k]);
     } else {
       for (int j = 0; j < 3; ++j)
         if (i + j < t.n) t.p[i + j] = p[k][j];
     }
   }
 }
-__global__ __launch_bounds__(256) void k_adamw8(AdamArgs a) {
+template <Stream S> __global__ __launch_bounds__(256) void k_adamw8(AdamArgs a) {
   const Control c = *a.c;
   if (c.skip) return;
   const PlanTensor t = a.tensors[a.chunk_tensor[blockIdx.x]];
   const long i0 = (blockIdx.x - t.chunk0) * CHUNK + (threadIdx.x >> 6) * (CHUNK / 4);
   if (i0 >= t.n) return;
-  if (t.g_bf16) step8<true>(a, c, t, i0);
-  else step8<false>(a, c, t, i0);
+  if (t.g_bf16) step8<true, S>(a, c, t, i0);
+  else step8<false, S>(a, c, t, i0);
 }
 
 // Sixteen codes per lane.
@@ -387,9 +406,18 @@ int check_plan(const dm_adamw_args* a) {
   return DM_OK;
 }
 const int* chunk_map(const dm_adamw_args* a) { return (const int*)((const char*)a->plan + tensor_bytes(a->n_tensors)); }
+double elements(const dm_adamw_args* a) { return (double)a->n_chunks * CHUNK; }   // at most
+Stream stream_of(const dm_adamw_args* a) {   // by fp32 gradients
+  if (elements(a) * 4 > CACHE_BYTES) return Stream::ALL;
+  return elements(a) * (a->state_bits == 32 ? 28 : 16) > CACHE_BYTES / 2 ? Stream::STATES : Stream::KEPT;
+}
 int run_sumsq(const dm_adamw_args* a, double* part, hipStream_t s) {
   const int parts = (int)std::min<long>(a->n_chunks, NORM_PARTS);
-  hipLaunchKernelGGL(k_grad_sumsq, dim3(parts), dim3(256), 0, s, (const PlanTensor*)a->plan, chunk_map(a), a->n_chunks, part);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(parts), dim3(256), 0, s, (const PlanTensor*)a->plan, chunk_map(a), (long)a->n_chunks, part);
+  };
+  if (elements(a) * 4 > CACHE_BYTES) go(k_grad_sumsq<true>);
+  else go(k_grad_sumsq<false>);
   return parts;
 }
 
@@ -440,8 +468,12 @@ int dm_adamw_step(const dm_adamw_args* a, void* stream) {
   const AdamArgs k{(const PlanTensor*)a->plan, chunk_map(a), a->exp_avg, a->exp_avg_sq, a->exp_avg_exponent,
                    a->exp_avg_sq_exponent, (float)a->beta1, (float)(1. - a->beta1), (float)a->beta2, (float)(1. - a->beta2),
                    (float)a->eps, w.c};
-  if (a->state_bits == 32) hipLaunchKernelGGL(k_adamw32, dim3(a->n_chunks), dim3(256), 0, s, k);
-  else hipLaunchKernelGGL(k_adamw8, dim3(a->n_chunks), dim3(256), 0, s, k);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a->n_chunks), dim3(256), 0, s, k); };
+  switch (stream_of(a)) {
+    case Stream::KEPT: a->state_bits == 32 ? go(k_adamw32<Stream::KEPT>) : go(k_adamw8<Stream::KEPT>); break;
+    case Stream::STATES: a->state_bits == 32 ? go(k_adamw32<Stream::STATES>) : go(k_adamw8<Stream::STATES>); break;
+    case Stream::ALL: a->state_bits == 32 ? go(k_adamw32<Stream::ALL>) : go(k_adamw8<Stream::ALL>); break;
+  }
   DM_HIP(hipGetLastError());
   return DM_OK;
 }
