@@ -61,6 +61,10 @@ template <int A, bool PAST, typename V, typename P> DM_DEV void store(P* p, cons
   if constexpr (PAST) __builtin_nontemporal_store(v, q);
   else *q = v;
 }
+DM_DEV u32x4 pack8(const float* v) {
+  const uint4 r = pack16<bf16>(v);
+  return u32x4{r.x, r.y, r.z, r.w};
+}
 // Four gradients from i on. Parameters and gradients may be views at any element of a buffer: their vectors are aligned
 // to their elements only.
 template <bool BF16, bool PAST> DM_DEV floatx4 grads4(const PlanTensor& t, long i) {
@@ -358,22 +362,33 @@ template <Stream S> __global__ __launch_bounds__(256) void k_adamw8(AdamArgs a) 
   else step8<false, S>(a, c, t, i0);
 }
 
-// Sixteen codes per lane.
-template <typename F> __global__ __launch_bounds__(256) void k_adamw_values(const uint8_t* codes, const uint8_t* exps, long n_blocks, bf16* out) {
+// Eight codes per lane: the numbers of a wave's store follow one another.
+template <typename F, bool PAST> __global__ __launch_bounds__(256) void k_adamw_values(const uint8_t* codes, const uint8_t* exps, long n_blocks, bf16* out) {
   constexpr bool SIGNED = F::BIAS == First::BIAS;
-  const long n = n_blocks * (BLOCK / 16);
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) {
-    const u32x4 c = ld_global<u32x4>(codes + 16 * i);
-    const int e = exps[i / (BLOCK / 16)];
-    float v[16];
+  constexpr int N = 4;   // vectors in flight
+  const long n = n_blocks * (BLOCK / 8), step = gridDim.x * 256L;
+  for (long i0 = blockIdx.x * 256L + threadIdx.x; i0 < n; i0 += N * step) {
+    u32x2 c[N];
+    int e[N];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t q = c[j / 4] >> 8 * (j % 4) & 255;
-      v[j] = decoded<F>(SIGNED ? q & 127 : q, e);
-      if (SIGNED && q & 128) v[j] = -v[j];
-      if (e == 255) v[j] = __builtin_nanf("");
+    for (int k = 0; k < N; ++k) {
+      const long i = min(i0 + k * step, n - 1);
+      c[k] = load<u32x2, 8, PAST>(codes + 8 * i);
+      e[k] = exps[i / (BLOCK / 8)];
     }
-    store_vec<bf16, 16>(out + 16 * i, v);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (i0 + k * step >= n) return;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t q = c[k][j / 4] >> 8 * (j % 4) & 255;
+        v[j] = decoded<F>(SIGNED ? q & 127 : q, e[k]);
+        if (SIGNED && q & 128) v[j] = -v[j];
+        if (e[k] == 255) v[j] = __builtin_nanf("");
+      }
+      store<16, PAST>(out + 8 * (i0 + k * step), pack8(v));
+    }
   }
 }
 
@@ -496,9 +511,12 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
   DM_REQUIRE(n_blocks >= 0 && n_blocks < (1L << 40), DM_ERR_INVALID, "n_blocks=%lld", (long long)n_blocks);
   if (n_blocks == 0) return DM_OK;
   DM_REQUIRE(codes && exponents && out && aligned16(codes) && aligned16(out), DM_ERR_INVALID, "null or unaligned operand");
-  const dim3 grid((unsigned)std::min<long>((n_blocks + 15) / 16, 1 << 16));
-  if (second) hipLaunchKernelGGL(k_adamw_values<Second>, grid, dim3(256), 0, S(stream), codes, exponents, (long)n_blocks, (bf16*)out);
-  else hipLaunchKernelGGL(k_adamw_values<First>, grid, dim3(256), 0, S(stream), codes, exponents, (long)n_blocks, (bf16*)out);
+  const dim3 grid((unsigned)std::min<long>((n_blocks + 31) / 32, 1 << 16));
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, S(stream), codes, exponents, (long)n_blocks, (bf16*)out);
+  };
+  if (n_blocks * BLOCK * 3. > CACHE_BYTES) second ? go(k_adamw_values<Second, true>) : go(k_adamw_values<First, true>);
+  else second ? go(k_adamw_values<Second, false>) : go(k_adamw_values<First, false>);
   DM_HIP(hipGetLastError());
   return DM_OK;
 }
