@@ -60,7 +60,7 @@ def test_weighted_step_matches_oracle(dtype, tol, coef, wavefront):
     m, sd = _model(cfg, dtype)
     tr = HipTrunk(m, B, T, schedule=SCHED, loss_chunk=48, objective="weighted", entropy_coef=coef, wavefront=wavefront)
     idx, tg = _batch(cfg, B, T)
-    w = _weights()
+    w = _weights() if dtype == torch.float32 else 0.5 + _weights().abs()   # bf16: no cancellation between tokens
     tr.train_step(idx.to(DEV), tg.to(DEV), w.to(DEV))
     torch.cuda.synchronize()
     loss, grads, logp, ent = _weighted(cfg, sd, idx, tg, w, coef)
