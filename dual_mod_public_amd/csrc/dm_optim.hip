@@ -272,7 +272,7 @@ struct Second {
   static constexpr int BIAS = 30;
 };
 template <typename F> DM_DEV float decoded(uint32_t code, int e) { return ldexpf(__uint_as_float(code << 20), e - F::BIAS); }
-// x >= 0 rounded by the 20 random bits r20
+// x >= 0 rounded by the 20 random bits r20 (in the smallest binade after fp32's own rounding, to 2^-20 of a code)
 template <typename F> DM_DEV uint32_t encoded(float x, int e, uint32_t r20) {
   return (__float_as_uint(ldexpf(x, F::BIAS - e)) + r20) >> 20;
 }

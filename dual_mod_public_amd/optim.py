@@ -33,10 +33,11 @@ class AdamW:
 
     def __init__(self, params, grads=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_norm=None,
                  skip_nonfinite=False, state_bits=32, seed=0):
-        groups = [g if isinstance(g, dict) else {"params": [g]} for g in params]
+        groups = [dict(g) if isinstance(g, dict) else {"params": g} for g in params]
         for g in groups:
-            if unknown := set(g) - {"params", "weight_decay", "lr_scale"}:
-                raise ValueError(f"parameter group with {sorted(unknown)}")
+            if "params" not in g or set(g) - {"params", "weight_decay", "lr_scale"}:
+                raise ValueError(f"parameter group of {sorted(g)}")
+            g["params"] = [g["params"]] if torch.is_tensor(g["params"]) else list(g["params"])
         self.params = [p for g in groups for p in g["params"]]
         self._decay = [float(g.get("weight_decay", weight_decay)) for g in groups for _ in g["params"]]
         self._scale = [float(g.get("lr_scale", 1.0)) for g in groups for _ in g["params"]]

@@ -440,6 +440,9 @@ def test_refusals():
         with pytest.raises((ValueError, NotImplementedError)):
             f()
             pytest.fail(f"call {i} was not refused")
+    # a group's parameters may be an iterator or one tensor
+    opt = AdamW([dict(params=(t for t in (p[:3], p[3:])), weight_decay=0.5), dict(params=torch.zeros(4, device=DEV))])
+    assert len(opt.params) == 3 and opt._decay == [0.5, 0.5, 0.01] and opt._scale == [1.0] * 3
     q = torch.zeros(10, device=DEV)
     AdamW([p[:5], p[5:]], grads=[q[:5], q[:5]])       # neighbours are not overlaps, and gradients may be shared
     both = torch.zeros(20, device=DEV)
