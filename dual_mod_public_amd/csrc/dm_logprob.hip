@@ -628,6 +628,37 @@ template <typename T> void run_bwd(const LpArgs<T>& a, hipStream_t s) {
 
 bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// whether what a call writes lies in anything else that it reads or writes (dlogits in the logits' place aside)
+bool outputs_overlap(const dm_logprob_args* a, bool bwd) {
+  typedef unsigned __int128 wide;
+  struct Range {
+    const void* p;
+    wide bytes;
+  };
+  const wide n = a->rows, e = esz(a->dtype);
+  const bool in_place = a->dlogits == a->logits && a->ld_d == a->ld;
+  const Range out[] = {{in_place ? nullptr : a->dlogits, ((n - 1) * a->ld_d + a->cols) * e}, {bwd ? nullptr : a->logp, n * 4},
+                       {bwd ? nullptr : a->lse, n * 4}, {bwd ? nullptr : a->entropy, n * 4}, {bwd ? nullptr : a->stats, n * 12},
+                       {bwd || !a->top ? nullptr : a->top_logp, n * a->top * 4}, {bwd || !a->top ? nullptr : a->top_ids, n * a->top * 8}};
+  const Range in[] = {{a->logits, ((n - 1) * a->ld + a->cols) * e}, {a->target, n * 8}, {a->dlogits ? a->g_logp : nullptr, n * 4},
+                      {a->dlogits ? a->g_entropy : nullptr, n * 4}, {bwd ? a->stats : nullptr, n * 12}};
+  auto meet = [](const Range& r, const Range& s) {
+    const wide p = reinterpret_cast<uintptr_t>(r.p), q = reinterpret_cast<uintptr_t>(s.p);
+    return p && q && p < q + s.bytes && q < p + r.bytes;
+  };
+  for (const Range& r : out) {
+    for (const Range& s : in)
+      if (meet(r, s)) return true;
+    for (const Range& s : out)
+      if (&s != &r && meet(r, s)) return true;
+  }
+  // written over the logits, the gradient meets the other inputs and outputs where the logits do
+  if (in_place)
+    for (const Range& s : in)
+      if (&s != in && meet(in[0], s)) return true;
+  return false;
+}
+
 // what both entry points ask of their arguments
 int check_logprob(const dm_logprob_args* a, bool bwd) {
   DM_REQUIRE(a != nullptr, DM_ERR_INVALID, "null arguments");
@@ -642,17 +673,15 @@ int check_logprob(const dm_logprob_args* a, bool bwd) {
     DM_REQUIRE(a->top >= 0 && a->top <= DM_TOP_MAX && a->top <= a->cols, DM_ERR_INVALID, "top=%d of cols=%d (at most %d)",
                a->top, a->cols, DM_TOP_MAX);
     DM_REQUIRE(a->top == 0 || (a->top_logp && a->top_ids), DM_ERR_INVALID, "null output of the most likely tokens");
-    if (!a->dlogits) return DM_OK;
   }
-  DM_REQUIRE(a->dlogits && aligned_to(a->dlogits, e) && a->ld_d >= a->cols, DM_ERR_INVALID, "null or unaligned dlogits, ld_d=%lld",
-             (long long)a->ld_d);
-  DM_REQUIRE(a->g_logp || a->g_entropy, DM_ERR_INVALID, "a gradient without coefficients");
-  DM_REQUIRE(!a->g_logp || a->target, DM_ERR_INVALID, "g_logp without targets");
-  DM_REQUIRE(!bwd || a->stats, DM_ERR_INVALID, "the forward's stats are needed");
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a->logits), d = reinterpret_cast<uintptr_t>(a->dlogits);
-  typedef unsigned __int128 wide;
-  const wide xe = ((wide)(a->rows - 1) * a->ld + a->cols) * e, de = ((wide)(a->rows - 1) * a->ld_d + a->cols) * e;
-  DM_REQUIRE((x == d && a->ld == a->ld_d) || x + xe <= d || d + de <= x, DM_ERR_INVALID, "dlogits overlaps the logits in part");
+  if (bwd || a->dlogits) {
+    DM_REQUIRE(a->dlogits && aligned_to(a->dlogits, e) && a->ld_d >= a->cols, DM_ERR_INVALID, "null or unaligned dlogits, ld_d=%lld",
+               (long long)a->ld_d);
+    DM_REQUIRE(a->g_logp || a->g_entropy, DM_ERR_INVALID, "a gradient without coefficients");
+    DM_REQUIRE(!a->g_logp || a->target, DM_ERR_INVALID, "g_logp without targets");
+    DM_REQUIRE(!bwd || a->stats, DM_ERR_INVALID, "the forward's stats are needed");
+  }
+  DM_REQUIRE(!outputs_overlap(a, bwd), DM_ERR_INVALID, "an output overlaps an input or another output");
   return DM_OK;
 }
 

@@ -20,7 +20,7 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from .decode import StaticTape
-from .logprobs import row_logprobs
+from .logprobs import RowLogprobs, row_logprobs
 
 
 class GraphDecoder:
@@ -52,6 +52,7 @@ class GraphDecoder:
             self.logp, self.entropy = (torch.zeros(B, 1, device=self.dev) for _ in range(2))
             self.top_logp = torch.zeros(B, 1, top, device=self.dev)
             self.top_ids = torch.zeros(B, 1, top, dtype=torch.long, device=self.dev)
+            self._lp = RowLogprobs(self.logp, self.entropy, None, None, *((self.top_logp, self.top_ids) if top else (None, None)))
         self.cos = model.rope_cos.to(self.dev, torch.float32).contiguous()
         self.sin = model.rope_sin.to(self.dev, torch.float32).contiguous()
         # compute-dtype weight copies at fixed addresses (the autocast casts, done once per version)
@@ -101,12 +102,7 @@ class GraphDecoder:
         L.check(L.lib().dm_argmax_rows(L.dtype_code(self.dt), L.ptr(lg), B, self.vocab, self.vocab,
                                        L.ptr(self.next), L.stream_ptr()))
         if self.top is not None:
-            r = row_logprobs(lg, self.next, top=self.top)
-            self.logp.copy_(r.logp)
-            self.entropy.copy_(r.entropy)
-            if self.top:
-                self.top_logp.copy_(r.top_logp)
-                self.top_ids.copy_(r.top_ids)
+            row_logprobs(lg, self.next, top=self.top, out=self._lp)
         self.pos += 1
 
     def _run_step(self):

@@ -66,6 +66,9 @@ def _per_row(t, logits, what, dtype):
 def _logits(logits):
     if not logits.is_cuda or logits.dim() < 1:
         raise ValueError(f"logits: shape {tuple(logits.shape)} on {logits.device}; rows [..., V] on a GPU are needed")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("row_logprobs and its like keep no autograd graph: token_logprobs does, or call them under "
+                                  "torch.no_grad() or on logits.detach()")
     return _rows(logits, "logits")
 
 
@@ -84,38 +87,60 @@ def _gradient(logits, targets, g_logp, g_entropy, dlogits):
                      dlogits.data_ptr(), _rows(dlogits, "dlogits")[1])
 
 
-def _forward(logits, targets, top, rows, ld, gradient=(None, None, None, 0)):
-    V, dev, lead = logits.shape[-1], logits.device, logits.shape[:-1]
+def _outputs(logits, targets, top):
+    lead, dev = logits.shape[:-1], logits.device
+    return RowLogprobs(
+        None if targets is None else torch.empty(lead, device=dev, dtype=torch.float32),
+        torch.empty(lead, device=dev, dtype=torch.float32),
+        torch.empty(lead, device=dev, dtype=torch.float32),
+        torch.empty((*lead, 3), device=dev, dtype=torch.float32),
+        torch.empty((*lead, top), device=dev, dtype=torch.float32) if top else None,
+        torch.empty((*lead, top), device=dev, dtype=torch.int64) if top else None)
+
+
+def _check_outputs(out, logits, targets, top):
+    lead = tuple(logits.shape[:-1])
+    if out.logp is not None and targets is None:
+        raise ValueError("out.logp without targets")
+    if (out.top_logp is None or out.top_ids is None) if top else (out.top_logp is not None or out.top_ids is not None):
+        raise ValueError(f"out.top_logp and out.top_ids belong to top > 0, both of them (top={top})")
+    for name, t, last in zip(RowLogprobs._fields, out, ((), (), (), (3,), (top,), (top,))):
+        dtype = torch.int64 if name == "top_ids" else torch.float32
+        if t is not None and (t.shape != lead + last or t.dtype != dtype or t.device != logits.device or not t.is_contiguous()):
+            raise ValueError(f"out.{name}: {t.dtype} {tuple(t.shape)} on {t.device}; contiguous {dtype} {lead + last} on {logits.device}")
+
+
+def _forward(logits, targets, top, out, rows, ld, gradient=(None, None, None, 0)):
+    V = logits.shape[-1]
     if not 0 <= top <= min(L.DM_TOP_MAX, V):
         raise ValueError(f"top={top} of {V} columns (at most {L.DM_TOP_MAX})")
     t = _per_row(targets, logits, "targets", torch.int64)
-    logp = None if targets is None else torch.empty(lead, device=dev, dtype=torch.float32)
-    entropy = torch.empty(lead, device=dev, dtype=torch.float32)
-    lse = torch.empty(lead, device=dev, dtype=torch.float32)
-    stats = torch.empty((*lead, 3), device=dev, dtype=torch.float32)
-    top_logp = top_ids = None
-    if top:
-        top_logp = torch.empty((*lead, top), device=dev, dtype=torch.float32)
-        top_ids = torch.empty((*lead, top), device=dev, dtype=torch.int64)
-    a = L.dm_logprob_args(L.dtype_code(logits.dtype), rows, V, top, logits.data_ptr(), ld, t, L.ptr(logp), lse.data_ptr(),
-                          entropy.data_ptr(), stats.data_ptr(), L.ptr(top_logp), L.ptr(top_ids), *gradient)
-    L.call_on(dev, L.lib().dm_logprob_rows, L.byref(a))
-    return RowLogprobs(logp, entropy, lse, stats, top_logp, top_ids)
+    if out is None:
+        out = _outputs(logits, targets, top)
+    else:
+        _check_outputs(out, logits, targets, top)
+    logp, entropy, lse, stats, top_logp, top_ids = out
+    a = L.dm_logprob_args(L.dtype_code(logits.dtype), rows, V, top, logits.data_ptr(), ld, t, L.ptr(logp), L.ptr(lse), L.ptr(entropy),
+                          L.ptr(stats), L.ptr(top_logp), L.ptr(top_ids), *gradient)
+    L.call_on(logits.device, L.lib().dm_logprob_rows, L.byref(a))
+    return out
 
 
-def row_logprobs(logits, targets=None, top=0):
+def row_logprobs(logits, targets=None, top=0, out=None):
     """The values of logits [..., V]: logp of ``targets`` (int64 [...], optional), entropy, lse and the ``top`` most
-    likely tokens of each row (at most 32). No gradient."""
-    return _forward(logits, targets, top, *_logits(logits))
+    likely tokens of each row (at most 32). No autograd graph: logits that would need one are refused. out: a RowLogprobs
+    of tensors to write into (static buffers of a decode loop), apart from each other and the inputs; a field that is None
+    is left out."""
+    return _forward(logits, targets, top, out, *_logits(logits))
 
 
-def row_logprobs_grad(logits, targets, g_logp, g_entropy=None, top=0, dlogits=None):
+def row_logprobs_grad(logits, targets, g_logp, g_entropy=None, top=0, dlogits=None, out=None):
     """row_logprobs, and the gradient of sum(g_logp logp + g_entropy entropy) to the logits (fp32 coefficients [...],
     either may be None) in the same pass: (RowLogprobs, dlogits). dlogits: a tensor for the gradient, the logits
     themselves too (in place); by default a new one."""
     rows, ld = _logits(logits)
     dlogits, gradient = _gradient(logits, targets, g_logp, g_entropy, dlogits)
-    return _forward(logits, targets, top, rows, ld, gradient), dlogits
+    return _forward(logits, targets, top, out, rows, ld, gradient), dlogits
 
 
 def row_logprobs_bwd(logits, targets, stats, g_logp, g_entropy=None, dlogits=None):

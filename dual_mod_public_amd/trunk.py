@@ -360,9 +360,8 @@ class HipTrunk:
             hf, r = _rms(xc, m.norm_f.weight, m.norm_f.eps)
             dl = hf @ self.w_emb.t()   # the logits, then their gradient
             if weighted:
-                v, _ = row_logprobs_grad(dl, t, g_logp[r0:r1], None if g_entropy is None else g_entropy[r0:r1], dlogits=dl)
-                logp[r0:r1].copy_(v.logp)
-                entropy[r0:r1].copy_(v.entropy)
+                row_logprobs_grad(dl, t, g_logp[r0:r1], None if g_entropy is None else g_entropy[r0:r1], dlogits=dl,
+                                  out=RowLogprobs(logp[r0:r1], entropy[r0:r1], None, None, None, None))
             else:
                 L.ce_rows(dl, t, nvalid, loss[r0:r1])
             gw.add_(_mm32(dl.t(), hf))

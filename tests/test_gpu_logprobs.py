@@ -382,6 +382,26 @@ def test_streams_and_graph(M, V):
         assert all(torch.equal(a, b) for a, b in zip(r, want[0]))
 
 
+def test_given_outputs():
+    """out=: the given tensors hold what new ones would, the fields left out nothing; wrong ones are refused."""
+    x, t, g, _ = rows_of(6, 333, torch.bfloat16)
+    w = torch.randn(6, generator=g, device=DEV)
+    want = lp.row_logprobs(x, t, top=4)
+    out = lp.RowLogprobs(*[torch.zeros_like(v) for v in want])
+    assert lp.row_logprobs(x, t, top=4, out=out) is out and all(torch.equal(a, b) for a, b in zip(out, want))
+    few = lp.RowLogprobs(None, torch.zeros(6, device=DEV), None, None, None, None)
+    _, dx = lp.row_logprobs_grad(x, t, w, out=few)
+    assert torch.equal(few.entropy, want.entropy) and torch.equal(dx, lp.row_logprobs_grad(x, t, w)[1])
+    none = few._replace(entropy=None)
+    assert torch.equal(lp.row_logprobs_grad(x, t, w, out=none)[1], dx)
+    for bad, top in ((out, 0), (out, 3), (few, 2), (few._replace(top_ids=out.top_ids), 4), (few._replace(lse=w[:5]), 0),
+                     (few._replace(lse=w.double()), 0), (few._replace(lse=w.cpu()), 0), (few._replace(stats=out.stats[:, :2]), 0)):
+        with pytest.raises(ValueError, match="out"):
+            lp.row_logprobs(x, t, top=top, out=bad)
+    with pytest.raises(ValueError, match="out.logp"):
+        lp.row_logprobs(x, None, out=few._replace(logp=w))
+
+
 def test_no_rows():
     x = torch.zeros(0, 10, device=DEV)
     t = torch.zeros(0, dtype=torch.int64, device=DEV)
@@ -409,6 +429,12 @@ def test_refusals():
         with pytest.raises((ValueError, NotImplementedError)):
             f()
             pytest.fail(f"call {i} was not refused")
+    leaf = x.clone().requires_grad_()
+    for f in (lambda: lp.row_logprobs(leaf, t), lambda: lp.row_logprobs_grad(leaf, t, w, dlogits=leaf)):
+        with pytest.raises(NotImplementedError, match="token_logprobs"):
+            f()
+    with torch.no_grad():
+        assert not lp.row_logprobs(leaf, t).logp.requires_grad
     wide = torch.zeros(4, 200, device=DEV)
     with pytest.raises(L.DMError, match="overlaps"):
         lp.row_logprobs_grad(wide[:, :100], t, w, dlogits=wide[:, 50:150])

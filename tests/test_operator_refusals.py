@@ -25,13 +25,21 @@ def rows_args(**kw):
                                 dict(dlogits=0x40001, ld_d=10, g_logp=0x50000),
                                 dict(dlogits=0x10004, ld_d=10, g_logp=0x50000), dict(dlogits=0x10000, ld_d=11, g_logp=0x50000),
                                 dict(dlogits=0x10000 - 40, ld_d=10, g_logp=0x50000),
-                                dict(target=None, logp=None, dlogits=0x40000, ld_d=10, g_logp=0x50000)])
+                                dict(target=None, logp=None, dlogits=0x40000, ld_d=10, g_logp=0x50000),
+                                # outputs over inputs and over each other (rows take 160 bytes, targets 32, values 16, stats 48)
+                                dict(lse=0x10000 + 156), dict(logp=0x20000 - 12), dict(stats=0x20000 + 28), dict(entropy=0x30000 + 12),
+                                dict(stats=0x30100 - 44), dict(top=2, top_logp=0x60000, top_ids=0x60000 + 28),
+                                dict(top=2, top_ids=0x60000, top_logp=0x10000 - 28),
+                                dict(dlogits=0x10000, ld_d=10, g_logp=0x10000 + 80), dict(dlogits=0x40000, ld_d=10, g_logp=0x40000 + 156),
+                                dict(dlogits=0x20000 + 28, ld_d=10, g_entropy=0x50000),
+                                dict(dlogits=0x40000, ld_d=10, g_logp=0x30000)])
 def test_logprob_rows_refuses(kw):
     lib = L.load()
     assert lib.dm_logprob_rows(L.byref(rows_args(**kw)), None) == -1 and lib.dm_last_error()
 
 
-@pytest.mark.parametrize("kw", [dict(dlogits=None), dict(stats=None), dict(g_logp=None)])
+@pytest.mark.parametrize("kw", [dict(dlogits=None), dict(stats=None), dict(g_logp=None), dict(stats=0x40000 + 156),
+                                dict(dlogits=0x10000, stats=0x10000 - 44)])
 def test_logprob_bwd_refuses(kw):
     a = rows_args(**dict(dict(dlogits=0x40000, ld_d=10, g_logp=0x50000), **kw))
     assert L.load().dm_logprob_rows_bwd(L.byref(a), None) == -1
@@ -114,6 +122,6 @@ def test_python_refuses_cpu_tensors_and_bad_settings():
     for f in (lambda: lp.row_logprobs(x, t), lambda: lp.token_logprobs(x, t), lambda: lp.row_logprobs_grad(x, t, torch.ones(2)),
               lambda: AdamW([x]), lambda: AdamW([]), lambda: AdamW([x], state_bits=16), lambda: AdamW([x], betas=(1.0, 0.9)),
               lambda: AdamW([x], eps=0.0), lambda: AdamW([x], max_norm=0.0), lambda: AdamW([x], max_norm=float("nan")),
-              lambda: AdamW([dict(params=[x], lr=1.0)]), lambda: AdamW([x], grads=[])):
+              lambda: AdamW([dict(params=[x], lr=1.0)]), lambda: AdamW([dict(weight_decay=0.1)]), lambda: AdamW([x], grads=[])):
         with pytest.raises(ValueError):
             f()
