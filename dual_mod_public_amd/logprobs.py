@@ -83,6 +83,8 @@ def _gradient(logits, targets, g_logp, g_entropy, dlogits):
     elif dlogits.shape != logits.shape or dlogits.dtype != logits.dtype or dlogits.device != logits.device:
         raise ValueError(f"dlogits: {dlogits.dtype} {tuple(dlogits.shape)} on {dlogits.device} for logits {logits.dtype} "
                          f"{tuple(logits.shape)} on {logits.device}")
+    else:   # what torch saved of it is no longer there
+        torch.autograd.graph.increment_version(dlogits)
     return dlogits, (_per_row(g_logp, logits, "g_logp", torch.float32), _per_row(g_entropy, logits, "g_entropy", torch.float32),
                      dlogits.data_ptr(), _rows(dlogits, "dlogits")[1])
 
@@ -119,6 +121,7 @@ def _forward(logits, targets, top, out, rows, ld, gradient=(None, None, None, 0)
         out = _outputs(logits, targets, top)
     else:
         _check_outputs(out, logits, targets, top)
+        torch.autograd.graph.increment_version([o for o in out if o is not None])
     logp, entropy, lse, stats, top_logp, top_ids = out
     a = L.dm_logprob_args(L.dtype_code(logits.dtype), rows, V, top, logits.data_ptr(), ld, t, L.ptr(logp), L.ptr(lse), L.ptr(entropy),
                           L.ptr(stats), L.ptr(top_logp), L.ptr(top_ids), *gradient)

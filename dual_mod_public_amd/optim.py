@@ -88,7 +88,7 @@ class AdamW:
         self.skipped = torch.zeros((), dtype=torch.int32, **kw)      # steps left out by skip_nonfinite
         self._ws = torch.empty(L.DM_ADAMW_WORKSPACE, dtype=torch.uint8, **kw)
         self._key = self._plan = self._a = None
-        self._in_graphs = []    # plans that captured steps read
+        self._in_graphs, self._graphs_hold = [], []    # plans that captured steps read, and what they write
         torch.cuda.current_stream(self.device).synchronize()   # the buffers are ready on every stream
 
     def _check_grad(self, i, p, g):
@@ -100,11 +100,14 @@ class AdamW:
         """dm_adamw_args of a step now; the plan is written again where a tensor has moved."""
         grads = self.grads if self.grads is not None else [p.grad for p in self.params]
         key = [None if t is None else t.data_ptr() for t in chain(self.params, grads)]
+        if self.grads is None:   # a new .grad may have an old one's address
+            key += [None if g is None else (g.dtype, g.is_contiguous()) for g in grads]
         if key != self._key:
             self._write_plan(grads)
             self._key = key
         if torch.cuda.is_current_stream_capturing() and not any(self._plan is t for t in self._in_graphs):
             self._in_graphs.append(self._plan)
+            self._graphs_hold.append(self._held)
         return self._a
 
     def _write_plan(self, grads):

@@ -402,6 +402,21 @@ def test_given_outputs():
         lp.row_logprobs(x, None, out=few._replace(logp=w))
 
 
+def test_written_tensors_are_known_to_autograd():
+    """A graph that saved the logits refuses to use them after a gradient in their place."""
+    x, t, g, _ = rows_of(4, 50, torch.float32)
+    w = torch.randn(4, generator=g, device=DEV)
+    leaf = x.clone().requires_grad_()
+    z = leaf * 1.0
+    loss, kept = z.square().sum(), z.detach()
+    out = lp.RowLogprobs(None, w.clone(), None, None, None, None)
+    versions = z._version, out.entropy._version
+    lp.row_logprobs_grad(kept, t, w, dlogits=kept, out=out)
+    assert z._version > versions[0] and out.entropy._version > versions[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_no_rows():
     x = torch.zeros(0, 10, device=DEV)
     t = torch.zeros(0, dtype=torch.int64, device=DEV)

@@ -349,6 +349,41 @@ def test_captured_step(bits):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_grad_of_another_order_at_an_old_address():
+    """A .grad that is new in the place of an old one is looked at again: strides that are not rows are refused."""
+    p = torch.nn.Parameter(torch.ones(8, 8, device=DEV))
+    p.grad = torch.arange(64.0, device=DEV).view(8, 8)
+    opt = AdamW([p], lr=0.5, weight_decay=0.0)
+    opt.step()
+    before = p.detach().clone()
+    p.grad = p.grad.t()
+    with pytest.raises(ValueError, match="gradient 0"):
+        opt.step()
+    assert torch.equal(p.detach(), before)
+    p.grad = p.grad.t()
+    opt.step()
+    assert not torch.equal(p.detach(), before) and int(opt.steps) == 2
+
+
+def test_old_graph_after_parameters_moved():
+    """A captured step keeps writing the storage that it was captured with, which stays allocated."""
+    p = torch.nn.Parameter(torch.ones(1000, device=DEV))
+    opt = AdamW([p], grads=[torch.ones(1000, device=DEV)], lr=0.5, weight_decay=0.0)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    old = p.data_ptr()
+    p.data = p.data.clone()
+    opt.step()
+    others = [torch.zeros(1000, device=DEV) for _ in range(64)]
+    assert old not in [t.data_ptr() for t in others]
+    kept = p.detach().clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p.detach(), kept) and not any(bool(t.any()) for t in others)
+
+
 def test_capture_needs_a_plan():
     p = torch.nn.Parameter(torch.ones(10, device=DEV))
     opt = AdamW([p])
