@@ -72,6 +72,7 @@ class AdamW:
 
         # flat states: tensor i's elements from block ``_block0[i]`` on
         self._block0, n = [], 0
+        self._sizes = [p.numel() for p in self.params]
         for p in self.params:
             self._block0.append(n)
             n += -(-p.numel() // L.DM_ADAMW_BLOCK)
@@ -101,7 +102,7 @@ class AdamW:
         grads = self.grads if self.grads is not None else [p.grad for p in self.params]
         key = [None if t is None else t.data_ptr() for t in chain(self.params, grads)]
         if self.grads is None:   # a new .grad may have an old one's address
-            key += [None if g is None else (g.dtype, g.is_contiguous()) for g in grads]
+            key += [None if g is None else (g.dtype, g.is_contiguous(), g.numel()) for g in grads]
         if key != self._key:
             self._write_plan(grads)
             self._key = key
@@ -116,6 +117,8 @@ class AdamW:
         self._key = None
         rows = []
         for i, (p, g) in enumerate(zip(self.params, grads)):
+            if p.numel() != self._sizes[i]:   # its states have their place between the others'
+                raise ValueError(f"parameter {i} now has {p.numel()} elements; its states were made for {self._sizes[i]}")
             if g is None or p.numel() == 0:
                 continue
             self._check_grad(i, p, g)
