@@ -9,8 +9,9 @@ global gradient norm.
 Parameters are the framework's fp32 masters. Gradients are fixed buffers given once (``grads``: fp32 or bf16, as
 HipTrunk's views of its flat buffer) or, without them, the parameters' ``.grad`` at each step. Everything a step
 changes beside the parameters lives on the device (``lr``, ``steps``, ``norm``, ``skipped``), so a step can be captured
-into a HIP graph and replayed. A replay does not tell torch that the parameters changed: call ``mark_updated()`` after
-it where something watches their versions (GraphDecoder, SwiGLU.decode).
+into a HIP graph and replayed. A replay works on the parameters and gradients that the step was captured with, which the
+optimizer keeps allocated from then on (keep the optimizer as long as the graph), and does not tell torch that the
+parameters changed: call ``mark_updated()`` after it where something watches their versions (GraphDecoder, SwiGLU.decode).
 
 8-bit states hold a byte per element and moment, and a byte per 256 elements and moment: blocks with a power-of-two
 scale, four significant bits per element, rounded stochastically by a hash of seed, step and element, so runs repeat
@@ -89,7 +90,7 @@ class AdamW:
         self.skipped = torch.zeros((), dtype=torch.int32, **kw)      # steps left out by skip_nonfinite
         self._ws = torch.empty(L.DM_ADAMW_WORKSPACE, dtype=torch.uint8, **kw)
         self._key = self._plan = self._a = None
-        self._in_graphs, self._graphs_hold = [], []    # plans that captured steps read, and what they write
+        self._in_graphs, self._graphs_hold = [], []    # plans that captured steps read, and what those read and write
         torch.cuda.current_stream(self.device).synchronize()   # the buffers are ready on every stream
 
     def _check_grad(self, i, p, g):
@@ -108,7 +109,7 @@ class AdamW:
             self._key = key
         if torch.cuda.is_current_stream_capturing() and not any(self._plan is t for t in self._in_graphs):
             self._in_graphs.append(self._plan)
-            self._graphs_hold.append(self._held)
+            self._graphs_hold.append((self._held, [g.detach() for g in grads if g is not None]))
         return self._a
 
     def _write_plan(self, grads):

@@ -59,3 +59,29 @@ def test_parameter_of_another_size(bits):
     a.grad = torch.ones(20, 15, device=DEV)
     opt.step()
     assert int(opt.steps) == 3
+
+
+def test_captured_gradients_stay():
+    """A captured step reads the gradients that it was captured with; they stay allocated when the parameters let go of
+    them."""
+    p, q = (torch.nn.Parameter(torch.zeros(n, device=DEV)) for n in (1000, 50))
+    opt = AdamW([p, q], lr=0.5, weight_decay=0.0, betas=(0.0, B2), max_norm=1e6)
+    p.grad, q.grad = torch.ones(1000, device=DEV), torch.ones(50, device=DEV)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        norm = opt.step()
+    held = {p.grad.data_ptr(), q.grad.data_ptr()}
+    p.grad = None
+    q.grad = None
+    others = [torch.full((n,), -7.0, device=DEV) for n in (1000, 50) for _ in range(64)]
+    assert not held & {t.data_ptr() for t in others}
+    graph.replay()
+    torch.cuda.synchronize()
+    assert abs(float(norm) - math.sqrt(1050)) <= 1e-5 * math.sqrt(1050)
+    # three steps against gradients of 1, the second captured but not run: two of them in all
+    assert (p + 1.0).abs().max() <= 1e-5 and (q + 1.0).abs().max() <= 1e-5
+    # a later plan's gradients are not kept by the graph's
+    p.grad, q.grad = torch.ones(1000, device=DEV), torch.ones(50, device=DEV)
+    opt.step()
+    assert int(opt.steps) == 3
