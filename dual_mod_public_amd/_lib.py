@@ -197,6 +197,7 @@ SIGNATURES = {
     "dm_adamw_plan_bytes": (ctypes.c_size_t, [P(dm_adamw_tensor), c_i32]),
     "dm_adamw_plan": (ctypes.c_int, [P(dm_adamw_tensor), c_i32, c_vp, ctypes.c_size_t, P(ctypes.c_int64)]),
     "dm_adamw_step": (ctypes.c_int, [P(dm_adamw_args), c_vp]),
+    "dm_adamw_step_counted": (ctypes.c_int, [P(dm_adamw_args), c_vp, c_vp]),
     "dm_grad_norm": (ctypes.c_int, [P(dm_adamw_args), c_vp]),
     "dm_adamw_values": (ctypes.c_int, [c_vp, c_vp, ctypes.c_int64, c_i32, c_vp, c_vp]),
     "dm_argmax_rows": (ctypes.c_int, [c_i32, c_vp, c_i32, c_i32, ctypes.c_int64, c_vp, c_vp]),

@@ -1,5 +1,5 @@
 // One AdamW step over many tensors, with 32-bit or 8-bit states, and the global gradient norm it clips by
-// (dm_adamw_step, dm_grad_norm).
+// (dm_adamw_step, dm_adamw_step_counted, dm_grad_norm).
 //
 // Three launches whatever the number of tensors: the sum of g^2 in NORM_PARTS parts (only where the norm is asked for),
 // one block that makes the step's scalars from them and from the step count, and the update, a block per chunk of a tensor;
@@ -28,18 +28,25 @@ struct PlanTensor {
   float weight_decay, lr_scale;
   int g_bf16, pad;
 };
+struct Rates {
+  float rate, v_scale;   // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
+};
 // what the step's kernels share: written by k_adamw_begin
 struct Control {
-  float coef, rate, v_scale, lr;   // c, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
-  uint32_t key;                    // the step's hash
+  float coef, lr;   // c
+  Rates all;        // of every tensor, where they have no step counts of their own
+  uint32_t key;     // the step's hash
   int skip;
 };
 static_assert(sizeof(Control) + 64 + NORM_PARTS * sizeof(double) <= DM_ADAMW_WORKSPACE, "workspace");
 struct Workspace {
   Control* c;
   double* part;
+  Rates* rates;   // per tensor, with step counts of their own
 };
-Workspace carve(void* base) { return {(Control*)base, (double*)((char*)base + 64)}; }
+Workspace carve(void* base) {
+  return {(Control*)base, (double*)((char*)base + 64), (Rates*)((char*)base + DM_ADAMW_WORKSPACE)};
+}
 
 struct AdamArgs {
   const PlanTensor* tensors;
@@ -48,6 +55,7 @@ struct AdamArgs {
   uint8_t *me, *ve;
   float b1, c1, b2, c2, eps;   // c = 1 - b
   const Control* c;
+  const Rates* rates;          // nullptr: Control's for all
 };
 
 DM_DEV float grad_at(const PlanTensor& t, long i) {
@@ -159,22 +167,40 @@ struct BeginArgs {
   int64_t* steps;
   float* norm;
   int* skipped;
+  const PlanTensor* tensors;
+  int n_tensors;
+  int64_t* tensor_steps;   // nullptr: all tensors' are *steps
+  Rates* rates;
 };
-// one block: the norm from its parts and the step's scalars
+DM_DEV Rates rates_at(const BeginArgs& a, int64_t t) {
+  const double power1 = exp2(t * a.log2_beta1), power2 = exp2(t * a.log2_beta2);
+  return {(float)(*a.lr / (1. - power1)), (float)(1. / sqrt(1. - power2))};
+}
+// one block: the norm from its parts and the step's scalars; a thread per tensor counts its steps and makes its rates
 __global__ __launch_bounds__(256) void k_adamw_begin(BeginArgs a) {
   __shared__ double red[4];
+  const bool step = a.steps != nullptr;   // else the norm alone
+  const int i = threadIdx.x;
+  int64_t t = step ? *a.steps + 1 : 0, ti = t;
+  long n = 0;
+  if (step && a.tensor_steps && i < a.n_tensors) n = a.tensors[i].n, ti = a.tensor_steps[i] + 1;
   double s = 0.;
-  for (int i = threadIdx.x; i < a.parts; i += 256) s += a.part[i];
-  const int64_t t = a.steps ? *a.steps + 1 : 0;
-  const double power1 = exp2(t * a.log2_beta1), power2 = exp2(t * a.log2_beta2);
+  for (int k = i; k < a.parts; k += 256) s += a.part[k];
+  const Rates r = step ? rates_at(a, ti) : Rates{};
   s = block_sum(s, red);
-  if (threadIdx.x > 0) return;
   const double norm = sqrt(s);
+  const bool skip = a.skip_nonfinite && !(norm < __builtin_inf());
+  if (step && !skip && a.tensor_steps) {
+    if (n > 0) a.tensor_steps[i] = ti, a.rates[i] = r;
+    for (int k = i + 256; k < a.n_tensors; k += 256)
+      if (a.tensors[k].n > 0) a.rates[k] = rates_at(a, a.tensor_steps[k] += 1);
+  }
+  if (i > 0) return;
   if (a.parts > 0 && a.norm) *a.norm = (float)norm;
-  if (!a.steps) return;   // the norm alone
+  if (!step) return;
   Control c{};
-  c.skip = a.skip_nonfinite && !(norm < __builtin_inf());
-  if (c.skip) {
+  c.skip = skip;
+  if (skip) {
     *a.skipped += 1;
     *a.c = c;
     return;
@@ -186,8 +212,7 @@ __global__ __launch_bounds__(256) void k_adamw_begin(BeginArgs a) {
     c.coef = k < 1. || k != k ? (float)k : 1.f;
   }
   c.lr = *a.lr;
-  c.rate = (float)(c.lr / (1. - power1));
-  c.v_scale = (float)(1. / sqrt(1. - power2));
+  c.all = r;
   c.key = mix(a.seed + (uint32_t)t * 0x9E3779B1u);
   *a.c = c;
 }
@@ -203,8 +228,8 @@ DM_DEV void moments(const AdamArgs& a, float b1, float b2, float g, float& m, fl
 // The parameters' part of a step, per tensor.
 struct Update {
   float keep, rate, v_scale, eps;
-  DM_DEV Update(const AdamArgs& a, const Control& c, const PlanTensor& t)
-      : keep((float)(1. - (double)c.lr * t.lr_scale * t.weight_decay)), rate(c.rate * t.lr_scale), v_scale(c.v_scale), eps(a.eps) {}
+  DM_DEV Update(const AdamArgs& a, const Control& c, const Rates& r, const PlanTensor& t)
+      : keep((float)(1. - (double)c.lr * t.lr_scale * t.weight_decay)), rate(r.rate * t.lr_scale), v_scale(r.v_scale), eps(a.eps) {}
   DM_DEV float of(float p, float m, float v) const {   // a square root and a reciprocal of one ulp each
     const float denom = fmaf(__builtin_amdgcn_sqrtf(v), v_scale, eps);
     return p * keep - rate * (m * __builtin_amdgcn_rcpf(denom));
@@ -212,8 +237,7 @@ struct Update {
 };
 
 // A block per chunk; bound by its 28 bytes per element (543M: 15.2 GB in 2.6 ms).
-template <bool BF16, Stream S> DM_DEV void step32(const AdamArgs& a, const Control& c, const PlanTensor& t, long i0, float* ms, float* vs) {
-  const Update u(a, c, t);
+template <bool BF16, Stream S> DM_DEV void step32(const AdamArgs& a, const Control& c, const Update& u, const PlanTensor& t, long i0, float* ms, float* vs) {
   constexpr int STEP = 256 * 4, N = CHUNK / STEP;
   constexpr bool PAST = S != Stream::KEPT;
   if (i0 + CHUNK <= t.n) {
@@ -255,12 +279,14 @@ template <bool BF16, Stream S> DM_DEV void step32(const AdamArgs& a, const Contr
 template <Stream S> __global__ __launch_bounds__(256) void k_adamw32(AdamArgs a) {
   const Control c = *a.c;
   if (c.skip) return;
-  const PlanTensor t = a.tensors[a.chunk_tensor[blockIdx.x]];
+  const int ti = a.chunk_tensor[blockIdx.x];
+  const PlanTensor t = a.tensors[ti];
+  const Update u(a, c, a.rates ? a.rates[ti] : c.all, t);
   const long i0 = (blockIdx.x - t.chunk0) * CHUNK;
   float* ms = (float*)a.m + t.block0 * BLOCK;
   float* vs = (float*)a.v + t.block0 * BLOCK;
-  if (t.g_bf16) step32<true, S>(a, c, t, i0, ms, vs);
-  else step32<false, S>(a, c, t, i0, ms, vs);
+  if (t.g_bf16) step32<true, S>(a, c, u, t, i0, ms, vs);
+  else step32<false, S>(a, c, u, t, i0, ms, vs);
 }
 
 // The two code formats. Shifted to the place of an fp32 number's exponent and upper mantissa bits, a code is one, its
@@ -286,10 +312,9 @@ DM_DEV bool too_large(float x) { return !(fabsf(x) < 0x1p127f); }
 // A wave per run of four 256-element blocks, four elements per lane and block: a block's largest magnitude is a wave's
 // reduction, its codes 4 bytes per lane. Bound by its 16 bytes per element (543M: 8.7 GB in 1.46 ms); the 85 vector
 // instructions per element, a hash of two quarter-rate products among them, run beside the streams.
-template <bool BF16, Stream S> DM_DEV void step8(const AdamArgs& a, const Control& c, const PlanTensor& t, long i0) {
+template <bool BF16, Stream S> DM_DEV void step8(const AdamArgs& a, const Control& c, const Update& u, const PlanTensor& t, long i0) {
   constexpr int N = CHUNK / BLOCK / 4;
   constexpr bool PAST = S != Stream::KEPT;
-  const Update u(a, c, t);
   const int lane = threadIdx.x & 63;
   const long blk0 = t.block0 + i0 / BLOCK;
   floatx4 p[N], g[N];
@@ -364,11 +389,13 @@ template <bool BF16, Stream S> DM_DEV void step8(const AdamArgs& a, const Contro
 template <Stream S> __global__ __launch_bounds__(256) void k_adamw8(AdamArgs a) {
   const Control c = *a.c;
   if (c.skip) return;
-  const PlanTensor t = a.tensors[a.chunk_tensor[blockIdx.x]];
+  const int ti = a.chunk_tensor[blockIdx.x];
+  const PlanTensor t = a.tensors[ti];
+  const Update u(a, c, a.rates ? a.rates[ti] : c.all, t);
   const long i0 = (blockIdx.x - t.chunk0) * CHUNK + (threadIdx.x >> 6) * (CHUNK / 4);
   if (i0 >= t.n) return;
-  if (t.g_bf16) step8<true, S>(a, c, t, i0);
-  else step8<false, S>(a, c, t, i0);
+  if (t.g_bf16) step8<true, S>(a, c, u, t, i0);
+  else step8<false, S>(a, c, u, t, i0);
 }
 
 // Eight codes per lane: the numbers of a wave's store follow one another. Bound by 3 bytes per element (543M: 0.28 ms).
@@ -471,7 +498,9 @@ int dm_adamw_plan(const dm_adamw_tensor* t, int32_t n_tensors, void* plan, size_
   return DM_OK;
 }
 
-int dm_adamw_step(const dm_adamw_args* a, void* stream) {
+int dm_adamw_step(const dm_adamw_args* a, void* stream) { return dm_adamw_step_counted(a, nullptr, stream); }
+
+int dm_adamw_step_counted(const dm_adamw_args* a, int64_t* tensor_steps, void* stream) {
   const int rc = check_plan(a);
   if (rc) return rc;
   DM_REQUIRE(a->state_bits == 32 || a->state_bits == 8, DM_ERR_INVALID, "state_bits %d (32 or 8)", a->state_bits);
@@ -483,15 +512,19 @@ int dm_adamw_step(const dm_adamw_args* a, void* stream) {
   DM_REQUIRE(a->max_norm < HUGE_VAL, DM_ERR_INVALID, "max_norm=%g", a->max_norm);
   const bool norm = a->max_norm > 0. || a->skip_nonfinite;
   DM_REQUIRE(a->lr && a->steps && (a->norm || !norm) && (a->skipped || !a->skip_nonfinite), DM_ERR_INVALID, "null scalar");
+  DM_REQUIRE(reinterpret_cast<uintptr_t>(tensor_steps) % 8 == 0, DM_ERR_INVALID, "unaligned tensor_steps");
+  const size_t need = DM_ADAMW_WORKSPACE + (tensor_steps ? a->n_tensors * sizeof(Rates) : 0);
+  DM_REQUIRE(a->workspace_bytes >= need, DM_ERR_WORKSPACE, "workspace %zu < %zu bytes", a->workspace_bytes, need);
   hipStream_t s = S(stream);
   const Workspace w = carve(a->workspace);
+  Rates* rates = tensor_steps ? w.rates : nullptr;
   const int parts = norm ? run_sumsq(a, w.part, s) : 0;
   hipLaunchKernelGGL(k_adamw_begin, dim3(1), dim3(256), 0, s,
                      BeginArgs{w.c, w.part, parts, std::log2(a->beta1), std::log2(a->beta2), a->max_norm, a->skip_nonfinite, a->seed, a->lr, a->steps,
-                               a->norm, a->skipped});
+                               a->norm, a->skipped, (const PlanTensor*)a->plan, a->n_tensors, tensor_steps, rates});
   const AdamArgs k{(const PlanTensor*)a->plan, chunk_map(a), a->exp_avg, a->exp_avg_sq, a->exp_avg_exponent,
                    a->exp_avg_sq_exponent, (float)a->beta1, (float)(1. - a->beta1), (float)a->beta2, (float)(1. - a->beta2),
-                   (float)a->eps, w.c};
+                   (float)a->eps, w.c, rates};
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a->n_chunks), dim3(256), 0, s, k); };
   switch (stream_of(a)) {
     case Stream::KEPT: a->state_bits == 32 ? go(k_adamw32<Stream::KEPT>) : go(k_adamw8<Stream::KEPT>); break;

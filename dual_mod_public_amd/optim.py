@@ -1,4 +1,4 @@
-"""AdamW over all tensors of a model in one launch (dm_adamw_step), with 32-bit or 8-bit states and clipping by the
+"""AdamW over all tensors of a model in one launch (dm_adamw_step_counted), with 32-bit or 8-bit states and clipping by the
 global gradient norm.
 
     opt = trunk.optimizer(lr=3e-4, weight_decay=0.1, max_norm=1.0)      # or AdamW(params, grads=..., ...)
@@ -7,11 +7,13 @@ global gradient norm.
     trunk.refresh()
 
 Parameters are the framework's fp32 masters. Gradients are fixed buffers given once (``grads``: fp32 or bf16, as
-HipTrunk's views of its flat buffer) or, without them, the parameters' ``.grad`` at each step. Everything a step
-changes beside the parameters lives on the device (``lr``, ``steps``, ``norm``, ``skipped``), so a step can be captured
-into a HIP graph and replayed. A replay works on the parameters and gradients that the step was captured with, which the
-optimizer keeps allocated from then on (keep the optimizer as long as the graph), and does not tell torch that the
-parameters changed: call ``mark_updated()`` after it where something watches their versions (GraphDecoder, SwiGLU.decode).
+HipTrunk's views of its flat buffer) or, without them, the parameters' ``.grad`` at each step: a parameter without one is
+left as it is, its states too, and its bias corrections count the steps that it took part in. Everything a step
+changes beside the parameters lives on the device (``lr``, ``steps``, ``tensor_steps``, ``norm``, ``skipped``), so a step
+can be captured into a HIP graph and replayed. A replay works on the parameters and gradients that the step was captured
+with, which the optimizer keeps allocated from then on (keep the optimizer as long as the graph), and does not tell torch
+that the parameters changed: call ``mark_updated()`` after it where something watches their versions (GraphDecoder,
+SwiGLU.decode).
 
 8-bit states hold a byte per element and moment, and a byte per 256 elements and moment: blocks with a power-of-two
 scale, four significant bits per element, rounded stochastically by a hash of seed, step and element, so runs repeat
@@ -88,7 +90,8 @@ class AdamW:
         self.steps = torch.zeros((), dtype=torch.int64, **kw)        # steps taken
         self.norm = torch.zeros((), dtype=torch.float32, **kw)       # the last step's gradient norm (before clipping)
         self.skipped = torch.zeros((), dtype=torch.int32, **kw)      # steps left out by skip_nonfinite
-        self._ws = torch.empty(L.DM_ADAMW_WORKSPACE, dtype=torch.uint8, **kw)
+        self.tensor_steps = torch.zeros(len(self.params), dtype=torch.int64, **kw)   # steps with a gradient, per parameter
+        self._ws = torch.empty(L.DM_ADAMW_WORKSPACE + 8 * len(self.params), dtype=torch.uint8, **kw)
         self._key = self._plan = self._a = None
         self._in_graphs, self._graphs_hold = [], []    # plans that captured steps read, and what those read and write
         torch.cuda.current_stream(self.device).synchronize()   # the buffers are ready on every stream
@@ -120,14 +123,15 @@ class AdamW:
         for i, (p, g) in enumerate(zip(self.params, grads)):
             if p.numel() != self._sizes[i]:   # its states have their place between the others'
                 raise ValueError(f"parameter {i} now has {p.numel()} elements; its states were made for {self._sizes[i]}")
-            if g is None or p.numel() == 0:
+            if g is None or p.numel() == 0:   # its place in tensor_steps
+                rows.append(L.dm_adamw_tensor(None, None, 0, 0, 0.0, 0.0, L.DM_F32, 0))
                 continue
             self._check_grad(i, p, g)
             if p.dtype != torch.float32 or p.device != self.device or not p.is_contiguous():
                 raise ValueError(f"parameter {i} is now {p.dtype} on {p.device}")
             rows.append(L.dm_adamw_tensor(p.data_ptr(), g.data_ptr(), p.numel(), self._block0[i], self._decay[i],
                                           self._scale[i], L.dtype_code(g.dtype), 0))
-        if not rows:
+        if not any(t.n for t in rows):
             raise ValueError("no parameter has a gradient")
         arr = (L.dm_adamw_tensor * len(rows))(*rows)
         nb = L.lib().dm_adamw_plan_bytes(arr, len(rows))
@@ -155,10 +159,13 @@ class AdamW:
                 return self._call(fn)
         L.call_on(self.device, fn, L.byref(self._args()))
 
+    def _counted(self, args, stream):
+        return L.lib().dm_adamw_step_counted(args, self.tensor_steps.data_ptr(), stream)
+
     def step(self):
         """One step. Returns the gradients' global norm before clipping (a device scalar, overwritten by the next
         step) where it is computed: with max_norm or skip_nonfinite; else None."""
-        self._call(L.lib().dm_adamw_step)
+        self._call(self._counted)
         self.mark_updated()
         return self.norm if self.max_norm is not None or self.skip_nonfinite else None
 
@@ -193,16 +200,17 @@ class AdamW:
         return tuple(out)
 
     def state_dict(self):
-        """The states (the live tensors, as torch's modules give theirs), the step count and the learning rate."""
+        """The states (the live tensors, as torch's modules give theirs), the step counts and the learning rate."""
         d = dict(steps=int(self.steps), lr=float(self.lr), state_bits=self.state_bits, exp_avg=self.exp_avg,
-                 exp_avg_sq=self.exp_avg_sq)
+                 exp_avg_sq=self.exp_avg_sq, tensor_steps=self.tensor_steps)
         if self.state_bits == 8:
             d.update(exp_avg_exponent=self.exp_avg_exponent, exp_avg_sq_exponent=self.exp_avg_sq_exponent)
         return d
 
     @torch.no_grad()
     def load_state_dict(self, d):
-        """Copies state_dict()'s values in; the learning rate only where it is given."""
+        """Copies state_dict()'s values in; the learning rate only where it is given. Without ``tensor_steps`` every parameter
+        counts as one that took part in all steps."""
         if d["state_bits"] != self.state_bits:
             raise ValueError(f"states of {d['state_bits']} bits for an optimizer of {self.state_bits}")
         names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_exponent", "exp_avg_sq_exponent"] if self.state_bits == 8 else [])
@@ -210,8 +218,15 @@ class AdamW:
             t = getattr(self, n)
             if d[n].shape != t.shape or d[n].dtype != t.dtype:
                 raise ValueError(f"{n}: {d[n].dtype} {tuple(d[n].shape)}, {t.dtype} {tuple(t.shape)} is needed")
+        counts = d.get("tensor_steps")
+        if counts is not None and tuple(counts.shape) != (len(self.params),):
+            raise ValueError(f"tensor_steps: {tuple(counts.shape)}, one per parameter ({len(self.params)}) is needed")
         for n in names:
             getattr(self, n).copy_(d[n])
         self.steps.fill_(int(d["steps"]))
+        if counts is None:
+            self.tensor_steps.fill_(int(d["steps"]))
+        else:
+            self.tensor_steps.copy_(counts)
         if "lr" in d:
             self.set_lr(d["lr"])

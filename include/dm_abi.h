@@ -572,14 +572,20 @@ int dm_logprob_rows_bwd(const dm_logprob_args* a, void* stream);
  * Rounding to codes is stochastic, by 16 bits each of a 32-bit hash of (seed, t, element): a step moves v by less
  * than a thousandth, a code is an eighth, and rounding to nearest would leave v where it is.
  * The parameters are updated from the unrounded states.
+ * dm_adamw_step_counted: with tensor_steps (device, int64 [n_tensors], the steps that each tensor has taken part in), t in
+ * the two powers is the tensor's own count, which a step increments for the plan's tensors of 1 element or more: a tensor
+ * whose gradients begin after the others' starts with t = 1. NULL, and in dm_adamw_step, t is steps for all tensors. (The
+ * hash's t is steps either way.)
  *
  * dm_adamw_plan writes the launch plan (host memory, *plan_bytes from dm_adamw_plan_bytes) of the tensors, which the
- * caller copies to the device; *n_chunks is the number of blocks to launch. Tensors of 0 elements are left out.
+ * caller copies to the device; *n_chunks is the number of blocks to launch. Tensors of 0 elements are left out
+ * (they keep their places in the plan and in tensor_steps).
  * The plan holds the tensors' addresses: it is written again when one moves. No parameter may overlap another.
  * lr (fp32), steps (int64, the number of steps taken, incremented), norm (fp32, written where the norm is computed:
  * max_norm > 0 or skip_nonfinite) and skipped (int32) are device scalars, so a captured step can be replayed.
  * skip_nonfinite: a step whose norm is not finite changes nothing but *skipped, which is incremented.
- * Workspace: DM_ADAMW_WORKSPACE bytes, 16-byte aligned, not shared by steps that may overlap. */
+ * Workspace: DM_ADAMW_WORKSPACE bytes, with tensor_steps 8 more per tensor, 16-byte aligned, not shared by steps that may
+ * overlap. */
 #define DM_ADAMW_BLOCK 256
 #define DM_ADAMW_WORKSPACE 16384
 typedef struct dm_adamw_tensor {
@@ -602,6 +608,7 @@ typedef struct dm_adamw_args {
 size_t dm_adamw_plan_bytes(const dm_adamw_tensor* t, int32_t n_tensors);
 int dm_adamw_plan(const dm_adamw_tensor* t, int32_t n_tensors, void* plan, size_t plan_bytes, int64_t* n_chunks);
 int dm_adamw_step(const dm_adamw_args* a, void* stream);
+int dm_adamw_step_counted(const dm_adamw_args* a, int64_t* tensor_steps, void* stream);
 /* norm = the gradients' global norm alone (fields plan, n_chunks, n_tensors, norm, workspace). */
 int dm_grad_norm(const dm_adamw_args* a, void* stream);
 /* The numbers that n_blocks blocks of codes stand for, as bf16 (exact: four significant bits; magnitudes below

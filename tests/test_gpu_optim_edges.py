@@ -85,3 +85,120 @@ def test_captured_gradients_stay():
     p.grad, q.grad = torch.ones(1000, device=DEV), torch.ones(50, device=DEV)
     opt.step()
     assert int(opt.steps) == 3
+
+
+def _follow(opt, params, counts, decay):
+    """One step, every parameter against 64-bit AdamW with its own step count (counts, advanced here)."""
+    before = [p.detach().double().cpu() for p in params]
+    m0, v0 = ([t.double().cpu().flatten() for t in opt.views(s)] for s in opt.state_values())
+    opt.step()
+    m1, v1 = ([t.double().cpu().flatten() for t in opt.views(s)] for s in opt.state_values())
+    for i, p in enumerate(params):
+        if p.grad is None:
+            assert torch.equal(p.detach().double().cpu(), before[i]) and torch.equal(m1[i], m0[i]) and torch.equal(v1[i], v0[i])
+            continue
+        counts[i] += 1
+        g = p.grad.double().cpu()
+        m, v = B1 * m0[i] + (1 - B1) * g, B2 * v0[i] + (1 - B2) * g * g
+        dm = U * (3 * (B1 * m0[i]).abs() + 5 * ((1 - B1) * g).abs())
+        dv = U * (3 * B2 * v0[i] + 8 * (1 - B2) * g * g)
+        want, tol = p_bound(before[i], decay, 1.0, m, v, dm, dv, counts[i])
+        assert ((p.detach().double().cpu() - want).abs() <= tol).all(), (i, counts)
+        if opt.state_bits == 32:
+            assert ((m1[i] - m).abs() <= dm).all() and ((v1[i] - v).abs() <= dv + 1e-44).all()
+    assert opt.tensor_steps.tolist() == counts
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradient_first_appears_later(bits):
+    """A parameter's bias corrections count the steps that it took part in: one whose first gradient comes late moves by
+    the learning rate as any other does, not by 0.1 / sqrt(0.001) of it; one that pauses goes on where it was."""
+    params = [torch.nn.Parameter(noise(n, n)) for n in (300, 70, 5000, 1)]
+    opt = AdamW(params, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=0.1, state_bits=bits, seed=3)
+    counts = [0] * 4
+    taking_part = ((0, 2), (0, 2), (0, 2, 3), (0, 1, 2), (1, 3), (0, 1, 2, 3), (1,), (0, 1, 2, 3))
+    for k, who in enumerate(taking_part):
+        for i, p in enumerate(params):
+            p.grad = noise(p.numel(), 100 * k + i) if i in who else None
+        _follow(opt, params, counts, 0.1)
+    assert int(opt.steps) == len(taking_part) and counts == [6, 5, 6, 4]
+
+
+def test_late_gradient_with_skipped_and_captured_steps():
+    """Steps left out count for no parameter, replayed ones for those that the captured plan holds."""
+    a, b = (torch.nn.Parameter(noise(n, n)) for n in (4100, 9))
+    opt = AdamW([a, b], lr=LR, betas=(B1, B2), eps=EPS, weight_decay=0.0, skip_nonfinite=True)
+    a.grad = torch.full((4100,), float("inf"), device=DEV)
+    opt.step()
+    assert opt.tensor_steps.tolist() == [0, 0] and int(opt.skipped) == 1
+    counts = [0, 0]
+    a.grad.fill_(0.5)
+    _follow(opt, [a, b], counts, 0.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        opt.step()
+    only_a = a.grad
+    for k in range(3):
+        graph.replay()
+        counts[0] += 1
+        a.grad, b.grad = noise(4100, k), noise(9, 10 + k)
+        _follow(opt, [a, b], counts, 0.0)
+        a.grad, b.grad = only_a, None
+    assert counts == [7, 3] and int(opt.steps) == 7
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_keeps_the_counts(bits):
+    def make():
+        params = [torch.nn.Parameter(noise(n, n)) for n in (300, 70)]
+        return params, AdamW(params, lr=LR, state_bits=bits, seed=3)
+
+    (p, opt), (q, other) = make(), make()
+    for k in range(3):
+        p[0].grad, p[1].grad = noise(300, k), noise(70, k) if k == 2 else None
+        opt.step()
+    other.load_state_dict(opt.state_dict())
+    assert other.tensor_steps.tolist() == [3, 1] and other.tensor_steps.data_ptr() != opt.tensor_steps.data_ptr()
+    for a, b in zip(p, q):
+        b.data.copy_(a.data)
+        a.grad = noise(a.numel(), 7)
+        b.grad = a.grad.clone()
+    opt.step()
+    other.step()
+    assert all(torch.equal(a, b) for a, b in zip(p, q)) and other.tensor_steps.tolist() == [4, 2]
+    # without the counts: every parameter took part in every step
+    d = opt.state_dict()
+    del d["tensor_steps"]
+    other.load_state_dict(d)
+    assert other.tensor_steps.tolist() == [4, 4] and int(other.steps) == 4
+    with pytest.raises(ValueError, match="tensor_steps"):
+        other.load_state_dict(dict(opt.state_dict(), tensor_steps=torch.zeros(3, dtype=torch.int64)))
+
+
+def test_counts_of_many_tensors():
+    """More tensors than the counting block has threads, every third of them from the second step on."""
+    params = [torch.nn.Parameter(noise(1 + k % 3, k)) for k in range(700)]
+    opt = AdamW(params, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=0.1)
+    counts = [0] * 700
+    for t in (1, 2):
+        for k, p in enumerate(params):
+            p.grad = noise(p.numel(), 1000 * t + k) if t == 2 or k % 3 else None
+        _follow(opt, params, counts, 0.1)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_without_counts_every_tensor_is_as_old(bits):
+    """dm_adamw_step, which takes no counts: the step count is every tensor's."""
+    runs = []
+    for counts in (True, False):
+        ps, gs = [noise(n, n) for n in (300, 5000)], [noise(n, n + 1) for n in (300, 5000)]
+        opt = AdamW(ps, grads=gs, lr=LR, max_norm=0.5, state_bits=bits, seed=2)
+        a = opt._args()
+        if not counts:
+            a.workspace_bytes = L.DM_ADAMW_WORKSPACE
+        for _ in range(3):
+            opt.step() if counts else L.check(L.lib().dm_adamw_step(L.byref(a), L.stream_ptr()))
+        torch.cuda.synchronize()
+        assert opt.tensor_steps.tolist() == ([3, 3] if counts else [0, 0]) and int(opt.steps) == 3
+        runs.append(ps + [opt.exp_avg, opt.exp_avg_sq])
+    assert all(torch.equal(x, y) for x, y in zip(*runs))
