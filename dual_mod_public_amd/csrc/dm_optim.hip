@@ -230,8 +230,12 @@ struct Update {
   float keep, rate, v_scale, eps;
   DM_DEV Update(const AdamArgs& a, const Control& c, const Rates& r, const PlanTensor& t)
       : keep((float)(1. - (double)c.lr * t.lr_scale * t.weight_decay)), rate(r.rate * t.lr_scale), v_scale(r.v_scale), eps(a.eps) {}
-  DM_DEV float of(float p, float m, float v) const {   // a square root and a reciprocal of one ulp each
-    const float denom = fmaf(__builtin_amdgcn_sqrtf(v), v_scale, eps);
+  // A square root and a reciprocal of one ulp each. The root's instruction takes numbers below 2^-126 for 0, so small ones
+  // are scaled up before it; the reciprocal's would too, but eps is not below 2^-126.
+  DM_DEV float of(float p, float m, float v) const {
+    const bool small = v < 0x1p-96f;
+    const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p32f : v);
+    const float denom = fmaf(root, small ? v_scale * 0x1p-16f : v_scale, eps);
     return p * keep - rate * (m * __builtin_amdgcn_rcpf(denom));
   }
 };
@@ -507,7 +511,7 @@ int dm_adamw_step_counted(const dm_adamw_args* a, int64_t* tensor_steps, void* s
   DM_REQUIRE(a->exp_avg && a->exp_avg_sq && aligned16(a->exp_avg) && aligned16(a->exp_avg_sq), DM_ERR_INVALID,
              "null or unaligned state");
   DM_REQUIRE(a->state_bits == 32 || (a->exp_avg_exponent && a->exp_avg_sq_exponent), DM_ERR_INVALID, "null block exponents");
-  DM_REQUIRE(a->beta1 >= 0. && a->beta1 < 1. && a->beta2 >= 0. && a->beta2 < 1. && (float)a->eps > 0.f && a->eps < HUGE_VAL,
+  DM_REQUIRE(a->beta1 >= 0. && a->beta1 < 1. && a->beta2 >= 0. && a->beta2 < 1. && (float)a->eps >= 0x1p-126f && (float)a->eps < INFINITY,
              DM_ERR_INVALID, "beta1=%g beta2=%g eps=%g", a->beta1, a->beta2, a->eps);
   DM_REQUIRE(a->max_norm < HUGE_VAL, DM_ERR_INVALID, "max_norm=%g", a->max_norm);
   const bool norm = a->max_norm > 0. || a->skip_nonfinite;

@@ -48,8 +48,8 @@ class AdamW:
             raise ValueError("no parameters")
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits={state_bits} (32 or 8)")
-        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps > 0):
-            raise ValueError(f"betas={betas} eps={eps}")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and 2.0 ** -126 <= eps < 2.0 ** 128):
+            raise ValueError(f"betas={betas} eps={eps} (eps a normal fp32 number)")
         if max_norm is not None and not 0 < max_norm < float("inf"):
             raise ValueError(f"max_norm={max_norm}")
         self.device = self.params[0].device

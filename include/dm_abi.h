@@ -599,7 +599,7 @@ typedef struct dm_adamw_args {
   int32_t n_tensors, state_bits;
   void* exp_avg; void* exp_avg_sq;           /* [n_blocks * DM_ADAMW_BLOCK] fp32 or codes, 16-byte aligned */
   uint8_t* exp_avg_exponent; uint8_t* exp_avg_sq_exponent;   /* [n_blocks], state_bits 8 */
-  double beta1, beta2, eps;
+  double beta1, beta2, eps;                  /* 0 <= beta < 1; eps a normal fp32 number, 2^-126 at least */
   double max_norm;                           /* <= 0: no clipping */
   int32_t skip_nonfinite; uint32_t seed;
   const float* lr; int64_t* steps; float* norm; int32_t* skipped;

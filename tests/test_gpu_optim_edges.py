@@ -202,3 +202,30 @@ def test_without_counts_every_tensor_is_as_old(bits):
         assert opt.tensor_steps.tolist() == ([3, 3] if counts else [0, 0]) and int(opt.steps) == 3
         runs.append(ps + [opt.exp_avg, opt.exp_avg_sq])
     assert all(torch.equal(x, y) for x, y in zip(*runs))
+
+
+@pytest.mark.parametrize("eps", [1e-8, 1e-15, 1e-30, 2.0 ** -126])
+def test_very_small_gradients(eps):
+    """Second moments below fp32's normal numbers: their square root is as exact as any other's."""
+    g = torch.logspace(-22, -15, 3000, device=DEV) * torch.where(noise(3000, 1) < 0, -1.0, 1.0)
+    g[::5] = 0
+    p = torch.zeros(3000, device=DEV)
+    opt = AdamW([p], grads=[g], lr=LR, betas=(B1, B2), eps=eps, weight_decay=0.0)
+    m, v = (torch.zeros(3000, dtype=torch.float64) for _ in range(2))
+    for t in (1, 2):
+        before = p.double().cpu()
+        opt.step()
+        g64 = g.double().cpu()
+        # the square, its product with 1 - b2 and the product with b2 each round to a multiple of 2^-149 at best
+        sub = 2.0 ** -150 * 3
+        dm = U * (3 * (B1 * m).abs() + 5 * ((1 - B1) * g64).abs())
+        dv = U * (3 * B2 * v + 8 * (1 - B2) * g64 * g64) + sub
+        m, v = B1 * m + (1 - B1) * g64, B2 * v + (1 - B2) * g64 * g64
+        have_m, have_v = opt.exp_avg.double().cpu()[:3000], opt.exp_avg_sq.double().cpu()[:3000]
+        assert ((have_m - m).abs() <= dm).all() and ((have_v - v).abs() <= dv).all()
+        # the update of the moments that are there: a square root, a quotient and a few products
+        rate, s2 = LR / (1 - B1 ** t), 1 / math.sqrt(1 - B2 ** t)
+        denom = have_v.sqrt() * s2 + eps
+        upd = rate * have_m / denom
+        assert ((p.double().cpu() - (before - upd)).abs() <= U * (16 * upd.abs() + 4 * before.abs()) + 2.0 ** -149).all(), t
+        m, v = have_m, have_v

@@ -2,6 +2,7 @@
 fp32's range."""
 
 import pytest
+import torch
 
 from dual_mod_public_amd import _lib as L
 from tests.test_operator_refusals import step_args
@@ -15,3 +16,12 @@ def test_step_counts_need_their_place():
         for have in (L.DM_ADAMW_WORKSPACE, L.DM_ADAMW_WORKSPACE + 8 * n - 1):
             a = step_args(n_tensors=n, workspace_bytes=have)
             assert lib.dm_adamw_step_counted(L.byref(a), 0x80000, None) == -3
+
+
+@pytest.mark.parametrize("eps", [1e-39, 1e-45, 2.0 ** -127, 1e39])
+def test_eps_out_of_range_is_refused(eps):
+    """eps is the least denominator of an update, in fp32: one that is no normal number there is refused."""
+    from dual_mod_public_amd.optim import AdamW
+    assert L.load().dm_adamw_step(L.byref(step_args(eps=eps)), None) == -1
+    with pytest.raises(ValueError, match="eps"):
+        AdamW([torch.zeros(3)], eps=eps)
