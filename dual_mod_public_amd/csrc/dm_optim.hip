@@ -432,13 +432,15 @@ template <typename F, bool PAST> __global__ __launch_bounds__(256) void k_adamw_
   }
 }
 
+constexpr long MAX_CHUNKS = 1L << 24;   // of a launch
+constexpr long MAX_BLOCKS = 1L << 40;   // of the states
 long chunks_of(long n) { return (n + CHUNK - 1) / CHUNK; }
 
 int check_tensors(const dm_adamw_tensor* t, int n, long* chunks) {
   DM_REQUIRE(t != nullptr && n > 0, DM_ERR_INVALID, "%d tensors", n);
   *chunks = 0;
   for (int i = 0; i < n; ++i) {
-    DM_REQUIRE(t[i].n >= 0 && t[i].block0 >= 0, DM_ERR_INVALID, "tensor %d: n=%lld block0=%lld", i, (long long)t[i].n,
+    DM_REQUIRE(t[i].n >= 0 && t[i].n < MAX_CHUNKS * CHUNK && t[i].block0 >= 0 && t[i].block0 < MAX_BLOCKS, DM_ERR_INVALID, "tensor %d: n=%lld block0=%lld", i, (long long)t[i].n,
                (long long)t[i].block0);
     DM_REQUIRE(t[i].g_dtype == DM_F32 || t[i].g_dtype == DM_BF16, DM_ERR_INVALID, "tensor %d: gradient dtype %d", i, t[i].g_dtype);
     if (t[i].n == 0) continue;
@@ -447,14 +449,14 @@ int check_tensors(const dm_adamw_tensor* t, int n, long* chunks) {
                "tensor %d: null or unaligned gradient", i);
     *chunks += chunks_of(t[i].n);
   }
-  DM_REQUIRE(*chunks > 0 && *chunks < (1L << 24), DM_ERR_INVALID, "%ld chunks of %d elements", *chunks, CHUNK);
+  DM_REQUIRE(*chunks > 0 && *chunks < MAX_CHUNKS, DM_ERR_INVALID, "%ld chunks of %d elements", *chunks, CHUNK);
   return DM_OK;
 }
 size_t tensor_bytes(int n) { return (size_t)n * sizeof(PlanTensor); }
 
 int check_plan(const dm_adamw_args* a) {
   DM_REQUIRE(a != nullptr, DM_ERR_INVALID, "null arguments");
-  DM_REQUIRE(a->plan && aligned16(a->plan) && a->n_tensors > 0 && a->n_chunks > 0 && a->n_chunks < (1L << 24), DM_ERR_INVALID,
+  DM_REQUIRE(a->plan && aligned16(a->plan) && a->n_tensors > 0 && a->n_chunks > 0 && a->n_chunks < MAX_CHUNKS, DM_ERR_INVALID,
              "null or unaligned plan, %d tensors, %lld chunks", a->n_tensors, (long long)a->n_chunks);
   DM_REQUIRE(a->workspace && aligned16(a->workspace) && a->workspace_bytes >= DM_ADAMW_WORKSPACE, DM_ERR_WORKSPACE,
              "workspace %zu < %d bytes", a->workspace_bytes, DM_ADAMW_WORKSPACE);
@@ -554,7 +556,7 @@ int dm_grad_norm(const dm_adamw_args* a, void* stream) {
 }
 
 int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_blocks, int32_t second, void* out, void* stream) {
-  DM_REQUIRE(n_blocks >= 0 && n_blocks < (1L << 40), DM_ERR_INVALID, "n_blocks=%lld", (long long)n_blocks);
+  DM_REQUIRE(n_blocks >= 0 && n_blocks < MAX_BLOCKS, DM_ERR_INVALID, "n_blocks=%lld", (long long)n_blocks);
   if (n_blocks == 0) return DM_OK;
   DM_REQUIRE(codes && exponents && out && aligned16(codes) && aligned16(out), DM_ERR_INVALID, "null or unaligned operand");
   const dim3 grid((unsigned)std::min<long>((n_blocks + 31) / 32, 1 << 16));

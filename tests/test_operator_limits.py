@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from dual_mod_public_amd import _lib as L
-from tests.test_operator_refusals import step_args
+from tests.test_operator_refusals import plan, step_args, tensor
 
 
 def test_step_counts_need_their_place():
@@ -25,3 +25,11 @@ def test_eps_out_of_range_is_refused(eps):
     assert L.load().dm_adamw_step(L.byref(step_args(eps=eps)), None) == -1
     with pytest.raises(ValueError, match="eps"):
         AdamW([torch.zeros(3)], eps=eps)
+
+
+def test_plan_of_lengths_past_64_bits():
+    """Lengths whose sum of launched blocks would pass 64 bits are refused one by one."""
+    big = (1 << 63) - 1
+    for ts in ([tensor(big)], [tensor(big), tensor((1 << 63) - 4096), tensor(5 * 4096)], [tensor(big, block0=1), tensor(4)],
+               [tensor(4, block0=big)]):
+        assert plan(*ts) is None
