@@ -200,8 +200,9 @@ class AdamW:
         return tuple(out)
 
     def state_dict(self):
-        """The states (the live tensors, as torch's modules give theirs), the step counts and the learning rate."""
-        d = dict(steps=int(self.steps), lr=float(self.lr), state_bits=self.state_bits, exp_avg=self.exp_avg,
+        """The states (the live tensors, as torch's modules give theirs), the parameters' sizes, the step counts and
+        the learning rate."""
+        d = dict(steps=int(self.steps), lr=float(self.lr), state_bits=self.state_bits, sizes=list(self._sizes), exp_avg=self.exp_avg,
                  exp_avg_sq=self.exp_avg_sq, tensor_steps=self.tensor_steps)
         if self.state_bits == 8:
             d.update(exp_avg_exponent=self.exp_avg_exponent, exp_avg_sq_exponent=self.exp_avg_sq_exponent)
@@ -209,8 +210,7 @@ class AdamW:
 
     @torch.no_grad()
     def load_state_dict(self, d):
-        """Copies state_dict()'s values in; the learning rate only where it is given. Without ``tensor_steps`` every parameter
-        counts as one that took part in all steps."""
+        """Copies state_dict()'s values in; the learning rate only where it is given. Without ``tensor_steps`` every parameter counts as one that took part in all steps."""
         if d["state_bits"] != self.state_bits:
             raise ValueError(f"states of {d['state_bits']} bits for an optimizer of {self.state_bits}")
         names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_exponent", "exp_avg_sq_exponent"] if self.state_bits == 8 else [])
@@ -218,6 +218,8 @@ class AdamW:
             t = getattr(self, n)
             if d[n].shape != t.shape or d[n].dtype != t.dtype:
                 raise ValueError(f"{n}: {d[n].dtype} {tuple(d[n].shape)}, {t.dtype} {tuple(t.shape)} is needed")
+        if list(d.get("sizes", self._sizes)) != self._sizes:
+            raise ValueError("states of parameters of other sizes or in another order")
         counts = d.get("tensor_steps")
         if counts is not None and tuple(counts.shape) != (len(self.params),):
             raise ValueError(f"tensor_steps: {tuple(counts.shape)}, one per parameter ({len(self.params)}) is needed")

@@ -229,3 +229,24 @@ def test_very_small_gradients(eps):
         upd = rate * have_m / denom
         assert ((p.double().cpu() - (before - upd)).abs() <= U * (16 * upd.abs() + 4 * before.abs()) + 2.0 ** -149).all(), t
         m, v = have_m, have_v
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_of_other_parameters(bits):
+    """States of parameters of other sizes or another order are refused, also where they fill as many blocks."""
+    def make(*sizes, seed=0):
+        params = [torch.zeros(n, device=DEV) for n in sizes]
+        return params, AdamW(params, grads=[noise(n, n) for n in sizes], lr=LR, state_bits=bits, seed=seed)
+
+    _, opt = make(100, 300)
+    opt.step()
+    saved = opt.state_dict()
+    for sizes in ((300, 100), (101, 300), (100, 300, 0)):
+        other = make(*sizes)[1]
+        assert other.exp_avg.shape == opt.exp_avg.shape
+        with pytest.raises(ValueError, match="sizes"):
+            other.load_state_dict(saved)
+        assert int(other.steps) == 0 and not other.exp_avg.any()
+    _, other = make(100, 300)
+    other.load_state_dict({k: v for k, v in saved.items() if k not in ("sizes", "seed")})    # states without them
+    assert torch.equal(other.exp_avg, opt.exp_avg) and other.seed == 0
