@@ -200,17 +200,18 @@ class AdamW:
         return tuple(out)
 
     def state_dict(self):
-        """The states (the live tensors, as torch's modules give theirs), the parameters' sizes, the step counts and
-        the learning rate."""
+        """The states (the live tensors, as torch's modules give theirs), the parameters' sizes, the step counts, the
+        learning rate and, of 8-bit states, the seed of their rounding."""
         d = dict(steps=int(self.steps), lr=float(self.lr), state_bits=self.state_bits, sizes=list(self._sizes), exp_avg=self.exp_avg,
                  exp_avg_sq=self.exp_avg_sq, tensor_steps=self.tensor_steps)
         if self.state_bits == 8:
-            d.update(exp_avg_exponent=self.exp_avg_exponent, exp_avg_sq_exponent=self.exp_avg_sq_exponent)
+            d.update(seed=self.seed, exp_avg_exponent=self.exp_avg_exponent, exp_avg_sq_exponent=self.exp_avg_sq_exponent)
         return d
 
     @torch.no_grad()
     def load_state_dict(self, d):
-        """Copies state_dict()'s values in; the learning rate only where it is given. Without ``tensor_steps`` every parameter counts as one that took part in all steps."""
+        """Copies state_dict()'s values in; the learning rate and the seed only where they are given (a step captured before
+        keeps its seed). Without ``tensor_steps`` every parameter counts as one that took part in all steps."""
         if d["state_bits"] != self.state_bits:
             raise ValueError(f"states of {d['state_bits']} bits for an optimizer of {self.state_bits}")
         names = ["exp_avg", "exp_avg_sq"] + (["exp_avg_exponent", "exp_avg_sq_exponent"] if self.state_bits == 8 else [])
@@ -232,3 +233,7 @@ class AdamW:
             self.tensor_steps.copy_(counts)
         if "lr" in d:
             self.set_lr(d["lr"])
+        if "seed" in d:
+            self.seed = int(d["seed"]) & 0xffffffff
+            if self._a is not None:
+                self._a.seed = self.seed

@@ -250,3 +250,20 @@ def test_state_of_other_parameters(bits):
     _, other = make(100, 300)
     other.load_state_dict({k: v for k, v in saved.items() if k not in ("sizes", "seed")})    # states without them
     assert torch.equal(other.exp_avg, opt.exp_avg) and other.seed == 0
+
+
+def test_state_keeps_the_seed():
+    """The rounding's seed belongs to the states: a run that is taken up again repeats bit for bit."""
+    def make(seed):
+        p = torch.zeros(1000, device=DEV)
+        return p, AdamW([p], grads=[noise(1000, 5)], lr=LR, state_bits=8, seed=seed)
+
+    (p, opt), (q, other) = make(11), make(0)
+    opt.step()
+    other.step()                                      # its plan is there already
+    other.load_state_dict(opt.state_dict())
+    q.copy_(p)
+    for _ in range(2):
+        opt.step()
+        other.step()
+    assert torch.equal(p, q) and torch.equal(opt.exp_avg, other.exp_avg) and torch.equal(opt.exp_avg_sq, other.exp_avg_sq)
