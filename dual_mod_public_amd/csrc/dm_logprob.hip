@@ -87,7 +87,8 @@ struct RowGrad {
   float value;    // 0 or NaN
   DM_DEV float of(float x) const {
     const float y = fmaf(x - M, LOG2E, -l2z), p = __builtin_amdgcn_exp2f(y);
-    return p * fmaf(b, fmaxf(y, -1e30f), a);   // p = 0 at -inf
+    // p = 0 at -inf. Each product with p for itself: b y would pass fp32's range for a large b, and 0 times it is NaN
+    return fmaf(p * b, fmaxf(y, -1e30f), p * a);
   }
   DM_DEV RowGrad(const GradCoef& k, const RowStats& s, bool no_token)
       : M(s.M), l2z(s.log_z * LOG2E), a(-k.g - (k.gh == 0.f ? 0.f : k.gh * s.entropy)), b(-k.gh * LN2), g(k.g) {

@@ -1,0 +1,38 @@
+"""Logit rows at the ends of what the calls take: large entropy coefficients beside masked columns, rows that one token
+dominates, forward-mode derivatives. Against the definitions in 64 bits, with the bounds of test_gpu_logprobs.py."""
+
+import pytest
+import torch
+
+from dual_mod_public_amd import _lib as L
+from dual_mod_public_amd import logprobs as lp
+from tests.hip_helpers import DEV, say
+from tests.test_gpu_logprobs import DTYPES, INF, check_grad, check_values, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    L.load()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [40, 3000, 70001])
+@pytest.mark.parametrize("scale", [1.0, 1e9, 1e20, 1e34])
+def test_large_entropy_coefficients(scale, V, dtype):
+    """A column of probability 0 has gradient 0 whatever the coefficients; the others follow the definition."""
+    say(f"coefficients {scale} V={V} {dtype}")
+    x, t, g, _ = rows_of(6, V, dtype)
+    x[:, 1::3] = -INF
+    x[1, 5:] = -INF
+    x[2] -= 60.0 * torch.rand(V, generator=g, device=DEV).to(dtype)      # probabilities down to e^-60 and less
+    x[3, 2], t[:] = -1e37, 0
+    w = scale * torch.randn(6, generator=g, device=DEV)
+    gh = scale * (0.5 + torch.rand(6, generator=g, device=DEV)) * torch.tensor([1.0, -1.0] * 3, device=DEV)
+    r, dx = lp.row_logprobs_grad(x, t, w, gh)
+    for name, d in (("fused", dx), ("backward", lp.row_logprobs_bwd(x, t, r.stats, w, gh))):
+        assert (d[:, 1::3] == 0).all() and (d[1, 5:] == 0).all() and d[3, 2] == 0, name
+        check_grad(x, t, w, gh, d, name)
