@@ -501,9 +501,10 @@ template <typename T, int NT, int NV, bool GRAD, bool ONCE> __global__ __launch_
     } else {
       s.M = u.m;
       const float l2 = __builtin_amdgcn_logf(u.z), shift = fmaf(u.m, LOG2E, u.c);   // what c's rounding left
-      s.log_z = (l2 - shift) * LN2;
+      // neither is below 0 but for the roundings of the two instructions, where one token has all of the probability
+      s.log_z = fmaxf((l2 - shift) * LN2, 0.f);
       s.lse = s.M + s.log_z;
-      s.entropy = (l2 - u.q / u.z) * LN2;
+      s.entropy = fmaxf((l2 - u.q / u.z) * LN2, 0.f);
     }
     if (threadIdx.x == 0) {
       if (a.logp) a.logp[r] = t < 0 ? 0.f : t < a.cols ? s.logp(xt) : NAN_;

@@ -36,3 +36,21 @@ def test_large_entropy_coefficients(scale, V, dtype):
     for name, d in (("fused", dx), ("backward", lp.row_logprobs_bwd(x, t, r.stats, w, gh))):
         assert (d[:, 1::3] == 0).all() and (d[1, 5:] == 0).all() and d[3, 2] == 0, name
         check_grad(x, t, w, gh, d, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [7, 64, 5000, 33000])
+def test_one_token_dominates(V, dtype):
+    """Log probabilities are at most 0 and entropies at least 0, where one token has all of the probability too."""
+    M = 512
+    for seed, others in enumerate((-INF, -25.0, -18.0, -15.0)):
+        x, t, g, _ = rows_of(M, V, dtype, seed=seed, scale=20.0)
+        value = x.float()[torch.arange(M, device=DEV), t]
+        x.copy_((value[:, None] + others).expand(M, V))
+        x[torch.arange(M, device=DEV), t] = value.to(dtype)
+        r, _ = lp.row_logprobs_grad(x, t, torch.ones(M, device=DEV), top=1)
+        r2 = lp.row_logprobs(x[:100], t[:100], top=min(V, 5))
+        assert (r.logp <= 0).all() and (r.top_logp <= 0).all() and (r.entropy >= 0).all() and (r.lse >= value).all(), others
+        assert (r2.logp <= 0).all() and (r2.top_logp <= 0).all() and (r2.entropy >= 0).all(), others
+        assert not torch.isnan(torch.log1p(-r.logp.exp())).any()
+        check_values(x[:64], t[:64], 1, lp.RowLogprobs(*[v[:64] for v in r]), f"others at {others}")
