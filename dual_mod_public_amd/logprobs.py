@@ -17,6 +17,7 @@ of nothing else gives every token -inf, entropy 0 and a zero gradient. A NaN mak
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -69,6 +70,8 @@ def _logits(logits):
     if logits.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("row_logprobs and its like keep no autograd graph: token_logprobs does, or call them under "
                                   "torch.no_grad() or on logits.detach()")
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("row_logprobs and its like carry no tangent: call them on logits.detach()")
     return _rows(logits, "logits")
 
 
@@ -131,9 +134,9 @@ def _forward(logits, targets, top, out, rows, ld, gradient=(None, None, None, 0)
 
 def row_logprobs(logits, targets=None, top=0, out=None):
     """The values of logits [..., V]: logp of ``targets`` (int64 [...], optional), entropy, lse and the ``top`` most
-    likely tokens of each row (at most 32). No autograd graph: logits that would need one are refused. out: a RowLogprobs
-    of tensors to write into (static buffers of a decode loop), apart from each other and the inputs; a field that is None
-    is left out."""
+    likely tokens of each row (at most 32). No autograd graph: logits that would need one, or that hold a forward-mode
+    tangent, are refused. out: a RowLogprobs of tensors to write into (static buffers of a decode loop), apart from each
+    other and the inputs; a field that is None is left out."""
     return _forward(logits, targets, top, out, *_logits(logits))
 
 

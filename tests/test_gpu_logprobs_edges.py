@@ -54,3 +54,22 @@ def test_one_token_dominates(V, dtype):
         assert (r2.logp <= 0).all() and (r2.top_logp <= 0).all() and (r2.entropy >= 0).all(), others
         assert not torch.isnan(torch.log1p(-r.logp.exp())).any()
         check_values(x[:64], t[:64], 1, lp.RowLogprobs(*[v[:64] for v in r]), f"others at {others}")
+
+
+def test_forward_mode_is_refused():
+    """The values carry no tangents: logits that hold one are refused, by token_logprobs too."""
+    import torch.autograd.forward_ad as fwd
+    x, t, g, _ = rows_of(4, 50, torch.float32)
+    w = torch.ones(4, device=DEV)
+    stats = lp.row_logprobs(x, t).stats
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for f in (lambda: lp.row_logprobs(dual, t), lambda: lp.row_logprobs_grad(dual, t, w),
+                  lambda: lp.row_logprobs_bwd(dual, t, stats, w)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                f()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
+                f()
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            lp.token_logprobs(dual, t)
+        assert torch.equal(lp.row_logprobs(dual.detach(), t).logp, lp.row_logprobs(x, t).logp)
