@@ -118,6 +118,7 @@ class dm_stack_bwd_layer(ctypes.Structure):
 
 
 DM_TOP_MAX = 32           # include/dm_abi.h: most likely tokens per row
+DM_LOGPROB_COLS = 1 << 27  # columns of a logit row
 DM_ADAMW_BLOCK = 256      # elements per block of the optimizer's states
 DM_ADAMW_WORKSPACE = 16384
 

@@ -578,7 +578,7 @@ template <typename T, int NT, int NV> __global__ __launch_bounds__(256) void k_l
   }
 }
 
-constexpr int MAX_COLS = 1 << 27;     // a row's bytes in 32 bits
+constexpr int MAX_COLS = DM_LOGPROB_COLS;   // a row's bytes in 32 bits
 constexpr int MAX_BLOCKS = 1 << 20;   // of a grid; further rows by the same blocks
 
 template <typename T> LpArgs<T> typed(const dm_logprob_args* a) {

@@ -33,13 +33,15 @@ class RowLogprobs(NamedTuple):
 
 def _rows(t, what):
     """(rows, row stride) of [..., V] with unit stride along V and one stride over all rows."""
-    V = t.shape[-1]
-    if t.numel() == 0:
+    V, n = t.shape[-1], t.numel()
+    if V > L.DM_LOGPROB_COLS or n > V * 0x7fffffff:
+        raise ValueError(f"{what}: rows of shape {tuple(t.shape)} (at most {L.DM_LOGPROB_COLS} columns and 2^31 - 1 rows)")
+    if n == 0:
         if V == 0:
             raise ValueError(f"{what}: no columns")
         return 0, V
     if t.is_contiguous():
-        return t.numel() // V, V
+        return n // V, V
     try:
         t2 = t.view(-1, V)
     except RuntimeError:

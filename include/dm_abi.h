@@ -538,9 +538,10 @@ int dm_ce_mean(const float* loss, int32_t M, const float* nvalid, float* out, vo
  * infinite ones, entropy NaN. The gradient of those two is NaN. A row whose coefficients are both 0 (g_logp counts
  * as 0 where the target is < 0) gets zeros whatever its logits; one with a target >= cols and g_logp != 0 NaN.
  * dlogits (storage dtype, stride ld_d >= cols) may be the logits themselves (same pointer and stride); no output may
- * overlap an input or another output otherwise. Pointers need their element's alignment only. At most 2^27 columns; rows may be 0. No workspace; rows are
+ * overlap an input or another output otherwise. Pointers need their element's alignment only. At most DM_LOGPROB_COLS columns; rows may be 0. No workspace; rows are
  * independent, a row's results do not depend on the others. */
 #define DM_TOP_MAX 32
+#define DM_LOGPROB_COLS (1 << 27)
 typedef struct dm_logprob_args {
   int32_t dtype, rows, cols;
   int32_t top;                       /* 0..min(DM_TOP_MAX, cols); dm_logprob_rows only */

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from dual_mod_public_amd import _lib as L
+from dual_mod_public_amd import logprobs as lp
 from tests.test_operator_refusals import plan, step_args, tensor
 
 
@@ -33,3 +34,15 @@ def test_plan_of_lengths_past_64_bits():
     for ts in ([tensor(big)], [tensor(big), tensor((1 << 63) - 4096), tensor(5 * 4096)], [tensor(big, block0=1), tensor(4)],
                [tensor(4, block0=big)]):
         assert plan(*ts) is None
+
+
+@pytest.mark.parametrize("shape", [((1 << 31), 1), ((1 << 32) + 4, 3), (2, 1 << 30, 2), (4, (1 << 27) + 1), (1, (1 << 32) + 5), (0, 1 << 32)])
+def test_rows_and_columns_past_their_limits(shape):
+    """More rows than a 32-bit count holds, or more columns than a row may have, are refused by size, not cut off."""
+    with pytest.raises(ValueError, match="at most"):
+        lp._rows(torch.empty(shape, device="meta", dtype=torch.bfloat16), "logits")
+
+
+def test_rows_at_their_limits():
+    assert lp._rows(torch.empty((1 << 31) - 1, 5, device="meta", dtype=torch.bfloat16), "logits") == ((1 << 31) - 1, 5)
+    assert lp._rows(torch.empty(2, 1 << 27, device="meta"), "logits") == (2, 1 << 27)
