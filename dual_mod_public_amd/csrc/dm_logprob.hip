@@ -648,9 +648,15 @@ bool outputs_overlap(const dm_logprob_args* a, bool bwd) {
     const wide p = reinterpret_cast<uintptr_t>(r.p), q = reinterpret_cast<uintptr_t>(s.p);
     return p && q && p < q + s.bytes && q < p + r.bytes;
   };
+  // rows of one stride side by side: the gradient's columns in the gaps of the logits'
+  const wide row = a->ld * e, used = a->cols * e;
+  const wide gap = a->dlogits && a->ld_d == a->ld
+                       ? ((wide)reinterpret_cast<uintptr_t>(a->dlogits) + ((wide)1 << 100) * row - reinterpret_cast<uintptr_t>(a->logits)) % row
+                       : 0;
+  const bool beside = gap >= used && gap + used <= row;
   for (const Range& r : out) {
     for (const Range& s : in)
-      if (meet(r, s)) return true;
+      if (meet(r, s) && !(beside && &r == out && &s == in)) return true;
     for (const Range& s : out)
       if (&s != &r && meet(r, s)) return true;
   }

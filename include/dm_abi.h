@@ -537,9 +537,10 @@ int dm_ce_mean(const float* loss, int32_t M, const float* nvalid, float* out, vo
  * log probabilities and entropy NaN. With +inf and no NaN: lse +inf, logp -inf for finite logits and NaN for the
  * infinite ones, entropy NaN. The gradient of those two is NaN. A row whose coefficients are both 0 (g_logp counts
  * as 0 where the target is < 0) gets zeros whatever its logits; one with a target >= cols and g_logp != 0 NaN.
- * dlogits (storage dtype, stride ld_d >= cols) may be the logits themselves (same pointer and stride); no output may
- * overlap an input or another output otherwise. Pointers need their element's alignment only. At most DM_LOGPROB_COLS columns; rows may be 0. No workspace; rows are
- * independent, a row's results do not depend on the others. */
+ * dlogits (storage dtype, stride ld_d >= cols) may be the logits themselves (same pointer and stride), or lie beside them
+ * in rows of the same stride; no output may overlap an input or another output otherwise, each taken from its first row's
+ * first element to its last row's last. Pointers need their element's alignment only. At most DM_LOGPROB_COLS columns;
+ * rows may be 0. No workspace; rows are independent, a row's results do not depend on the others. */
 #define DM_TOP_MAX 32
 #define DM_LOGPROB_COLS (1 << 27)
 typedef struct dm_logprob_args {

@@ -73,3 +73,31 @@ def test_forward_mode_is_refused():
         with pytest.raises((RuntimeError, NotImplementedError)):
             lp.token_logprobs(dual, t)
         assert torch.equal(lp.row_logprobs(dual.detach(), t).logp, lp.row_logprobs(x, t).logp)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_beside_the_logits(dtype):
+    """Logits and gradient as columns of one buffer: rows that lie side by side do not overlap; rows that meet are refused."""
+    M, V = 5, 333
+    for at_x, at_d in ((0, V), (V + 4, 1), (0, V + 9)):
+        wide = torch.full((M, 2 * V + 9), 7.0, device=DEV, dtype=dtype)
+        x, d = wide[:, at_x:at_x + V], wide[:, at_d:at_d + V]
+        g = torch.Generator(device=DEV).manual_seed(at_d)
+        x.copy_(torch.randn(M, V, generator=g, device=DEV).to(dtype))
+        t = torch.randint(0, V, (M,), generator=g, device=DEV)
+        w = torch.randn(M, generator=g, device=DEV)
+        r, want = lp.row_logprobs_grad(x.clone(), t, w)
+        before = wide.clone()
+        lp.row_logprobs_grad(x, t, w, dlogits=d)
+        assert torch.equal(d, want)
+        d.fill_(7.0)
+        assert torch.equal(wide, before)
+        lp.row_logprobs_bwd(x, t, r.stats, w, dlogits=d)
+        check_grad(x, t, w, None, d)
+        d.fill_(7.0)
+        assert torch.equal(wide, before)
+    for at_x, at_d in ((0, V - 1), (5, 0), (0, 2 * V + 9 - V + 1)):
+        flat = torch.zeros((M + 1) * (2 * V + 9), device=DEV, dtype=dtype)
+        x, d = (torch.as_strided(flat, (M, V), (2 * V + 9, 1), o) for o in (at_x, at_d))
+        with pytest.raises(L.DMError, match="overlaps"):
+            lp.row_logprobs_grad(x, t, w, dlogits=d)
