@@ -451,6 +451,8 @@ class HipTrunk:
         """The forward alone: RowLogprobs of targets [B, T] (logprobs.row_logprobs: a target of -1 is ignored) after
         idx [B, T], with the ``top`` most likely tokens of each position. Overwrites the activations of the last
         step, none of its gradients."""
+        if tuple(targets.shape) != (self.B, self.T):
+            raise ValueError(f"targets {tuple(targets.shape)}; [B, T] = {(self.B, self.T)} is needed")
         self.idx.copy_(idx)
         self._embed()
         if self.wavefront:
