@@ -7,9 +7,12 @@
 // -p (g + gh (logp + H)) + g [target] needs lse and H, so a row's logits wait in registers for them: 16 vectors of
 // 16 bytes in each of 256 threads hold 32768 bf16 logits, and the row is read and written once.
 // The `top` most likely tokens: the 64 lanes' largest logits are logits of 64 different places, so the top-th of them is
-// reached by at least `top` of the row; the few tens of logits that reach it are listed in LDS and ranked there.
+// reached by at least `top` of the row; the few tens of logits that reach it are listed in LDS and ranked there. A row with
+// more than 1024 such logits (equal ones or of few values, or masked by a finite number with fewer lanes of allowed ones than
+// `top`) and one of -inf are scanned once per alternative instead: 64 rows of 50257 bf16 with 8 alternatives 83 to 100 us
+// (ordinary ones 12), 4096 of 32000 1.34 to 1.42 ms (53).
 // Bound by HBM (44 us for 262 MB of logits, 6.0 TB/s; with the gradient 524 MB in 98 us, 5.4 TB/s; a large copy reaches
-// 5.0 to 5.4); close behind come the 10 vector instructions per logit, 4 of whose slots are the exponential.
+// 5.0 to 5.4); close behind come the 11 vector instructions per logit, 4 of whose slots are the exponential.
 #include "dm_common.h"
 #include "dm_error.h"
 
@@ -592,7 +595,10 @@ template <bool GRAD, typename T, int NT, int NV, bool ONCE = true> void launch_r
 // The threads of a row and their vectors per tile, by the row's 16-byte vectors (bf16: 8 logits, fp32: 4).
 // Fewer rows than CUs: as many threads as a block has, since nothing else hides a row's latencies (one row of 32000 bf16
 // with 5 alternatives 7.0 us, at 256 threads 9.6; without them 4.9, where a block of so many threads takes 3.8 for a row
-// of 8). Several blocks per row with a second launch to join them would cost that launch.
+// of 8). Up to a row per CU that is faster, from two on the CU's other blocks hide them better: 1024 and 256 threads take
+// for 64, 255, 320, 1000 rows of 50257 bf16 7.5 / 9.8, 8.6 / 11.1, 14.2 / 12.3, 29 / 21 us, with 8 alternatives 10.4 / 17.5,
+// 11.6 / 18.4, 19.8 / 20.3, 40 / 28; of 12000 bf16 4.7 / 4.5, 5.1 / 4.8, 8.0 / 5.7, 15 / 8. Several blocks per row have not
+// been tried: joined by a second launch they would cost that launch.
 // Otherwise the smallest blocks that fill a CU's memory pipes while others of the CU wait at their barriers (4096 rows of
 // 32000 bf16: 64 threads of 4 vectors 47 us, 256 of 8 44, 1024 of 4 72). With the gradient a row is best read once and
 // held until it is written (the same rows: 256 threads of 16 vectors, all of a row, 98 us; of 8 vectors, read twice,

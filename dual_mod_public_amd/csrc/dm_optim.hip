@@ -4,8 +4,8 @@
 // Three launches whatever the number of tensors: the sum of g^2 in NORM_PARTS parts (only where the norm is asked for),
 // one block that makes the step's scalars from them and from the step count, and the update, a block per chunk of a tensor;
 // a plan in device memory says which. All of it streams: 543M parameters (fp32 gradients) move 15.2 GB, and 2.2 GB for
-// the norm, in 2.98 ms (5.8 TB/s, where a large copy reaches 5.0); with 8-bit states 8.7 and 2.2 GB in 1.84 ms (5.9 TB/s).
-// A small model's step (2.9M) takes 20 us, of which 5 are the scalars' launch.
+// the norm, in 3.01 ms (5.8 TB/s, where a large copy reaches 5.0); with 8-bit states 8.7 and 2.2 GB in 1.81 ms (6.0 TB/s).
+// A small model's step (2.9M) takes 21 us, of which 4 are the scalars' launch (3.3 with one step count for all tensors).
 #include "dm_common.h"
 #include "dm_error.h"
 
@@ -90,11 +90,13 @@ template <bool BF16, bool PAST> DM_DEV floatx4 grads4(const PlanTensor& t, long 
     return load<floatx4, 4, PAST>((const float*)t.g + i);
   }
 }
-// What goes past the caches. A small model's step finds its data in the last one, of 256 MB (2.9M parameters, 80 MB: 20.1 us
-// kept, 22.6 past). A larger step's parameters and states, read and written, only push one another out: past the caches 15M
-// parameters take 78 us (93), with 8-bit states 59 (70), 47M 237 (283). The gradients stay as long as they fit by
-// themselves, since the norm has read them just before (past as well: 85, 250); beyond, they go past too (543M: 2.98 ms;
-// 3.07 with the gradients kept, 3.26 with everything; with 8-bit states 1.84 ms, 2.07 with everything).
+// What goes past the caches. A small model's step finds its data in the last one, of 256 MB (2.9M parameters, 80 MB). A
+// larger step's parameters and states, read and written, only push one another and what else the program uses out. Steps of
+// three models in turn, kept / states and parameters past / gradients past as well: 6M parameters 47 / 42 / 44 us, 15M 103 /
+// 84 / 91, 47M 299 / 254 / 263; with 8-bit states 38 / 37 / 37, 75 / 64 / 64, 189 / 164 / 166. (One model's steps with nothing
+// between them find more of it: 6M 40 / 42 / 41, 15M 80 / 84 / 89, 47M 297 / 230 / 256.) The gradients stay as long as they
+// fit by themselves, since the norm has read them just before; beyond, they go past too (543M: 3.24 / 3.09 / 3.01 ms, with
+// 8-bit states 2.02 / 1.79 / 1.81).
 enum class Stream { KEPT, STATES, ALL };
 constexpr double CACHE_BYTES = 256 << 20;
 
@@ -240,7 +242,7 @@ struct Update {
   }
 };
 
-// A block per chunk; bound by its 28 bytes per element (543M: 15.2 GB in 2.6 ms).
+// A block per chunk; bound by its 28 bytes per element (543M: 15.2 GB in 2.64 ms).
 template <bool BF16, Stream S> DM_DEV void step32(const AdamArgs& a, const Control& c, const Update& u, const PlanTensor& t, long i0, float* ms, float* vs) {
   constexpr int STEP = 256 * 4, N = CHUNK / STEP;
   constexpr bool PAST = S != Stream::KEPT;
@@ -314,7 +316,7 @@ DM_DEV int block_exponent(float largest, bool bad) {
 DM_DEV bool too_large(float x) { return !(fabsf(x) < 0x1p127f); }
 
 // A wave per run of four 256-element blocks, four elements per lane and block: a block's largest magnitude is a wave's
-// reduction, its codes 4 bytes per lane. Bound by its 16 bytes per element (543M: 8.7 GB in 1.46 ms); the 85 vector
+// reduction, its codes 4 bytes per lane. Bound by its 16 bytes per element (543M: 8.7 GB in 1.55 ms); the 89 vector
 // instructions per element, a hash of two quarter-rate products among them, run beside the streams.
 template <bool BF16, Stream S> DM_DEV void step8(const AdamArgs& a, const Control& c, const Update& u, const PlanTensor& t, long i0) {
   constexpr int N = CHUNK / BLOCK / 4;

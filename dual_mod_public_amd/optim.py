@@ -15,6 +15,9 @@ with, which the optimizer keeps allocated from then on (keep the optimizer as lo
 that the parameters changed: call ``mark_updated()`` after it where something watches their versions (GraphDecoder,
 SwiGLU.decode).
 
+A step whose tensors lie where they lay before is launches alone. One that finds a tensor moved writes the launch plan again,
+which waits for the device: let ``.grad`` stay (``zero_grad(set_to_none=False)``) or give ``grads`` where steps are short.
+
 8-bit states hold a byte per element and moment, and a byte per 256 elements and moment: blocks with a power-of-two
 scale, four significant bits per element, rounded stochastically by a hash of seed, step and element, so runs repeat
 bit for bit. A NaN or infinity in a state makes its block NaN; ``skip_nonfinite`` leaves such steps out.
