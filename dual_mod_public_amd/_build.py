@@ -14,7 +14,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libdm_hip.so")
-SOURCES = ["dm_lib.hip", "dm_bwd.hip", "dm_stack.hip", "dm_logprob.hip", "dm_optim.hip"]
+SOURCES = ["dm_lib.hip", "dm_bwd.hip", "dm_stack.hip", "dm_logprob.hip", "dm_optim.hip", "dm_paged.hip", "dm_drafts.hip"]
 HEADERS = ["dm_common.h", "dm_group.h", "dm_gemm.h", "dm_attn.h", "dm_kernels.h", "dm_decode.h", "dm_bwd.h", "dm_block.h", "dm_host.h",
            "dm_fwd_host.h", "dm_rows.h", "dm_prof.h", "dm_error.h", "../../include/dm_abi.h"]
 

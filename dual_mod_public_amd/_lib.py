@@ -144,6 +144,35 @@ class dm_adamw_args(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
+DM_PAGE_MAX = 1024        # include/dm_abi.h: rows of a page
+DM_PAGED_ROWS = 1 << 26    # rows of a sequence's table
+c_i64 = ctypes.c_int64
+
+
+class dm_paged_args(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("B", c_i32), ("h", c_i32), ("h_kv", c_i32), ("dh", c_i32), ("page", c_i32),
+                ("n_pages", c_i32), ("table_cols", c_i32), ("n_tokens", c_i32), ("window", c_i32), ("scale", ctypes.c_float),
+                ("reserved", c_i32), ("q", c_vp), ("q_token", c_i64), ("q_head", c_i64), ("K", c_vp), ("V", c_vp),
+                ("k_page", c_i64), ("v_page", c_i64), ("table", c_vp), ("lengths", c_vp), ("starts", c_vp), ("k_rows", c_vp),
+                ("k_token", c_i64), ("k_head", c_i64), ("v_rows", c_vp), ("v_token", c_i64), ("v_head", c_i64), ("o", c_vp),
+                ("lse", c_vp), ("weights", c_vp), ("workspace", c_vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class dm_evict_args(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("B", c_i32), ("h_kv", c_i32), ("dh", c_i32), ("page", c_i32), ("n_pages", c_i32),
+                ("table_cols", c_i32), ("new_cols", c_i32), ("keep", c_i32), ("sinks", c_i32), ("recent", c_i32),
+                ("reserved", c_i32), ("K", c_vp), ("V", c_vp), ("k_page", c_i64), ("v_page", c_i64), ("table", c_vp),
+                ("lengths", c_vp), ("new_table", c_vp), ("weights", c_vp), ("weights_out", c_vp), ("rows", c_vp),
+                ("lengths_out", c_vp)]
+
+
+class dm_verify_args(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("rows", c_i32), ("cols", c_i32), ("B", c_i32), ("logits", c_vp), ("ld", c_i64),
+                ("draft_logits", c_vp), ("ld_draft", c_i64), ("ids", c_vp), ("uniforms", c_vp), ("temperature", c_vp),
+                ("starts", c_vp), ("tokens", c_vp), ("accepted", c_vp), ("logp", c_vp), ("workspace", c_vp),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 P = ctypes.POINTER
 
 # name -> (restype, argtypes); every symbol include/dm_abi.h declares
@@ -201,6 +230,12 @@ SIGNATURES = {
     "dm_adamw_step_counted": (ctypes.c_int, [P(dm_adamw_args), c_vp, c_vp]),
     "dm_grad_norm": (ctypes.c_int, [P(dm_adamw_args), c_vp]),
     "dm_adamw_values": (ctypes.c_int, [c_vp, c_vp, ctypes.c_int64, c_i32, c_vp, c_vp]),
+    "dm_paged_workspace_bytes": (ctypes.c_size_t, [P(dm_paged_args)]),
+    "dm_paged_write": (ctypes.c_int, [P(dm_paged_args), c_vp]),
+    "dm_paged_attention": (ctypes.c_int, [P(dm_paged_args), c_vp]),
+    "dm_paged_evict": (ctypes.c_int, [P(dm_evict_args), c_vp]),
+    "dm_verify_workspace_bytes": (ctypes.c_size_t, [P(dm_verify_args)]),
+    "dm_verify_drafts": (ctypes.c_int, [P(dm_verify_args), c_vp]),
     "dm_argmax_rows": (ctypes.c_int, [c_i32, c_vp, c_i32, c_i32, ctypes.c_int64, c_vp, c_vp]),
     "dm_stack_fwd_plan_bytes": (ctypes.c_size_t, [P(dm_config), c_i32, P(dm_stack_layer), P(c_i32), c_i32, c_i32]),
     "dm_stack_fwd": (ctypes.c_int, [P(dm_config), c_i32, P(dm_stack_layer), c_fp, c_fp, P(c_i32), c_i32, c_i32,

@@ -1,0 +1,795 @@
+// Attention of new tokens over a paged cache (dm_paged_write, dm_paged_attention) and eviction from it
+// (dm_paged_evict).
+//
+// Sequence b has lengths[b] cached rows with its new tokens, whose rows are the last ones; row r lies in page
+// table[b, r / page] of [n_pages, h_kv, page, dh]. The query rows of a sequence and key head are its n tokens times
+// the g = h / h_kv heads that share the key head, token by token, in tiles of TILE_Q.
+//
+// How the work is split is decided on the device, from the lengths (a captured call is replayed with other ones): every
+// kernel derives the same plan from them (Plan), in which a sequence's rows are cut into as many pieces as bring the
+// whole call to about `want` pieces. Partial results of a query tile (unnormalised sums with their maximum) wait in the
+// workspace and k_paged_join adds them in the order of the pieces, so a call's results repeat bit for bit.
+#include "dm_common.h"
+#include "dm_error.h"
+
+#include <algorithm>
+
+using namespace dm;
+
+namespace {
+
+constexpr float INF = __builtin_inff(), NAN_ = __builtin_nanf("");
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int CUS = 256;
+constexpr int TILE_Q = 16;      // query rows of a tile
+constexpr int TILE_K = 64;      // cached rows that the plan counts in
+
+struct PagedArgs {
+  const void *q, *K, *V, *k_rows, *v_rows;
+  void* o;
+  float *lse, *weights, *part;         // part: the pieces' sums, then their maxima and sums of exponentials
+  const int32_t *table, *lengths, *starts;
+  long q_token, q_head, k_page, v_page, kr_token, kr_head, vr_token, vr_head;
+  int B, h, h_kv, g, n_pages, cols, page_shift, N, window;
+  float scale2;                        // scale log2 e
+  int want, least;                     // the plan: pieces wanted, least tiles of cached rows in one
+};
+
+// A sequence as the call gives it. A table that does not hold its rows, or fewer rows than new tokens: bad, NaN results.
+struct Seq {
+  int first, n, len;
+  bool bad;
+  DM_DEV Seq() : first(0), n(0), len(0), bad(false) {}
+  DM_DEV Seq(const PagedArgs& a, int b) {
+    len = a.lengths[b];
+    if (a.starts) {
+      first = min(max(a.starts[b], 0), a.N);
+      n = min(max(a.starts[b + 1], first), a.N) - first;
+    } else {
+      first = b;
+      n = len != 0;   // an empty place of the batch
+    }
+    bad = len < n || len > (a.cols << a.page_shift);
+    if (bad) len = n;
+  }
+  // rows [low, high) that token j reads (with a self pair its own row is not among them)
+  DM_DEV int high(const PagedArgs& a, int j) const { return len - n + j + (a.k_rows ? 0 : 1); }
+  DM_DEV int low(const PagedArgs& a, int j) const { return a.window ? max(0, len - n + j - a.window + 1) : 0; }
+  DM_DEV int tiles_k(const PagedArgs& a) const {   // of all its tokens' rows
+    if (n == 0 || bad) return 0;
+    return (max(0, high(a, n - 1) - (low(a, 0) & -TILE_K)) + TILE_K - 1) / TILE_K;
+  }
+};
+
+struct Item {
+  int b = -1;      // -1: there is none
+  Seq s;
+  int tile, piece, pieces, slot;   // slot of the query tile's piece 0 in the workspace, where pieces > 1
+};
+
+DM_DEV long wave_sum_long(long v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// The plan: sequence b's query tiles (of ROWS query rows; 1 with ROWS = 0) times its pieces, in order. PIECES: find item
+// number `at` of those; otherwise of the query tiles alone. Called by whole waves.
+template <int ROWS, bool PIECES> DM_DEV Item find_item(const PagedArgs& a, int at) {
+  const int lane = threadIdx.x & 63;
+  auto tiles_q = [&](const Seq& s) { return ROWS ? (s.n * a.g + ROWS - 1) / (ROWS ? ROWS : 1) : (s.n > 0); };
+  Seq s;
+  long cost = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    s = Seq(a, b);
+    cost += (long)tiles_q(s) * s.tiles_k(a);
+  }
+  cost = wave_sum_long(cost);
+  const int each = (int)max((long)a.least, (cost + a.want - 1) / a.want);   // tiles of cached rows per piece
+  Item it;
+  long done = 0, slots = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    if (a.B > 64) s = b < a.B ? Seq(a, b) : Seq();
+    const int tq = b < a.B ? tiles_q(s) : 0;
+    const int pieces = tq ? max(1, (s.tiles_k(a) + each - 1) / each) : 1;
+    const long mine = PIECES ? (long)tq * pieces : tq, kept = pieces > 1 ? (long)tq * pieces : 0;
+    long sum = mine, ksum = kept;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const long u = __shfl_up(sum, o, 64), ku = __shfl_up(ksum, o, 64);
+      if (lane >= o) sum += u, ksum += ku;
+    }
+    const uint64_t hit = __ballot(mine > 0 && done + sum > at);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      const int rest = (int)(at - (done + __shfl(sum - mine, l, 64)));
+      it.b = b0 + l;
+      it.s.first = __shfl(s.first, l, 64);
+      it.s.n = __shfl(s.n, l, 64);
+      it.s.len = __shfl(s.len, l, 64);
+      it.s.bad = __shfl((int)s.bad, l, 64);
+      it.pieces = __shfl(pieces, l, 64);
+      it.tile = PIECES ? rest / it.pieces : rest;
+      it.piece = PIECES ? rest % it.pieces : 0;
+      it.slot = (int)(slots + __shfl(ksum - kept, l, 64)) + it.tile * it.pieces;
+      return it;
+    }
+    done += __shfl(sum, 63, 64);
+    slots += __shfl(ksum, 63, 64);
+  }
+  return it;
+}
+
+// the item in scalar registers: every lane holds the same
+DM_DEV void make_uniform(Item& it) {
+  auto u = [](int& x) { x = __builtin_amdgcn_readfirstlane(x); };
+  u(it.b), u(it.s.first), u(it.s.n), u(it.s.len), u(it.tile), u(it.piece), u(it.pieces), u(it.slot);
+  it.s.bad = __builtin_amdgcn_readfirstlane((int)it.s.bad);
+}
+
+// ---- rows into the pages ---------------------------------------------------------------------
+// One thread per 16 bytes of a new token's key or value row.
+template <typename T> __global__ __launch_bounds__(256) void k_paged_write(PagedArgs a, int dh) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int per = dh / V;
+  const long each = (long)a.h_kv * per * 2, at = blockIdx.x * 256L + threadIdx.x;
+  if (at >= a.N * each) return;
+  const int t = (int)(at / each), rest = (int)(at % each);
+  const bool value = rest >= a.h_kv * per;
+  const int c = (rest / per) % a.h_kv, v = rest % per;
+  int b = t;
+  if (a.starts) {   // the last sequence that starts at t or before
+    int lo = 0, hi = a.B;
+    while (lo + 1 < hi) {
+      const int mid = (lo + hi) / 2;
+      if (a.starts[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+  }
+  const Seq s(a, b);
+  if (s.bad || t < s.first || t >= s.first + s.n) return;
+  const int row = s.len - s.n + (t - s.first);
+  const int page = a.table[(long)b * a.cols + (row >> a.page_shift)];
+  if (page < 0 || page >= a.n_pages) return;
+  const T* src = value ? (const T*)a.v_rows + t * a.vr_token + c * a.vr_head : (const T*)a.k_rows + t * a.kr_token + c * a.kr_head;
+  T* dst = value ? (T*)a.V + page * a.v_page : (T*)a.K + page * a.k_page;
+  dst += ((long)c << a.page_shift) * dh + (long)(row & ((1 << a.page_shift) - 1)) * dh;
+  *reinterpret_cast<u32x4*>(dst + v * V) = *reinterpret_cast<const u32x4*>(src + v * V);
+}
+
+// ---- the read ----------------------------------------------------------------------------------
+template <typename T, int DH> struct Tile {
+  static constexpr int KT = 32;                                   // cached rows of a wave's step
+  static constexpr int V = 16 / (int)sizeof(T);
+  static constexpr int LDV = DH + (sizeof(T) == 2 ? 16 : 4);      // 8 rows (fp32: 4 groups) fill the banks once
+  static constexpr int NF = DH * (int)sizeof(T) / 64;             // 16-byte loads of a lane for 16 rows in fragments
+  static constexpr int NV = KT * DH * (int)sizeof(T) / 1024;      // 16-byte loads of a lane for the step's V rows
+  static constexpr int VPR = DH / V;
+  static constexpr int NDT = DH / 16;
+};
+
+// S^T[16 cached rows][16 query rows] += K Q^T for one 16-byte chunk per lane of each: bf16 lane l holds columns
+// 8 (l / 16) .. + 7 of a 32-column step, fp32 4 (l / 16) .. + 3 of 16 columns (the same in K and Q, so the order of the
+// columns in an instruction does not matter).
+template <typename T> DM_DEV floatx4 mma_chunk(const u32x4& k, const u32x4& q, floatx4 acc) {
+  if constexpr (sizeof(T) == 2) {
+    return Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q), acc);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = Mfma<float>::mma(__uint_as_float(k[j]), __uint_as_float(q[j]), acc);
+    return acc;
+  }
+}
+
+// O^T[16 columns][16 query rows] += V^T P^T over 32 rows. Lane l's probabilities are those of rows 16 t + 4 (l / 16) + i
+// of query row l % 16, which is how the scores' tiles leave them; V's fragments take their rows in the same order.
+template <typename T, int LDV> DM_DEV floatx4 mma_values(const T* Vs, const float (&p)[2][4], floatx4 acc) {
+  const int lane = threadIdx.x & 63, grp = lane >> 4, s = lane & 15;
+  if constexpr (sizeof(T) == 2) {
+    const bf16* v = (const bf16*)Vs + (4 * grp + (s >> 2)) * LDV + 4 * (s & 3);
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 16 * LDV));
+    const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    bf16x8 pb;   // probabilities in [0, 1] rounded to bf16 beside values that are bf16 themselves; their sum is not
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pb[4 * t + i] = (bf16)p[t][i];
+    return Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, both), pb, acc);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc = Mfma<float>::mma(to_f(Vs[(16 * t + 4 * grp + i) * LDV + s]), p[t][i], acc);
+    return acc;
+  }
+}
+
+template <typename T> DM_DEV bool any_nonfinite(const u32x4& v) {
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 2) bad |= (v[j] & 0x7f80u) == 0x7f80u || (v[j] & 0x7f800000u) == 0x7f800000u;
+    else bad |= (v[j] & 0x7f800000u) == 0x7f800000u;
+  }
+  return bad;
+}
+
+// A step's rows [r0, r0 + 16 t .. + 16) lie in one page each (pages hold 16 rows or more and begin at a multiple of 16).
+// needed: some query of the tile reads some of them. A page outside the pool is read as page 0 and marks the sequence.
+DM_DEV long page_of(const PagedArgs& a, const int32_t* table, int r, bool needed, bool& bad) {
+  if (!needed) return 0;
+  const int p = __builtin_amdgcn_readfirstlane(table[r >> a.page_shift]);
+  if (p < 0 || p >= a.n_pages) {
+    bad = true;
+    return 0;
+  }
+  return p;
+}
+
+// One block: a query tile of 16 rows, a key head and a piece of its cached rows. The four waves take steps of 32 rows in
+// turn, each with a running maximum m and sum z per query row (scores in units of ln 2) and O^T in registers, and are
+// joined through LDS.
+template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_read(PagedArgs a) {
+  using C = Tile<T, DH>;
+  constexpr int VBYTES = C::KT * C::LDV * (int)sizeof(T), OBYTES = TILE_Q * DH * 4;
+  __shared__ __attribute__((aligned(16))) char smem[4 * (VBYTES > OBYTES ? VBYTES : OBYTES)];
+  __shared__ float sm[4][TILE_Q], sz[4][TILE_Q];
+  const int c = blockIdx.x % a.h_kv, lane = threadIdx.x & 63, grp = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Item it = find_item<TILE_Q, true>(a, blockIdx.x / a.h_kv);
+  if (it.b < 0) return;
+  make_uniform(it);
+  const Seq& s = it.s;
+  const int rows = s.n * a.g, rho0 = it.tile * TILE_Q;            // query rows of the sequence, the tile's first
+  const int j_first = rho0 / a.g, j_last = (min(rho0 + TILE_Q, rows) - 1) / a.g;
+  // the lane's query row
+  const int rho = rho0 + col, j = rho / a.g, head = c * a.g + rho % a.g;
+  const bool live = rho < rows;
+  const int high = live ? s.high(a, j) : 0, low = live ? s.low(a, j) : 0;
+  // the tile's rows, and this piece's
+  const int t_low = s.low(a, j_first), t_high = s.bad ? 0 : s.high(a, j_last);
+  const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
+  const int each = (tiles + it.pieces - 1) / it.pieces;
+  const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
+  // rows below this and from that on are read by all live query rows
+  const int all_low = s.low(a, j_last), all_high = s.high(a, j_first);
+
+  u32x4 qf[C::NF];
+  {
+    const T* q = (const T*)a.q + (long)(s.first + j) * a.q_token + (long)head * a.q_head;
+#pragma unroll
+    for (int i = 0; i < C::NF; ++i) qf[i] = live ? ld_global<u32x4>(q + i * 4 * C::V + grp * C::V) : u32x4{0, 0, 0, 0};
+  }
+  floatx4 O[C::NDT];
+#pragma unroll
+  for (int d = 0; d < C::NDT; ++d) O[d] = zero4();
+  float m = -INF, z = 0.f;    // z: this lane's share
+  if (a.k_rows && it.piece == 0 && wave == 0) {   // the self pair: one more row
+    const long kr = (long)(s.first + j) * a.kr_token + (long)c * a.kr_head, vr = (long)(s.first + j) * a.vr_token + (long)c * a.vr_head;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < C::NF; ++i) {
+      const u32x4 k = live ? ld_global<u32x4>((const T*)a.k_rows + kr + i * 4 * C::V + grp * C::V) : u32x4{0, 0, 0, 0};
+      float x[C::V], y[C::V];
+      unpack16<T>(uint4{k[0], k[1], k[2], k[3]}, x);
+      unpack16<T>(uint4{qf[i][0], qf[i][1], qf[i][2], qf[i][3]}, y);
+#pragma unroll
+      for (int e = 0; e < C::V; ++e) dot = fmaf(x[e], y[e], dot);
+    }
+    m = xor_sum<32>(xor_sum<16>(dot)) * a.scale2;
+    const float p = __builtin_amdgcn_exp2f(m - (m == -INF ? 0.f : m));
+    z = grp == 0 ? p : 0.f;
+#pragma unroll
+    for (int d = 0; d < C::NDT; ++d) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (live) unpack4<T>(ld_global<typename Raw4<T>::type>((const T*)a.v_rows + vr + 16 * d + 4 * grp), v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) O[d][i] = p * v[i];
+    }
+  }
+
+  const int32_t* table = a.table + (long)it.b * a.cols;
+  const int in_page = (1 << a.page_shift) - 1;
+  T* Vs = reinterpret_cast<T*>(smem) + wave * C::KT * C::LDV;
+  bool bad = s.bad;
+  u32x4 kf[2][C::NF], vf[C::NV];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int r = r0 + 16 * t;
+      const long page = page_of(a, table, r, r < t_high && r + 16 > t_low, bad);
+      const long off = (((long)c << a.page_shift) + (r & in_page)) * DH;
+      const T* K = (const T*)a.K + page * a.k_page + off;
+      const T* Vp = (const T*)a.V + page * a.v_page + off;
+#pragma unroll
+      for (int i = 0; i < C::NF; ++i) kf[t][i] = ld_global<u32x4>(K + col * DH + i * 4 * C::V + grp * C::V);
+#pragma unroll
+      for (int i = 0; i < C::NV / 2; ++i) {
+        const int v = i * 64 + lane;
+        vf[t * (C::NV / 2) + i] = ld_global<u32x4>(Vp + v * C::V);
+      }
+    }
+  };
+  int r0 = k0 + C::KT * wave;
+  if (r0 < k1) load(r0);
+  for (; r0 < k1; r0 += 4 * C::KT) {
+    const bool masked = r0 < all_low || r0 + C::KT > all_high;
+    bool odd = false;    // masked values that no probability of 0 may meet
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < C::NV / 2; ++i) {
+        const int v = i * 64 + lane, row = 16 * t + v / C::VPR;
+        u32x4 x = vf[t * (C::NV / 2) + i];
+        if (masked) {
+          if (r0 + row < t_low || r0 + row >= t_high) x = u32x4{0, 0, 0, 0};   // whatever lies there
+          odd |= any_nonfinite<T>(x);
+        }
+        *reinterpret_cast<u32x4*>(Vs + row * C::LDV + (v % C::VPR) * C::V) = x;
+      }
+    float p[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      floatx4 acc = zero4();
+#pragma unroll
+      for (int i = 0; i < C::NF; ++i) acc = mma_chunk<T>(kf[t][i], qf[i], acc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[t][i] = acc[i] * a.scale2;
+    }
+    if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT);
+    float top = -INF;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 16 * t + 4 * grp + i;
+        if (masked && (r < low || r >= high)) p[t][i] = -INF;
+        top = fmaxf(top, p[t][i]);
+      }
+    const float was = m;
+    m = fmaxf(m, xor_max<32>(xor_max<16>(top)));
+    const float ref = m == -INF ? 0.f : m;
+    const float alpha = __builtin_amdgcn_exp2f(was - ref);
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[t][i] = __builtin_amdgcn_exp2f(p[t][i] - ref);
+        sum += p[t][i];
+      }
+    z = z * alpha + sum;
+#pragma unroll
+    for (int d = 0; d < C::NDT; ++d) O[d] *= alpha;
+    __builtin_amdgcn_wave_barrier();   // LDS operations of one wave complete in order
+    if (masked && __ballot(odd)) {
+      // rows that some of the tile's queries do not read hold infinities or NaN, which a product with 0 would spread
+      for (int r = 0; r < C::KT; ++r) {
+        const int t = r >> 4, i = r & 3, from = ((r >> 2) & 3) * 16 + col;
+        float x = 0.f;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int ii = 0; ii < 4; ++ii) {
+            const float y = __shfl(p[tt][ii], from, 64);
+            if (tt == t && ii == i) x = y;
+          }
+        if (r0 + r < low || r0 + r >= high) continue;
+#pragma unroll
+        for (int d = 0; d < C::NDT; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[d][e] = fmaf(x, to_f(Vs[r * C::LDV + 16 * d + 4 * grp + e]), O[d][e]);
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < C::NDT; ++d) O[d] = mma_values<T, C::LDV>(Vs + 16 * d, p, O[d]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  z = xor_sum<32>(xor_sum<16>(z));
+  if (bad) z = NAN_;
+  if (grp == 0) sm[wave][col] = m, sz[wave][col] = z;
+  __syncthreads();
+  float M = fmaxf(fmaxf(sm[0][col], sm[1][col]), fmaxf(sm[2][col], sm[3][col]));
+  const float mine = __builtin_amdgcn_exp2f(m - (M == -INF ? 0.f : M));
+  float* Os = reinterpret_cast<float*>(smem) + wave * TILE_Q * DH;
+#pragma unroll
+  for (int d = 0; d < C::NDT; ++d)
+    *reinterpret_cast<floatx4*>(Os + col * DH + 16 * d + 4 * grp) = O[d] * mine;
+  __syncthreads();
+  // 16 threads per query row, DH / 16 columns each
+  constexpr int E = DH / 16;
+  const int row = threadIdx.x >> 4, e0 = (threadIdx.x & 15) * E;
+  M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row]));
+  const float ref = M == -INF ? 0.f : M;
+  float Z = 0.f, x[E];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) Z += sz[w][row] * __builtin_amdgcn_exp2f(sm[w][row] - ref);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    x[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x[e] += reinterpret_cast<float*>(smem)[(w * TILE_Q + row) * DH + e0 + e];
+  }
+  if (rho0 + row >= rows) return;
+  if (it.pieces > 1) {
+    const long at = ((long)(it.slot + it.piece) * a.h_kv + c) * TILE_Q + row;
+    float* part = a.part + at * (DH + 2);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<floatx2*>(part + e0 + e) = floatx2{x[e], x[e + 1]};
+    if (e0 == 0) *reinterpret_cast<floatx2*>(part + DH) = floatx2{M, Z};
+    return;
+  }
+  const long at = (long)(s.first + (rho0 + row) / a.g) * a.h + c * a.g + (rho0 + row) % a.g;
+  const float inv = Z == 0.f ? 0.f : 1.f / Z;
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = Z == 0.f ? 0.f : x[e] * inv;
+#pragma unroll
+  for (int e = 0; e < E; e += 4) st4<T>((T*)a.o + at * DH + e0 + e, x + e);
+  if (e0 == 0) a.lse[at] = Z == 0.f ? -INF : (ref + __builtin_amdgcn_logf(Z)) * LN2;
+}
+
+// The pieces of a query tile, in their order.
+template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
+  const int c = blockIdx.x % a.h_kv;
+  Item it = find_item<TILE_Q, false>(a, blockIdx.x / a.h_kv);
+  if (it.b < 0 || it.pieces == 1) return;
+  make_uniform(it);
+  constexpr int E = DH / 16;
+  const int row = threadIdx.x >> 4, e0 = (threadIdx.x & 15) * E, rho = it.tile * TILE_Q + row;
+  if (rho >= it.s.n * a.g) return;
+  const long step = (long)a.h_kv * TILE_Q * (DH + 2);
+  const float* part = a.part + (((long)it.slot * a.h_kv + c) * TILE_Q + row) * (DH + 2);
+  float M = -INF, Z = 0.f, x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = 0.f;
+  for (int i = 0; i < it.pieces; ++i) M = fmaxf(M, part[i * step + DH]);
+  const float ref = M == -INF ? 0.f : M;
+  for (int i = 0; i < it.pieces; ++i) {
+    const float* p = part + i * step;
+    const floatx2 mz = *reinterpret_cast<const floatx2*>(p + DH);
+    const float f = __builtin_amdgcn_exp2f(mz[0] - ref);
+    Z += f * mz[1];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const floatx2 v = *reinterpret_cast<const floatx2*>(p + e0 + e);
+      x[e] = fmaf(f, v[0], x[e]);
+      x[e + 1] = fmaf(f, v[1], x[e + 1]);
+    }
+  }
+  const long at = (long)(it.s.first + rho / a.g) * a.h + c * a.g + rho % a.g;
+  const float inv = 1.f / Z;
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = Z == 0.f ? 0.f : x[e] * inv;
+#pragma unroll
+  for (int e = 0; e < E; e += 4) st4<T>((T*)a.o + at * DH + e0 + e, x + e);
+  if (e0 == 0) a.lse[at] = Z == 0.f ? -INF : (ref + __builtin_amdgcn_logf(Z)) * LN2;
+}
+
+// ---- the weights -------------------------------------------------------------------------------
+// weights[b, c, r] += the sum over the sequence's query rows of exp(score - lse), the scores computed again: a wave holds
+// 32 cached rows as fragments and goes over all query tiles, so each weight has one writer and one order of its sum.
+template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_weights(PagedArgs a) {
+  using C = Tile<T, DH>;
+  const int c = blockIdx.x % a.h_kv, lane = threadIdx.x & 63, grp = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Item it = find_item<0, true>(a, blockIdx.x / a.h_kv);
+  if (it.b < 0) return;
+  make_uniform(it);
+  const Seq& s = it.s;
+  if (s.bad) return;
+  const int rows = s.n * a.g, t_low = s.low(a, 0), t_high = s.high(a, s.n - 1);
+  const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
+  const int each = (tiles + it.pieces - 1) / it.pieces;
+  const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
+  const int32_t* table = a.table + (long)it.b * a.cols;
+  const int in_page = (1 << a.page_shift) - 1;
+  float* w = a.weights + ((long)it.b * a.h_kv + c) * ((long)a.cols << a.page_shift);
+  for (int r0 = k0 + C::KT * wave; r0 < k1; r0 += 4 * C::KT) {
+    u32x4 kf[2][C::NF];
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int r = r0 + 16 * t;
+      const long page = page_of(a, table, r, r < t_high && r + 16 > t_low, bad);
+      const T* K = (const T*)a.K + page * a.k_page + (((long)c << a.page_shift) + (r & in_page)) * DH;
+#pragma unroll
+      for (int i = 0; i < C::NF; ++i) kf[t][i] = ld_global<u32x4>(K + col * DH + i * 4 * C::V + grp * C::V);
+    }
+    float sum[2][4] = {};
+    for (int rho0 = 0; rho0 < rows; rho0 += TILE_Q) {
+      const int rho = rho0 + col, j = rho / a.g, head = c * a.g + rho % a.g;
+      const bool live = rho < rows;
+      const long at = (long)(s.first + j) * a.h + head;
+      const int high = live ? s.high(a, j) : 0, low = live ? s.low(a, j) : 0;
+      const T* q = (const T*)a.q + (long)(s.first + j) * a.q_token + (long)head * a.q_head;
+      u32x4 qf[C::NF];
+#pragma unroll
+      for (int i = 0; i < C::NF; ++i) qf[i] = live ? ld_global<u32x4>(q + i * 4 * C::V + grp * C::V) : u32x4{0, 0, 0, 0};
+      const float lse2 = live ? a.lse[at] * LOG2E : 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        floatx4 acc = zero4();
+#pragma unroll
+        for (int i = 0; i < C::NF; ++i) acc = mma_chunk<T>(kf[t][i], qf[i], acc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = r0 + 16 * t + 4 * grp + i;
+          if (r >= low && r < high) sum[t][i] += __builtin_amdgcn_exp2f(fmaf(acc[i], a.scale2, -lse2));
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 16 * t + 4 * grp + i;
+        const float x = group16_sum(sum[t][i]);
+        if (col == 0 && r >= t_low && r < t_high) w[r] += bad ? NAN_ : x;
+      }
+  }
+}
+
+// ---- eviction ------------------------------------------------------------------------------------
+struct EvictArgs {
+  const void *K, *V;
+  void *K_out, *V_out;
+  const float* weights;
+  float* weights_out;
+  const int32_t *table, *lengths, *new_table;
+  int32_t *rows, *lengths_out;
+  long k_page, v_page;
+  int B, h, n_pages, cols, new_cols, page_shift, keep, sinks, recent;
+};
+
+// The order of weights as whole numbers (NaN above all, -0 as 0).
+DM_DEV uint32_t weight_order(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return x != x ? 0xffffffffu : (b >> 31 ? ~b : b | 0x80000000u);
+}
+
+// One block per sequence and key head: the weight of the last row to be kept by its bits, eight at a time from the top
+// (a histogram over the rows that agree so far), then the rows in order: those above it, and of those equal to it the first.
+__global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
+  __shared__ int hist[256], total[2][16], found[2];
+  const int c = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long cap = (long)a.cols << a.page_shift;
+  const int len = a.lengths[b] < 0 || a.lengths[b] > cap ? 0 : a.lengths[b];
+  const int left = min(len, a.keep);
+  int32_t* rows = a.rows + ((long)b * a.h + c) * a.keep;
+  if (c == 0 && threadIdx.x == 0) a.lengths_out[b] = left;
+  for (int i = left + threadIdx.x; i < a.keep; i += 1024) rows[i] = -1;
+  if (len <= a.keep) {
+    for (int i = threadIdx.x; i < left; i += 1024) rows[i] = i;
+    return;
+  }
+  const float* w = a.weights + ((long)b * a.h + c) * cap;
+  const int lo = a.sinks, hi = len - a.recent;      // rows that may go
+  uint32_t key = 0;
+  int need = a.keep - a.sinks - a.recent;           // of them stay (less than there are)
+  if (need > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+      __syncthreads();
+      const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+      for (int i = lo + threadIdx.x; i < hi; i += 1024) {
+        const uint32_t u = weight_order(w[i]);
+        if ((u & mask) == key) atomicAdd(&hist[(u >> shift) & 255], 1);
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int d = 255, above = 0;
+        while (d > 0 && above + hist[d] < need) above += hist[d--];
+        found[0] = d;
+        found[1] = above;
+      }
+      __syncthreads();
+      key |= (uint32_t)found[0] << shift;
+      need -= found[1];
+    }
+  } else {
+    key = 0xffffffffu;
+  }
+  // need: how many of the rows equal to key stay
+  int at = 0, equal = 0;
+  for (int i0 = 0; i0 < len; i0 += 1024) {
+    const int i = i0 + threadIdx.x;
+    bool sure = false, tie = false;
+    if (i < len) {
+      if (i < lo || i >= hi) sure = true;
+      else {
+        const uint32_t u = weight_order(w[i]);
+        sure = u > key;
+        tie = u == key;
+      }
+    }
+    const uint64_t bs = __ballot(sure), bt = __ballot(tie), before = (1ull << lane) - 1;
+    __syncthreads();
+    if (lane == 0) total[0][wave] = __popcll(bs), total[1][wave] = __popcll(bt);
+    __syncthreads();
+    int s = at + __popcll(bs & before), e = equal + __popcll(bt & before);
+    for (int k = 0; k < 16; ++k) {
+      if (k < wave) s += total[0][k], e += total[1][k];
+      at += total[0][k];
+      equal += total[1][k];
+    }
+    if (sure || (tie && e < need)) rows[s + min(e, need)] = i;
+  }
+}
+
+// One thread per 16 bytes of a kept row of K and of V.
+__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a, int row_bytes, int esize) {
+  const int c = blockIdx.y, b = blockIdx.z, per = row_bytes / 16;
+  const long at = blockIdx.x * 256L + threadIdx.x;
+  const long i = at / per;
+  const int v = (int)(at % per);
+  const long cap = (long)a.cols << a.page_shift, new_cap = (long)a.new_cols << a.page_shift;
+  if (i >= new_cap) return;
+  const int len = a.lengths[b] < 0 || a.lengths[b] > cap ? 0 : a.lengths[b];
+  const int left = min(len, a.keep), in_page = (1 << a.page_shift) - 1;
+  if (i >= left) {
+    if (v == 0) a.weights_out[((long)b * a.h + c) * new_cap + i] = 0.f;
+    return;
+  }
+  const int r = a.rows[((long)b * a.h + c) * a.keep + i];
+  if (v == 0) a.weights_out[((long)b * a.h + c) * new_cap + i] = a.weights[((long)b * a.h + c) * cap + r];
+  const int src = a.table[(long)b * a.cols + (r >> a.page_shift)], dst = a.new_table[(long)b * a.new_cols + (i >> a.page_shift)];
+  if (dst < 0 || dst >= a.n_pages) return;
+  const bool bad = src < 0 || src >= a.n_pages;
+  const long from = (((long)c << a.page_shift) + (r & in_page)) * row_bytes + v * 16;
+  const long to = (((long)c << a.page_shift) + (i & in_page)) * row_bytes + v * 16;
+  u32x4 k = {~0u, ~0u, ~0u, ~0u}, x = k;   // NaN in either type
+  if (!bad) {
+    k = *reinterpret_cast<const u32x4*>((const char*)a.K + src * a.k_page * esize + from);
+    x = *reinterpret_cast<const u32x4*>((const char*)a.V + src * a.v_page * esize + from);
+  }
+  *reinterpret_cast<u32x4*>((char*)a.K_out + dst * a.k_page * esize + to) = k;
+  *reinterpret_cast<u32x4*>((char*)a.V_out + dst * a.v_page * esize + to) = x;
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+int log2_of(int x) {
+  for (int i = 0; i < 31; ++i)
+    if (x == 1 << i) return i;
+  return -1;
+}
+
+// The plan's numbers for query tiles of `rows` rows: about four blocks per CU over the key heads, in pieces of 128 rows or
+// more (a step of each of a block's waves).
+int wanted(const dm_paged_args* a, int blocks) { return std::max(1, cdiv(blocks, a->h_kv)); }
+long query_tiles(const dm_paged_args* a, int rows) { return (long)a->n_tokens * (a->h / a->h_kv) / rows + a->B; }
+constexpr int READ_BLOCKS = 4 * CUS, READ_LEAST = 2, WEIGHT_BLOCKS = 8 * CUS;
+
+size_t part_floats(const dm_paged_args* a) { return (size_t)2 * wanted(a, READ_BLOCKS) * a->h_kv * TILE_Q * (a->dh + 2); }
+
+int check_pages(int dtype, int dh, int page, int n_pages, int cols, int B, int h_kv, const void* K, const void* V, int64_t k_page,
+                int64_t v_page) {
+  DM_REQUIRE(dtype == DM_BF16 || dtype == DM_F32, DM_ERR_INVALID, "dtype %d", dtype);
+  DM_REQUIRE(dh == 64 || dh == 128, DM_ERR_UNSUPPORTED, "dh=%d (64 or 128)", dh);
+  DM_REQUIRE(log2_of(page) >= 4 && page <= DM_PAGE_MAX, DM_ERR_UNSUPPORTED, "page=%d rows (a power of two, 16..%d)", page, DM_PAGE_MAX);
+  DM_REQUIRE(B > 0 && h_kv > 0 && n_pages > 0 && cols > 0 && (int64_t)cols * page <= DM_PAGED_ROWS, DM_ERR_INVALID,
+             "B=%d h_kv=%d n_pages=%d table_cols=%d of %d rows (at most %d rows)", B, h_kv, n_pages, cols, page, DM_PAGED_ROWS);
+  DM_REQUIRE(B <= 65535 && h_kv <= 65535, DM_ERR_INVALID, "B=%d h_kv=%d (at most 65535)", B, h_kv);
+  const int64_t least = (int64_t)h_kv * page * dh, unit = dtype == DM_BF16 ? 8 : 4;
+  DM_REQUIRE(K && V && aligned16(K) && aligned16(V) && k_page >= least && v_page >= least && k_page % unit == 0 && v_page % unit == 0,
+             DM_ERR_INVALID, "null or unaligned pages, strides %lld %lld (at least %lld, 16-byte steps)", (long long)k_page,
+             (long long)v_page, (long long)least);
+  return DM_OK;
+}
+
+int check_rows(const char* what, const void* p, int64_t token, int64_t head, int dtype) {
+  const int64_t unit = dtype == DM_BF16 ? 8 : 4;
+  DM_REQUIRE(p && aligned16(p) && token >= 0 && head >= 0 && token % unit == 0 && head % unit == 0, DM_ERR_INVALID,
+             "%s: null or unaligned, strides %lld %lld (16-byte steps)", what, (long long)token, (long long)head);
+  return DM_OK;
+}
+
+int check_paged(const dm_paged_args* a, bool write) {
+  DM_REQUIRE(a != nullptr, DM_ERR_INVALID, "null arguments");
+  if (const int rc = check_pages(a->dtype, a->dh, a->page, a->n_pages, a->table_cols, a->B, a->h_kv, a->K, a->V, a->k_page, a->v_page)) return rc;
+  DM_REQUIRE(a->n_tokens >= 0 && (a->starts || a->n_tokens == a->B), DM_ERR_INVALID,
+             "n_tokens=%d (without starts one per sequence, B=%d)", a->n_tokens, a->B);
+  DM_REQUIRE(a->table && a->lengths, DM_ERR_INVALID, "null table or lengths");
+  if (a->n_tokens == 0) return DM_OK;
+  DM_REQUIRE((int64_t)a->n_tokens * std::max(a->h_kv, write ? 0 : a->h) <= DM_PAGED_TOKENS, DM_ERR_INVALID,
+             "%d tokens of %d heads (at most %d rows)", a->n_tokens, std::max(a->h_kv, write ? 0 : a->h), DM_PAGED_TOKENS);
+  if (write || a->k_rows || a->v_rows) {
+    if (const int rc = check_rows("k_rows", a->k_rows, a->k_token, a->k_head, a->dtype)) return rc;
+    if (const int rc = check_rows("v_rows", a->v_rows, a->v_token, a->v_head, a->dtype)) return rc;
+  }
+  if (write) return DM_OK;
+  DM_REQUIRE(a->h > 0 && a->h % a->h_kv == 0 && a->h / a->h_kv <= 1024, DM_ERR_INVALID, "h=%d h_kv=%d", a->h, a->h_kv);
+  DM_REQUIRE(a->window >= 0 && a->scale == a->scale && a->scale > -INF && a->scale < INF, DM_ERR_INVALID, "window=%d scale=%g", a->window,
+             a->scale);
+  if (const int rc = check_rows("q", a->q, a->q_token, a->q_head, a->dtype)) return rc;
+  DM_REQUIRE(a->o && aligned16(a->o) && a->lse, DM_ERR_INVALID, "null or unaligned o, null lse");
+  const size_t need = dm_paged_workspace_bytes(a);
+  DM_REQUIRE(a->workspace_bytes >= need && (need == 0 || (a->workspace && aligned16(a->workspace))), DM_ERR_WORKSPACE,
+             "workspace %zu < %zu bytes", a->workspace_bytes, need);
+  return DM_OK;
+}
+
+PagedArgs paged(const dm_paged_args* a) {
+  PagedArgs r = {};
+  r.q = a->q, r.K = a->K, r.V = a->V, r.k_rows = a->k_rows, r.v_rows = a->v_rows, r.o = a->o, r.lse = a->lse, r.weights = a->weights;
+  r.part = (float*)a->workspace, r.table = a->table, r.lengths = a->lengths, r.starts = a->starts;
+  r.q_token = a->q_token, r.q_head = a->q_head, r.k_page = a->k_page, r.v_page = a->v_page;
+  r.kr_token = a->k_token, r.kr_head = a->k_head, r.vr_token = a->v_token, r.vr_head = a->v_head;
+  r.B = a->B, r.h = a->h, r.h_kv = a->h_kv, r.g = a->h_kv ? a->h / a->h_kv : 1, r.n_pages = a->n_pages, r.cols = a->table_cols;
+  r.page_shift = log2_of(a->page), r.N = a->n_tokens, r.window = a->window, r.scale2 = a->scale * LOG2E;
+  r.want = wanted(a, READ_BLOCKS), r.least = READ_LEAST;
+  return r;
+}
+
+template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStream_t s) {
+  PagedArgs p = paged(a);
+  const long tiles = query_tiles(a, TILE_Q);
+  hipLaunchKernelGGL((k_paged_read<T, DH>), dim3((unsigned)((p.want + tiles) * a->h_kv)), dim3(256), 0, s, p);
+  // pieces there are only where a sequence can have more tiles than the least of one piece
+  if ((int64_t)a->table_cols * a->page > READ_LEAST * TILE_K)
+    hipLaunchKernelGGL((k_paged_join<T, DH>), dim3((unsigned)(tiles * a->h_kv)), dim3(256), 0, s, p);
+  if (a->weights) {
+    p.want = wanted(a, WEIGHT_BLOCKS);
+    hipLaunchKernelGGL((k_paged_weights<T, DH>), dim3((unsigned)((p.want + (long)a->B) * a->h_kv)), dim3(256), 0, s, p);
+  }
+  DM_HIP(hipGetLastError());
+  return DM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dm_paged_workspace_bytes(const dm_paged_args* a) {
+  if (!a || a->h_kv <= 0 || a->B <= 0 || (a->dh != 64 && a->dh != 128)) return 0;
+  return part_floats(a) * 4;
+}
+
+int dm_paged_write(const dm_paged_args* a, void* stream) {
+  const int rc = check_paged(a, true);
+  if (rc || a->n_tokens == 0) return rc;
+  const PagedArgs p = paged(a);
+  const long n = (long)a->n_tokens * a->h_kv * 2 * (a->dh * (long)esz(a->dtype) / 16);
+  const dim3 grid((unsigned)((n + 255) / 256));
+  if (a->dtype == DM_BF16) hipLaunchKernelGGL(k_paged_write<bf16>, grid, dim3(256), 0, S(stream), p, a->dh);
+  else hipLaunchKernelGGL(k_paged_write<float>, grid, dim3(256), 0, S(stream), p, a->dh);
+  DM_HIP(hipGetLastError());
+  return DM_OK;
+}
+
+int dm_paged_attention(const dm_paged_args* a, void* stream) {
+  const int rc = check_paged(a, false);
+  if (rc || a->n_tokens == 0) return rc;
+  if (a->dtype == DM_BF16) return a->dh == 64 ? run_attention<bf16, 64>(a, S(stream)) : run_attention<bf16, 128>(a, S(stream));
+  return a->dh == 64 ? run_attention<float, 64>(a, S(stream)) : run_attention<float, 128>(a, S(stream));
+}
+
+int dm_paged_evict(const dm_evict_args* a, void* stream) {
+  DM_REQUIRE(a != nullptr, DM_ERR_INVALID, "null arguments");
+  if (const int rc = check_pages(a->dtype, a->dh, a->page, a->n_pages, a->table_cols, a->B, a->h_kv, a->K, a->V, a->k_page, a->v_page)) return rc;
+  const int64_t cap = (int64_t)a->table_cols * a->page, new_cap = (int64_t)a->new_cols * a->page;
+  DM_REQUIRE(a->keep > 0 && a->sinks >= 0 && a->recent >= 0 && (int64_t)a->sinks + a->recent <= a->keep, DM_ERR_INVALID,
+             "keep=%d sinks=%d recent=%d", a->keep, a->sinks, a->recent);
+  DM_REQUIRE(a->new_cols > 0 && new_cap <= DM_PAGED_ROWS && new_cap >= std::min<int64_t>(a->keep, cap), DM_ERR_INVALID,
+             "new_cols=%d pages do not hold %d rows", a->new_cols, a->keep);
+  DM_REQUIRE(a->table && a->lengths && a->new_table && a->weights && a->weights_out && a->rows && a->lengths_out, DM_ERR_INVALID,
+             "null argument");
+  DM_REQUIRE(a->weights != a->weights_out && a->lengths != a->lengths_out, DM_ERR_INVALID, "an output in an input's place");
+  EvictArgs p = {};
+  p.K = a->K, p.V = a->V, p.K_out = a->K, p.V_out = a->V, p.weights = a->weights, p.weights_out = a->weights_out;
+  p.table = a->table, p.lengths = a->lengths, p.new_table = a->new_table, p.rows = a->rows, p.lengths_out = a->lengths_out;
+  p.k_page = a->k_page, p.v_page = a->v_page, p.B = a->B, p.h = a->h_kv, p.n_pages = a->n_pages, p.cols = a->table_cols;
+  p.new_cols = a->new_cols, p.page_shift = log2_of(a->page), p.keep = a->keep, p.sinks = a->sinks, p.recent = a->recent;
+  const int bytes = a->dh * (int)esz(a->dtype);
+  hipLaunchKernelGGL(k_evict_select, dim3(a->h_kv, a->B), dim3(1024), 0, S(stream), p);
+  hipLaunchKernelGGL(k_evict_move, dim3((unsigned)((new_cap * (bytes / 16) + 255) / 256), a->h_kv, a->B), dim3(256), 0, S(stream), p, bytes,
+                     (int)esz(a->dtype));
+  DM_HIP(hipGetLastError());
+  return DM_OK;
+}
+
+}  // extern "C"

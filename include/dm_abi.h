@@ -618,6 +618,92 @@ int dm_grad_norm(const dm_adamw_args* a, void* stream);
 int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_blocks, int32_t second, void* out,
                     void* stream);
 
+/* ---- a paged cache -----------------------------------------------------------------------
+ * B sequences of different lengths. Pages K, V [n_pages, h_kv, page, dh] (a page's h_kv * page rows contiguous, pages k_page /
+ * v_page elements apart, 16-byte aligned; page a power of two, 16..DM_PAGE_MAX); row r of sequence b lies in page
+ * table[b, r / page] (int32 [B, table_cols], unused entries anything). lengths [B]: cached rows, the new tokens' among
+ * them; starts [B + 1]: the new tokens starts[b] .. starts[b + 1] - 1 (0 or more) of sequence b, whose token j has row
+ * lengths[b] - n + j; NULL: one token per sequence, none where lengths[b] is 0. All three lie on the device and may change between replays of a
+ * captured call. Tokens of no sequence (behind starts[B]) are neither read nor written,
+ * nor are their rows of o and lse.
+ * A sequence that its table does not hold (lengths[b] > table_cols * page, or less than its new tokens), or one that reads a
+ * page outside [0, n_pages), gets NaN; what such a page would be written is left out.
+ *
+ * dm_paged_write: the tokens' rows k_rows, v_rows [n_tokens, h_kv, dh] (any token and head strides) into the pages.
+ * dm_paged_attention: for query head a of key head a / (h / h_kv) and a token with row p, over the rows r <= p with
+ *   r > p - window (window 0: all),   s_r = scale q . K[r],  lse = log sum e^s,  o = sum e^(s - lse) V[r]
+ *   (fp32; bf16: the probabilities rounded to bf16 before the product with V). With k_rows, v_rows: r < p, and the token's own
+ *   pair takes the place of row p (the raw self pair of dm_attend_one; row p itself is not read). Rows that a token does
+ *   not read do not reach its result, whatever they hold; a token that reads nothing: o 0, lse -inf. o [n_tokens, h, dh]
+ *   storage dtype, lse [n_tokens, h] fp32, both contiguous.
+ *   weights (fp32 [B, h_kv, table_cols * page], may be NULL): weights[b, c, r] += the sum over b's new tokens and the heads
+ *   of c of e^(s_r - lse), for the rows that are read. One writer per weight, in a fixed order.
+ * Workspace: dm_paged_workspace_bytes(a) (from the sizes alone), 16-byte aligned, not shared by calls that may overlap.
+ * At most DM_PAGED_ROWS rows per sequence, n_tokens * h at most DM_PAGED_TOKENS. */
+#define DM_PAGE_MAX 1024
+#define DM_PAGED_ROWS (1 << 26)
+#define DM_PAGED_TOKENS (1 << 27)
+typedef struct dm_paged_args {
+  int32_t dtype, B, h, h_kv, dh;             /* dh 64 or 128 */
+  int32_t page, n_pages, table_cols, n_tokens;
+  int32_t window;
+  float scale; int32_t reserved;
+  const void* q; int64_t q_token, q_head;    /* [n_tokens, h, dh], strides in elements, 16-byte steps */
+  void* K; void* V; int64_t k_page, v_page;
+  const int32_t* table; const int32_t* lengths; const int32_t* starts;
+  const void* k_rows; int64_t k_token, k_head;
+  const void* v_rows; int64_t v_token, v_head;
+  void* o; float* lse; float* weights;
+  void* workspace; size_t workspace_bytes;
+} dm_paged_args;
+size_t dm_paged_workspace_bytes(const dm_paged_args* a);
+int dm_paged_write(const dm_paged_args* a, void* stream);
+int dm_paged_attention(const dm_paged_args* a, void* stream);
+
+/* dm_paged_evict: of each sequence and key head the rows 0 .. sinks - 1, the last `recent` ones and those of the others with
+ * the largest weights (of equal ones the lower row; a NaN before every number), min(lengths[b], keep) in all, copied in their
+ * order to rows 0, 1, ... of the pages new_table [B, new_cols] (which hold min(keep, table_cols * page) rows), with their
+ * weights: weights_out [B, h_kv, new_cols * page], 0 behind them. rows [B, h_kv, keep]: the rows kept, -1 behind them;
+ * lengths_out [B]. The new pages are none that a table of the call names (pages that sequences share may be read, so a
+ * shared prefix stays). A length that the table does not hold counts as 0; rows of a page outside the pool become NaN. */
+typedef struct dm_evict_args {
+  int32_t dtype, B, h_kv, dh;
+  int32_t page, n_pages, table_cols, new_cols;
+  int32_t keep, sinks, recent, reserved;
+  void* K; void* V; int64_t k_page, v_page;
+  const int32_t* table; const int32_t* lengths; const int32_t* new_table;
+  const float* weights; float* weights_out;
+  int32_t* rows; int32_t* lengths_out;
+} dm_evict_args;
+int dm_paged_evict(const dm_evict_args* a, void* stream);
+
+/* ---- drafted tokens ------------------------------------------------------------------------
+ * Sequence b's rows starts[b] .. starts[b + 1] - 1 of logits [rows, cols] (storage dtype bf16 or fp32, row stride ld): row
+ * t is the target's distribution p = softmax(x / T) after input token ids[t], and ids[t + 1] the token drafted for it (the last row of a
+ * sequence has none), from q = softmax(y / T) of draft_logits' row t, or with NULL for certain (q = 1 at it).
+ *   accepted at row t: uniforms[t, 0] q(d) < p(d)
+ *   The sequence's first row without an accepted draft gets the first token v with sum_{w <= v} r_w > uniforms[t, 1] sum r,
+ *   r = max(p - q, 0); r = p in its last row, and where r is 0.
+ *   temperature[b] = 0: accepted where the draft is the first of the largest logits, which is the token otherwise.
+ * tokens [rows]: the accepted drafts and the new token, each at the row it was predicted by; -1 behind them, in rows of no
+ * sequence and where the row that ends the sequence is no distribution (a NaN, +inf, nothing but -inf; greedy: a NaN, nothing but
+ * -inf). accepted [B]: drafts accepted. logp [rows]: the tokens' target log probabilities (at T = 1 where T is 0), 0 where there is
+ * none, NaN where there is no distribution. A draft outside [0, cols) is not accepted. Probabilities, sums and places in 64 bits.
+ * At most 65535 rows and sequences. */
+typedef struct dm_verify_args {
+  int32_t dtype, rows, cols, B;
+  const void* logits; int64_t ld;
+  const void* draft_logits; int64_t ld_draft;
+  const int64_t* ids;                        /* [rows] */
+  const float* uniforms;                     /* [rows, 2], in [0, 1) */
+  const float* temperature;                  /* [B], 0 or more */
+  const int32_t* starts;                     /* [B + 1] */
+  int64_t* tokens; int32_t* accepted; float* logp;
+  void* workspace; size_t workspace_bytes;
+} dm_verify_args;
+size_t dm_verify_workspace_bytes(const dm_verify_args* a);
+int dm_verify_drafts(const dm_verify_args* a, void* stream);
+
 /* ---- RMSNorm weight gradient -----------------------------------------------------------
  * dw [d] fp32 += sum over the M rows of dy x r (dy, x [M, d] storage dtype, r [M] fp32 the rows' scales
  * rsqrt(mean x^2 + eps)): attention.py:74-83's weight, summed in a fixed order over 64 chunks of rows.
