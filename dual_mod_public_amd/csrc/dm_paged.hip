@@ -111,6 +111,7 @@ template <int ROWS, bool PIECES> DM_DEV Item find_item(const PagedArgs& a, int a
       it.s.bad = __shfl((int)s.bad, l, 64);
       it.pieces = __shfl(pieces, l, 64);
       it.tile = PIECES ? rest / it.pieces : rest;
+      if (ROWS) it.tile = __shfl(tq, l, 64) - 1 - it.tile;      // the tiles with the most rows to read first
       it.piece = PIECES ? rest % it.pieces : 0;
       it.slot = (int)(slots + __shfl(ksum - kept, l, 64)) + it.tile * it.pieces;
       return it;
@@ -185,29 +186,6 @@ template <typename T> DM_DEV floatx4 mma_chunk(const u32x4& k, const u32x4& q, f
 
 // O^T[16 columns][16 query rows] += V^T P^T over 32 rows. Lane l's probabilities are those of rows 16 t + 4 (l / 16) + i
 // of query row l % 16, which is how the scores' tiles leave them; V's fragments take their rows in the same order.
-template <typename T, int LDV> DM_DEV floatx4 mma_values(const T* Vs, const float (&p)[2][4], floatx4 acc) {
-  const int lane = threadIdx.x & 63, grp = lane >> 4, s = lane & 15;
-  if constexpr (sizeof(T) == 2) {
-    const bf16* v = (const bf16*)Vs + (4 * grp + (s >> 2)) * LDV + 4 * (s & 3);
-    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
-    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 16 * LDV));
-    const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    bf16x8 pb;   // probabilities in [0, 1] rounded to bf16 beside values that are bf16 themselves; their sum is not
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pb[4 * t + i] = (bf16)p[t][i];
-    return Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, both), pb, acc);
-  } else {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        acc = Mfma<float>::mma(to_f(Vs[(16 * t + 4 * grp + i) * LDV + s]), p[t][i], acc);
-    return acc;
-  }
-}
-
 template <typename T> DM_DEV bool any_nonfinite(const u32x4& v) {
   bool bad = false;
 #pragma unroll
@@ -216,6 +194,80 @@ template <typename T> DM_DEV bool any_nonfinite(const u32x4& v) {
     else bad |= (v[j] & 0x7f800000u) == 0x7f800000u;
   }
   return bad;
+}
+
+// Steps in which a query row does not read every row, and some value among them is not finite: a product with a probability
+// of 0 would make it NaN. Such values count 0 in the product, and a second one, of 1 for each row that is read with 1 for
+// +inf, 2^7 for -inf and 2^14 for NaN (at most 64 rows of a step, exact in bf16 and fp32), says what to add.
+DM_DEV uint32_t code_of(bool nonfinite, bool nan, bool negative, uint32_t one, uint32_t two7, uint32_t two14) {
+  return !nonfinite ? 0u : nan ? two14 : negative ? two7 : one;
+}
+DM_DEV i16x8 split_nonfinite(i16x8& v) {
+  i16x8 code;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = (uint16_t)v[i];
+    const bool odd = (u & 0x7f80u) == 0x7f80u;
+    code[i] = (short)code_of(odd, u & 0x7fu, u >> 15, 0x3f80u, 0x4300u, 0x4680u);
+    if (odd) v[i] = 0;
+  }
+  return code;
+}
+DM_DEV float split_nonfinite(float& v) {
+  const uint32_t u = __float_as_uint(v);
+  const bool odd = (u & 0x7f800000u) == 0x7f800000u;
+  if (odd) v = 0.f;
+  return __uint_as_float(code_of(odd, u & 0x7fffffu, u >> 31, 0x3f800000u, 0x43000000u, 0x46800000u));
+}
+DM_DEV float said_by(float code) {
+  const int c = (int)code;
+  float x = 0.f;
+  if (c & 0x7f) x += INF;
+  if ((c >> 7) & 0x7f) x -= INF;
+  if (c >> 14) x = NAN_;
+  return x;
+}
+
+// O^T[16 columns][16 query rows] += V^T P^T over 32 rows. Lane l's probabilities are those of rows 16 t + 4 (l / 16) + i
+// of query row l % 16, which is how the scores' tiles leave them; V's fragments take their rows in the same order.
+// The probabilities are rounded to bf16 beside values that are bf16 themselves; their sum z is not. ODD: see
+// split_nonfinite; read: the rows that the query row reads.
+DM_DEV i16x8 values_fragment(const bf16* v, int ldv) {
+  const int lane = threadIdx.x & 63, grp = lane >> 4, s = lane & 15;
+  v += (4 * grp + (s >> 2)) * ldv + 4 * (s & 3);
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
+  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 16 * ldv));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int N> DM_DEV bf16x8 to_bf16x8(const float (&p)[N], int at) {
+  bf16x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (bf16)p[at + i];
+  return r;
+}
+template <typename T, int LDV, bool ODD> DM_DEV floatx4 mma_values(const T* Vs, const float (&p)[8], const float (&read)[8], floatx4 acc) {
+  floatx4 said = zero4();
+  if constexpr (sizeof(T) == 2) {
+    i16x8 v = values_fragment((const bf16*)Vs, LDV);
+    if constexpr (ODD) {
+      const i16x8 code = split_nonfinite(v);
+      said = Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, code), to_bf16x8(read, 0), said);
+    }
+    acc = Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, v), to_bf16x8(p, 0), acc);
+  } else {
+    const int lane = threadIdx.x & 63, grp = lane >> 4, s = lane & 15;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = to_f(Vs[(16 * (i >> 2) + 4 * grp + (i & 3)) * LDV + s]);
+      if constexpr (ODD) said = Mfma<float>::mma(split_nonfinite(v), read[i], said);
+      acc = Mfma<float>::mma(v, p[i], acc);
+    }
+  }
+  if constexpr (ODD) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += said_by(said[i]);
+  }
+  return acc;
 }
 
 // A step's rows [r0, r0 + 16 t .. + 16) lie in one page each (pages hold 16 rows or more and begin at a multiple of 16).
@@ -331,62 +383,49 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
         }
         *reinterpret_cast<u32x4*>(Vs + row * C::LDV + (v % C::VPR) * C::V) = x;
       }
-    float p[2][4];
+    float p[8];      // of rows r0 + 16 (i / 4) + 4 grp + i % 4
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       floatx4 acc = zero4();
 #pragma unroll
       for (int i = 0; i < C::NF; ++i) acc = mma_chunk<T>(kf[t][i], qf[i], acc);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[t][i] = acc[i] * a.scale2;
+      for (int i = 0; i < 4; ++i) p[4 * t + i] = acc[i] * a.scale2;
     }
     if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT);
+    float read[8];
     float top = -INF;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + 16 * (i >> 2) + 4 * grp + (i & 3);
+      const bool hidden = masked && (r < low || r >= high);
+      read[i] = hidden ? 0.f : 1.f;
+      if (hidden) p[i] = -INF;
+      top = fmaxf(top, p[i]);
+    }
+    top = xor_max<32>(xor_max<16>(top));
+    // the reference follows the maximum only where that has risen by 2^8: sums and probabilities are relative to it
+    if (__ballot(top > m + 8.f)) {
+      const float was = m;
+      m = fmaxf(m, top);
+      const float alpha = __builtin_amdgcn_exp2f(was - (m == -INF ? 0.f : m));
+      z *= alpha;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + 16 * t + 4 * grp + i;
-        if (masked && (r < low || r >= high)) p[t][i] = -INF;
-        top = fmaxf(top, p[t][i]);
-      }
-    const float was = m;
-    m = fmaxf(m, xor_max<32>(xor_max<16>(top)));
+      for (int d = 0; d < C::NDT; ++d) O[d] *= alpha;
+    }
     const float ref = m == -INF ? 0.f : m;
-    const float alpha = __builtin_amdgcn_exp2f(was - ref);
-    float sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[t][i] = __builtin_amdgcn_exp2f(p[t][i] - ref);
-        sum += p[t][i];
-      }
-    z = z * alpha + sum;
-#pragma unroll
-    for (int d = 0; d < C::NDT; ++d) O[d] *= alpha;
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(p[i] - ref);
+      z += p[i];
+    }
     __builtin_amdgcn_wave_barrier();   // LDS operations of one wave complete in order
     if (masked && __ballot(odd)) {
-      // rows that some of the tile's queries do not read hold infinities or NaN, which a product with 0 would spread
-      for (int r = 0; r < C::KT; ++r) {
-        const int t = r >> 4, i = r & 3, from = ((r >> 2) & 3) * 16 + col;
-        float x = 0.f;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int ii = 0; ii < 4; ++ii) {
-            const float y = __shfl(p[tt][ii], from, 64);
-            if (tt == t && ii == i) x = y;
-          }
-        if (r0 + r < low || r0 + r >= high) continue;
-#pragma unroll
-        for (int d = 0; d < C::NDT; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) O[d][e] = fmaf(x, to_f(Vs[r * C::LDV + 16 * d + 4 * grp + e]), O[d][e]);
-      }
+      for (int d = 0; d < C::NDT; ++d) O[d] = mma_values<T, C::LDV, true>(Vs + 16 * d, p, read, O[d]);
     } else {
 #pragma unroll
-      for (int d = 0; d < C::NDT; ++d) O[d] = mma_values<T, C::LDV>(Vs + 16 * d, p, O[d]);
+      for (int d = 0; d < C::NDT; ++d) O[d] = mma_values<T, C::LDV, false>(Vs + 16 * d, p, read, O[d]);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -433,17 +472,264 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
   if (e0 == 0) a.lse[at] = Z == 0.f ? -INF : (ref + __builtin_amdgcn_logf(Z)) * LN2;
 }
 
+// ---- the read of many query rows -------------------------------------------------------------------
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+DM_DEV floatx16 mma32(const u32x4& a, const u32x4& b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// V^T's fragment for 32 columns and 16 rows: lane l column l % 32, rows 4 (l / 32) + 0..3 and 8 + those, the order in which
+// a 32 x 32 tile of scores leaves its rows to its lanes.
+DM_DEV i16x8 values_fragment32(const bf16* v, int ldv) {
+  const int lane = threadIdx.x & 63, s = lane & 15;
+  v += (4 * (lane >> 5) + (s >> 2)) * ldv + 16 * ((lane >> 4) & 1) + 4 * (s & 3);
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
+  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * ldv));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <int DH> struct WideTile {
+  static constexpr int KT = 64;            // cached rows of a step
+  static constexpr int LDK = DH + 8;       // 16 rows' 16-byte pieces fill the banks once
+  static constexpr int LDV = DH + 32;      // 4 rows' 64-byte pieces do
+  static constexpr int BUF = KT * (LDK + LDV);
+  static constexpr int VPR = DH / 8, NK = DH / 16, ND = DH / 32;
+};
+
+// One block: a tile of 32 NW query rows (32 per wave), a key head and a piece of its cached rows, which pass through LDS in
+// steps of 64 that all waves share (two buffers, the next step's rows on their way in registers). Scores as 32 x 32 tiles
+// S^T = K Q^T: a lane holds one query row's scores, so maximum and sum need one exchange per step.
+template <int DH, int NW> __global__ __launch_bounds__(64 * NW) void k_paged_read_wide(PagedArgs a) {
+  using C = WideTile<DH>;
+  constexpr int NT = 64 * NW, ROWS = 32 * NW, NL = C::KT * C::VPR / NT;    // 16-byte loads per thread of K and of V
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  bf16* lds = reinterpret_cast<bf16*>(smem);
+  __shared__ int odd_step[2];
+  const int c = blockIdx.x % a.h_kv, lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Item it = find_item<ROWS, true>(a, blockIdx.x / a.h_kv);
+  if (it.b < 0) return;
+  make_uniform(it);
+  const Seq& s = it.s;
+  const int rows = s.n * a.g, rho0 = it.tile * ROWS;
+  const int j_first = rho0 / a.g, j_last = (min(rho0 + ROWS, rows) - 1) / a.g;
+  const int rho = rho0 + 32 * wave + col, j = rho / a.g, head = c * a.g + rho % a.g;
+  const bool live = rho < rows;
+  const int high = live ? s.high(a, j) : 0, low = live ? s.low(a, j) : 0;
+  const int t_low = s.low(a, j_first), t_high = s.bad ? 0 : s.high(a, j_last);
+  const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
+  const int each = (tiles + it.pieces - 1) / it.pieces;
+  const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
+  // rows that all, and that any, of the wave's live query rows read
+  const int w_first = min(rho0 + 32 * wave, rows - 1) / a.g, w_last = min(rho0 + 32 * wave + 31, rows - 1) / a.g;
+  const int all_low = s.low(a, w_last), all_high = s.high(a, w_first), any_low = s.low(a, w_first), any_high = s.high(a, w_last);
+
+  u32x4 qf[C::NK];
+  {
+    const bf16* q = (const bf16*)a.q + (long)(s.first + j) * a.q_token + (long)head * a.q_head;
+    const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;    // the maximum is taken before the scale
+#pragma unroll
+    for (int i = 0; i < C::NK; ++i) {
+      qf[i] = live ? ld_global<u32x4>(q + 16 * i + 8 * half) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[i][e] = a.scale2 == 0.f ? 0u : qf[i][e] ^ flip;
+    }
+  }
+  const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
+  floatx16 O[C::ND];
+#pragma unroll
+  for (int d = 0; d < C::ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) O[d][i] = 0.f;
+  float m = -INF, z = 0.f;     // z: this lane's share
+  if (a.k_rows && it.piece == 0) {
+    const long kr = (long)(s.first + j) * a.kr_token + (long)c * a.kr_head, vr = (long)(s.first + j) * a.vr_token + (long)c * a.vr_head;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < C::NK; ++i) {
+      const u32x4 k = live ? ld_global<u32x4>((const bf16*)a.k_rows + kr + 16 * i + 8 * half) : u32x4{0, 0, 0, 0};
+      float x[8], y[8];
+      unpack16<bf16>(uint4{k[0], k[1], k[2], k[3]}, x);
+      unpack16<bf16>(uint4{qf[i][0], qf[i][1], qf[i][2], qf[i][3]}, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
+    }
+    m = xor_sum<32>(dot) * scale2;
+    const float p = __builtin_amdgcn_exp2f(m - (m == -INF ? 0.f : m));
+    z = half == 0 ? p : 0.f;
+#pragma unroll
+    for (int d = 0; d < C::ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (live) unpack4<bf16>(ld_global<u32x2>((const bf16*)a.v_rows + vr + 32 * d + 8 * i + 4 * half), v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[d][4 * i + e] = p * v[e];
+      }
+  }
+
+  const int32_t* table = a.table + (long)it.b * a.cols;
+  const int in_page = (1 << a.page_shift) - 1;
+  bool bad = s.bad;
+  u32x4 kx[NL], vx[NL];
+  // a wave's load takes 64 / VPR (4 or 8) rows: of one page
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int v = i * NT + threadIdx.x, row = v / C::VPR;
+      const int r = r0 + (i * NT + 64 * wave) / C::VPR;
+      const long page = page_of(a, table, r, r < t_high && r + 64 / C::VPR > t_low, bad);
+      const long off = (((long)c << a.page_shift) + ((r0 + row) & in_page)) * DH + (v % C::VPR) * 8;
+      kx[i] = ld_global<u32x4>((const bf16*)a.K + page * a.k_page + off);
+      vx[i] = ld_global<u32x4>((const bf16*)a.V + page * a.v_page + off);
+    }
+  };
+  auto store = [&](int r0, int buf) {
+    bf16* Ks = lds + buf * C::BUF;
+    bf16* Vs = Ks + C::KT * C::LDK;
+    const bool edge = r0 < s.low(a, j_last) || r0 + C::KT > s.high(a, j_first);   // some query row does not read all of it
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int v = i * NT + threadIdx.x, row = v / C::VPR, e = (v % C::VPR) * 8;
+      if (edge) {
+        if (r0 + row < t_low || r0 + row >= t_high) vx[i] = u32x4{0, 0, 0, 0};    // whatever lies there
+        odd |= any_nonfinite<bf16>(vx[i]);
+      }
+      *reinterpret_cast<u32x4*>(Ks + row * C::LDK + e) = kx[i];
+      *reinterpret_cast<u32x4*>(Vs + row * C::LDV + e) = vx[i];
+    }
+    if (odd) odd_step[buf] = r0;
+  };
+  if (threadIdx.x < 2) odd_step[threadIdx.x] = -1;
+  if (k0 < k1) load(k0);
+  __syncthreads();
+  if (k0 < k1) store(k0, 0);
+  __syncthreads();
+  int buf = 0;
+  for (int r0 = k0; r0 < k1; r0 += C::KT, buf ^= 1) {
+    const bool more = r0 + C::KT < k1;
+    if (more) load(r0 + C::KT);
+    if (r0 < any_high && r0 + C::KT > any_low) {
+      const bf16* Ks = lds + buf * C::BUF;
+      const bf16* Vs = Ks + C::KT * C::LDK;
+      const bool masked = r0 < all_low || r0 + C::KT > all_high;
+      float p[32];      // of rows r0 + 8 (i / 4) + 4 half + i % 4
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        floatx16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::NK; ++i)
+          acc = mma32(*reinterpret_cast<const u32x4*>(Ks + (32 * t + col) * C::LDK + 16 * i + 8 * half), qf[i], acc);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[16 * t + i] = acc[i];
+      }
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int r = r0 + 8 * (i >> 2) + 4 * half + (i & 3);
+          if (r < low || r >= high) p[i] = -INF;
+        }
+      }
+      float top = -INF;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) top = fmaxf(top, p[i]);
+      top = xor_max<32>(top) * scale2;
+      if (__ballot(top > m + 8.f)) {
+        const float was = m;
+        m = fmaxf(m, top);
+        const float alpha = __builtin_amdgcn_exp2f(was - (m == -INF ? 0.f : m));
+        z *= alpha;
+#pragma unroll
+        for (int d = 0; d < C::ND; ++d) O[d] *= alpha;
+      }
+      const float ref = m == -INF ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], scale2, -ref));
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sum[i & 3] += p[i];
+      z += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (masked && odd_step[buf] == r0) {
+        float read[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int r = r0 + 8 * (i >> 2) + 4 * half + (i & 3);
+          read[i] = r < low || r >= high ? 0.f : 1.f;
+        }
+#pragma unroll
+        for (int d = 0; d < C::ND; ++d) {
+          floatx16 said;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) said[i] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            i16x8 v = values_fragment32(Vs + 16 * k * C::LDV + 32 * d, C::LDV);
+            const i16x8 code = split_nonfinite(v);
+            said = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, code), to_bf16x8(read, 8 * k), said, 0, 0, 0);
+            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), to_bf16x8(p, 8 * k), O[d], 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) O[d][i] += said_by(said[i]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bf16x8 pb = to_bf16x8(p, 8 * k);
+#pragma unroll
+          for (int d = 0; d < C::ND; ++d)
+            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values_fragment32(Vs + 16 * k * C::LDV + 32 * d, C::LDV)),
+                                                           pb, O[d], 0, 0, 0);
+        }
+      }
+    }
+    if (more) store(r0 + C::KT, buf ^ 1);
+    __syncthreads();
+  }
+  z = xor_sum<32>(z);
+  // a page outside the pool is seen by the waves whose rows lie there
+  if (threadIdx.x == 0) odd_step[0] = 0;
+  __syncthreads();
+  if (bad) odd_step[0] = 1;
+  __syncthreads();
+  if (odd_step[0]) z = NAN_;
+  if (!live) return;
+  const float ref = m == -INF ? 0.f : m;
+  if (it.pieces > 1) {
+    float* part = a.part + (((long)(it.slot + it.piece) * a.h_kv + c) * ROWS + 32 * wave + col) * (DH + 2);
+#pragma unroll
+    for (int d = 0; d < C::ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) *reinterpret_cast<floatx2*>(part + 32 * d + 8 * (i >> 2) + 4 * half + (i & 3)) = floatx2{O[d][i], O[d][i + 1]};
+    if (half == 0) *reinterpret_cast<floatx2*>(part + DH) = floatx2{m, z};
+    return;
+  }
+  const long at = (long)(s.first + j) * a.h + head;
+  const float inv = 1.f / z;
+#pragma unroll
+  for (int d = 0; d < C::ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = z == 0.f ? 0.f : O[d][4 * i + e] * inv;
+      st4<bf16>((bf16*)a.o + at * DH + 32 * d + 8 * i + 4 * half, x);
+    }
+  if (half == 0) a.lse[at] = z == 0.f ? -INF : (ref + __builtin_amdgcn_logf(z)) * LN2;
+}
+
 // The pieces of a query tile, in their order.
-template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
+template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
   const int c = blockIdx.x % a.h_kv;
-  Item it = find_item<TILE_Q, false>(a, blockIdx.x / a.h_kv);
+  Item it = find_item<ROWS, false>(a, blockIdx.x / a.h_kv);
   if (it.b < 0 || it.pieces == 1) return;
   make_uniform(it);
   constexpr int E = DH / 16;
-  const int row = threadIdx.x >> 4, e0 = (threadIdx.x & 15) * E, rho = it.tile * TILE_Q + row;
+  const int row = blockIdx.y * 16 + (threadIdx.x >> 4), e0 = (threadIdx.x & 15) * E, rho = it.tile * ROWS + row;
   if (rho >= it.s.n * a.g) return;
-  const long step = (long)a.h_kv * TILE_Q * (DH + 2);
-  const float* part = a.part + (((long)it.slot * a.h_kv + c) * TILE_Q + row) * (DH + 2);
+  const long step = (long)a.h_kv * ROWS * (DH + 2);
+  const float* part = a.part + (((long)it.slot * a.h_kv + c) * ROWS + row) * (DH + 2);
   float M = -INF, Z = 0.f, x[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = 0.f;
@@ -658,13 +944,24 @@ int log2_of(int x) {
   return -1;
 }
 
-// The plan's numbers for query tiles of `rows` rows: about four blocks per CU over the key heads, in pieces of 128 rows or
-// more (a step of each of a block's waves).
+// The plan's numbers: about `blocks` blocks over the key heads.
 int wanted(const dm_paged_args* a, int blocks) { return std::max(1, cdiv(blocks, a->h_kv)); }
 long query_tiles(const dm_paged_args* a, int rows) { return (long)a->n_tokens * (a->h / a->h_kv) / rows + a->B; }
-constexpr int READ_BLOCKS = 4 * CUS, READ_LEAST = 2, WEIGHT_BLOCKS = 8 * CUS;
+constexpr int WEIGHT_BLOCKS = 8 * CUS;
 
-size_t part_floats(const dm_paged_args* a) { return (size_t)2 * wanted(a, READ_BLOCKS) * a->h_kv * TILE_Q * (a->dh + 2); }
+// Which read a call takes, by the mean number of query rows of a sequence and key head.
+struct Form {
+  int rows, blocks, least;     // query rows of a tile; blocks wanted; least tiles of cached rows in a piece
+};
+Form form_of(const dm_paged_args* a) {
+  const int64_t mean = (int64_t)a->n_tokens * (a->h / a->h_kv) / a->B;
+  if (a->dtype != DM_BF16 || mean <= TILE_Q) return {TILE_Q, 4 * CUS, 2};
+  return mean <= 128 ? Form{128, 2 * CUS, 2} : Form{256, CUS, 2};
+}
+size_t part_floats(const dm_paged_args* a) {
+  const Form f = form_of(a);
+  return (size_t)2 * wanted(a, f.blocks) * a->h_kv * f.rows * (a->dh + 2);
+}
 
 int check_pages(int dtype, int dh, int page, int n_pages, int cols, int B, int h_kv, const void* K, const void* V, int64_t k_page,
                 int64_t v_page) {
@@ -721,17 +1018,40 @@ PagedArgs paged(const dm_paged_args* a) {
   r.kr_token = a->k_token, r.kr_head = a->k_head, r.vr_token = a->v_token, r.vr_head = a->v_head;
   r.B = a->B, r.h = a->h, r.h_kv = a->h_kv, r.g = a->h_kv ? a->h / a->h_kv : 1, r.n_pages = a->n_pages, r.cols = a->table_cols;
   r.page_shift = log2_of(a->page), r.N = a->n_tokens, r.window = a->window, r.scale2 = a->scale * LOG2E;
-  r.want = wanted(a, READ_BLOCKS), r.least = READ_LEAST;
   return r;
 }
 
+template <int DH, int NW> int launch_wide(const PagedArgs& p, unsigned blocks, hipStream_t s) {
+  constexpr int BYTES = 2 * WideTile<DH>::BUF * 2;
+  static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_read_wide<DH, NW>),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+  DM_HIP(rc);
+  hipLaunchKernelGGL((k_paged_read_wide<DH, NW>), dim3(blocks), dim3(64 * NW), BYTES, s, p);
+  return DM_OK;
+}
+
 template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStream_t s) {
+  const Form f = form_of(a);
   PagedArgs p = paged(a);
-  const long tiles = query_tiles(a, TILE_Q);
-  hipLaunchKernelGGL((k_paged_read<T, DH>), dim3((unsigned)((p.want + tiles) * a->h_kv)), dim3(256), 0, s, p);
+  p.want = wanted(a, f.blocks), p.least = f.least;
+  const long tiles = query_tiles(a, f.rows);
+  const unsigned blocks = (unsigned)((p.want + tiles) * a->h_kv);
   // pieces there are only where a sequence can have more tiles than the least of one piece
-  if ((int64_t)a->table_cols * a->page > READ_LEAST * TILE_K)
-    hipLaunchKernelGGL((k_paged_join<T, DH>), dim3((unsigned)(tiles * a->h_kv)), dim3(256), 0, s, p);
+  const bool join = (int64_t)a->table_cols * a->page > f.least * TILE_K;
+  const dim3 joined((unsigned)(tiles * a->h_kv), f.rows / 16);
+  if (f.rows == TILE_Q) {
+    hipLaunchKernelGGL((k_paged_read<T, DH>), dim3(blocks), dim3(256), 0, s, p);
+    if (join) hipLaunchKernelGGL((k_paged_join<T, DH, TILE_Q>), joined, dim3(256), 0, s, p);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (f.rows == 128) {
+      if (const int rc = launch_wide<DH, 4>(p, blocks, s)) return rc;
+      if (join) hipLaunchKernelGGL((k_paged_join<T, DH, 128>), joined, dim3(256), 0, s, p);
+    } else if (f.rows == 256) {
+      if (const int rc = launch_wide<DH, 8>(p, blocks, s)) return rc;
+      if (join) hipLaunchKernelGGL((k_paged_join<T, DH, 256>), joined, dim3(256), 0, s, p);
+    }
+  }
   if (a->weights) {
     p.want = wanted(a, WEIGHT_BLOCKS);
     hipLaunchKernelGGL((k_paged_weights<T, DH>), dim3((unsigned)((p.want + (long)a->B) * a->h_kv)), dim3(256), 0, s, p);
@@ -745,7 +1065,7 @@ template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStrea
 extern "C" {
 
 size_t dm_paged_workspace_bytes(const dm_paged_args* a) {
-  if (!a || a->h_kv <= 0 || a->B <= 0 || (a->dh != 64 && a->dh != 128)) return 0;
+  if (!a || a->h_kv <= 0 || a->B <= 0 || a->h < a->h_kv || a->n_tokens < 0 || (a->dh != 64 && a->dh != 128)) return 0;
   return part_floats(a) * 4;
 }
 

@@ -51,7 +51,7 @@ def attention(q, K, V, table, lengths, counts, k_self=None, v_self=None, window=
                     total = torch.logsumexp(s, 0)
                     e = torch.exp(s - total)
                     o[t, a], lse[t, a] = e @ v, total
-                    d = u * ((dh + 8) * (scale * (k.abs() @ q[t, a].abs())).max() + 8 * (s.abs().max() + total.abs()) + len(k) + 16)
+                    d = u * ((dh + 8) * (abs(scale) * (k.abs() @ q[t, a].abs())).max() + 8 * (s.abs().max() + total.abs()) + len(k) + 16)
                     share = e @ v.abs()
                     bo[t, a] = share * (2 * d + (half if half > u else 0)) + half * o[t, a].abs()
                     bl[t, a] = d + 2 * u * total.abs()

@@ -104,6 +104,13 @@ def test_long_chunks(dtype, new):
     check(s, counts, True, window=100)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 3.0])
+@pytest.mark.parametrize("new", [1, 30, 150])
+def test_scales(scale, new):
+    counts, lengths = [new, new], [new + 70, new]
+    check(make(lengths, counts, 4, 2, 64, 32, torch.bfloat16, seed=new), counts, True, scale=scale)
+
+
 @pytest.mark.parametrize("with_self", [False, True])
 def test_many_sequences(with_self):
     """More sequences than a wave has lanes."""
