@@ -270,16 +270,16 @@ template <typename T, int LDV, bool ODD> DM_DEV floatx4 mma_values(const T* Vs, 
   return acc;
 }
 
-// A step's rows [r0, r0 + 16 t .. + 16) lie in one page each (pages hold 16 rows or more and begin at a multiple of 16).
-// needed: some query of the tile reads some of them. A page outside the pool is read as page 0 and marks the sequence.
-DM_DEV long page_of(const PagedArgs& a, const int32_t* table, int r, bool needed, bool& bad) {
-  if (!needed) return 0;
-  const int p = __builtin_amdgcn_readfirstlane(table[r >> a.page_shift]);
-  if (p < 0 || p >= a.n_pages) {
-    bad = true;
-    return 0;
-  }
-  return p;
+// The page of rows r .. that lie in one (pages hold 16 rows or more and begin at a multiple of 16). needed: some query of
+// the tile reads some of them. A page outside the pool is read as page 0 and marks the sequence. The table is read through
+// the scalar cache: a vector load of it would be waited for together with all rows that are on their way (prompt_chunk's
+// read 2.50 ms so), and pages are looked up a step ahead of their rows.
+DM_DEV int page_of(const PagedArgs& a, const int32_t* table, int r, bool needed, bool& bad) {
+  typedef const __attribute__((address_space(4))) int32_t* Scalar;
+  const int p = needed ? ((Scalar)table)[r >> a.page_shift] : 0;
+  const bool in = p >= 0 && p < a.n_pages;
+  bad |= !in;
+  return in ? p : 0;
 }
 
 // One block: a query tile of 16 rows, a key head and a piece of its cached rows. The four waves take steps of 32 rows in
@@ -349,11 +349,16 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
   T* Vs = reinterpret_cast<T*>(smem) + wave * C::KT * C::LDV;
   bool bad = s.bad;
   u32x4 kf[2][C::NF], vf[C::NV];
+  int pages[2];
+  auto look_up = [&](int r0) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) pages[t] = page_of(a, table, r0 + 16 * t, r0 + 16 * t < t_high && r0 + 16 * t + 16 > t_low, bad);
+  };
   auto load = [&](int r0) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int r = r0 + 16 * t;
-      const long page = page_of(a, table, r, r < t_high && r + 16 > t_low, bad);
+      const long page = pages[t];
       const long off = (((long)c << a.page_shift) + (r & in_page)) * DH;
       const T* K = (const T*)a.K + page * a.k_page + off;
       const T* Vp = (const T*)a.V + page * a.v_page + off;
@@ -367,7 +372,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
     }
   };
   int r0 = k0 + C::KT * wave;
-  if (r0 < k1) load(r0);
+  if (r0 < k1) look_up(r0), load(r0), look_up(min(r0 + 4 * C::KT, k1));
   for (; r0 < k1; r0 += 4 * C::KT) {
     const bool masked = r0 < all_low || r0 + C::KT > all_high;
     bool odd = false;    // masked values that no probability of 0 may meet
@@ -392,7 +397,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[4 * t + i] = acc[i] * a.scale2;
     }
-    if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT);
+    if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT), look_up(min(r0 + 8 * C::KT, k1));
     float read[8];
     float top = -INF;
 #pragma unroll
@@ -571,13 +576,20 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW) void k_paged_rea
   const int in_page = (1 << a.page_shift) - 1;
   bool bad = s.bad;
   u32x4 kx[NL], vx[NL];
+  int pages[NL];
   // a wave's load takes 64 / VPR (4 or 8) rows: of one page
+  auto look_up = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int r = r0 + (i * NT + 64 * wave) / C::VPR;
+      pages[i] = page_of(a, table, r, r < t_high && r + 64 / C::VPR > t_low, bad);
+    }
+  };
   auto load = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int v = i * NT + threadIdx.x, row = v / C::VPR;
-      const int r = r0 + (i * NT + 64 * wave) / C::VPR;
-      const long page = page_of(a, table, r, r < t_high && r + 64 / C::VPR > t_low, bad);
+      const long page = pages[i];
       const long off = (((long)c << a.page_shift) + ((r0 + row) & in_page)) * DH + (v % C::VPR) * 8;
       kx[i] = ld_global<u32x4>((const bf16*)a.K + page * a.k_page + off);
       vx[i] = ld_global<u32x4>((const bf16*)a.V + page * a.v_page + off);
@@ -601,14 +613,14 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW) void k_paged_rea
     if (odd) odd_step[buf] = r0;
   };
   if (threadIdx.x < 2) odd_step[threadIdx.x] = -1;
-  if (k0 < k1) load(k0);
+  if (k0 < k1) look_up(k0), load(k0), look_up(min(k0 + C::KT, k1));
   __syncthreads();
   if (k0 < k1) store(k0, 0);
   __syncthreads();
   int buf = 0;
   for (int r0 = k0; r0 < k1; r0 += C::KT, buf ^= 1) {
     const bool more = r0 + C::KT < k1;
-    if (more) load(r0 + C::KT);
+    if (more) load(r0 + C::KT), look_up(min(r0 + 2 * C::KT, k1));
     if (r0 < any_high && r0 + C::KT > any_low) {
       const bf16* Ks = lds + buf * C::BUF;
       const bf16* Vs = Ks + C::KT * C::LDK;
