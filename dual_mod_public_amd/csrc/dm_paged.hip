@@ -13,6 +13,7 @@
 #include "dm_error.h"
 
 #include <algorithm>
+#include <cstdlib>
 
 using namespace dm;
 
@@ -496,19 +497,22 @@ template <int DH> struct WideTile {
   static constexpr int KT = 64;            // cached rows of a step
   static constexpr int LDK = DH + 8;       // 16 rows' 16-byte pieces fill the banks once
   static constexpr int LDV = DH + 32;      // 4 rows' 64-byte pieces do
-  static constexpr int BUF = KT * (LDK + LDV);
+  static constexpr int KS = KT * LDK, VS = KT * LDV;      // a buffer of K, of V
   static constexpr int VPR = DH / 8, NK = DH / 16, ND = DH / 32;
 };
 
 // One block: a tile of 32 NW query rows (32 per wave), a key head and a piece of its cached rows, which pass through LDS in
-// steps of 64 that all waves share (two buffers, the next step's rows on their way in registers). Scores as 32 x 32 tiles
-// S^T = K Q^T: a lane holds one query row's scores, so maximum and sum need one exchange per step.
-template <int DH, int NW> __global__ __launch_bounds__(64 * NW) void k_paged_read_wide(PagedArgs a) {
+// steps of 64 that all waves share. Scores as 32 x 32 tiles S^T = K Q^T: a lane holds one query row's scores, so maximum and
+// sum need one exchange per step. The next step's scores run on the matrix cores while this one's exponentials run on the
+// vector units, and this one's product with V beside the next one's maximum: K is a step ahead of V (two buffers each, their
+// rows on their way in registers).
+template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_paged_read_wide(PagedArgs a) {
   using C = WideTile<DH>;
   constexpr int NT = 64 * NW, ROWS = 32 * NW, NL = C::KT * C::VPR / NT;    // 16-byte loads per thread of K and of V
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  bf16* lds = reinterpret_cast<bf16*>(smem);
-  __shared__ int odd_step[2];
+  bf16* const Ks = reinterpret_cast<bf16*>(smem);
+  bf16* const Vs = Ks + 2 * C::KS;
+  __shared__ int any_odd, any_bad;
   const int c = blockIdx.x % a.h_kv, lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Item it = find_item<ROWS, true>(a, blockIdx.x / a.h_kv);
@@ -575,137 +579,194 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW) void k_paged_rea
   const int32_t* table = a.table + (long)it.b * a.cols;
   const int in_page = (1 << a.page_shift) - 1;
   bool bad = s.bad;
-  u32x4 kx[NL], vx[NL];
-  int pages[NL];
-  // a wave's load takes 64 / VPR (4 or 8) rows: of one page
-  auto look_up = [&](int r0) {
+  // load i of a wave: 64 / VPR (4 or 8) rows, of one page; the lane's place from the first of them on
+  constexpr int AT_ONCE = 64 / C::VPR;
+  const int my_row = lane / C::VPR, my_col = lane % C::VPR * 8;
+  const uint32_t my_off = (uint32_t)(my_row * DH + my_col) * 2;
+  auto first_row = [&](int i) { return (i * NW + wave) * AT_ONCE; };
+  struct Rows {
+    int page[NL];
+    u32x4 x[NL];
+  } kr, vr;
+  auto look_up = [&](Rows& w, int r0) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int r = r0 + (i * NT + 64 * wave) / C::VPR;
-      pages[i] = page_of(a, table, r, r < t_high && r + 64 / C::VPR > t_low, bad);
+      const int r = r0 + first_row(i);
+      w.page[i] = page_of(a, table, r, r < t_high && r + AT_ONCE > t_low, bad);
     }
   };
-  auto load = [&](int r0) {
+  auto load = [&](Rows& w, int r0, const void* pages, long stride) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int v = i * NT + threadIdx.x, row = v / C::VPR;
-      const long page = pages[i];
-      const long off = (((long)c << a.page_shift) + ((r0 + row) & in_page)) * DH + (v % C::VPR) * 8;
-      kx[i] = ld_global<u32x4>((const bf16*)a.K + page * a.k_page + off);
-      vx[i] = ld_global<u32x4>((const bf16*)a.V + page * a.v_page + off);
+      const long off = w.page[i] * stride + (((long)c << a.page_shift) + ((r0 + first_row(i)) & in_page)) * DH;
+      w.x[i] = ld_global<u32x4>((const char*)((const bf16*)pages + off) + my_off);
     }
   };
-  auto store = [&](int r0, int buf) {
-    bf16* Ks = lds + buf * C::BUF;
-    bf16* Vs = Ks + C::KT * C::LDK;
-    const bool edge = r0 < s.low(a, j_last) || r0 + C::KT > s.high(a, j_first);   // some query row does not read all of it
-    bool odd = false;
+  auto store_k = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int v = i * NT + threadIdx.x, row = v / C::VPR, e = (v % C::VPR) * 8;
-      if (edge) {
-        if (r0 + row < t_low || r0 + row >= t_high) vx[i] = u32x4{0, 0, 0, 0};    // whatever lies there
-        odd |= any_nonfinite<bf16>(vx[i]);
+    for (int i = 0; i < NL; ++i)
+      *reinterpret_cast<u32x4*>(Ks + buf * C::KS + (first_row(i) + my_row) * C::LDK + my_col) = kr.x[i];
+  };
+  const int edge_low = s.low(a, j_last), edge_high = s.high(a, j_first);   // rows that all query rows of the tile read
+  // In steps that some query row does not read all of, values that are not finite count 0 here (a product with a probability
+  // of 0 would make it NaN) and are added at the end, for the query rows that read them.
+  auto is_edge = [&](int r0) { return r0 < edge_low || r0 + C::KT > edge_high; };
+  auto store_v = [&](int r0, int buf) {
+    if (is_edge(r0)) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int r = r0 + first_row(i) + my_row;
+        if (r < t_low || r >= t_high) vr.x[i] = u32x4{0, 0, 0, 0};    // whatever lies there
+        if (any_nonfinite<bf16>(vr.x[i])) {
+          any_odd = 1;
+          i16x8 v = __builtin_bit_cast(i16x8, vr.x[i]);
+          split_nonfinite(v);
+          vr.x[i] = __builtin_bit_cast(u32x4, v);
+        }
       }
-      *reinterpret_cast<u32x4*>(Ks + row * C::LDK + e) = kx[i];
-      *reinterpret_cast<u32x4*>(Vs + row * C::LDV + e) = vx[i];
     }
-    if (odd) odd_step[buf] = r0;
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      *reinterpret_cast<u32x4*>(Vs + buf * C::VS + (first_row(i) + my_row) * C::LDV + my_col) = vr.x[i];
   };
-  if (threadIdx.x < 2) odd_step[threadIdx.x] = -1;
-  if (k0 < k1) look_up(k0), load(k0), look_up(min(k0 + C::KT, k1));
+  auto scores = [&](int buf, floatx16 (&S)[2]) {
+    const bf16* K = Ks + buf * C::KS + col * C::LDK + 8 * half;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[t][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < C::NK; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) S[t] = mma32(*reinterpret_cast<const u32x4*>(K + 32 * t * C::LDK + 16 * i), qf[i], S[t]);
+  };
+  // scores of rows r0 + 32 t + 8 (i / 4) + 4 half + i % 4 in S[t][i]
+  auto is_masked = [&](int r0) { return r0 < all_low || r0 + C::KT > all_high; };
+  auto mask = [&](int r0, floatx16 (&S)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = r0 + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
+        if (r < low || r >= high) S[t][i] = -INF;
+      }
+  };
+  auto largest = [&](const floatx16 (&S)[2]) {
+    float top = fmaxf(S[0][0], S[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(S[0][i], S[1][i]));
+    return xor_max<32>(top) * scale2;
+  };
+  auto follow = [&](float top) {     // as in k_paged_read
+    if (__ballot(top > m + 8.f)) {
+      const float was = m;
+      m = fmaxf(m, top);
+      const float alpha = __builtin_amdgcn_exp2f(was - (m == -INF ? 0.f : m));
+      z *= alpha;
+#pragma unroll
+      for (int d = 0; d < C::ND; ++d) O[d] *= alpha;
+    }
+  };
+  u32x4 p[4];
+  auto exponentials = [&](const floatx16 (&S)[2]) {
+    const float ref = m == -INF ? 0.f : m;
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(fmaf(S[k >> 1][8 * (k & 1) + i], scale2, -ref));
+        sum[i & 1] += e[i];
+      }
+      p[k] = __builtin_bit_cast(u32x4, to_bf16x8(e, 0));
+    }
+    z += sum[0] + sum[1];
+  };
+  auto product = [&](int buf) {
+    const bf16* V = Vs + buf * C::VS;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int d = 0; d < C::ND; ++d)
+        O[d] = mma32(__builtin_bit_cast(u32x4, values_fragment32(V + 16 * k * C::LDV + 32 * d, C::LDV)), p[k], O[d]);
+  };
+  if (threadIdx.x == 0) any_odd = any_bad = 0;
   __syncthreads();
-  if (k0 < k1) store(k0, 0);
-  __syncthreads();
-  int buf = 0;
-  for (int r0 = k0; r0 < k1; r0 += C::KT, buf ^= 1) {
-    const bool more = r0 + C::KT < k1;
-    if (more) load(r0 + C::KT), look_up(min(r0 + 2 * C::KT, k1));
-    if (r0 < any_high && r0 + C::KT > any_low) {
-      const bf16* Ks = lds + buf * C::BUF;
-      const bf16* Vs = Ks + C::KT * C::LDK;
-      const bool masked = r0 < all_low || r0 + C::KT > all_high;
-      float p[32];      // of rows r0 + 8 (i / 4) + 4 half + i % 4
+  const int steps = k0 < k1 ? (k1 - k0 + C::KT - 1) / C::KT : 0;
+  auto step_row = [&](int n) { return min(k0 + n * C::KT, k1); };     // step n's first row; k1: there is no such step
+  if (steps) {
+    look_up(kr, k0), load(kr, k0, a.K, a.k_page);
+    vr = kr, load(vr, k0, a.V, a.v_page);
+    store_k(0), store_v(k0, 0);
+    look_up(kr, step_row(1)), load(kr, step_row(1), a.K, a.k_page), store_k(1);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        floatx16 acc;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < C::NK; ++i)
-          acc = mma32(*reinterpret_cast<const u32x4*>(Ks + (32 * t + col) * C::LDK + 16 * i + 8 * half), qf[i], acc);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[16 * t + i] = acc[i];
-      }
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int r = r0 + 8 * (i >> 2) + 4 * half + (i & 3);
-          if (r < low || r >= high) p[i] = -INF;
-        }
-      }
-      float top = -INF;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) top = fmaxf(top, p[i]);
-      top = xor_max<32>(top) * scale2;
-      if (__ballot(top > m + 8.f)) {
-        const float was = m;
-        m = fmaxf(m, top);
-        const float alpha = __builtin_amdgcn_exp2f(was - (m == -INF ? 0.f : m));
-        z *= alpha;
-#pragma unroll
-        for (int d = 0; d < C::ND; ++d) O[d] *= alpha;
-      }
-      const float ref = m == -INF ? 0.f : m;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], scale2, -ref));
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 32; ++i) sum[i & 3] += p[i];
-      z += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      if (masked && odd_step[buf] == r0) {
-        float read[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int r = r0 + 8 * (i >> 2) + 4 * half + (i & 3);
-          read[i] = r < low || r >= high ? 0.f : 1.f;
-        }
-#pragma unroll
-        for (int d = 0; d < C::ND; ++d) {
-          floatx16 said;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) said[i] = 0.f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            i16x8 v = values_fragment32(Vs + 16 * k * C::LDV + 32 * d, C::LDV);
-            const i16x8 code = split_nonfinite(v);
-            said = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, code), to_bf16x8(read, 8 * k), said, 0, 0, 0);
-            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), to_bf16x8(p, 8 * k), O[d], 0, 0, 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) O[d][i] += said_by(said[i]);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bf16x8 pb = to_bf16x8(p, 8 * k);
-#pragma unroll
-          for (int d = 0; d < C::ND; ++d)
-            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values_fragment32(Vs + 16 * k * C::LDV + 32 * d, C::LDV)),
-                                                           pb, O[d], 0, 0, 0);
-        }
-      }
-    }
-    if (more) store(r0 + C::KT, buf ^ 1);
+    for (int i = 0; i < NL; ++i) vr.page[i] = kr.page[i];       // V follows K by a step
+    look_up(kr, step_row(2));
     __syncthreads();
+    floatx16 S[2];
+    scores(0, S);
+    if (is_masked(k0)) mask(k0, S);
+    follow(largest(S));
+    __syncthreads();
+    for (int n = 0; n + 1 < steps; ++n) {
+      const int buf = n & 1;
+      int next[NL];
+      load(kr, step_row(n + 2), a.K, a.k_page);      // (past the last step: of page 0, not used)
+      load(vr, step_row(n + 1), a.V, a.v_page);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) next[i] = kr.page[i];
+      look_up(kr, step_row(n + 3));
+      floatx16 T[2];
+      scores(buf ^ 1, T);
+      exponentials(S);
+      if (is_masked(step_row(n + 1))) mask(step_row(n + 1), T);
+      product(buf);
+      follow(largest(T));
+      S[0] = T[0], S[1] = T[1];
+      // into the buffers of K of step n and V of step n - 1, which every wave has done with since the last barrier
+      store_k(buf);
+      store_v(step_row(n + 1), buf ^ 1);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) vr.page[i] = next[i];
+      __syncthreads();
+    }
+    exponentials(S);
+    product((steps - 1) & 1);
+  }
+  __syncthreads();
+  if (any_odd) {
+    for (int r0 = k0; r0 < k1; r0 += 16) {
+      if (!is_edge(k0 + (r0 - k0) / C::KT * C::KT)) continue;
+      float read[8];
+      const bf16* v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {      // the lane's rows
+        const int r = r0 + 8 * (i >> 2) + 4 * half + (i & 3);
+        read[i] = r < low || r >= high ? 0.f : 1.f;
+        const int page = r >= t_low && r < t_high ? table[r >> a.page_shift] : -1;
+        v[i] = page < 0 || page >= a.n_pages ? nullptr
+                                             : (const bf16*)a.V + page * a.v_page + (((long)c << a.page_shift) + (r & in_page)) * DH + col;
+      }
+#pragma unroll
+      for (int d = 0; d < C::ND; ++d) {
+        i16x8 x;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = v[i] ? (short)ld_global<unsigned short>(v[i] + 32 * d) : (short)0;
+        const i16x8 code = split_nonfinite(x);
+        floatx16 said;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) said[i] = 0.f;
+        said = mma32(__builtin_bit_cast(u32x4, code), __builtin_bit_cast(u32x4, to_bf16x8(read, 0)), said);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[d][i] += said_by(said[i]);
+      }
+    }
   }
   z = xor_sum<32>(z);
-  // a page outside the pool is seen by the waves whose rows lie there
-  if (threadIdx.x == 0) odd_step[0] = 0;
+  if (bad) any_bad = 1;      // seen by the waves whose rows lie there
   __syncthreads();
-  if (bad) odd_step[0] = 1;
-  __syncthreads();
-  if (odd_step[0]) z = NAN_;
+  if (any_bad) z = NAN_;
   if (!live) return;
   const float ref = m == -INF ? 0.f : m;
   if (it.pieces > 1) {
@@ -968,7 +1029,7 @@ struct Form {
 Form form_of(const dm_paged_args* a) {
   const int64_t mean = (int64_t)a->n_tokens * (a->h / a->h_kv) / a->B;
   if (a->dtype != DM_BF16 || mean <= TILE_Q) return {TILE_Q, 4 * CUS, 2};
-  return mean <= 128 ? Form{128, 2 * CUS, 2} : Form{256, CUS, 2};
+  return Form{getenv("DMW") && atoi(getenv("DMW")) == 8 ? 256 : 128, 2 * CUS, 2};
 }
 size_t part_floats(const dm_paged_args* a) {
   const Form f = form_of(a);
@@ -1034,7 +1095,7 @@ PagedArgs paged(const dm_paged_args* a) {
 }
 
 template <int DH, int NW> int launch_wide(const PagedArgs& p, unsigned blocks, hipStream_t s) {
-  constexpr int BYTES = 2 * WideTile<DH>::BUF * 2;
+  constexpr int BYTES = 2 * (WideTile<DH>::KS + WideTile<DH>::VS) * 2;
   static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_read_wide<DH, NW>),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
   DM_HIP(rc);
