@@ -13,7 +13,7 @@
 #include "dm_error.h"
 
 #include <algorithm>
-#include <cstdlib>
+#include <type_traits>
 
 using namespace dm;
 
@@ -34,6 +34,7 @@ struct PagedArgs {
   int B, h, h_kv, g, n_pages, cols, page_shift, N, window;
   float scale2;                        // scale log2 e
   int want, least;                     // the plan: pieces wanted, least tiles of cached rows in one
+  float* scores;                       // [N, h, cols * page] in units of ln 2, for the weights; nullptr: not kept
 };
 
 // A sequence as the call gives it. A table that does not hold its rows, or fewer rows than new tokens: bad, NaN results.
@@ -123,6 +124,9 @@ template <int ROWS, bool PIECES> DM_DEV Item find_item(const PagedArgs& a, int a
   return it;
 }
 
+// A number that every lane holds, as a scalar: quotients come from vector instructions, and what is computed from them (rows,
+// pages, addresses) would stay with those.
+DM_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 // the item in scalar registers: every lane holds the same
 DM_DEV void make_uniform(Item& it) {
   auto u = [](int& x) { x = __builtin_amdgcn_readfirstlane(x); };
@@ -291,14 +295,14 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
   constexpr int VBYTES = C::KT * C::LDV * (int)sizeof(T), OBYTES = TILE_Q * DH * 4;
   __shared__ __attribute__((aligned(16))) char smem[4 * (VBYTES > OBYTES ? VBYTES : OBYTES)];
   __shared__ float sm[4][TILE_Q], sz[4][TILE_Q];
-  const int c = blockIdx.x % a.h_kv, lane = threadIdx.x & 63, grp = lane >> 4, col = lane & 15;
+  const int c = uniform(blockIdx.x % a.h_kv), lane = threadIdx.x & 63, grp = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Item it = find_item<TILE_Q, true>(a, blockIdx.x / a.h_kv);
   if (it.b < 0) return;
   make_uniform(it);
   const Seq& s = it.s;
   const int rows = s.n * a.g, rho0 = it.tile * TILE_Q;            // query rows of the sequence, the tile's first
-  const int j_first = rho0 / a.g, j_last = (min(rho0 + TILE_Q, rows) - 1) / a.g;
+  const int j_first = uniform(rho0 / a.g), j_last = uniform((min(rho0 + TILE_Q, rows) - 1) / a.g);
   // the lane's query row
   const int rho = rho0 + col, j = rho / a.g, head = c * a.g + rho % a.g;
   const bool live = rho < rows;
@@ -306,7 +310,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
   // the tile's rows, and this piece's
   const int t_low = s.low(a, j_first), t_high = s.bad ? 0 : s.high(a, j_last);
   const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
-  const int each = (tiles + it.pieces - 1) / it.pieces;
+  const int each = uniform((tiles + it.pieces - 1) / it.pieces);
   const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
   // rows below this and from that on are read by all live query rows
   const int all_low = s.low(a, j_last), all_high = s.high(a, j_first);
@@ -408,6 +412,11 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
       read[i] = hidden ? 0.f : 1.f;
       if (hidden) p[i] = -INF;
       top = fmaxf(top, p[i]);
+    }
+    if (a.scores && live) {
+      float* x = a.scores + ((long)(s.first + j) * a.h + head) * ((long)a.cols << a.page_shift) + r0 + 4 * grp;
+      *reinterpret_cast<floatx4*>(x) = floatx4{p[0], p[1], p[2], p[3]};
+      if (r0 + 16 < k1) *reinterpret_cast<floatx4*>(x + 16) = floatx4{p[4], p[5], p[6], p[7]};
     }
     top = xor_max<32>(xor_max<16>(top));
     // the reference follows the maximum only where that has risen by 2^8: sums and probabilities are relative to it
@@ -513,23 +522,23 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
   bf16* const Ks = reinterpret_cast<bf16*>(smem);
   bf16* const Vs = Ks + 2 * C::KS;
   __shared__ int any_odd, any_bad;
-  const int c = blockIdx.x % a.h_kv, lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const int c = uniform(blockIdx.x % a.h_kv), lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Item it = find_item<ROWS, true>(a, blockIdx.x / a.h_kv);
   if (it.b < 0) return;
   make_uniform(it);
   const Seq& s = it.s;
   const int rows = s.n * a.g, rho0 = it.tile * ROWS;
-  const int j_first = rho0 / a.g, j_last = (min(rho0 + ROWS, rows) - 1) / a.g;
+  const int j_first = uniform(rho0 / a.g), j_last = uniform((min(rho0 + ROWS, rows) - 1) / a.g);
   const int rho = rho0 + 32 * wave + col, j = rho / a.g, head = c * a.g + rho % a.g;
   const bool live = rho < rows;
   const int high = live ? s.high(a, j) : 0, low = live ? s.low(a, j) : 0;
   const int t_low = s.low(a, j_first), t_high = s.bad ? 0 : s.high(a, j_last);
   const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
-  const int each = (tiles + it.pieces - 1) / it.pieces;
+  const int each = uniform((tiles + it.pieces - 1) / it.pieces);
   const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
   // rows that all, and that any, of the wave's live query rows read
-  const int w_first = min(rho0 + 32 * wave, rows - 1) / a.g, w_last = min(rho0 + 32 * wave + 31, rows - 1) / a.g;
+  const int w_first = uniform(min(rho0 + 32 * wave, rows - 1) / a.g), w_last = uniform(min(rho0 + 32 * wave + 31, rows - 1) / a.g);
   const int all_low = s.low(a, w_last), all_high = s.high(a, w_first), any_low = s.low(a, w_first), any_high = s.high(a, w_last);
 
   u32x4 qf[C::NK];
@@ -643,19 +652,24 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
   // scores of rows r0 + 32 t + 8 (i / 4) + 4 half + i % 4 in S[t][i]
   auto is_masked = [&](int r0) { return r0 < all_low || r0 + C::KT > all_high; };
   auto mask = [&](int r0, floatx16 (&S)[2]) {
+    const int from = low - r0 - 4 * half, to = high - r0 - 4 * half;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int r = r0 + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3);
-        if (r < low || r >= high) S[t][i] = -INF;
+        const int r = 32 * t + 8 * (i >> 2) + (i & 3);
+        if (r < from || r >= to) S[t][i] = -INF;
       }
   };
   auto largest = [&](const floatx16 (&S)[2]) {
-    float top = fmaxf(S[0][0], S[1][0]);
+    float top = S[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(S[0][i], S[1][i]));
-    return xor_max<32>(top) * scale2;
+    for (int i = 0; i < 16; ++i) {
+      if (i) top = __builtin_elementwise_maximum(top, S[0][i]);
+      top = __builtin_elementwise_maximum(top, S[1][i]);
+    }
+    const LanePair both = lane_pair<32>(top);
+    return __builtin_elementwise_maximum(both.a, both.b) * scale2;
   };
   auto follow = [&](float top) {     // as in k_paged_read
     if (__ballot(top > m + 8.f)) {
@@ -667,29 +681,24 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
       for (int d = 0; d < C::ND; ++d) O[d] *= alpha;
     }
   };
+  // the exponentials number at .. at + n - 1 of a step's 32, packed eight by eight
   u32x4 p[4];
-  auto exponentials = [&](const floatx16 (&S)[2]) {
-    const float ref = m == -INF ? 0.f : m;
-    float sum[2] = {0.f, 0.f};
+  float e[32], sum[2];
+  auto exponentials = [&](const floatx16 (&S)[2], float ref, int at, int n) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(fmaf(S[k >> 1][8 * (k & 1) + i], scale2, -ref));
-        sum[i & 1] += e[i];
-      }
-      p[k] = __builtin_bit_cast(u32x4, to_bf16x8(e, 0));
+    for (int i = at; i < at + n; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(fmaf(S[i >> 4][i & 15], scale2, -ref));
+      sum[i & 1] = i < 2 ? e[i] : sum[i & 1] + e[i];
+      if ((i & 7) == 7) p[i >> 3] = __builtin_bit_cast(u32x4, to_bf16x8(e, i - 7));
     }
-    z += sum[0] + sum[1];
   };
-  auto product = [&](int buf) {
-    const bf16* V = Vs + buf * C::VS;
+  // V^T's fragments of columns 64 u and rows 16 k of the step, and the products with them: number i = (k, u)
+  constexpr int PAIRS = C::ND / 2;
+  u32x4 vf[2];
+  auto read_v = [&](const bf16* V, int i) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int d = 0; d < C::ND; ++d)
-        O[d] = mma32(__builtin_bit_cast(u32x4, values_fragment32(V + 16 * k * C::LDV + 32 * d, C::LDV)), p[k], O[d]);
+    for (int d = 0; d < 2; ++d)
+      vf[d] = __builtin_bit_cast(u32x4, values_fragment32(V + 16 * (i / PAIRS) * C::LDV + 64 * (i % PAIRS) + 32 * d, C::LDV));
   };
   if (threadIdx.x == 0) any_odd = any_bad = 0;
   __syncthreads();
@@ -709,7 +718,7 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
     if (is_masked(k0)) mask(k0, S);
     follow(largest(S));
     __syncthreads();
-    for (int n = 0; n + 1 < steps; ++n) {
+    auto step = [&](int n, auto masked) {
       const int buf = n & 1;
       int next[NL];
       load(kr, step_row(n + 2), a.K, a.k_page);      // (past the last step: of page 0, not used)
@@ -717,12 +726,55 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
 #pragma unroll
       for (int i = 0; i < NL; ++i) next[i] = kr.page[i];
       look_up(kr, step_row(n + 3));
+      // Each matrix product stands beside a share of the vector work, in this order (the compiler's own puts all
+      // exponentials first, and each LDS read right before its product): the next step's scores beside the first 24 exponentials,
+      // the products with V beside the others and the next maximum.
       floatx16 T[2];
-      scores(buf ^ 1, T);
-      exponentials(S);
-      if (is_masked(step_row(n + 1))) mask(step_row(n + 1), T);
-      product(buf);
-      follow(largest(T));
+      const float ref = m == -INF ? 0.f : m;
+      const bf16* K = Ks + (buf ^ 1) * C::KS + col * C::LDK + 8 * half;
+      const bf16* V = Vs + buf * C::VS;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) T[t][i] = 0.f;
+      u32x4 kf[2] = {*reinterpret_cast<const u32x4*>(K), *reinterpret_cast<const u32x4*>(K + 32 * C::LDK)};
+#pragma unroll
+      for (int i = 0; i < C::NK; ++i) {
+        const u32x4 k0 = kf[0], k1 = kf[1];
+        if (i + 1 < C::NK) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) kf[t] = *reinterpret_cast<const u32x4*>(K + 32 * t * C::LDK + 16 * (i + 1));
+        } else {
+          read_v(V, 0);
+        }
+        T[0] = mma32(k0, qf[i], T[0]);
+        T[1] = mma32(k1, qf[i], T[1]);
+        exponentials(S, ref, i * (24 / C::NK), 24 / C::NK);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (masked) mask(step_row(n + 1), T);
+      float top = T[0][0];
+#pragma unroll
+      for (int i = 0; i < 4 * PAIRS; ++i) {
+        const u32x4 v0 = vf[0], v1 = vf[1];
+        if (i + 1 < 4 * PAIRS) read_v(V, i + 1);
+        const int d = 2 * (i % PAIRS);
+        O[d] = mma32(v0, p[i / PAIRS], O[d]);
+        O[d + 1] = mma32(v1, p[i / PAIRS], O[d + 1]);
+        if (i < 2 * PAIRS) {
+          exponentials(S, ref, 24 + i * (4 / PAIRS), 4 / PAIRS);
+        } else {     // NaN where a score is NaN: the reference stays then, and the sum becomes NaN
+#pragma unroll
+          for (int x = (i - 2 * PAIRS) * (8 / PAIRS); x < (i - 2 * PAIRS + 1) * (8 / PAIRS); ++x) {
+            top = __builtin_elementwise_maximum(top, T[0][x]);
+            top = __builtin_elementwise_maximum(top, T[1][x]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      z += sum[0] + sum[1];
+      const LanePair both = lane_pair<32>(top);
+      follow(__builtin_elementwise_maximum(both.a, both.b) * scale2);
       S[0] = T[0], S[1] = T[1];
       // into the buffers of K of step n and V of step n - 1, which every wave has done with since the last barrier
       store_k(buf);
@@ -730,9 +782,20 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
 #pragma unroll
       for (int i = 0; i < NL; ++i) vr.page[i] = next[i];
       __syncthreads();
+    };
+    for (int n = 0; n + 1 < steps; ++n) {
+      if (is_masked(step_row(n + 1))) step(n, std::true_type());
+      else step(n, std::false_type());
     }
-    exponentials(S);
-    product((steps - 1) & 1);
+    exponentials(S, m == -INF ? 0.f : m, 0, 32);
+    z += sum[0] + sum[1];
+    const bf16* V = Vs + ((steps - 1) & 1) * C::VS;
+#pragma unroll
+    for (int i = 0; i < 4 * PAIRS; ++i) {
+      read_v(V, i);
+#pragma unroll
+      for (int d = 0; d < 2; ++d) O[2 * (i % PAIRS) + d] = mma32(vf[d], p[i / PAIRS], O[2 * (i % PAIRS) + d]);
+    }
   }
   __syncthreads();
   if (any_odd) {
@@ -804,15 +867,22 @@ template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k
   const long step = (long)a.h_kv * ROWS * (DH + 2);
   const float* part = a.part + (((long)it.slot * a.h_kv + c) * ROWS + row) * (DH + 2);
   float M = -INF, Z = 0.f, x[E];
+  // the row's 16 threads share its pieces' maxima and sums, then each adds its columns
+  const int lane16 = threadIdx.x & 15;
+  for (int i = lane16; i < it.pieces; i += 16) M = fmaxf(M, part[i * step + DH]);
+  M = group16_max(M);
+  const float ref = M == -INF ? 0.f : M;
+  for (int i = lane16; i < it.pieces; i += 16) {
+    const floatx2 mz = *reinterpret_cast<const floatx2*>(part + i * step + DH);
+    Z += __builtin_amdgcn_exp2f(mz[0] - ref) * mz[1];
+  }
+  Z = group16_sum(Z);
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = 0.f;
-  for (int i = 0; i < it.pieces; ++i) M = fmaxf(M, part[i * step + DH]);
-  const float ref = M == -INF ? 0.f : M;
+#pragma unroll 8
   for (int i = 0; i < it.pieces; ++i) {
     const float* p = part + i * step;
-    const floatx2 mz = *reinterpret_cast<const floatx2*>(p + DH);
-    const float f = __builtin_amdgcn_exp2f(mz[0] - ref);
-    Z += f * mz[1];
+    const float f = __builtin_amdgcn_exp2f(p[DH] - ref);
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
       const floatx2 v = *reinterpret_cast<const floatx2*>(p + e0 + e);
@@ -830,11 +900,50 @@ template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k
 }
 
 // ---- the weights -------------------------------------------------------------------------------
-// weights[b, c, r] += the sum over the sequence's query rows of exp(score - lse), the scores computed again: a wave holds
+// The logarithm of a sum in units of ln 2, with what a sum of 0 (no row read, or scores of -inf) stands for: weights of 0.
+DM_DEV float lse_of(float lse) { return lse == -INF ? INF : lse * LOG2E; }
+
+// weights[b, c, r] += the sum over the sequence's query rows of exp(score - lse), from scores that the read kept: a thread
+// takes 4 cached rows and goes over the query rows.
+__global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
+  const int c = uniform(blockIdx.x % a.h_kv);
+  Item it = find_item<0, true>(a, blockIdx.x / a.h_kv);
+  if (it.b < 0) return;
+  make_uniform(it);
+  const Seq& s = it.s;
+  if (s.bad) return;
+  const int t_low = s.low(a, 0), t_high = s.high(a, s.n - 1);
+  const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
+  const int each = uniform((tiles + it.pieces - 1) / it.pieces);
+  const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
+  const long cap = (long)a.cols << a.page_shift;
+  float* w = a.weights + ((long)it.b * a.h_kv + c) * cap;
+  for (int r = k0 + 4 * threadIdx.x; r < k1; r += 1024) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < s.n; ++j) {
+      const int low = s.low(a, j), high = s.high(a, j);
+      if (r >= high || r + 4 <= low) continue;
+      const long at = (long)(s.first + j) * a.h + c * a.g;
+      const float* x = a.scores + at * cap + r;
+#pragma unroll 4
+      for (int i = 0; i < a.g; ++i) {
+        const floatx4 v = *reinterpret_cast<const floatx4*>(x + i * cap);
+        const float lse2 = lse_of(a.lse[at + i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += r + e >= low && r + e < high ? __builtin_amdgcn_exp2f(v[e] - lse2) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (r + e >= t_low && r + e < t_high) w[r + e] += sum[e];
+  }
+}
+
+// The same with the scores computed again: weights[b, c, r] += the sum over the sequence's query rows of exp(score - lse), the scores computed again: a wave holds
 // 32 cached rows as fragments and goes over all query tiles, so each weight has one writer and one order of its sum.
 template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_weights(PagedArgs a) {
   using C = Tile<T, DH>;
-  const int c = blockIdx.x % a.h_kv, lane = threadIdx.x & 63, grp = lane >> 4, col = lane & 15;
+  const int c = uniform(blockIdx.x % a.h_kv), lane = threadIdx.x & 63, grp = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Item it = find_item<0, true>(a, blockIdx.x / a.h_kv);
   if (it.b < 0) return;
@@ -843,7 +952,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
   if (s.bad) return;
   const int rows = s.n * a.g, t_low = s.low(a, 0), t_high = s.high(a, s.n - 1);
   const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
-  const int each = (tiles + it.pieces - 1) / it.pieces;
+  const int each = uniform((tiles + it.pieces - 1) / it.pieces);
   const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
   const int32_t* table = a.table + (long)it.b * a.cols;
   const int in_page = (1 << a.page_shift) - 1;
@@ -869,7 +978,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
       u32x4 qf[C::NF];
 #pragma unroll
       for (int i = 0; i < C::NF; ++i) qf[i] = live ? ld_global<u32x4>(q + i * 4 * C::V + grp * C::V) : u32x4{0, 0, 0, 0};
-      const float lse2 = live ? a.lse[at] * LOG2E : 0.f;
+      const float lse2 = live ? lse_of(a.lse[at]) : 0.f;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         floatx4 acc = zero4();
@@ -1022,19 +1131,31 @@ int wanted(const dm_paged_args* a, int blocks) { return std::max(1, cdiv(blocks,
 long query_tiles(const dm_paged_args* a, int rows) { return (long)a->n_tokens * (a->h / a->h_kv) / rows + a->B; }
 constexpr int WEIGHT_BLOCKS = 8 * CUS;
 
-// Which read a call takes, by the mean number of query rows of a sequence and key head.
+// Which read a call takes, by the mean number of query rows of a sequence and key head: tiles of 16 rows while two of them
+// hold those, of 128, or of 256 (us, bf16, 16 sequences of 4096 rows, 16 heads of 64 and 32 of 128 on 8 key heads:
+// 24 rows 60 / 69 / 115 and 60 / 62 / 82, 48 rows 78 / 71 / 115 and 84 / 65 / 86, 256 rows 303 / 123 / 134 and 307 / 117 / 119,
+// 512 rows 572 / 225 / 215 and 596 / 195 / 188; two sequences of 16384 rows, 8192 query rows: 4110 / 1340 / 1150). Pieces:
+// what fills the CUs with the blocks that one holds (at 8192 query rows 1, 2 and 4 times as many: 1150, 1184, 1206 us).
 struct Form {
   int rows, blocks, least;     // query rows of a tile; blocks wanted; least tiles of cached rows in a piece
 };
 Form form_of(const dm_paged_args* a) {
   const int64_t mean = (int64_t)a->n_tokens * (a->h / a->h_kv) / a->B;
-  if (a->dtype != DM_BF16 || mean <= TILE_Q) return {TILE_Q, 4 * CUS, 2};
-  return Form{getenv("DMW") && atoi(getenv("DMW")) == 8 ? 256 : 128, 2 * CUS, 2};
+  if (a->dtype != DM_BF16 || mean <= 2 * TILE_Q) return {TILE_Q, 4 * CUS, 2};
+  return mean <= 512 ? Form{128, 2 * CUS, 2} : Form{256, CUS, 2};
+}
+// The scores of a call with weights are kept where they take no more room than the pages' keys; else they are computed
+// again from the keys.
+size_t score_floats(const dm_paged_args* a) {
+  if (!a->weights || form_of(a).rows != TILE_Q) return 0;
+  const double n = (double)a->n_tokens * a->h * a->table_cols * a->page;
+  return n * 4 <= (double)a->n_pages * a->h_kv * a->page * a->dh * esz(a->dtype) ? (size_t)n : 0;
 }
 size_t part_floats(const dm_paged_args* a) {
   const Form f = form_of(a);
   return (size_t)2 * wanted(a, f.blocks) * a->h_kv * f.rows * (a->dh + 2);
 }
+size_t part_bytes(const dm_paged_args* a) { return align256(part_floats(a) * 4); }
 
 int check_pages(int dtype, int dh, int page, int n_pages, int cols, int B, int h_kv, const void* K, const void* V, int64_t k_page,
                 int64_t v_page) {
@@ -1107,6 +1228,7 @@ template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStrea
   const Form f = form_of(a);
   PagedArgs p = paged(a);
   p.want = wanted(a, f.blocks), p.least = f.least;
+  if (score_floats(a)) p.scores = (float*)((char*)a->workspace + part_bytes(a));
   const long tiles = query_tiles(a, f.rows);
   const unsigned blocks = (unsigned)((p.want + tiles) * a->h_kv);
   // pieces there are only where a sequence can have more tiles than the least of one piece
@@ -1127,7 +1249,13 @@ template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStrea
   }
   if (a->weights) {
     p.want = wanted(a, WEIGHT_BLOCKS);
-    hipLaunchKernelGGL((k_paged_weights<T, DH>), dim3((unsigned)((p.want + (long)a->B) * a->h_kv)), dim3(256), 0, s, p);
+    const dim3 grid((unsigned)((p.want + (long)a->B) * a->h_kv));
+    if (p.scores) {
+      p.least = 1024 / TILE_K;     // a round of a block's threads
+      hipLaunchKernelGGL(k_paged_weights_of, grid, dim3(256), 0, s, p);
+    } else {
+      hipLaunchKernelGGL((k_paged_weights<T, DH>), grid, dim3(256), 0, s, p);
+    }
   }
   DM_HIP(hipGetLastError());
   return DM_OK;
@@ -1139,7 +1267,7 @@ extern "C" {
 
 size_t dm_paged_workspace_bytes(const dm_paged_args* a) {
   if (!a || a->h_kv <= 0 || a->B <= 0 || a->h < a->h_kv || a->n_tokens < 0 || (a->dh != 64 && a->dh != 128)) return 0;
-  return part_floats(a) * 4;
+  return part_bytes(a) + score_floats(a) * 4;
 }
 
 int dm_paged_write(const dm_paged_args* a, void* stream) {
