@@ -34,7 +34,7 @@ struct PagedArgs {
   int B, h, h_kv, g, n_pages, cols, page_shift, N, window;
   float scale2;                        // scale log2 e
   int want, least;                     // the plan: pieces wanted, least tiles of cached rows in one
-  float* scores;                       // [N, h, cols * page] in units of ln 2, for the weights; nullptr: not kept
+  float* scores;                       // N h cols * page of them in units of ln 2, for the weights; nullptr: not kept
 };
 
 // A sequence as the call gives it. A table that does not hold its rows, or fewer rows than new tokens: bad, NaN results.
@@ -174,6 +174,7 @@ template <typename T, int DH> struct Tile {
   static constexpr int NV = KT * DH * (int)sizeof(T) / 1024;      // 16-byte loads of a lane for the step's V rows
   static constexpr int VPR = DH / V;
   static constexpr int NDT = DH / 16;
+  static constexpr int WAVES = sizeof(T) == 2 ? 3 : 3 - DH / 64;      // per SIMD (bf16 rows of 64 at 4: 97 us, at 3 92)
 };
 
 // S^T[16 cached rows][16 query rows] += K Q^T for one 16-byte chunk per lane of each: bf16 lane l holds columns
@@ -202,27 +203,22 @@ template <typename T> DM_DEV bool any_nonfinite(const u32x4& v) {
 }
 
 // Steps in which a query row does not read every row, and some value among them is not finite: a product with a probability
-// of 0 would make it NaN. Such values count 0 in the product, and a second one, of 1 for each row that is read with 1 for
-// +inf, 2^7 for -inf and 2^14 for NaN (at most 64 rows of a step, exact in bf16 and fp32), says what to add.
-DM_DEV uint32_t code_of(bool nonfinite, bool nan, bool negative, uint32_t one, uint32_t two7, uint32_t two14) {
-  return !nonfinite ? 0u : nan ? two14 : negative ? two7 : one;
+// of 0 would make it NaN. Such values count 0 in the product; at the end a second one, of 1 for each row that is read with 1
+// for +inf, 2^7 for -inf and 2^14 for NaN (of at most 32 rows, exact in bf16 and fp32), says what to add.
+DM_DEV float split_nonfinite(float v) {      // the code of a value
+  const uint32_t u = __float_as_uint(v), top = u & 0x7fffffffu;
+  return top < 0x7f800000u ? 0.f : top > 0x7f800000u ? 16384.f : u >> 31 ? 128.f : 1.f;
 }
-DM_DEV i16x8 split_nonfinite(i16x8& v) {
-  i16x8 code;
+template <typename T> DM_DEV void clear_nonfinite(u32x4& v) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t u = (uint16_t)v[i];
-    const bool odd = (u & 0x7f80u) == 0x7f80u;
-    code[i] = (short)code_of(odd, u & 0x7fu, u >> 15, 0x3f80u, 0x4300u, 0x4680u);
-    if (odd) v[i] = 0;
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 2) {
+      if ((v[j] & 0x7f80u) == 0x7f80u) v[j] &= 0xffff0000u;
+      if ((v[j] & 0x7f800000u) == 0x7f800000u) v[j] &= 0xffffu;
+    } else {
+      if ((v[j] & 0x7f800000u) == 0x7f800000u) v[j] = 0;
+    }
   }
-  return code;
-}
-DM_DEV float split_nonfinite(float& v) {
-  const uint32_t u = __float_as_uint(v);
-  const bool odd = (u & 0x7f800000u) == 0x7f800000u;
-  if (odd) v = 0.f;
-  return __uint_as_float(code_of(odd, u & 0x7fffffu, u >> 31, 0x3f800000u, 0x43000000u, 0x46800000u));
 }
 DM_DEV float said_by(float code) {
   const int c = (int)code;
@@ -235,8 +231,7 @@ DM_DEV float said_by(float code) {
 
 // O^T[16 columns][16 query rows] += V^T P^T over 32 rows. Lane l's probabilities are those of rows 16 t + 4 (l / 16) + i
 // of query row l % 16, which is how the scores' tiles leave them; V's fragments take their rows in the same order.
-// The probabilities are rounded to bf16 beside values that are bf16 themselves; their sum z is not. ODD: see
-// split_nonfinite; read: the rows that the query row reads.
+// The probabilities are rounded to bf16 beside values that are bf16 themselves; their sum z is not.
 DM_DEV i16x8 values_fragment(const bf16* v, int ldv) {
   const int lane = threadIdx.x & 63, grp = lane >> 4, s = lane & 15;
   v += (4 * grp + (s >> 2)) * ldv + 4 * (s & 3);
@@ -250,29 +245,15 @@ template <int N> DM_DEV bf16x8 to_bf16x8(const float (&p)[N], int at) {
   for (int i = 0; i < 8; ++i) r[i] = (bf16)p[at + i];
   return r;
 }
-template <typename T, int LDV, bool ODD> DM_DEV floatx4 mma_values(const T* Vs, const float (&p)[8], const float (&read)[8], floatx4 acc) {
-  floatx4 said = zero4();
+template <typename T, int LDV> DM_DEV floatx4 mma_values(const T* Vs, const float (&p)[8], floatx4 acc) {
   if constexpr (sizeof(T) == 2) {
-    i16x8 v = values_fragment((const bf16*)Vs, LDV);
-    if constexpr (ODD) {
-      const i16x8 code = split_nonfinite(v);
-      said = Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, code), to_bf16x8(read, 0), said);
-    }
-    acc = Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, v), to_bf16x8(p, 0), acc);
+    return Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, values_fragment((const bf16*)Vs, LDV)), to_bf16x8(p, 0), acc);
   } else {
     const int lane = threadIdx.x & 63, grp = lane >> 4, s = lane & 15;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = to_f(Vs[(16 * (i >> 2) + 4 * grp + (i & 3)) * LDV + s]);
-      if constexpr (ODD) said = Mfma<float>::mma(split_nonfinite(v), read[i], said);
-      acc = Mfma<float>::mma(v, p[i], acc);
-    }
+    for (int i = 0; i < 8; ++i) acc = Mfma<float>::mma(to_f(Vs[(16 * (i >> 2) + 4 * grp + (i & 3)) * LDV + s]), p[i], acc);
+    return acc;
   }
-  if constexpr (ODD) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += said_by(said[i]);
-  }
-  return acc;
 }
 
 // The page of rows r .. that lie in one (pages hold 16 rows or more and begin at a multiple of 16). needed: some query of
@@ -287,10 +268,22 @@ DM_DEV int page_of(const PagedArgs& a, const int32_t* table, int r, bool needed,
   return in ? p : 0;
 }
 
+// Row r of V, nullptr: not among [t_low, t_high), or of no page of the pool.
+template <typename T> DM_DEV const T* value_row(const PagedArgs& a, const int32_t* table, int c, int r, int t_low, int t_high, int dh) {
+  const int page = r >= t_low && r < t_high ? table[r >> a.page_shift] : -1;
+  if (page < 0 || page >= a.n_pages) return nullptr;
+  return (const T*)a.V + page * a.v_page + (((long)c << a.page_shift) + (r & ((1 << a.page_shift) - 1))) * dh;
+}
+// (rows in steps of 32)
+DM_DEV long scores_at(const PagedArgs& a, const Seq& s, int c) {
+  return ((long)s.first * a.h_kv + (long)c * s.n) * a.g * ((((long)a.cols << a.page_shift) + 31) & -32L);
+}
+
 // One block: a query tile of 16 rows, a key head and a piece of its cached rows. The four waves take steps of 32 rows in
 // turn, each with a running maximum m and sum z per query row (scores in units of ln 2) and O^T in registers, and are
-// joined through LDS.
-template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_read(PagedArgs a) {
+// joined through LDS. KEEP: the scores are kept for the weights (of the lanes behind the last query row too, which work on that
+// one again: a store that some lanes skip would have the next rows' loads wait for it, tokens_shared 276 us).
+template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile<T, DH>::WAVES)) void k_paged_read(PagedArgs a) {
   using C = Tile<T, DH>;
   constexpr int VBYTES = C::KT * C::LDV * (int)sizeof(T), OBYTES = TILE_Q * DH * 4;
   __shared__ __attribute__((aligned(16))) char smem[4 * (VBYTES > OBYTES ? VBYTES : OBYTES)];
@@ -303,23 +296,22 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
   const Seq& s = it.s;
   const int rows = s.n * a.g, rho0 = it.tile * TILE_Q;            // query rows of the sequence, the tile's first
   const int j_first = uniform(rho0 / a.g), j_last = uniform((min(rho0 + TILE_Q, rows) - 1) / a.g);
-  // the lane's query row
-  const int rho = rho0 + col, j = rho / a.g, head = c * a.g + rho % a.g;
-  const bool live = rho < rows;
-  const int high = live ? s.high(a, j) : 0, low = live ? s.low(a, j) : 0;
+  // the lane's query row; behind the last one that one again
+  const int rho = min(rho0 + col, rows - 1), j = rho / a.g, head = c * a.g + rho % a.g;
+  const int high = s.high(a, j), low = s.low(a, j);
   // the tile's rows, and this piece's
   const int t_low = s.low(a, j_first), t_high = s.bad ? 0 : s.high(a, j_last);
   const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
   const int each = uniform((tiles + it.pieces - 1) / it.pieces);
   const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
-  // rows below this and from that on are read by all live query rows
+  // rows from this on and below that are read by all query rows of the tile
   const int all_low = s.low(a, j_last), all_high = s.high(a, j_first);
 
   u32x4 qf[C::NF];
   {
     const T* q = (const T*)a.q + (long)(s.first + j) * a.q_token + (long)head * a.q_head;
 #pragma unroll
-    for (int i = 0; i < C::NF; ++i) qf[i] = live ? ld_global<u32x4>(q + i * 4 * C::V + grp * C::V) : u32x4{0, 0, 0, 0};
+    for (int i = 0; i < C::NF; ++i) qf[i] = ld_global<u32x4>(q + i * 4 * C::V + grp * C::V);
   }
   floatx4 O[C::NDT];
 #pragma unroll
@@ -330,7 +322,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < C::NF; ++i) {
-      const u32x4 k = live ? ld_global<u32x4>((const T*)a.k_rows + kr + i * 4 * C::V + grp * C::V) : u32x4{0, 0, 0, 0};
+      const u32x4 k = ld_global<u32x4>((const T*)a.k_rows + kr + i * 4 * C::V + grp * C::V);
       float x[C::V], y[C::V];
       unpack16<T>(uint4{k[0], k[1], k[2], k[3]}, x);
       unpack16<T>(uint4{qf[i][0], qf[i][1], qf[i][2], qf[i][3]}, y);
@@ -342,17 +334,19 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
     z = grp == 0 ? p : 0.f;
 #pragma unroll
     for (int d = 0; d < C::NDT; ++d) {
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (live) unpack4<T>(ld_global<typename Raw4<T>::type>((const T*)a.v_rows + vr + 16 * d + 4 * grp), v);
+      float v[4];
+      unpack4<T>(ld_global<typename Raw4<T>::type>((const T*)a.v_rows + vr + 16 * d + 4 * grp), v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) O[d][i] = p * v[i];
     }
   }
 
+  // kept scores of the lane's query row: [cached rows / 4][query rows][4] for each sequence and key head
+  float* scores = a.scores + scores_at(a, s, c) + 4 * rho + grp * (4 * rows);
   const int32_t* table = a.table + (long)it.b * a.cols;
   const int in_page = (1 << a.page_shift) - 1;
   T* Vs = reinterpret_cast<T*>(smem) + wave * C::KT * C::LDV;
-  bool bad = s.bad;
+  bool bad = s.bad, odd = false;
   u32x4 kf[2][C::NF], vf[C::NV];
   int pages[2];
   auto look_up = [&](int r0) {
@@ -380,19 +374,19 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
   if (r0 < k1) look_up(r0), load(r0), look_up(min(r0 + 4 * C::KT, k1));
   for (; r0 < k1; r0 += 4 * C::KT) {
     const bool masked = r0 < all_low || r0 + C::KT > all_high;
-    bool odd = false;    // masked values that no probability of 0 may meet
+    if (masked) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < C::NV / 2; ++i) {
-        const int v = i * 64 + lane, row = 16 * t + v / C::VPR;
-        u32x4 x = vf[t * (C::NV / 2) + i];
-        if (masked) {
-          if (r0 + row < t_low || r0 + row >= t_high) x = u32x4{0, 0, 0, 0};   // whatever lies there
-          odd |= any_nonfinite<T>(x);
-        }
-        *reinterpret_cast<u32x4*>(Vs + row * C::LDV + (v % C::VPR) * C::V) = x;
+      for (int i = 0; i < C::NV; ++i) {
+        const int row = r0 + (i * 64 + lane) / C::VPR;
+        if (row < t_low || row >= t_high) vf[i] = u32x4{0, 0, 0, 0};   // whatever lies there
+        if (any_nonfinite<T>(vf[i])) odd = true, clear_nonfinite<T>(vf[i]);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < C::NV; ++i) {
+      const int v = i * 64 + lane;
+      *reinterpret_cast<u32x4*>(Vs + v / C::VPR * C::LDV + (v % C::VPR) * C::V) = vf[i];
+    }
     float p[8];      // of rows r0 + 16 (i / 4) + 4 grp + i % 4
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -402,22 +396,22 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[4 * t + i] = acc[i] * a.scale2;
     }
-    if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT), look_up(min(r0 + 8 * C::KT, k1));
-    float read[8];
-    float top = -INF;
+    if (masked) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = r0 + 16 * (i >> 2) + 4 * grp + (i & 3);
-      const bool hidden = masked && (r < low || r >= high);
-      read[i] = hidden ? 0.f : 1.f;
-      if (hidden) p[i] = -INF;
-      top = fmaxf(top, p[i]);
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + 16 * (i >> 2) + 4 * grp + (i & 3);
+        if (r < low || r >= high) p[i] = -INF;
+      }
     }
-    if (a.scores && live) {
-      float* x = a.scores + ((long)(s.first + j) * a.h + head) * ((long)a.cols << a.page_shift) + r0 + 4 * grp;
+    float top = p[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, p[i]);
+    if constexpr (KEEP) {
+      float* x = scores + (long)(r0 >> 2) * (4 * rows);
       *reinterpret_cast<floatx4*>(x) = floatx4{p[0], p[1], p[2], p[3]};
-      if (r0 + 16 < k1) *reinterpret_cast<floatx4*>(x + 16) = floatx4{p[4], p[5], p[6], p[7]};
+      *reinterpret_cast<floatx4*>(x + 16 * rows) = floatx4{p[4], p[5], p[6], p[7]};
     }
+    if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT), look_up(min(r0 + 8 * C::KT, k1));
     top = xor_max<32>(xor_max<16>(top));
     // the reference follows the maximum only where that has risen by 2^8: sums and probabilities are relative to it
     if (__ballot(top > m + 8.f)) {
@@ -435,14 +429,40 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_rea
       z += p[i];
     }
     __builtin_amdgcn_wave_barrier();   // LDS operations of one wave complete in order
-    if (masked && __ballot(odd)) {
 #pragma unroll
-      for (int d = 0; d < C::NDT; ++d) O[d] = mma_values<T, C::LDV, true>(Vs + 16 * d, p, read, O[d]);
-    } else {
-#pragma unroll
-      for (int d = 0; d < C::NDT; ++d) O[d] = mma_values<T, C::LDV, false>(Vs + 16 * d, p, read, O[d]);
-    }
+    for (int d = 0; d < C::NDT; ++d) O[d] = mma_values<T, C::LDV>(Vs + 16 * d, p, O[d]);
     __builtin_amdgcn_wave_barrier();
+  }
+  if (__ballot(odd)) {      // see split_nonfinite
+    for (r0 = k0 + C::KT * wave; r0 < k1; r0 += 4 * C::KT) {
+      if (r0 >= all_low && r0 + C::KT <= all_high) continue;
+      float read[8];
+      const T* v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + 16 * (i >> 2) + 4 * grp + (i & 3);
+        read[i] = r < low || r >= high ? 0.f : 1.f;
+        v[i] = value_row<T>(a, table, c, r, t_low, t_high, DH);
+      }
+      for (int d = 0; d < C::NDT; ++d) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = v[i] ? to_f(v[i][16 * d + col]) : 0.f;
+        floatx4 said = zero4();
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = split_nonfinite(x[i]);
+          said = Mfma<bf16>::mma(to_bf16x8(x, 0), to_bf16x8(read, 0), said);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) said = Mfma<float>::mma(split_nonfinite(x[i]), read[i], said);
+        }
+#pragma unroll
+        for (int dd = 0; dd < C::NDT; ++dd)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) O[dd][i] += dd == d ? said_by(said[i]) : 0.f;
+      }
+    }
   }
   z = xor_sum<32>(xor_sum<16>(z));
   if (bad) z = NAN_;
@@ -628,9 +648,7 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
         if (r < t_low || r >= t_high) vr.x[i] = u32x4{0, 0, 0, 0};    // whatever lies there
         if (any_nonfinite<bf16>(vr.x[i])) {
           any_odd = 1;
-          i16x8 v = __builtin_bit_cast(i16x8, vr.x[i]);
-          split_nonfinite(v);
-          vr.x[i] = __builtin_bit_cast(u32x4, v);
+          clear_nonfinite<bf16>(vr.x[i]);
         }
       }
     }
@@ -807,20 +825,17 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
       for (int i = 0; i < 8; ++i) {      // the lane's rows
         const int r = r0 + 8 * (i >> 2) + 4 * half + (i & 3);
         read[i] = r < low || r >= high ? 0.f : 1.f;
-        const int page = r >= t_low && r < t_high ? table[r >> a.page_shift] : -1;
-        v[i] = page < 0 || page >= a.n_pages ? nullptr
-                                             : (const bf16*)a.V + page * a.v_page + (((long)c << a.page_shift) + (r & in_page)) * DH + col;
+        v[i] = value_row<bf16>(a, table, c, r, t_low, t_high, DH);
       }
 #pragma unroll
       for (int d = 0; d < C::ND; ++d) {
-        i16x8 x;
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = v[i] ? (short)ld_global<unsigned short>(v[i] + 32 * d) : (short)0;
-        const i16x8 code = split_nonfinite(x);
+        for (int i = 0; i < 8; ++i) x[i] = split_nonfinite(v[i] ? to_f(v[i][32 * d + col]) : 0.f);
         floatx16 said;
 #pragma unroll
         for (int i = 0; i < 16; ++i) said[i] = 0.f;
-        said = mma32(__builtin_bit_cast(u32x4, code), __builtin_bit_cast(u32x4, to_bf16x8(read, 0)), said);
+        said = mma32(__builtin_bit_cast(u32x4, to_bf16x8(x, 0)), __builtin_bit_cast(u32x4, to_bf16x8(read, 0)), said);
 #pragma unroll
         for (int i = 0; i < 16; ++i) O[d][i] += said_by(said[i]);
       }
@@ -920,15 +935,14 @@ __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
   float* w = a.weights + ((long)it.b * a.h_kv + c) * cap;
   for (int r = k0 + 4 * threadIdx.x; r < k1; r += 1024) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* x = a.scores + scores_at(a, s, c) + (long)r * (s.n * a.g);
     for (int j = 0; j < s.n; ++j) {
       const int low = s.low(a, j), high = s.high(a, j);
       if (r >= high || r + 4 <= low) continue;
-      const long at = (long)(s.first + j) * a.h + c * a.g;
-      const float* x = a.scores + at * cap + r;
 #pragma unroll 4
       for (int i = 0; i < a.g; ++i) {
-        const floatx4 v = *reinterpret_cast<const floatx4*>(x + i * cap);
-        const float lse2 = lse_of(a.lse[at + i]);
+        const floatx4 v = *reinterpret_cast<const floatx4*>(x + 4 * (j * a.g + i));
+        const float lse2 = lse_of(a.lse[(long)(s.first + j) * a.h + c * a.g + i]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] += r + e >= low && r + e < high ? __builtin_amdgcn_exp2f(v[e] - lse2) : 0.f;
       }
@@ -1022,8 +1036,44 @@ DM_DEV uint32_t weight_order(float x) {
 
 // One block per sequence and key head: the weight of the last row to be kept by its bits, eight at a time from the top
 // (a histogram over the rows that agree so far), then the rows in order: those above it, and of those equal to it the first.
+// A thread takes 4 rows in turn; the first KEYS * 4096 rows' weights stay in registers. Eight histograms, by lane, since weights
+// share their first bits; bound by its passes' latencies (one sequence of 2304 rows 11 us, 16384 rows 17).
+constexpr int KEYS = 4, COPIES = 8;
+struct Selection {
+  int hist[256 * COPIES];
+  int total[2][KEYS][16];
+  int digit, above;
+};
+
+// of the need-th largest: its digit, and how many rows have a larger one. By the first wave: lane l takes digits 4 (63 - l) ..
+// + 3, from the largest.
+DM_DEV void find_digit(Selection& sh, int need) {
+  const int lane = threadIdx.x & 63, d0 = 4 * (63 - lane);
+  int n[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    n[i] = 0;
+#pragma unroll
+    for (int k = 0; k < COPIES; ++k) n[i] += sh.hist[(d0 + i) * COPIES + k];
+    sum += n[i];
+  }
+  int upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += v;
+  }
+  int above = upto - sum;
+  if (above < need && upto >= need) {
+    int d = 3;
+    while (d > 0 && above + n[d] < need) above += n[d--];
+    sh.digit = d0 + d;
+    sh.above = above;
+  }
+}
+
 __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
-  __shared__ int hist[256], total[2][16], found[2];
+  __shared__ Selection sh;
   const int c = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long cap = (long)a.cols << a.page_shift;
   const int len = a.lengths[b] < 0 || a.lengths[b] > cap ? 0 : a.lengths[b];
@@ -1037,55 +1087,91 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
   }
   const float* w = a.weights + ((long)b * a.h + c) * cap;
   const int lo = a.sinks, hi = len - a.recent;      // rows that may go
+  // rows 4 q .. 4 q + 3 (the capacity is a multiple of 16)
+  auto keys_of = [&](int q, uint32_t (&u)[4]) {
+    if (4 * q < len) {
+      const floatx4 v = *reinterpret_cast<const floatx4*>(w + 4 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = weight_order(v[e]);
+    }
+  };
+  uint32_t held[KEYS][4];
+#pragma unroll
+  for (int k = 0; k < KEYS; ++k) keys_of(threadIdx.x + 1024 * k, held[k]);
   uint32_t key = 0;
   int need = a.keep - a.sinks - a.recent;           // of them stay (less than there are)
   if (need > 0) {
     for (int shift = 24; shift >= 0; shift -= 8) {
-      if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+      for (int i = threadIdx.x; i < 256 * COPIES; i += 1024) sh.hist[i] = 0;
       __syncthreads();
       const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i = lo + threadIdx.x; i < hi; i += 1024) {
-        const uint32_t u = weight_order(w[i]);
-        if ((u & mask) == key) atomicAdd(&hist[(u >> shift) & 255], 1);
+      auto count = [&](int q, const uint32_t (&u)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * q + e >= lo && 4 * q + e < hi && (u[e] & mask) == key)
+            atomicAdd(&sh.hist[((u[e] >> shift) & 255) * COPIES + (lane & (COPIES - 1))], 1);
+      };
+#pragma unroll
+      for (int k = 0; k < KEYS; ++k) count(threadIdx.x + 1024 * k, held[k]);
+      for (int q = threadIdx.x + 1024 * KEYS; 4 * q < hi; q += 1024) {
+        uint32_t u[4];
+        keys_of(q, u);
+        count(q, u);
       }
       __syncthreads();
-      if (threadIdx.x == 0) {
-        int d = 255, above = 0;
-        while (d > 0 && above + hist[d] < need) above += hist[d--];
-        found[0] = d;
-        found[1] = above;
-      }
+      if (wave == 0) find_digit(sh, need);
       __syncthreads();
-      key |= (uint32_t)found[0] << shift;
-      need -= found[1];
+      key |= (uint32_t)sh.digit << shift;
+      need -= sh.above;
     }
   } else {
     key = 0xffffffffu;
   }
   // need: how many of the rows equal to key stay
   int at = 0, equal = 0;
-  for (int i0 = 0; i0 < len; i0 += 1024) {
-    const int i = i0 + threadIdx.x;
-    bool sure = false, tie = false;
-    if (i < len) {
-      if (i < lo || i >= hi) sure = true;
-      else {
-        const uint32_t u = weight_order(w[i]);
-        sure = u > key;
-        tie = u == key;
+  for (int q0 = 0; 4 * q0 < len; q0 += 1024 * KEYS) {
+    int sure[KEYS], tie[KEYS], before[KEYS];     // bits of a thread's rows; rows of the wave before the thread's, ties << 16
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) {
+      const int q = q0 + threadIdx.x + 1024 * k;
+      uint32_t u[4];
+      if (q0) keys_of(q, u);
+      else u[0] = held[k][0], u[1] = held[k][1], u[2] = held[k][2], u[3] = held[k][3];
+      sure[k] = tie[k] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * q + e;
+        if (i < len && (i < lo || i >= hi || u[e] > key)) sure[k] |= 1 << e;
+        else if (i < len && u[e] == key) tie[k] |= 1 << e;
+      }
+      const int mine = __popc(sure[k]) + (__popc(tie[k]) << 16);
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += v;
+      }
+      before[k] = sum - mine;
+      if (lane == 63) sh.total[0][k][wave] = sum & 0xffff, sh.total[1][k][wave] = sum >> 16;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) {
+      int s = at + (before[k] & 0xffff), t = equal + (before[k] >> 16);
+      for (int x = 0; x < 16; ++x) {
+        if (x < wave) s += sh.total[0][k][x], t += sh.total[1][k][x];
+        at += sh.total[0][k][x];
+        equal += sh.total[1][k][x];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool is_sure = sure[k] >> e & 1, is_tie = tie[k] >> e & 1;
+        if (is_sure || (is_tie && t < need)) rows[s + min(t, need)] = 4 * (q0 + (int)threadIdx.x + 1024 * k) + e;
+        s += is_sure;
+        t += is_tie;
       }
     }
-    const uint64_t bs = __ballot(sure), bt = __ballot(tie), before = (1ull << lane) - 1;
     __syncthreads();
-    if (lane == 0) total[0][wave] = __popcll(bs), total[1][wave] = __popcll(bt);
-    __syncthreads();
-    int s = at + __popcll(bs & before), e = equal + __popcll(bt & before);
-    for (int k = 0; k < 16; ++k) {
-      if (k < wave) s += total[0][k], e += total[1][k];
-      at += total[0][k];
-      equal += total[1][k];
-    }
-    if (sure || (tie && e < need)) rows[s + min(e, need)] = i;
   }
 }
 
@@ -1148,7 +1234,7 @@ Form form_of(const dm_paged_args* a) {
 // again from the keys.
 size_t score_floats(const dm_paged_args* a) {
   if (!a->weights || form_of(a).rows != TILE_Q) return 0;
-  const double n = (double)a->n_tokens * a->h * a->table_cols * a->page;
+  const double n = (double)a->n_tokens * a->h * (((int64_t)a->table_cols * a->page + 31) & -32);
   return n * 4 <= (double)a->n_pages * a->h_kv * a->page * a->dh * esz(a->dtype) ? (size_t)n : 0;
 }
 size_t part_floats(const dm_paged_args* a) {
@@ -1235,7 +1321,8 @@ template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStrea
   const bool join = (int64_t)a->table_cols * a->page > f.least * TILE_K;
   const dim3 joined((unsigned)(tiles * a->h_kv), f.rows / 16);
   if (f.rows == TILE_Q) {
-    hipLaunchKernelGGL((k_paged_read<T, DH>), dim3(blocks), dim3(256), 0, s, p);
+    if (p.scores) hipLaunchKernelGGL((k_paged_read<T, DH, true>), dim3(blocks), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((k_paged_read<T, DH, false>), dim3(blocks), dim3(256), 0, s, p);
     if (join) hipLaunchKernelGGL((k_paged_join<T, DH, TILE_Q>), joined, dim3(256), 0, s, p);
   }
   if constexpr (sizeof(T) == 2) {
