@@ -190,8 +190,20 @@ template <typename T> DM_DEV floatx4 mma_chunk(const u32x4& k, const u32x4& q, f
   }
 }
 
-// O^T[16 columns][16 query rows] += V^T P^T over 32 rows. Lane l's probabilities are those of rows 16 t + 4 (l / 16) + i
-// of query row l % 16, which is how the scores' tiles leave them; V's fragments take their rows in the same order.
+// the same for two tiles, whose chains of sums take turns
+template <typename T> DM_DEV void mma_chunks(const u32x4& k0, const u32x4& k1, const u32x4& q, floatx4 (&acc)[2]) {
+  if constexpr (sizeof(T) == 2) {
+    acc[0] = mma_chunk<T>(k0, q, acc[0]);
+    acc[1] = mma_chunk<T>(k1, q, acc[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      acc[0] = Mfma<float>::mma(__uint_as_float(k0[j]), __uint_as_float(q[j]), acc[0]);
+      acc[1] = Mfma<float>::mma(__uint_as_float(k1[j]), __uint_as_float(q[j]), acc[1]);
+    }
+  }
+}
+
 template <typename T> DM_DEV bool any_nonfinite(const u32x4& v) {
   bool bad = false;
 #pragma unroll
@@ -388,14 +400,11 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
       *reinterpret_cast<u32x4*>(Vs + v / C::VPR * C::LDV + (v % C::VPR) * C::V) = vf[i];
     }
     float p[8];      // of rows r0 + 16 (i / 4) + 4 grp + i % 4
+    floatx4 acc[2] = {zero4(), zero4()};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      floatx4 acc = zero4();
+    for (int i = 0; i < C::NF; ++i) mma_chunks<T>(kf[0][i], kf[1][i], qf[i], acc);
 #pragma unroll
-      for (int i = 0; i < C::NF; ++i) acc = mma_chunk<T>(kf[t][i], qf[i], acc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[4 * t + i] = acc[i] * a.scale2;
-    }
+    for (int i = 0; i < 8; ++i) p[i] = acc[i >> 2][i & 3] * a.scale2;
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -971,7 +980,13 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
   const int32_t* table = a.table + (long)it.b * a.cols;
   const int in_page = (1 << a.page_shift) - 1;
   float* w = a.weights + ((long)it.b * a.h_kv + c) * ((long)a.cols << a.page_shift);
-  for (int r0 = k0 + C::KT * wave; r0 < k1; r0 += 4 * C::KT) {
+  // Few query rows: each wave takes cached rows of its own; many: the waves share them and take the query tiles in turn
+  // (window_fp32: 23.2 us without)
+  __shared__ float part[2][4][C::KT];
+  const bool shared = rows > 4 * TILE_Q;
+  const int step = shared ? C::KT : 4 * C::KT, q_first = shared ? TILE_Q * wave : 0, q_step = shared ? 4 * TILE_Q : TILE_Q;
+  int buf = 0;
+  for (int r0 = k0 + (shared ? 0 : C::KT * wave); r0 < k1; r0 += step, buf ^= 1) {
     u32x4 kf[2][C::NF];
     bool bad = false;
 #pragma unroll
@@ -983,27 +998,37 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
       for (int i = 0; i < C::NF; ++i) kf[t][i] = ld_global<u32x4>(K + col * DH + i * 4 * C::V + grp * C::V);
     }
     float sum[2][4] = {};
-    for (int rho0 = 0; rho0 < rows; rho0 += TILE_Q) {
-      const int rho = rho0 + col, j = rho / a.g, head = c * a.g + rho % a.g;
-      const bool live = rho < rows;
-      const long at = (long)(s.first + j) * a.h + head;
-      const int high = live ? s.high(a, j) : 0, low = live ? s.low(a, j) : 0;
+    // the tokens that read one of these rows; a tile of their query rows is on its way while the one before is used
+    const int past = s.len - s.n;
+    const int j0 = max(0, r0 - past + (a.k_rows ? 1 : 0)), j1 = a.window ? min((long)s.n, (long)r0 - past + C::KT - 1 + a.window) : s.n;
+    u32x4 qf[C::NF];
+    float lse2 = 0.f;
+    auto fetch = [&](int rho0) {
+      const int rho = min(rho0 + col, rows - 1), j = rho / a.g, head = c * a.g + rho % a.g;
       const T* q = (const T*)a.q + (long)(s.first + j) * a.q_token + (long)head * a.q_head;
-      u32x4 qf[C::NF];
 #pragma unroll
-      for (int i = 0; i < C::NF; ++i) qf[i] = live ? ld_global<u32x4>(q + i * 4 * C::V + grp * C::V) : u32x4{0, 0, 0, 0};
-      const float lse2 = live ? lse_of(a.lse[at]) : 0.f;
+      for (int i = 0; i < C::NF; ++i) qf[i] = ld_global<u32x4>(q + i * 4 * C::V + grp * C::V);
+      lse2 = lse_of(a.lse[(long)(s.first + j) * a.h + head]);
+    };
+    int rho0 = j0 * a.g + q_first;
+    if (rho0 < j1 * a.g) fetch(rho0);
+    for (; rho0 < j1 * a.g; rho0 += q_step) {
+      const int rho = rho0 + col, j = rho / a.g;
+      const bool live = rho < rows;
+      const int high = live ? s.high(a, j) : 0, low = live ? s.low(a, j) : 0;
+      floatx4 acc[2];
+      const float minus = -lse2;
+      acc[0] = acc[1] = zero4();
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        floatx4 acc = zero4();
+      for (int i = 0; i < C::NF; ++i) mma_chunks<T>(kf[0][i], kf[1][i], qf[i], acc);
+      if (rho0 + q_step < j1 * a.g) fetch(rho0 + q_step);
 #pragma unroll
-        for (int i = 0; i < C::NF; ++i) acc = mma_chunk<T>(kf[t][i], qf[i], acc);
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = r0 + 16 * t + 4 * grp + i;
-          if (r >= low && r < high) sum[t][i] += __builtin_amdgcn_exp2f(fmaf(acc[i], a.scale2, -lse2));
+          if (r >= low && r < high) sum[t][i] += __builtin_amdgcn_exp2f(fmaf(acc[t][i], a.scale2, minus));
         }
-      }
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -1011,8 +1036,18 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
       for (int i = 0; i < 4; ++i) {
         const int r = r0 + 16 * t + 4 * grp + i;
         const float x = group16_sum(sum[t][i]);
-        if (col == 0 && r >= t_low && r < t_high) w[r] += bad ? NAN_ : x;
+        if (shared) {
+          if (col == 0) part[buf][wave][r - r0] = bad ? NAN_ : x;
+        } else if (col == 0 && r >= t_low && r < t_high) {
+          w[r] += bad ? NAN_ : x;
+        }
       }
+    if (shared) {     // (the other buffer's sums are read before the next barrier)
+      __syncthreads();
+      const int r = r0 + threadIdx.x;
+      if (threadIdx.x < C::KT && r >= t_low && r < t_high)
+        w[r] += (part[buf][0][threadIdx.x] + part[buf][1][threadIdx.x]) + (part[buf][2][threadIdx.x] + part[buf][3][threadIdx.x]);
+    }
   }
 }
 
@@ -1227,7 +1262,7 @@ struct Form {
 };
 Form form_of(const dm_paged_args* a) {
   const int64_t mean = (int64_t)a->n_tokens * (a->h / a->h_kv) / a->B;
-  if (a->dtype != DM_BF16 || mean <= 2 * TILE_Q) return {TILE_Q, 4 * CUS, 2};
+  if (a->dtype != DM_BF16 || mean <= 2 * TILE_Q) return {TILE_Q, 5 * CUS, 2};
   return mean <= 512 ? Form{128, 2 * CUS, 2} : Form{256, CUS, 2};
 }
 // The scores of a call with weights are kept where they take no more room than the pages' keys; else they are computed
@@ -1341,6 +1376,7 @@ template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStrea
       p.least = 1024 / TILE_K;     // a round of a block's threads
       hipLaunchKernelGGL(k_paged_weights_of, grid, dim3(256), 0, s, p);
     } else {
+      p.least = 1;
       hipLaunchKernelGGL((k_paged_weights<T, DH>), grid, dim3(256), 0, s, p);
     }
   }
