@@ -1051,6 +1051,105 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
   }
 }
 
+// The same for many query rows: a block takes 64 cached rows, each wave all of them against 32 query rows at a time (every
+// fragment of Q is used twice), the waves' sums are added through LDS. Bound by the exponentials beside the products: two
+// sequences of 16384 rows, 8192 query rows of 128: 0.6 ms, with 16-row tiles 1.84.
+template <int DH> __global__ __launch_bounds__(256, 2) void k_paged_weights_wide(PagedArgs a) {
+  constexpr int NK = DH / 16;
+  __shared__ float part[2][4][TILE_K];
+  const int c = uniform(blockIdx.x % a.h_kv), lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Item it = find_item<0, true>(a, blockIdx.x / a.h_kv);
+  if (it.b < 0) return;
+  make_uniform(it);
+  const Seq& s = it.s;
+  if (s.bad) return;
+  const int rows = s.n * a.g, t_low = s.low(a, 0), t_high = s.high(a, s.n - 1), past = s.len - s.n;
+  const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
+  const int each = uniform((tiles + it.pieces - 1) / it.pieces);
+  const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
+  const int32_t* table = a.table + (long)it.b * a.cols;
+  const int in_page = (1 << a.page_shift) - 1;
+  float* w = a.weights + ((long)it.b * a.h_kv + c) * ((long)a.cols << a.page_shift);
+  int buf = 0;
+  for (int r0 = k0; r0 < k1; r0 += TILE_K, buf ^= 1) {
+    u32x4 kf[2][NK];
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int page[2];     // of 16 rows each
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = r0 + 32 * t + 16 * e;
+        page[e] = page_of(a, table, r, r < t_high && r + 16 > t_low, bad);
+      }
+      const long at = ((long)c << a.page_shift) + ((r0 + 32 * t + col) & in_page);
+      const bf16* K = (const bf16*)a.K + (col < 16 ? page[0] : page[1]) * a.k_page + at * DH + 8 * half;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) kf[t][i] = ld_global<u32x4>(K + 16 * i);
+    }
+    const int j0 = max(0, r0 - past + (a.k_rows ? 1 : 0)), j1 = a.window ? min((long)s.n, (long)r0 - past + TILE_K - 1 + a.window) : s.n;
+    float sum[2][16];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[t][i] = 0.f;
+    u32x4 qf[NK];
+    float lse2 = INF;
+    auto fetch = [&](int rho0) {
+      const int rho = min(rho0 + col, rows - 1), j = rho / a.g, head = c * a.g + rho % a.g;
+      const bf16* q = (const bf16*)a.q + (long)(s.first + j) * a.q_token + (long)head * a.q_head + 8 * half;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) qf[i] = ld_global<u32x4>(q + 16 * i);
+      lse2 = rho0 + col < rows ? lse_of(a.lse[(long)(s.first + j) * a.h + head]) : INF;
+    };
+    int rho0 = j0 * a.g + 32 * wave;
+    if (rho0 < j1 * a.g) fetch(rho0);
+    for (; rho0 < j1 * a.g; rho0 += 128) {
+      const int j = min(rho0 + col, rows - 1) / a.g;
+      const float minus = -lse2;
+      floatx16 S[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[t][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        S[0] = mma32(kf[0][i], qf[i], S[0]);
+        S[1] = mma32(kf[1][i], qf[i], S[1]);
+      }
+      if (rho0 + 128 < j1 * a.g) fetch(rho0 + 128);
+      const int first = uniform(rho0 / a.g), last = uniform((min(rho0 + 32, rows) - 1) / a.g);
+      if (r0 < s.low(a, last) || r0 + TILE_K > s.high(a, first)) {
+        const int from = s.low(a, j) - r0 - 4 * half, to = s.high(a, j) - r0 - 4 * half;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = 32 * t + 8 * (i >> 2) + (i & 3);
+            sum[t][i] += r < from || r >= to ? 0.f : __builtin_amdgcn_exp2f(fmaf(S[t][i], a.scale2, minus));
+          }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[t][i] += __builtin_amdgcn_exp2f(fmaf(S[t][i], a.scale2, minus));
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = lanes_sum<1, 16>(sum[t][i]);
+        if (col == 0) part[buf][wave][32 * t + 8 * (i >> 2) + 4 * half + (i & 3)] = bad ? NAN_ : x;
+      }
+    __syncthreads();     // (the other buffer's sums are read before the next barrier)
+    const int r = r0 + threadIdx.x;
+    if (threadIdx.x < TILE_K && r >= t_low && r < t_high)
+      w[r] += (part[buf][0][threadIdx.x] + part[buf][1][threadIdx.x]) + (part[buf][2][threadIdx.x] + part[buf][3][threadIdx.x]);
+  }
+}
+
 // ---- eviction ------------------------------------------------------------------------------------
 struct EvictArgs {
   const void *K, *V;
@@ -1377,7 +1476,10 @@ template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStrea
       hipLaunchKernelGGL(k_paged_weights_of, grid, dim3(256), 0, s, p);
     } else {
       p.least = 1;
-      hipLaunchKernelGGL((k_paged_weights<T, DH>), grid, dim3(256), 0, s, p);
+      if constexpr (sizeof(T) == 2) {
+        if (f.rows != TILE_Q) hipLaunchKernelGGL(k_paged_weights_wide<DH>, grid, dim3(256), 0, s, p);
+      }
+      if (f.rows == TILE_Q) hipLaunchKernelGGL((k_paged_weights<T, DH>), grid, dim3(256), 0, s, p);
     }
   }
   DM_HIP(hipGetLastError());
