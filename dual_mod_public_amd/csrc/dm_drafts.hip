@@ -15,7 +15,41 @@ namespace {
 
 constexpr float INF = __builtin_inff(), NAN_ = __builtin_nanf("");
 constexpr int PART = 4096;      // columns of a block's part of a row
-constexpr int EACH = PART / 256;
+
+// 2^(w / 32) for w <= 0 (w = 32 x / (T ln 2) for e^(x / T), x a difference of logits), relative error below 2e-12: 2^(n / 32)
+// 2^(f / 32) with n the nearest whole number to w, the 32 roots from a table in LDS (one in each pair of its banks), and the Taylor
+// sum of 2^(f / 32) up to f^4 (|f| <= 1/2 leaves (ln 2 / 64)^5 / 120 = 1.3e-12). Half of the instructions of the library's
+// function, whose range and last bits are not needed here. Below 2^-1000 it stays there: a probability that has to be 0 is
+// made so by its logit. No NaN.
+__constant__ const double ROOTS[32] = {      // 2^(i / 32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+constexpr int LEAST = 1000;
+struct Roots {
+  double v[32];            // 2^(i / 32 - LEAST)
+  DM_DEV void fill() {     // a barrier has to follow
+    if (threadIdx.x < 32) v[threadIdx.x] = ROOTS[threadIdx.x] * 0x1p-1000;
+  }
+};
+DM_DEV double scale_of(double T) { return 32.0 / (T * 0.6931471805599453); }
+DM_DEV double exp_of(double w, const Roots& roots) {
+  constexpr double SHIFT = 0x1.8p52 + 32 * LEAST;      // the sum with it holds n + 32 LEAST in its low bits
+  w = fmax(w, -32.0 * LEAST);
+  const double big = w + SHIFT, f = w - (big - SHIFT);
+  double e = fma(f, 9.172562701824643e-09, 1.693850972437182e-06);
+  e = fma(e, f, 0.0002345961982022468);
+  e = fma(e, f, 0.02166084939249829);
+  e = fma(e, f, 1.0);
+  const uint32_t k = (uint32_t)__double_as_longlong(big);
+  const uint64_t root = (uint64_t)__double_as_longlong(roots.v[k & 31]);
+  return e * __longlong_as_double((long long)(root + ((uint64_t)(k >> 5) << 52)));
+}
 
 // A part's sum of exp((x - m) / T) relative to its own maximum, with the first place of that; m is NaN where the part holds
 // one.
@@ -28,9 +62,12 @@ struct Part {
 struct Choice {
   double zp, zq;      // sums of exponentials of its target and draft rows (zq 0: p alone)
   float mp, mq;       // their maxima
-  int row;            // token row, -1: none
+  int row;            // token row
   int drop;           // a column that counts 0 (the draft without a distribution), -1: none
-  int token;          // -2: to be drawn; else the token, -1 where there is no distribution
+  int token;          // -2: to be drawn; else there is nothing more to do
+  double scale, T;    // scale_of its temperature, and that
+  double log_zp;
+  float u;            // its place
 };
 
 struct VerifyArgs {
@@ -56,81 +93,111 @@ struct Rows {
   }
 };
 
-// the sequence of token row t, -1: none
+// The sequence of token row t, the same in all lanes of a wave; -1: none.
 DM_DEV int sequence_of(const VerifyArgs& a, int t) {
-  int lo = 0, hi = a.B;
-  while (lo + 1 < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.starts[mid] <= t) lo = mid;
-    else hi = mid;
+  int n = 0;     // sequences that start at t or before
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + (threadIdx.x & 63);
+    n += __popcll(__ballot(b < a.B && a.starts[b] <= t));
   }
-  const Rows r(a, lo);
-  return t >= r.first && t < r.first + r.n ? lo : -1;
+  if (n == 0) return -1;
+  const Rows r(a, n - 1);
+  return t >= r.first && t < r.first + r.n ? n - 1 : -1;
 }
 // a temperature of 0 is greedy; the log probabilities are those at 1 then
 DM_DEV double divisor(float T) { return T == 0.f ? 1.0 : (double)T; }
 
+// sums and minima over a wave without the LDS crossbar (lane_pair)
+template <int O> DM_DEV double pair_sum(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const LanePair lo = lane_pair<O>(__uint_as_float((uint32_t)u)), hi = lane_pair<O>(__uint_as_float((uint32_t)(u >> 32)));
+  const auto join = [](float l, float h) { return __longlong_as_double((long long)((uint64_t)__float_as_uint(h) << 32 | __float_as_uint(l))); };
+  return join(lo.a, hi.a) + join(lo.b, hi.b);
+}
 DM_DEV double wave_sum_double(double v) {
+  return pair_sum<32>(pair_sum<16>(pair_sum<8>(pair_sum<4>(pair_sum<2>(pair_sum<1>(v))))));
+}
+template <int O> DM_DEV int pair_min(int v) {
+  const LanePair p = lane_pair<O>(__uint_as_float((uint32_t)v));
+  return min((int)__float_as_uint(p.a), (int)__float_as_uint(p.b));
+}
+DM_DEV int wave_min(int v) { return pair_min<32>(pair_min<16>(pair_min<8>(pair_min<4>(pair_min<2>(pair_min<1>(v)))))); }
+
+// N elements from column c on; -inf behind the row. Rows have their elements' alignment only.
+template <typename T, int N> DM_DEV void load_columns(const T* x, int c, int cols, float (&v)[N]) {
+  constexpr int V = 16 / (int)sizeof(T) < N ? 16 / (int)sizeof(T) : N;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  for (int i = 0; i < N; i += V) {
+    if (c + i + V <= cols) {
+      const auto r = ld_global_a<typename RawV<T, V>::type, (int)sizeof(T)>(x + c + i);
+      float u[V];
+      unpackv<T, V>(r, u);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i + e] = u[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i + e] = c + i + e < cols ? to_f(x[c + i + e]) : -INF;
+    }
+  }
 }
 
-// One block per row and part of it, of the target and of the draft (blockIdx.z).
+// One block per row and part of it, of the target and of the draft (blockIdx.z). Bound by the exponentials in 64 bits (about
+// 20 instructions each), close to the rows' bytes.
 template <typename T> __global__ __launch_bounds__(256) void k_verify_parts(VerifyArgs a) {
-  const int t = blockIdx.y, c0 = blockIdx.x * PART;
+  constexpr int V = 16 / (int)sizeof(T), EACH = PART / 256;
+  __shared__ Roots roots;
+  __shared__ float sm[4];
+  __shared__ double sz[4];
+  __shared__ int sarg[4], snan[4];
+  const int t = blockIdx.y, c0 = blockIdx.x * PART, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool draft = blockIdx.z;
+  const T* x = draft ? (const T*)a.y + t * a.ld_y : (const T*)a.x + t * a.ld_x;
+  float v[EACH / V][V];
+#pragma unroll
+  for (int i = 0; i < EACH / V; ++i) load_columns(x, c0 + (threadIdx.x + 256 * i) * V, a.V, v[i]);
   const int b = sequence_of(a, t);
   if (b < 0) return;
   const Rows rows(a, b);
-  if (draft && t == rows.first + rows.n - 1) return;
-  const T* x = (draft ? (const T*)a.y + t * a.ld_y : (const T*)a.x + t * a.ld_x) + c0;
-  const int n = min(PART, a.V - c0);
-  const double inv = 1.0 / divisor(a.temperature[b]);
-  float v[EACH];
+  const float temperature = a.temperature[b];
+  if (draft && (t == rows.first + rows.n - 1 || temperature == 0.f)) return;
+  const double scale = scale_of(divisor(temperature));
+  roots.fill();
   float m = -INF;
   bool nan = false;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const int c = threadIdx.x + 256 * i;
-    v[i] = c < n ? to_f(x[c]) : -INF;
-    m = fmaxf(m, v[i]);
-    nan |= v[i] != v[i];
+    m = fmaxf(m, v[i / V][i % V]);
+    nan |= v[i / V][i % V] != v[i / V][i % V];
   }
-  __shared__ float sm[4];
-  __shared__ double sz[4];
-  __shared__ int sarg[4], snan;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x == 0) snan = 0;
   m = wave_max(m);
-  if (lane == 0) sm[wave] = m;
+  nan = __ballot(nan) != 0;
+  if (lane == 0) sm[wave] = m, snan[wave] = nan;
   __syncthreads();
-  if (nan) snan = 1;
   m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  const double ref = m == -INF ? 0.0 : (double)m;
+  const double minus = m == -INF ? 0.0 : -(double)m * scale;
   double z = 0.0;
   int arg = 0x7fffffff;
 #pragma unroll
-  for (int i = EACH - 1; i >= 0; --i) {
-    if (v[i] == m) arg = threadIdx.x + 256 * i;
+  for (int i = 0; i < EACH; ++i) z += exp_of(fma((double)v[i / V][i % V], scale, minus), roots);
+  z = m == -INF ? 0.0 : wave_sum_double(z);
+  if (temperature == 0.f) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (v[i / V][i % V] == m) arg = min(arg, c0 + ((int)threadIdx.x + 256 * (i / V)) * V + i % V);
+    arg = wave_min(arg);
   }
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) z += exp(((double)v[i] - ref) * inv);
-  z = wave_sum_double(z);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o, 64));
   if (lane == 0) sz[wave] = z, sarg[wave] = arg;
   __syncthreads();
   if (threadIdx.x) return;
   Part p;
   p.z = (sz[0] + sz[1]) + (sz[2] + sz[3]);
-  p.m = snan ? NAN_ : m;
-  p.arg = c0 + min(min(sarg[0], sarg[1]), min(sarg[2], sarg[3]));
+  p.m = snan[0] | snan[1] | snan[2] | snan[3] ? NAN_ : m;
+  p.arg = min(min(sarg[0], sarg[1]), min(sarg[2], sarg[3]));
   a.parts[((long)draft * a.N + t) * a.n_parts + blockIdx.x] = p;
 }
 
 // A row's parts joined by a wave: the maximum (NaN if there is one), the sum relative to it and the first place of it.
-DM_DEV Part join_parts(const VerifyArgs& a, bool draft, int t, double inv) {
+DM_DEV Part join_parts(const VerifyArgs& a, bool draft, int t, double scale, const Roots& roots) {
   const Part* p = a.parts + ((long)draft * a.N + t) * a.n_parts;
   const int lane = threadIdx.x & 63;
   float m = -INF;
@@ -144,200 +211,228 @@ DM_DEV Part join_parts(const VerifyArgs& a, bool draft, int t, double inv) {
   int arg = 0x7fffffff;
   for (int i = lane; i < a.n_parts; i += 64) {
     if (p[i].m == m) arg = min(arg, p[i].arg);
-    z += p[i].z * (p[i].m == -INF ? 0.0 : exp(((double)p[i].m - m) * inv));
+    z += p[i].z * (p[i].m == -INF ? 0.0 : exp_of(((double)p[i].m - m) * scale, roots));
   }
   Part r;
   r.z = wave_sum_double(z);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) arg = min(arg, __shfl_xor(arg, o, 64));
-  r.arg = arg;
+  r.arg = wave_min(arg);
   r.m = __ballot(nan) ? NAN_ : m;
   return r;
 }
 // whether the parts are those of a distribution: something finite, no NaN, no +inf
 DM_DEV bool is_distribution(const Part& p) { return fabsf(p.m) < INF; }
 
-// Every block of a sequence's parts decides over its rows (a wave each, in turn), the first one writes what is decided; then
-// each sums its part of the chosen row.
-template <typename T> __global__ __launch_bounds__(256) void k_verify_choose(VerifyArgs a) {
-  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Rows rows(a, b);
-  __shared__ Choice ch;
-  __shared__ int end;
-  __shared__ double sums[2][4];
-  if (threadIdx.x == 0) end = rows.n;
-  __syncthreads();
-  const float temperature = a.temperature[b];
-  const double inv = 1.0 / divisor(temperature);
-  const bool greedy = temperature == 0.f;
-  for (int i = wave; i < rows.n; i += 4) {
-    const int t = rows.first + i;
-    const bool last = i == rows.n - 1;
-    const Part p = join_parts(a, false, t, inv);
-    Part q;
-    q.z = 0.0, q.m = 0.f;
-    if (!last && a.y && !greedy) q = join_parts(a, true, t, inv);
-    const long d = last ? -1 : a.ids[t + 1];
-    const bool in_range = d >= 0 && d < a.V;
-    bool ok = false;
-    double pd = 0.0, lp = NAN_;
-    const bool valid = is_distribution(p) && is_distribution(q);
-    if (valid && in_range) {
-      lp = ((double)to_f(((const T*)a.x)[t * a.ld_x + d]) - p.m) * inv;
-      pd = exp(lp) / p.z;
-      lp -= log(p.z);
-    }
-    if (greedy) {
-      ok = !last && d == p.arg && p.m == p.m && p.m > -INF;
-    } else if (valid && in_range) {
-      const double qd = a.y ? exp(((double)to_f(((const T*)a.y)[t * a.ld_y + d]) - q.m) * inv) / q.z : 1.0;
-      ok = (double)a.u[2 * t] * qd < pd;
-    }
-    if (!ok && lane == 0) atomicMin(&end, i);
-    if (ok && blockIdx.x == 0 && lane == 0) {
-      a.tokens[t] = d;
-      a.logp[t] = (float)lp;
+// 4 columns of the chosen row's p, and r
+template <typename T> struct Residual {
+  float x[4];
+  double p[4], r[4];
+  DM_DEV Residual(const VerifyArgs& a, const Choice& ch, int c, const Roots& roots) {
+    float y[4];
+    load_columns((const T*)a.x + ch.row * a.ld_x, c, a.V, x);
+    if (ch.zq > 0.0) load_columns((const T*)a.y + ch.row * a.ld_y, c, a.V, y);
+    const double ip = 1.0 / ch.zp, iq = ch.zq > 0.0 ? 1.0 / ch.zq : 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i] = x[i] == -INF ? 0.0 : exp_of(((double)x[i] - ch.mp) * ch.scale, roots) * ip;
+      const double q = ch.zq > 0.0 && y[i] != -INF ? exp_of(((double)y[i] - ch.mq) * ch.scale, roots) * iq : 0.0;
+      r[i] = c + i == ch.drop ? 0.0 : fmax(p[i] - q, 0.0);
     }
   }
-  __syncthreads();
-  const int e = end;
+};
+
+// One block per sequence decides over its rows (a wave each, 16 at a time).
+template <typename T> __global__ __launch_bounds__(1024) void k_verify_judge(VerifyArgs a) {
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ Roots roots;
+  __shared__ Part sp[16], sq[16];
+  __shared__ bool refused[16];
+  int end = 0;
+  const float temperature = a.temperature[b];
+  const Rows rows(a, b);
   if (rows.n == 0) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (threadIdx.x == 0) {
       a.accepted[b] = 0;
-      a.choice[b].row = -1;
+      a.choice[b].token = -1;
     }
     return;
   }
-  const int t = rows.first + e;
-  const bool last = e == rows.n - 1;
-  if (wave == 0) {
-    const Part p = join_parts(a, false, t, inv);
-    Part q;
-    q.z = 0.0, q.m = 0.f, q.arg = 0;
-    const bool with_q = !last && a.y && !greedy;
-    if (with_q) q = join_parts(a, true, t, inv);
-    if (lane == 0) {
-      ch.zp = p.z, ch.zq = with_q ? q.z : 0.0, ch.mp = p.m, ch.mq = q.m, ch.row = t;
-      ch.drop = last || a.y ? -1 : (int)max(-1l, min((long)a.ids[t + 1], 0x7fffffffl));
-      ch.token = greedy ? (p.m == p.m && p.m > -INF ? p.arg : -1) : is_distribution(p) && is_distribution(q) ? -2 : -1;
-      if (blockIdx.x == 0) {
-        a.choice[b] = ch;
-        a.accepted[b] = e;
+  roots.fill();
+  __syncthreads();
+  const double by = divisor(temperature), scale = scale_of(by);
+  const bool greedy = temperature == 0.f;
+  int i0 = 0;
+  for (;; i0 += 16) {      // the last row takes no draft, so one of them ends it
+    const int i = i0 + wave;
+    if (i < rows.n) {
+      const int t = rows.first + i;
+      const bool last = i == rows.n - 1, with_q = !last && a.y && !greedy;
+      const long d = last ? -1 : a.ids[t + 1];
+      const float u = a.u[2 * t];
+      const bool in_range = d >= 0 && d < a.V;
+      const float xd = in_range ? to_f(((const T*)a.x)[t * a.ld_x + d]) : 0.f;
+      const float yd = in_range && with_q ? to_f(((const T*)a.y)[t * a.ld_y + d]) : 0.f;
+      const Part p = join_parts(a, false, t, scale, roots);
+      Part q;
+      q.z = 0.0, q.m = 0.f, q.arg = 0;
+      if (with_q) q = join_parts(a, true, t, scale, roots);
+      const bool valid = is_distribution(p) && is_distribution(q);
+      bool ok = false;
+      if (greedy) {
+        ok = !last && d == p.arg && p.m == p.m && p.m > -INF;
+      } else if (valid && in_range) {
+        const double qd = !with_q ? 1.0 : yd == -INF ? 0.0 : exp_of(((double)yd - q.m) * scale, roots) / q.z;
+        ok = xd != -INF && (double)u * qd < exp_of(((double)xd - p.m) * scale, roots) / p.z;
+      }
+      if (lane == 0) {
+        sp[wave] = p, sq[wave] = q;
+        refused[wave] = !ok;
+        if (ok) a.tokens[t] = d, a.logp[t] = valid ? (float)(((double)xd - p.m) / by - log(p.z)) : NAN_;
       }
     }
+    __syncthreads();
+    const uint64_t first = __ballot(lane < 16 && i0 + lane < rows.n && refused[lane & 15]);
+    if (first) {
+      end = i0 + __ffsll((unsigned long long)first) - 1;
+      break;
+    }
+    __syncthreads();
   }
-  // the rows behind
-  if (blockIdx.x == 0)
-    for (int i = e + 1 + threadIdx.x; i < rows.n; i += 256) a.tokens[rows.first + i] = -1, a.logp[rows.first + i] = 0.f;
-  __syncthreads();
+  const int t = rows.first + end;
+  if (threadIdx.x == 0) {
+    const bool last = end == rows.n - 1;
+    const Part p = sp[end - i0], q = sq[end - i0];
+    Choice ch;
+    ch.zp = p.z, ch.zq = q.z, ch.mp = p.m, ch.mq = q.m, ch.row = t, ch.scale = scale, ch.u = a.u[2 * t + 1];
+    ch.drop = last || a.y ? -1 : (int)max(-1l, min((long)a.ids[t + 1], 0x7fffffffl));
+    ch.token = greedy ? (p.m == p.m && p.m > -INF ? p.arg : -1) : is_distribution(p) && is_distribution(q) ? -2 : -1;
+    ch.T = by, ch.log_zp = log(p.z);
+    a.choice[b] = ch;
+    a.accepted[b] = end;
+    if (ch.token != -2) a.tokens[t] = ch.token, a.logp[t] = ch.token >= 0 && is_distribution(p) ? (float)-ch.log_zp : NAN_;
+  }
+  for (int i = end + 1 + threadIdx.x; i < rows.n; i += 1024) a.tokens[rows.first + i] = -1, a.logp[rows.first + i] = 0.f;
+}
+
+// The sums of r and p over each part of a sequence's chosen row.
+template <typename T> __global__ __launch_bounds__(1024) void k_verify_sums(VerifyArgs a) {
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ Roots roots;
+  __shared__ double sums[2][16];
+  const Choice ch = a.choice[b];
   if (ch.token != -2) return;
-  double r = 0.0, s = 0.0;
-  const T* x = (const T*)a.x + t * a.ld_x;
-  const T* y = (const T*)a.y + t * a.ld_y;
-  const int c0 = blockIdx.x * PART + threadIdx.x * EACH;
-  for (int i = 0; i < EACH; ++i) {
-    const int c = c0 + i;
-    if (c >= a.V) break;
-    const double pc = exp(((double)to_f(x[c]) - ch.mp) * inv) / ch.zp;
-    const double qc = ch.zq > 0.0 ? exp(((double)to_f(y[c]) - ch.mq) * inv) / ch.zq : 0.0;
-    s += pc;
-    r += c == ch.drop ? 0.0 : fmax(pc - qc, 0.0);
-  }
-  r = wave_sum_double(r);
-  s = wave_sum_double(s);
+  roots.fill();
+  __syncthreads();
+  const Residual<T> v(a, ch, blockIdx.x * PART + threadIdx.x * 4, roots);
+  const double r = wave_sum_double((v.r[0] + v.r[1]) + (v.r[2] + v.r[3])), s = wave_sum_double((v.p[0] + v.p[1]) + (v.p[2] + v.p[3]));
   if (lane == 0) sums[0][wave] = r, sums[1][wave] = s;
   __syncthreads();
-  if (threadIdx.x < 2)
-    a.sums[((long)b * 2 + threadIdx.x) * a.n_parts + blockIdx.x] =
-        (sums[threadIdx.x][0] + sums[threadIdx.x][1]) + (sums[threadIdx.x][2] + sums[threadIdx.x][3]);
+  if (threadIdx.x < 2) {
+    double sum = 0.0;
+    for (int w = 0; w < 16; ++w) sum += sums[threadIdx.x][w];
+    a.sums[((long)b * 2 + threadIdx.x) * a.n_parts + blockIdx.x] = sum;
+  }
+}
+
+DM_DEV double wave_upto(double v) {      // the sum over the lanes up to this one
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
 }
 
 // One block per sequence: the part of the chosen row in which the place lies, then the thread, then the column. Rows of no
 // sequence get token -1.
-template <typename T> __global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a) {
+template <typename T> __global__ __launch_bounds__(1024) void k_verify_pick(VerifyArgs a) {
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (b == a.B) {
-    for (int t = threadIdx.x; t < a.N; t += 256)
-      if (sequence_of(a, t) < 0) a.tokens[t] = -1, a.logp[t] = 0.f;
+  if (b >= a.B) {
+    const int t = (b - a.B) * 16 + wave;
+    if (t < a.N && sequence_of(a, t) < 0 && lane == 0) a.tokens[t] = -1, a.logp[t] = 0.f;
     return;
   }
+  const double* sums_of = a.sums + (long)b * 2 * a.n_parts;
+  const double ahead = wave == 0 && lane < a.n_parts ? sums_of[lane] : 0.0;      // beside the choice
   const Choice ch = a.choice[b];
-  if (ch.row < 0) return;
-  const double inv = 1.0 / divisor(a.temperature[b]);
-  const T* x = (const T*)a.x + ch.row * a.ld_x;
-  const T* y = (const T*)a.y + ch.row * a.ld_y;
-  __shared__ double base, place, sums[4];
-  __shared__ int part, plain, hit[4], positive[4];
-  int token = ch.token;
-  if (token == -2) {
-    if (threadIdx.x == 0) {
-      const double* s = a.sums + (long)b * 2 * a.n_parts;
-      double total = 0.0;
-      for (int i = 0; i < a.n_parts; ++i) total += s[i];
-      plain = !(total > 0.0);
-      if (plain) {
-        s += a.n_parts;
-        total = 0.0;
-        for (int i = 0; i < a.n_parts; ++i) total += s[i];
+  if (ch.token != -2) return;
+  __shared__ Roots roots;
+  __shared__ double base, place, sums[16];
+  __shared__ int part, plain, hit[16], most[16];
+  roots.fill();
+  if (wave == 0) {
+    const double* s = sums_of;
+    double total = 0.0;
+    for (int kind = 0; kind < 2; ++kind) {      // r, and p where r is 0
+      if (kind) s += a.n_parts;
+      total = kind ? (lane < a.n_parts ? s[lane] : 0.0) : ahead;
+      for (int i = lane + 64; i < a.n_parts; i += 64) total += s[i];
+      total = wave_sum_double(total);
+      if (lane == 0) plain = kind;
+      if (total > 0.0) break;
+    }
+    const double to = (double)ch.u * total;
+    // the part in which the sum passes the place; by rounding none: the last part with any
+    double before = 0.0, found_base = 0.0;
+    int found = -1, any = 0;
+    double any_base = 0.0;
+    for (int i0 = 0; i0 < a.n_parts && found < 0; i0 += 64) {
+      const int i = i0 + lane;
+      const double mine = s == sums_of && i0 == 0 ? ahead : i < a.n_parts ? s[i] : 0.0, upto = before + wave_upto(mine);
+      const uint64_t over = __ballot(mine > 0.0 && upto > to), some = __ballot(mine > 0.0);
+      if (some) {
+        const int l = 63 - __clzll((long long)some);
+        any = i0 + l, any_base = __shfl(upto - mine, l, 64);
       }
-      place = (double)a.u[2 * ch.row + 1] * total;
-      // the part after whose sum the place lies; past the last one's (by rounding) the last with any
-      double before = 0.0;
-      part = -1;
-      int any = 0;
-      double any_base = 0.0;
-      for (int i = 0; i < a.n_parts; ++i) {
-        if (s[i] > 0.0) any = i, any_base = before;
-        if (before + s[i] > place) {
-          part = i, base = before;
-          break;
-        }
-        before += s[i];
+      if (over) {
+        const int l = __ffsll((unsigned long long)over) - 1;
+        found = i0 + l, found_base = __shfl(upto - mine, l, 64);
       }
-      if (part < 0) part = any, base = any_base;
+      before = __shfl(upto, 63, 64);
     }
-    __syncthreads();
-    const int c0 = part * PART + threadIdx.x * EACH;
-    double r[EACH], mine = 0.0;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int c = c0 + i;
-      r[i] = 0.0;
-      if (c < a.V) {
-        const double pc = exp(((double)to_f(x[c]) - ch.mp) * inv) / ch.zp;
-        const double qc = !plain && ch.zq > 0.0 ? exp(((double)to_f(y[c]) - ch.mq) * inv) / ch.zq : 0.0;
-        r[i] = !plain && c == ch.drop ? 0.0 : fmax(pc - qc, 0.0);
-      }
-      mine += r[i];
+    if (lane == 0) {
+      part = found < 0 ? any : found;
+      base = found < 0 ? any_base : found_base;
+      place = to;
     }
-    double sum = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double v = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += v;
-    }
-    if (lane == 63) sums[wave] = sum;
-    __syncthreads();
-    double before = base + (sum - mine);
-    for (int w = 0; w < wave; ++w) before += sums[w];
-    int first = 0x7fffffff, most = -1;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      before += r[i];
-      if (r[i] > 0.0) most = c0 + i;
-      if (before > place && r[i] > 0.0 && first == 0x7fffffff) first = c0 + i;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64)), most = max(most, __shfl_xor(most, o, 64));
-    if (lane == 0) hit[wave] = first, positive[wave] = most;
-    __syncthreads();
-    token = min(min(hit[0], hit[1]), min(hit[2], hit[3]));
-    if (token == 0x7fffffff) token = max(max(positive[0], positive[1]), max(positive[2], positive[3]));
   }
-  if (threadIdx.x == 0) {
-    a.tokens[ch.row] = token;
-    a.logp[ch.row] = token < 0 ? NAN_ : (float)(((double)to_f(x[token]) - ch.mp) * inv - log(ch.zp));
+  __syncthreads();
+  const int c0 = part * PART + threadIdx.x * 4;
+  const Residual<T> v(a, ch, c0, roots);
+  double r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = plain ? v.p[i] : v.r[i];
+  const double mine = (r[0] + r[1]) + (r[2] + r[3]), upto = wave_upto(mine);
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  double before = base;
+  for (int w = 0; w < wave; ++w) before += sums[w];
+  before += upto - mine;
+  int first = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    before += r[i];
+    if (r[i] > 0.0) last = c0 + i;
+    if (before > place && r[i] > 0.0) first = min(first, c0 + i);
   }
+  // columns ascend with the lanes and the waves
+  const uint64_t hits = __ballot(first != 0x7fffffff), some = __ballot(last >= 0);
+  if (hits && lane == __ffsll((unsigned long long)hits) - 1) hit[wave] = first;
+  else if (!hits && lane == 0) hit[wave] = -1;
+  if (some && lane == 63 - __clzll((long long)some)) most[wave] = last;
+  else if (!some && lane == 0) most[wave] = -1;
+  __syncthreads();
+  int token = -1;
+#pragma unroll
+  for (int w = 0; w < 16; ++w)
+    if (most[w] >= 0) token = most[w];
+#pragma unroll
+  for (int w = 15; w >= 0; --w)
+    if (hit[w] >= 0) token = hit[w];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c0 + i == token) a.tokens[ch.row] = token, a.logp[ch.row] = (float)(((double)v.x[i] - ch.mp) / ch.T - ch.log_zp);
+  if (token < 0 && threadIdx.x == 0) a.tokens[ch.row] = -1, a.logp[ch.row] = NAN_;
 }
 
 int n_parts(int V) { return cdiv(V, PART); }
@@ -346,8 +441,9 @@ size_t sums_bytes(const dm_verify_args* a) { return align256((size_t)2 * a->B * 
 
 template <typename T> void run_verify(const VerifyArgs& p, hipStream_t s) {
   hipLaunchKernelGGL(k_verify_parts<T>, dim3(p.n_parts, p.N, p.y ? 2 : 1), dim3(256), 0, s, p);
-  hipLaunchKernelGGL(k_verify_choose<T>, dim3(p.n_parts, p.B), dim3(256), 0, s, p);
-  hipLaunchKernelGGL(k_verify_pick<T>, dim3(p.B + 1), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(k_verify_judge<T>, dim3(p.B), dim3(1024), 0, s, p);
+  hipLaunchKernelGGL(k_verify_sums<T>, dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
+  hipLaunchKernelGGL(k_verify_pick<T>, dim3(p.B + cdiv(p.N, 16)), dim3(1024), 0, s, p);
 }
 
 }  // namespace
