@@ -22,8 +22,8 @@ class Verified(NamedTuple):
 
 
 def _like(t, name, shape, dtype, device):
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; contiguous {dtype} {shape} on {device} is needed")
+    if t.dtype != dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; contiguous {dtype} {shape} on cuda:{device} is needed")
     return t.data_ptr()
 
 
@@ -35,36 +35,33 @@ def verify_drafts(logits, ids, uniforms, starts, draft_logits=None, temperature=
     but -inf) ends its sequence with token -1."""
     if not logits.is_cuda or logits.dim() != 2:
         raise ValueError(f"logits: shape {tuple(logits.shape)} on {logits.device}; rows [N, V] on a GPU are needed")
-    dev = logits.device
+    dev = logits.get_device()
     dtype = L.dtype_code(logits.dtype)
-    if starts.dim() != 1 or starts.numel() < 1:
+    if starts.dim() != 1 or starts.shape[0] < 1:
         raise ValueError(f"starts: {tuple(starts.shape)}; [B + 1] is needed")
-    (N, V), B = logits.shape, starts.numel() - 1
+    (N, V), B = logits.shape, starts.shape[0] - 1
     if N > 65535 or B > 65535:
         raise ValueError(f"{N} rows of {B} sequences (at most 65535)")
-    ld = _rows(logits, "logits")[1]
-    ld_draft = 0
+    ld, draft, ld_draft = _rows(logits, "logits")[1], None, 0
     if draft_logits is not None:
-        if draft_logits.shape != logits.shape or draft_logits.dtype != logits.dtype or draft_logits.device != dev:
+        if draft_logits.shape != logits.shape or draft_logits.dtype != logits.dtype or draft_logits.get_device() != dev:
             raise ValueError(f"draft_logits: {draft_logits.dtype} {tuple(draft_logits.shape)} on {draft_logits.device} for logits "
-                             f"{logits.dtype} {tuple(logits.shape)} on {dev}")
-        ld_draft = _rows(draft_logits, "draft_logits")[1]
-    if torch.is_tensor(temperature):
-        T = temperature
-    else:
+                             f"{logits.dtype} {tuple(logits.shape)} on {logits.device}")
+        draft, ld_draft = draft_logits.data_ptr(), _rows(draft_logits, "draft_logits")[1]
+    if not torch.is_tensor(temperature):
         if not 0 <= temperature < float("inf"):
             raise ValueError(f"temperature={temperature}")
-        T = torch.full((B,), float(temperature), device=dev)
+        temperature = torch.full((B,), float(temperature), device=logits.device)
     args = (_like(ids, "ids", (N,), torch.int64, dev), _like(uniforms, "uniforms", (N, 2), torch.float32, dev),
-            _like(T, "temperature", (B,), torch.float32, dev), _like(starts, "starts", (B + 1,), torch.int32, dev))
-    out = Verified(torch.empty(N, dtype=torch.int64, device=dev), torch.empty(B, dtype=torch.int32, device=dev),
-                   torch.empty(N, device=dev))
+            _like(temperature, "temperature", (B,), torch.float32, dev), _like(starts, "starts", (B + 1,), torch.int32, dev))
+    out = Verified(ids.new_empty((N,)), starts.new_empty((B,)), uniforms.new_empty((N,)))
     if N == 0 or B == 0:
         out.tokens.fill_(-1), out.accepted.zero_(), out.logp.zero_()
         return out
-    a = L.dm_verify_args(dtype, N, V, B, logits.data_ptr(), ld, L.ptr(draft_logits), ld_draft, *args, out.tokens.data_ptr(),
-                         out.accepted.data_ptr(), out.logp.data_ptr(), None, 0)
-    ws = torch.empty(L.lib().dm_verify_workspace_bytes(L.byref(a)), dtype=torch.uint8, device=dev)
+    a = L.dm_verify_args(dtype, N, V, B, logits.data_ptr(), ld, draft, ld_draft, *args, out.tokens.data_ptr(), out.accepted.data_ptr(),
+                         out.logp.data_ptr())
+    args = L.byref(a)
+    ws = torch.empty(L.lib().dm_verify_workspace_bytes(args), dtype=torch.uint8, device=logits.device)
     a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    L.call_on(dev, L.lib().dm_verify_drafts, L.byref(a))
+    L.call_on(logits.device, L.lib().dm_verify_drafts, args)
     return out
