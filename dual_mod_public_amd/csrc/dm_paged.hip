@@ -69,43 +69,46 @@ struct Item {
   int tile, piece, pieces, slot;   // slot of the query tile's piece 0 in the workspace, where pieces > 1
 };
 
-DM_DEV long wave_sum_long(long v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// The sum over the lanes up to this one, by moves inside the rows of 16 lanes and broadcasts of the rows' last lanes.
+DM_DEV int wave_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);     // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);     // row_bcast 15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);     // row_bcast 31 into rows 2 and 3
   return v;
 }
 
 // The plan: sequence b's query tiles (of ROWS query rows; 1 with ROWS = 0) times its pieces, in order. PIECES: find item
-// number `at` of those; otherwise of the query tiles alone. Called by whole waves.
+// number `at` of those; otherwise of the query tiles alone. Called by whole waves. Items and slots are fewer than the blocks of a
+// launch; the cost (query tiles times tiles of cached rows) may pass 32 bits and is summed in fp32, rounded up, so that a piece's
+// tiles are never too few for the slots that the workspace has.
 template <int ROWS, bool PIECES> DM_DEV Item find_item(const PagedArgs& a, int at) {
   const int lane = threadIdx.x & 63;
   auto tiles_q = [&](const Seq& s) { return ROWS ? (s.n * a.g + ROWS - 1) / (ROWS ? ROWS : 1) : (s.n > 0); };
   Seq s;
-  long cost = 0;
+  float cost = 0.f;
   for (int b = lane; b < a.B; b += 64) {
     s = Seq(a, b);
-    cost += (long)tiles_q(s) * s.tiles_k(a);
+    cost += (float)tiles_q(s) * (float)s.tiles_k(a);
   }
-  cost = wave_sum_long(cost);
-  const int each = (int)max((long)a.least, (cost + a.want - 1) / a.want);   // tiles of cached rows per piece
+  cost = wave_sum(cost) * (1.f + 1e-4f);                   // 1024 + 6 additions of half a step, 2^-24, each
+  const int each = max(a.least, (int)fminf(ceilf(cost / (float)a.want), 1e9f));   // tiles of cached rows per piece
   Item it;
-  long done = 0, slots = 0;
+  int done = 0, slots = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
     if (a.B > 64) s = b < a.B ? Seq(a, b) : Seq();
     const int tq = b < a.B ? tiles_q(s) : 0;
     const int pieces = tq ? max(1, (s.tiles_k(a) + each - 1) / each) : 1;
-    const long mine = PIECES ? (long)tq * pieces : tq, kept = pieces > 1 ? (long)tq * pieces : 0;
-    long sum = mine, ksum = kept;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const long u = __shfl_up(sum, o, 64), ku = __shfl_up(ksum, o, 64);
-      if (lane >= o) sum += u, ksum += ku;
-    }
-    const uint64_t hit = __ballot(mine > 0 && done + sum > at);
+    const int mine = PIECES ? tq * pieces : tq, kept = pieces > 1 ? tq * pieces : 0;
+    const int upto = wave_upto(mine), kept_upto = wave_upto(kept);
+    const uint64_t hit = __ballot(mine > 0 && done + upto > at);
     if (hit) {
       const int l = __ffsll((unsigned long long)hit) - 1;
-      const int rest = (int)(at - (done + __shfl(sum - mine, l, 64)));
+      const int rest = at - (done + __shfl(upto - mine, l, 64));
+      if (rest < 0 || rest >= __shfl(mine, l, 64)) return it;     // (starts that do not ascend: more than 32 bits of tiles)
       it.b = b0 + l;
       it.s.first = __shfl(s.first, l, 64);
       it.s.n = __shfl(s.n, l, 64);
@@ -115,11 +118,11 @@ template <int ROWS, bool PIECES> DM_DEV Item find_item(const PagedArgs& a, int a
       it.tile = PIECES ? rest / it.pieces : rest;
       if (ROWS) it.tile = __shfl(tq, l, 64) - 1 - it.tile;      // the tiles with the most rows to read first
       it.piece = PIECES ? rest % it.pieces : 0;
-      it.slot = (int)(slots + __shfl(ksum - kept, l, 64)) + it.tile * it.pieces;
+      it.slot = slots + __shfl(kept_upto - kept, l, 64) + it.tile * it.pieces;
       return it;
     }
-    done += __shfl(sum, 63, 64);
-    slots += __shfl(ksum, 63, 64);
+    done += __shfl(upto, 63, 64);
+    slots += __shfl(kept_upto, 63, 64);
   }
   return it;
 }
@@ -1347,11 +1350,18 @@ int log2_of(int x) {
 }
 
 // The plan's numbers: about `blocks` blocks over the key heads.
-int wanted(const dm_paged_args* a, int blocks) { return std::max(1, cdiv(blocks, a->h_kv)); }
 long query_tiles(const dm_paged_args* a, int rows) { return (long)a->n_tokens * (a->h / a->h_kv) / rows + a->B; }
 constexpr int WEIGHT_BLOCKS = 8 * CUS;
 
 // Which read a call takes, by the mean number of query rows of a sequence and key head: tiles of 16 rows while two of them
+// ... but no more than there can be, by the table's and the window's rows: blocks without a piece cost their look at the plan
+// (one_token 8.2 us with 8 blocks per CU, 7.0 with 5).
+int wanted(const dm_paged_args* a, int blocks, long tiles, int least) {
+  long rows = (long)a->table_cols * a->page;
+  if (a->window) rows = std::min(rows, (long)a->window + a->n_tokens);
+  const long each = (rows / TILE_K + 2 + least - 1) / least;     // pieces of a tile
+  return (int)std::max(1L, std::min((long)cdiv(blocks, a->h_kv), tiles * each));
+}
 // hold those, of 128, or of 256 (us, bf16, 16 sequences of 4096 rows, 16 heads of 64 and 32 of 128 on 8 key heads:
 // 24 rows 60 / 69 / 115 and 60 / 62 / 82, 48 rows 78 / 71 / 115 and 84 / 65 / 86, 256 rows 303 / 123 / 134 and 307 / 117 / 119,
 // 512 rows 572 / 225 / 215 and 596 / 195 / 188; two sequences of 16384 rows, 8192 query rows: 4110 / 1340 / 1150). Pieces:
@@ -1373,7 +1383,8 @@ size_t score_floats(const dm_paged_args* a) {
 }
 size_t part_floats(const dm_paged_args* a) {
   const Form f = form_of(a);
-  return (size_t)2 * wanted(a, f.blocks) * a->h_kv * f.rows * (a->dh + 2);
+  return (size_t)2 * wanted(a, f) * a->h_kv * f.rows * (a->dh + 2);
+int wanted(const dm_paged_args* a, const Form& f) { return wanted(a, f.blocks, query_tiles(a, f.rows), f.least); }
 }
 size_t part_bytes(const dm_paged_args* a) { return align256(part_floats(a) * 4); }
 
@@ -1447,7 +1458,7 @@ template <int DH, int NW> int launch_wide(const PagedArgs& p, unsigned blocks, h
 template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStream_t s) {
   const Form f = form_of(a);
   PagedArgs p = paged(a);
-  p.want = wanted(a, f.blocks), p.least = f.least;
+  p.want = wanted(a, f), p.least = f.least;
   if (score_floats(a)) p.scores = (float*)((char*)a->workspace + part_bytes(a));
   const long tiles = query_tiles(a, f.rows);
   const unsigned blocks = (unsigned)((p.want + tiles) * a->h_kv);
@@ -1469,13 +1480,12 @@ template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStrea
     }
   }
   if (a->weights) {
-    p.want = wanted(a, WEIGHT_BLOCKS);
+    p.least = p.scores ? 1024 / TILE_K : 1;     // a round of a block's threads; a step
+    p.want = wanted(a, WEIGHT_BLOCKS, a->B, p.least);
     const dim3 grid((unsigned)((p.want + (long)a->B) * a->h_kv));
     if (p.scores) {
-      p.least = 1024 / TILE_K;     // a round of a block's threads
       hipLaunchKernelGGL(k_paged_weights_of, grid, dim3(256), 0, s, p);
     } else {
-      p.least = 1;
       if constexpr (sizeof(T) == 2) {
         if (f.rows != TILE_Q) hipLaunchKernelGGL(k_paged_weights_wide<DH>, grid, dim3(256), 0, s, p);
       }
