@@ -138,34 +138,35 @@ DM_DEV void make_uniform(Item& it) {
 }
 
 // ---- rows into the pages ---------------------------------------------------------------------
-// One thread per 16 bytes of a new token's key or value row.
+// One thread per 16 bytes of a new token's key or value row (in turns where there are more of them than a launch has threads).
 template <typename T> __global__ __launch_bounds__(256) void k_paged_write(PagedArgs a, int dh) {
   constexpr int V = 16 / (int)sizeof(T);
   const int per = dh / V;
-  const long each = (long)a.h_kv * per * 2, at = blockIdx.x * 256L + threadIdx.x;
-  if (at >= a.N * each) return;
-  const int t = (int)(at / each), rest = (int)(at % each);
-  const bool value = rest >= a.h_kv * per;
-  const int c = (rest / per) % a.h_kv, v = rest % per;
-  int b = t;
-  if (a.starts) {   // the last sequence that starts at t or before
-    int lo = 0, hi = a.B;
-    while (lo + 1 < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.starts[mid] <= t) lo = mid;
-      else hi = mid;
+  const long each = (long)a.h_kv * per * 2, all = a.N * each;
+  for (long at = blockIdx.x * 256L + threadIdx.x; at < all; at += gridDim.x * 256L) {
+    const int t = (int)(at / each), rest = (int)(at % each);
+    const bool value = rest >= a.h_kv * per;
+    const int c = (rest / per) % a.h_kv, v = rest % per;
+    int b = t;
+    if (a.starts) {   // the last sequence that starts at t or before
+      int lo = 0, hi = a.B;
+      while (lo + 1 < hi) {
+        const int mid = (lo + hi) / 2;
+        if (a.starts[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      b = lo;
     }
-    b = lo;
+    const Seq s(a, b);
+    if (s.bad || t < s.first || t >= s.first + s.n) continue;
+    const int row = s.len - s.n + (t - s.first);
+    const int page = a.table[(long)b * a.cols + (row >> a.page_shift)];
+    if (page < 0 || page >= a.n_pages) continue;
+    const T* src = value ? (const T*)a.v_rows + t * a.vr_token + c * a.vr_head : (const T*)a.k_rows + t * a.kr_token + c * a.kr_head;
+    T* dst = value ? (T*)a.V + page * a.v_page : (T*)a.K + page * a.k_page;
+    dst += ((long)c << a.page_shift) * dh + (long)(row & ((1 << a.page_shift) - 1)) * dh;
+    *reinterpret_cast<u32x4*>(dst + v * V) = *reinterpret_cast<const u32x4*>(src + v * V);
   }
-  const Seq s(a, b);
-  if (s.bad || t < s.first || t >= s.first + s.n) return;
-  const int row = s.len - s.n + (t - s.first);
-  const int page = a.table[(long)b * a.cols + (row >> a.page_shift)];
-  if (page < 0 || page >= a.n_pages) return;
-  const T* src = value ? (const T*)a.v_rows + t * a.vr_token + c * a.vr_head : (const T*)a.k_rows + t * a.kr_token + c * a.kr_head;
-  T* dst = value ? (T*)a.V + page * a.v_page : (T*)a.K + page * a.k_page;
-  dst += ((long)c << a.page_shift) * dh + (long)(row & ((1 << a.page_shift) - 1)) * dh;
-  *reinterpret_cast<u32x4*>(dst + v * V) = *reinterpret_cast<const u32x4*>(src + v * V);
 }
 
 // ---- the read ----------------------------------------------------------------------------------
@@ -733,7 +734,9 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
   if (threadIdx.x == 0) any_odd = any_bad = 0;
   __syncthreads();
   const int steps = k0 < k1 ? (k1 - k0 + C::KT - 1) / C::KT : 0;
-  auto step_row = [&](int n) { return min(k0 + n * C::KT, k1); };     // step n's first row; k1: there is no such step
+  // step n's first row. Past the last step the next 64 rows again and again: a load's rows lie in one page from any multiple
+  // of 16 on, but not from k1 on
+  auto step_row = [&](int n) { return k0 + min(n, steps) * C::KT; };
   if (steps) {
     look_up(kr, k0), load(kr, k0, a.K, a.k_page);
     vr = kr, load(vr, k0, a.V, a.v_page);
@@ -1351,9 +1354,6 @@ int log2_of(int x) {
 
 // The plan's numbers: about `blocks` blocks over the key heads.
 long query_tiles(const dm_paged_args* a, int rows) { return (long)a->n_tokens * (a->h / a->h_kv) / rows + a->B; }
-constexpr int WEIGHT_BLOCKS = 8 * CUS;
-
-// Which read a call takes, by the mean number of query rows of a sequence and key head: tiles of 16 rows while two of them
 // ... but no more than there can be, by the table's and the window's rows: blocks without a piece cost their look at the plan
 // (one_token 8.2 us with 8 blocks per CU, 7.0 with 5).
 int wanted(const dm_paged_args* a, int blocks, long tiles, int least) {
@@ -1362,6 +1362,9 @@ int wanted(const dm_paged_args* a, int blocks, long tiles, int least) {
   const long each = (rows / TILE_K + 2 + least - 1) / least;     // pieces of a tile
   return (int)std::max(1L, std::min((long)cdiv(blocks, a->h_kv), tiles * each));
 }
+constexpr int WEIGHT_BLOCKS = 8 * CUS;
+
+// Which read a call takes, by the mean number of query rows of a sequence and key head: tiles of 16 rows while two of them
 // hold those, of 128, or of 256 (us, bf16, 16 sequences of 4096 rows, 16 heads of 64 and 32 of 128 on 8 key heads:
 // 24 rows 60 / 69 / 115 and 60 / 62 / 82, 48 rows 78 / 71 / 115 and 84 / 65 / 86, 256 rows 303 / 123 / 134 and 307 / 117 / 119,
 // 512 rows 572 / 225 / 215 and 596 / 195 / 188; two sequences of 16384 rows, 8192 query rows: 4110 / 1340 / 1150). Pieces:
@@ -1381,10 +1384,10 @@ size_t score_floats(const dm_paged_args* a) {
   const double n = (double)a->n_tokens * a->h * (((int64_t)a->table_cols * a->page + 31) & -32);
   return n * 4 <= (double)a->n_pages * a->h_kv * a->page * a->dh * esz(a->dtype) ? (size_t)n : 0;
 }
+int wanted(const dm_paged_args* a, const Form& f) { return wanted(a, f.blocks, query_tiles(a, f.rows), f.least); }
 size_t part_floats(const dm_paged_args* a) {
   const Form f = form_of(a);
   return (size_t)2 * wanted(a, f) * a->h_kv * f.rows * (a->dh + 2);
-int wanted(const dm_paged_args* a, const Form& f) { return wanted(a, f.blocks, query_tiles(a, f.rows), f.least); }
 }
 size_t part_bytes(const dm_paged_args* a) { return align256(part_floats(a) * 4); }
 
@@ -1395,7 +1398,8 @@ int check_pages(int dtype, int dh, int page, int n_pages, int cols, int B, int h
   DM_REQUIRE(log2_of(page) >= 4 && page <= DM_PAGE_MAX, DM_ERR_UNSUPPORTED, "page=%d rows (a power of two, 16..%d)", page, DM_PAGE_MAX);
   DM_REQUIRE(B > 0 && h_kv > 0 && n_pages > 0 && cols > 0 && (int64_t)cols * page <= DM_PAGED_ROWS, DM_ERR_INVALID,
              "B=%d h_kv=%d n_pages=%d table_cols=%d of %d rows (at most %d rows)", B, h_kv, n_pages, cols, page, DM_PAGED_ROWS);
-  DM_REQUIRE(B <= 65535 && h_kv <= 65535, DM_ERR_INVALID, "B=%d h_kv=%d (at most 65535)", B, h_kv);
+  DM_REQUIRE(B <= 65535 && h_kv <= 65535 && (int64_t)B * h_kv <= DM_PAGED_HEADS, DM_ERR_INVALID, "B=%d h_kv=%d (at most 65535, %d in all)",
+             B, h_kv, DM_PAGED_HEADS);
   const int64_t least = (int64_t)h_kv * page * dh, unit = dtype == DM_BF16 ? 8 : 4;
   DM_REQUIRE(K && V && aligned16(K) && aligned16(V) && k_page >= least && v_page >= least && k_page % unit == 0 && v_page % unit == 0,
              DM_ERR_INVALID, "null or unaligned pages, strides %lld %lld (at least %lld, 16-byte steps)", (long long)k_page,
@@ -1448,9 +1452,8 @@ PagedArgs paged(const dm_paged_args* a) {
 
 template <int DH, int NW> int launch_wide(const PagedArgs& p, unsigned blocks, hipStream_t s) {
   constexpr int BYTES = 2 * (WideTile<DH>::KS + WideTile<DH>::VS) * 2;
-  static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_read_wide<DH, NW>),
-                                                   hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
-  DM_HIP(rc);
+  DM_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_read_wide<DH, NW>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                             BYTES));     // of the current device, so in every call
   hipLaunchKernelGGL((k_paged_read_wide<DH, NW>), dim3(blocks), dim3(64 * NW), BYTES, s, p);
   return DM_OK;
 }
@@ -1510,7 +1513,7 @@ int dm_paged_write(const dm_paged_args* a, void* stream) {
   if (rc || a->n_tokens == 0) return rc;
   const PagedArgs p = paged(a);
   const long n = (long)a->n_tokens * a->h_kv * 2 * (a->dh * (long)esz(a->dtype) / 16);
-  const dim3 grid((unsigned)((n + 255) / 256));
+  const dim3 grid((unsigned)std::min((n + 255) / 256, 1L << 20));
   if (a->dtype == DM_BF16) hipLaunchKernelGGL(k_paged_write<bf16>, grid, dim3(256), 0, S(stream), p, a->dh);
   else hipLaunchKernelGGL(k_paged_write<float>, grid, dim3(256), 0, S(stream), p, a->dh);
   DM_HIP(hipGetLastError());

@@ -626,8 +626,9 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
  * lengths[b] - n + j; NULL: one token per sequence, none where lengths[b] is 0. All three lie on the device and may change between replays of a
  * captured call. Tokens of no sequence (behind starts[B]) are neither read nor written,
  * nor are their rows of o and lse.
- * A sequence that its table does not hold (lengths[b] > table_cols * page, or less than its new tokens), or one that reads a
- * page outside [0, n_pages), gets NaN; what such a page would be written is left out.
+ * starts do not descend. A sequence that its table does not hold (lengths[b] > table_cols * page, or less than its new tokens),
+ * or one that reads a page outside [0, n_pages), gets NaN; what such a page would be written is left out. weights of the first
+ * kind of sequence stay as they are, of the second they become NaN.
  *
  * dm_paged_write: the tokens' rows k_rows, v_rows [n_tokens, h_kv, dh] (any token and head strides) into the pages.
  * dm_paged_attention: for query head a of key head a / (h / h_kv) and a token with row p, over the rows r <= p with
@@ -639,10 +640,11 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
  *   weights (fp32 [B, h_kv, table_cols * page], may be NULL): weights[b, c, r] += the sum over b's new tokens and the heads
  *   of c of e^(s_r - lse), for the rows that are read. One writer per weight, in a fixed order.
  * Workspace: dm_paged_workspace_bytes(a) (from the sizes and whether there are weights), 16-byte aligned, not shared by calls that may overlap.
- * At most DM_PAGED_ROWS rows per sequence, n_tokens * h at most DM_PAGED_TOKENS. */
+ * At most DM_PAGED_ROWS rows per sequence, n_tokens * h at most DM_PAGED_TOKENS, B * h_kv at most DM_PAGED_HEADS. */
 #define DM_PAGE_MAX 1024
 #define DM_PAGED_ROWS (1 << 26)
 #define DM_PAGED_TOKENS (1 << 27)
+#define DM_PAGED_HEADS (1 << 22)
 typedef struct dm_paged_args {
   int32_t dtype, B, h, h_kv, dh;             /* dh 64 or 128 */
   int32_t page, n_pages, table_cols, n_tokens;
@@ -687,7 +689,7 @@ int dm_paged_evict(const dm_evict_args* a, void* stream);
  *   temperature[b] = 0: accepted where the draft is the first of the largest logits, which is the token otherwise.
  * tokens [rows]: the accepted drafts and the new token, each at the row it was predicted by; -1 behind them, in rows of no
  * sequence and where the row that ends the sequence is no distribution (a NaN, +inf, nothing but -inf; greedy: a NaN, nothing but
- * -inf). accepted [B]: drafts accepted. logp [rows]: the tokens' target log probabilities (at T = 1 where T is 0), 0 where there is
+ * -inf; a temperature that is negative or not finite). accepted [B]: drafts accepted. logp [rows]: the tokens' target log probabilities (at T = 1 where T is 0), 0 where there is
  * none, NaN where there is no distribution. A draft outside [0, cols) is not accepted. Probabilities, sums and places in 64 bits.
  * At most 65535 rows and sequences. */
 typedef struct dm_verify_args {
@@ -696,7 +698,7 @@ typedef struct dm_verify_args {
   const void* draft_logits; int64_t ld_draft;
   const int64_t* ids;                        /* [rows] */
   const float* uniforms;                     /* [rows, 2], in [0, 1) */
-  const float* temperature;                  /* [B], 0 or more */
+  const float* temperature;                  /* [B], 0 or more, finite */
   const int32_t* starts;                     /* [B + 1] */
   int64_t* tokens; int32_t* accepted; float* logp;
   void* workspace; size_t workspace_bytes;

@@ -337,3 +337,36 @@ def test_evict_bad_sequences():
     assert got[:11].isnan().all() and torch.equal(got[12:28], torch.cat([K[s["table"][1, 2], 0, 8:], K[s["table"][1, 3], 0, :8]]))
     for p in free[:2] + sorted(used):
         assert torch.equal(d["K"][p].nan_to_num(7), K[p].nan_to_num(7))
+
+
+@pytest.mark.parametrize("h,lengths,page", [(8, [13], 16), (8, [125], 128), (16, [77], 128), (4, [200, 45], 16), (8, [1], 16)])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_sequences_that_end_with_the_pool(h, lengths, page, dh):
+    """Prompts whose last page is the pool's last one, not full, so that nothing may be read behind its rows."""
+    check(make(lengths, lengths, h, 1, dh, page, torch.bfloat16, seed=h, spare=0), lengths, weights=False)
+
+
+def test_starts_that_descend():
+    """No result is defined, but every place that is read and written lies in the call's tensors, and a right call follows."""
+    s = make([64] * 200, [1] * 200, 4, 2, 64, 16, torch.bfloat16, seed=3)
+    d = dev(s)
+    want = paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], d["starts"])
+    starts = torch.tensor([0, 200] * 100 + [-7], dtype=torch.int32, device=DEV)
+    w = torch.zeros(200, 2, s["table"].shape[1] * 16, device=DEV)
+    paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], starts, weights=w)
+    got = paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], d["starts"])
+    assert torch.equal(got.o, want.o) and torch.equal(got.lse, want.lse)
+
+
+def test_many_sequences_and_key_heads():
+    """More sequences than lanes with key heads in the thousands: a launch of B h_kv blocks at least."""
+    B, h = 130, 1024
+    s = make([3] * B, [1] * B, h, h, 64, 16, torch.bfloat16, seed=4, spare=0)
+    d = dev(s)
+    r = paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"])
+    i = torch.tensor([0, 1, 500, h - 1])
+    for b in (0, 63, 64, B - 1):
+        part = dict(q=s["q"][b:b + 1, i], K=s["K"][:, i], V=s["V"][:, i], table=s["table"][b:b + 1])
+        o, lse, _, bo, bl, _ = ref.attention(part["q"], part["K"], part["V"], part["table"], [3], [1])
+        near(r.o[b:b + 1, i.to(DEV)], o, bo, "o")
+        near(r.lse[b:b + 1, i.to(DEV)], lse, bl, "lse")

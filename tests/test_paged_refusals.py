@@ -91,3 +91,12 @@ def test_python_refuses_tensors_of_the_cpu():
             f()
     with pytest.raises(NotImplementedError, match="no autograd"):
         paged.paged_attention(q.requires_grad_(), K, V, table, lengths)
+
+
+def test_more_blocks_than_a_launch_has():
+    """B h_kv blocks are the least of a launch; of 2^22 and more of them a launch's threads would pass 32 bits."""
+    lib = L.load()
+    big = dict(B=4097, h_kv=1024, h=1024, n_tokens=4097, k_page=1024 * 16 * 64, v_page=1024 * 16 * 64)
+    rows = dict(k_rows=0x80000, v_rows=0x90000, k_token=1024 * 64, k_head=64, v_token=1024 * 64, v_head=64)
+    assert lib.dm_paged_attention(L.byref(paged_args(**big)), None) == -1 and b"in all" in lib.dm_last_error()
+    assert lib.dm_paged_write(L.byref(paged_args(**big, **rows)), None) == -1
