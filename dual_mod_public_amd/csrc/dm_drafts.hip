@@ -19,8 +19,8 @@ constexpr int PART = 4096;      // columns of a block's part of a row
 // 2^(w / 32) for w <= 0 (w = 32 x / (T ln 2) for e^(x / T), x a difference of logits), relative error below 2e-12: 2^(n / 32)
 // 2^(f / 32) with n the nearest whole number to w, the 32 roots from a table in LDS (one in each pair of its banks), and the Taylor
 // sum of 2^(f / 32) up to f^4 (|f| <= 1/2 leaves (ln 2 / 64)^5 / 120 = 1.3e-12). Half of the instructions of the library's
-// function, whose range and last bits are not needed here. Below 2^-1000 it stays there: a probability that has to be 0 is
-// made so by its logit. No NaN.
+// function, whose range and last bits are not needed here. Below 2^-1000 it stays there, which a sum of at least 1 does not see;
+// a probability is 0 there (prob_of). No NaN.
 __constant__ const double ROOTS[32] = {      // 2^(i / 32)
     1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
     1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
@@ -50,6 +50,9 @@ DM_DEV double exp_of(double w, const Roots& roots) {
   const uint64_t root = (uint64_t)__double_as_longlong(roots.v[k & 31]);
   return e * __longlong_as_double((long long)(root + ((uint64_t)(k >> 5) << 52)));
 }
+
+// ... as a probability: 0 below 2^-1000, and of a logit of -inf
+DM_DEV double prob_of(double w, const Roots& roots) { return w > -32.0 * LEAST ? exp_of(w, roots) : 0.0; }
 
 // A part's sum of exp((x - m) / T) relative to its own maximum, with the first place of that; m is NaN where the part holds
 // one.
@@ -174,11 +177,12 @@ template <typename T> __global__ __launch_bounds__(256) void k_verify_parts(Veri
   if (lane == 0) sm[wave] = m, snan[wave] = nan;
   __syncthreads();
   m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  const double minus = m == -INF ? 0.0 : -(double)m * scale;
+  // the difference first: at a temperature of 10^-6 a product's rounding would be as large as the logits' steps
+  const double top = m == -INF ? 0.0 : (double)m;
   double z = 0.0;
   int arg = 0x7fffffff;
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) z += exp_of(fma((double)v[i / V][i % V], scale, minus), roots);
+  for (int i = 0; i < EACH; ++i) z += exp_of(((double)v[i / V][i % V] - top) * scale, roots);
   z = m == -INF ? 0.0 : wave_sum_double(z);
   if (temperature == 0.f) {
 #pragma unroll
@@ -219,6 +223,8 @@ DM_DEV Part join_parts(const VerifyArgs& a, bool draft, int t, double scale, con
   r.m = __ballot(nan) ? NAN_ : m;
   return r;
 }
+// whether a number is a temperature
+DM_DEV bool is_temperature(float T) { return T >= 0.f && T < INF; }
 // whether the parts are those of a distribution: something finite, no NaN, no +inf
 DM_DEV bool is_distribution(const Part& p) { return fabsf(p.m) < INF; }
 
@@ -233,8 +239,8 @@ template <typename T> struct Residual {
     const double ip = 1.0 / ch.zp, iq = ch.zq > 0.0 ? 1.0 / ch.zq : 0.0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      p[i] = x[i] == -INF ? 0.0 : exp_of(((double)x[i] - ch.mp) * ch.scale, roots) * ip;
-      const double q = ch.zq > 0.0 && y[i] != -INF ? exp_of(((double)y[i] - ch.mq) * ch.scale, roots) * iq : 0.0;
+      p[i] = prob_of(((double)x[i] - ch.mp) * ch.scale, roots) * ip;
+      const double q = ch.zq > 0.0 ? prob_of(((double)y[i] - ch.mq) * ch.scale, roots) * iq : 0.0;
       r[i] = c + i == ch.drop ? 0.0 : fmax(p[i] - q, 0.0);
     }
   }
@@ -275,13 +281,13 @@ template <typename T> DM_DEV void judge(const VerifyArgs& a, int b, bool writes,
       Part q;
       q.z = 0.0, q.m = 0.f, q.arg = 0;
       if (with_q) q = join_parts(a, true, t, scale, roots);
-      const bool valid = is_distribution(p) && is_distribution(q);
+      const bool valid = is_temperature(temperature) && is_distribution(p) && is_distribution(q);
       bool ok = false;
       if (greedy) {
         ok = !last && d == p.arg && p.m == p.m && p.m > -INF;
       } else if (valid && in_range) {
-        const double qd = !with_q ? 1.0 : yd == -INF ? 0.0 : exp_of(((double)yd - q.m) * scale, roots) / q.z;
-        ok = xd != -INF && (double)u * qd < exp_of(((double)xd - p.m) * scale, roots) / p.z;
+        const double qd = !with_q ? 1.0 : prob_of(((double)yd - q.m) * scale, roots) / q.z;
+        ok = (double)u * qd < prob_of(((double)xd - p.m) * scale, roots) / p.z;
       }
       if (lane == 0) {
         sh.p[wave] = p, sh.q[wave] = q;
@@ -304,7 +310,7 @@ template <typename T> DM_DEV void judge(const VerifyArgs& a, int b, bool writes,
     Choice ch;
     ch.zp = p.z, ch.zq = q.z, ch.mp = p.m, ch.mq = q.m, ch.row = t, ch.scale = scale, ch.u = a.u[2 * t + 1];
     ch.drop = last || a.y ? -1 : (int)max(-1l, min((long)a.ids[t + 1], 0x7fffffffl));
-    ch.token = greedy ? (p.m == p.m && p.m > -INF ? p.arg : -1) : is_distribution(p) && is_distribution(q) ? -2 : -1;
+    ch.token = greedy ? (p.m == p.m && p.m > -INF ? p.arg : -1) : is_temperature(temperature) && is_distribution(p) && is_distribution(q) ? -2 : -1;
     ch.T = by, ch.log_zp = log(p.z);
     sh.choice = ch;
     if (writes) {

@@ -32,7 +32,10 @@ def verify_drafts(logits, ids, uniforms, starts, draft_logits=None, temperature=
     the device): sequence b's rows are starts[b] .. starts[b + 1] - 1. uniforms [N, 2] fp32 in [0, 1). draft_logits [N, V]: the
     distribution that ids[t + 1] was drawn from in row t (a sequence's last row is not read); None: the drafts are certain.
     temperature: one number, or [B] fp32. Returns Verified; no gradients. A row without a distribution (a NaN, +inf, nothing
-    but -inf) ends its sequence with token -1."""
+    but -inf; a temperature that is negative or not finite) ends its sequence with token -1."""
+    for t in (logits, draft_logits):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("verify_drafts keeps no autograd graph; call it under torch.no_grad() or on detached tensors")
     if not logits.is_cuda or logits.dim() != 2:
         raise ValueError(f"logits: shape {tuple(logits.shape)} on {logits.device}; rows [N, V] on a GPU are needed")
     dev = logits.get_device()

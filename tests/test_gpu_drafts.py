@@ -153,3 +153,29 @@ def test_rows_of_no_sequence():
     b = verify_drafts(pad(d["x"], 2), pad(d["ids"], 2), pad(d["u"], 2), d["starts"] + 2, draft_logits=pad(d["y"], 2), temperature=d["T"])
     assert torch.equal(b.tokens[2:7], a.tokens) and torch.equal(b.logp[2:7], a.logp) and torch.equal(b.accepted, a.accepted)
     assert (b.tokens[:2] == -1).all() and (b.tokens[7:] == -1).all() and (b.logp[7:] == 0).all()
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_small_and_large_temperatures(draft, dtype):
+    """Down to those of which a logit's quotient is far beyond its 64 bits' whole numbers, where only the largest logits have any
+    probability, and up to a uniform distribution."""
+    counts = [4, 6, 2, 5, 3, 4, 1]
+    s = make(counts, 5000, dtype, 77, draft)
+    s["T"] = torch.tensor([1e-3, 1e-8, 1e-20, 1e-30, 1e-44, 1e10, 3e38])
+    s["x"][5, 10] = s["x"][5, 4200] = s["x"][5].max() + 1      # two largest ones
+    s["x"] += 30
+    check(s, counts)
+
+
+@pytest.mark.parametrize("T", [-1.0, -1e-30, math.inf, -math.inf, math.nan])
+def test_numbers_that_are_no_temperature(T):
+    counts = [4, 3, 5]
+    s = make(counts, 700, torch.bfloat16, 78)
+    want = check(s, counts)
+    d = {n: t.to(DEV) for n, t in s.items()}
+    d["T"][1] = T
+    r = verify_drafts(d["x"], d["ids"], d["u"], d["starts"], draft_logits=d["y"], temperature=d["T"])
+    assert r.accepted[1] == 0 and (r.tokens[4:7] == -1).all() and r.logp[4].isnan() and (r.logp[5:7] == 0).all()
+    keep = [0, 1, 2, 3, 7, 8, 9, 10, 11]
+    assert torch.equal(r.tokens[keep], want.tokens[keep]) and torch.equal(r.logp[keep], want.logp[keep])
