@@ -48,6 +48,21 @@ def _no_graph(t):
         raise NotImplementedError("the paged cache keeps no autograd graph; call it under torch.no_grad() or on detached tensors")
 
 
+def _extent(t):
+    """The addresses [from, to) that a tensor's elements lie in."""
+    p = t.data_ptr()
+    return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else p
+
+
+def _apart(what, out, *others):
+    lo, hi = _extent(out)
+    for t in others:
+        if t is not None:
+            a, b = _extent(t)
+            if a < hi and lo < b:
+                raise ValueError(f"{what} overlaps a tensor that the call reads")
+
+
 # The checks compare device numbers and whole tuples: small calls are bound by the host, and torch's device objects and
 # generators over tensors cost more than the rest of a check.
 
@@ -150,7 +165,13 @@ def paged_attention(q, K, V, table, lengths, starts=None, k_self=None, v_self=No
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError(f"out: {out.dtype} {tuple(out.shape)} on {out.device}; contiguous {q.dtype} {tuple(q.shape)} on {K.device}")
     else:
+        _no_graph(out)
+        _apart("out", out, q, K, V, k_self, v_self, weights)
         torch.autograd.graph.increment_version(out)
+    if weights is not None:
+        _no_graph(weights)
+        if K.dtype == torch.float32:
+            _apart("weights", weights, q, K, V, k_self, v_self)
     lse = torch.empty((N, h), dtype=torch.float32, device=K.device)
     if N == 0 or B == 0:
         return PagedAttention(out, lse)

@@ -54,14 +54,19 @@ class PagedTape:
             n_sweeps = 1
         if n_sweeps < 1:
             raise ValueError(f"n_sweeps={n_sweeps}")
-        cfg, N = self.cfg, xhat.shape[0]
-        d, h, dh = cfg.d_model, cfg.n_heads, cfg.head_dim
+        N, d = xhat.shape[0], self.cfg.d_model
         if xhat.dtype != self.dtype or xhat.shape != (N, d) or xhat.device != self.device:
             raise ValueError(f"xhat: {xhat.dtype} {tuple(xhat.shape)} on {xhat.device}; {self.dtype} [N, {d}] on {self.device} is needed")
         if positions.shape != (N,) or positions.dtype != torch.int64:
             raise ValueError(f"positions: {positions.dtype} {tuple(positions.shape)}; int64 [{N}] is needed")
         if N == 0:
             return xhat.new_empty(0, d)
+        with torch.cuda.device(self.device):     # the launches below are the current device's
+            return self._extend(xhat, positions, cos, sin, (self.K, self.V, table, lengths, starts), n_sweeps, weights)
+
+    def _extend(self, xhat, positions, cos, sin, cache, n_sweeps, weights):
+        cfg, N = self.cfg, xhat.shape[0]
+        d, h, dh = cfg.d_model, cfg.n_heads, cfg.head_dim
         self.refresh()
         xhat = xhat.contiguous()
         cos, sin = (t.index_select(0, positions).float().contiguous() for t in (cos, sin))
@@ -72,7 +77,6 @@ class PagedTape:
         K, V = (torch.empty(h, N, dh, device=self.device, dtype=self.dtype) for _ in range(2))
         nb = L.lib().dm_refine_kv_workspace_bytes(conf, N)
         ws = torch.empty(nb, device=self.device, dtype=torch.uint8)
-        cache = (self.K, self.V, table, lengths, starts)
         if n_sweeps > 1:     # the first sweep reads the chunk's raw rows
             paged_write(k_self, v_self, *cache)
         for i in range(n_sweeps):

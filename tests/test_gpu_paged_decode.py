@@ -328,3 +328,27 @@ def test_sizes_of_nothing():
     assert r.o.shape == (0, 4, 64)
     v = verify_drafts(torch.zeros(3, 9, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV), torch.zeros(3, 2, device=DEV), i32(0))
     assert v.tokens.tolist() == [-1] * 3 and v.accepted.numel() == 0
+
+
+def test_outputs_in_the_place_of_inputs():
+    K, V = paged.new_pages(4, 2, 16, 64, dtype=torch.float32)
+    table, lengths = torch.zeros(2, 2, dtype=torch.int32, device=DEV), i32(3, 4)
+    q = torch.zeros(4, 4, 64, device=DEV)
+    pair = torch.zeros(2, 2, 64, device=DEV)
+    for kw in (dict(out=q[:2]), dict(out=q[1:3]), dict(out=K[2].view(-1)[:512].view(2, 4, 64)), dict(weights=V[1].view(-1)[:128].view(2, 2, 32)),
+               dict(weights=q[:2].view(-1)[:128].view(2, 2, 32))):
+        with pytest.raises(ValueError, match="overlaps"):
+            paged.paged_attention(q[:2], K, V, table, lengths, k_self=pair, v_self=pair, **kw)
+    r = paged.paged_attention(q[:2], K, V, table, lengths, out=q[2:])       # beside it
+    assert r.o.data_ptr() == q[2:].data_ptr()
+    w = torch.zeros(2, 2, 32, device=DEV, requires_grad=True)
+    with pytest.raises(NotImplementedError):
+        paged.paged_attention(q[:2], K, V, table, lengths, weights=w)
+    x = torch.zeros(4, 9, device=DEV)
+    rest = (torch.zeros(4, dtype=torch.int64, device=DEV), torch.zeros(4, 2, device=DEV), i32(0, 4))
+    y = x.clone().requires_grad_()
+    for kw in (dict(logits=y), dict(logits=x, draft_logits=y)):
+        with pytest.raises(NotImplementedError):
+            verify_drafts(kw.pop("logits"), *rest, **kw)
+    with torch.no_grad():
+        verify_drafts(y, *rest)
