@@ -1177,32 +1177,25 @@ DM_DEV uint32_t weight_order(float x) {
 // One block per sequence and key head: the weight of the last row to be kept by its bits, eight at a time from the top
 // (a histogram over the rows that agree so far), then the rows in order: those above it, and of those equal to it the first.
 // A thread takes 4 rows in turn; the first KEYS * 4096 rows' weights stay in registers. Eight histograms, by lane, since weights
-// share their first bits; bound by its passes' latencies (one sequence of 2304 rows 11 us, 16384 rows 17).
-constexpr int KEYS = 4, COPIES = 8;
+// share their first bits; one set for each pass, cleared before the first. Bound by its passes'
+// latencies (one sequence of 2304 rows and 16 heads 8.4 us, 32 of 3000 to 16384 rows and 8 heads 15.3; with scans by shuffles, one set of histograms and a sum over
+// the waves' totals in each thread 15.7 and 22.4).
+constexpr int KEYS = 4, COPIES = 8, COPY = 256 + 8;      // a copy's first banks lie 8 behind the one's before
 struct Selection {
-  int hist[256 * COPIES];
-  int total[2][KEYS][16];
+  int hist[4][COPIES * COPY];
+  int total[KEYS][16];      // rows kept of wave w's turn k, ties << 16
   int digit, above;
 };
 
 // of the need-th largest: its digit, and how many rows have a larger one. By the first wave: lane l takes digits 4 (63 - l) ..
 // + 3, from the largest.
-DM_DEV void find_digit(Selection& sh, int need) {
+DM_DEV void find_digit(Selection& sh, const int* hist, int need) {
   const int lane = threadIdx.x & 63, d0 = 4 * (63 - lane);
-  int n[4], sum = 0;
+  typedef int intx4 __attribute__((ext_vector_type(4)));
+  intx4 n = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    n[i] = 0;
-#pragma unroll
-    for (int k = 0; k < COPIES; ++k) n[i] += sh.hist[(d0 + i) * COPIES + k];
-    sum += n[i];
-  }
-  int upto = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int v = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += v;
-  }
+  for (int k = 0; k < COPIES; ++k) n += *reinterpret_cast<const intx4*>(hist + k * COPY + d0);
+  const int sum = (n[0] + n[1]) + (n[2] + n[3]), upto = wave_upto(sum);
   int above = upto - sum;
   if (above < need && upto >= need) {
     int d = 3;
@@ -1214,7 +1207,7 @@ DM_DEV void find_digit(Selection& sh, int need) {
 
 __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
   __shared__ Selection sh;
-  const int c = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long cap = (long)a.cols << a.page_shift;
   const int len = a.lengths[b] < 0 || a.lengths[b] > cap ? 0 : a.lengths[b];
   const int left = min(len, a.keep);
@@ -1241,15 +1234,16 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
   uint32_t key = 0;
   int need = a.keep - a.sinks - a.recent;           // of them stay (less than there are)
   if (need > 0) {
+    for (int i = threadIdx.x; i < 4 * COPIES * COPY; i += 1024) (&sh.hist[0][0])[i] = 0;
+    __syncthreads();
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256 * COPIES; i += 1024) sh.hist[i] = 0;
-      __syncthreads();
+      int* hist = sh.hist[shift >> 3];
       const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
       auto count = [&](int q, const uint32_t (&u)[4]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (4 * q + e >= lo && 4 * q + e < hi && (u[e] & mask) == key)
-            atomicAdd(&sh.hist[((u[e] >> shift) & 255) * COPIES + (lane & (COPIES - 1))], 1);
+            atomicAdd(hist + (lane & (COPIES - 1)) * COPY + ((u[e] >> shift) & 255), 1);
       };
 #pragma unroll
       for (int k = 0; k < KEYS; ++k) count(threadIdx.x + 1024 * k, held[k]);
@@ -1259,7 +1253,7 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
         count(q, u);
       }
       __syncthreads();
-      if (wave == 0) find_digit(sh, need);
+      if (wave == 0) find_digit(sh, hist, need);
       __syncthreads();
       key |= (uint32_t)sh.digit << shift;
       need -= sh.above;
@@ -1285,24 +1279,17 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
         else if (i < len && u[e] == key) tie[k] |= 1 << e;
       }
       const int mine = __popc(sure[k]) + (__popc(tie[k]) << 16);
-      int sum = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += v;
-      }
-      before[k] = sum - mine;
-      if (lane == 63) sh.total[0][k][wave] = sum & 0xffff, sh.total[1][k][wave] = sum >> 16;
+      const int upto = wave_upto(mine);
+      before[k] = upto - mine;
+      if (lane == 63) sh.total[k][wave] = upto;
     }
     __syncthreads();
+    // rows before each wave's turn (16384 rows at most: ties stay below 32 bits)
+    const int turn = sh.total[lane >> 4][lane & 15], turns = wave_upto(turn);
 #pragma unroll
     for (int k = 0; k < KEYS; ++k) {
-      int s = at + (before[k] & 0xffff), t = equal + (before[k] >> 16);
-      for (int x = 0; x < 16; ++x) {
-        if (x < wave) s += sh.total[0][k][x], t += sh.total[1][k][x];
-        at += sh.total[0][k][x];
-        equal += sh.total[1][k][x];
-      }
+      const int ahead = before[k] + __builtin_amdgcn_readlane(turns - turn, 16 * k + wave);
+      int s = at + (ahead & 0xffff), t = equal + (ahead >> 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool is_sure = sure[k] >> e & 1, is_tie = tie[k] >> e & 1;
@@ -1311,6 +1298,9 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
         t += is_tie;
       }
     }
+    const int all = __builtin_amdgcn_readlane(turns, 63);
+    at += all & 0xffff;
+    equal += all >> 16;
     __syncthreads();
   }
 }
