@@ -357,13 +357,20 @@ template <typename T, bool JUDGE> __global__ __launch_bounds__(1024) void k_veri
   }
 }
 
-DM_DEV double wave_upto(double v) {      // the sum over the lanes up to this one
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
+// the sum over the lanes up to this one, by moves inside the rows of 16 lanes and broadcasts of the rows' last lanes
+template <int CTRL, int ROWS> DM_DEV double moved(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+DM_DEV double wave_upto(double v) {
+  v += moved<0x111, 0xf>(v);     // row_shr 1, 2, 4, 8
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);     // row_bcast 15, 31
+  v += moved<0x143, 0xc>(v);
   return v;
 }
 
