@@ -81,9 +81,9 @@ DM_DEV int wave_upto(int v) {
 }
 
 // The plan: sequence b's query tiles (of ROWS query rows; 1 with ROWS = 0) times its pieces, in order. PIECES: find item
-// number `at` of those; otherwise of the query tiles alone. Called by whole waves. Items and slots are fewer than the blocks of a
-// launch; the cost (query tiles times tiles of cached rows) may pass 32 bits and is summed in fp32, rounded up, so that a piece's
-// tiles are never too few for the slots that the workspace has.
+// number `at` of those; otherwise of the query tiles alone. Called by whole waves. Items and slots are fewer than the blocks
+// of a launch; the cost (query tiles times tiles of cached rows) may pass 32 bits and is summed in fp32, rounded up, so that a
+// piece's tiles are never too few for the slots that the workspace has.
 template <int ROWS, bool PIECES> DM_DEV Item find_item(const PagedArgs& a, int at) {
   const int lane = threadIdx.x & 63;
   auto tiles_q = [&](const Seq& s) { return ROWS ? (s.n * a.g + ROWS - 1) / (ROWS ? ROWS : 1) : (s.n > 0); };
@@ -138,7 +138,8 @@ DM_DEV void make_uniform(Item& it) {
 }
 
 // ---- rows into the pages ---------------------------------------------------------------------
-// One thread per 16 bytes of a new token's key or value row (in turns where there are more of them than a launch has threads).
+// One thread per 16 bytes of a new token's key or value row (in turns where there are more of them than a launch has
+// threads). Bound by latency at ordinary sizes: 4 us for 200 tokens, 12 for 4096 tokens of 8 key heads of 128 (34 MB moved).
 template <typename T> __global__ __launch_bounds__(256) void k_paged_write(PagedArgs a, int dh) {
   constexpr int V = 16 / (int)sizeof(T);
   const int per = dh / V;
@@ -178,7 +179,9 @@ template <typename T, int DH> struct Tile {
   static constexpr int NV = KT * DH * (int)sizeof(T) / 1024;      // 16-byte loads of a lane for the step's V rows
   static constexpr int VPR = DH / V;
   static constexpr int NDT = DH / 16;
-  static constexpr int WAVES = sizeof(T) == 2 ? 3 : 3 - DH / 64;      // per SIMD (bf16 rows of 64 at 4: 97 us, at 3 92)
+  // per SIMD at least: what the registers of rows on their way leave (bf16 rows of 64: 105 registers, 4 waves fit; asked for 4 the
+  // compiler keeps fewer loads on their way: 64 sequences of 100 to 8192 rows 97 us instead of 92)
+  static constexpr int WAVES = sizeof(T) == 2 ? 3 : 3 - DH / 64;
 };
 
 // S^T[16 cached rows][16 query rows] += K Q^T for one 16-byte chunk per lane of each: bf16 lane l holds columns
@@ -274,8 +277,8 @@ template <typename T, int LDV> DM_DEV floatx4 mma_values(const T* Vs, const floa
 
 // The page of rows r .. that lie in one (pages hold 16 rows or more and begin at a multiple of 16). needed: some query of
 // the tile reads some of them. A page outside the pool is read as page 0 and marks the sequence. The table is read through
-// the scalar cache: a vector load of it would be waited for together with all rows that are on their way (prompt_chunk's
-// read 2.50 ms so), and pages are looked up a step ahead of their rows.
+// the scalar cache: a vector load of it would be waited for together with all rows that are on their way (two prompts' chunks
+// of 2048 tokens over 16384 rows 2.50 ms so, 1.66 with scalar loads), and pages are looked up a step ahead of their rows.
 DM_DEV int page_of(const PagedArgs& a, const int32_t* table, int r, bool needed, bool& bad) {
   typedef const __attribute__((address_space(4))) int32_t* Scalar;
   const int p = needed ? ((Scalar)table)[r >> a.page_shift] : 0;
@@ -297,8 +300,15 @@ DM_DEV long scores_at(const PagedArgs& a, const Seq& s, int c) {
 
 // One block: a query tile of 16 rows, a key head and a piece of its cached rows. The four waves take steps of 32 rows in
 // turn, each with a running maximum m and sum z per query row (scores in units of ln 2) and O^T in registers, and are
-// joined through LDS. KEEP: the scores are kept for the weights (of the lanes behind the last query row too, which work on that
-// one again: a store that some lanes skip would have the next rows' loads wait for it, tokens_shared 276 us).
+// joined through LDS. S^T = K Q^T rather than S = Q K^T: a lane then holds scores of one query row only, the maximum needs two
+// exchanges, and the probabilities are already the operand of the product with V, whose columns come from LDS transposed. K goes
+// to the matrix cores straight from memory. The next step's rows of K and V are on their way in registers meanwhile.
+// Bound by the rows' bytes: 64 sequences of 100 to 8192 rows of 64 on 16 key heads (484 MB) 90 us, 5.4 TB/s, of random pages of
+// 64 rows; more blocks per CU or more rows on their way bring nothing. One token over 1024 rows 6 us, most of it latency: the
+// plan, the table, the rows.
+// KEEP: the scores are kept for the weights (of the lanes behind the last query row too, which work on that one again: a store
+// that some lanes skip would have the next rows' loads wait for it, 276 instead of 273 us). 32 sequences of 3000 to 16384 rows of
+// 128 on 8 key heads, 1.28 GB: 229 us without, 273 with; computing the scores again costs 172.
 template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile<T, DH>::WAVES)) void k_paged_read(PagedArgs a) {
   using C = Tile<T, DH>;
   constexpr int VBYTES = C::KT * C::LDV * (int)sizeof(T), OBYTES = TILE_Q * DH * 4;
@@ -547,7 +557,11 @@ template <int DH> struct WideTile {
 // steps of 64 that all waves share. Scores as 32 x 32 tiles S^T = K Q^T: a lane holds one query row's scores, so maximum and
 // sum need one exchange per step. The next step's scores run on the matrix cores while this one's exponentials run on the
 // vector units, and this one's product with V beside the next one's maximum: K is a step ahead of V (two buffers each, their
-// rows on their way in registers).
+// rows on their way in registers; rows sent to LDS directly were slower, since the compiler then waits for all of them before
+// it reads V transposed). Rows of K are padded by 16 bytes, of V by 64: no bank conflicts.
+// Bound by the matrix cores beside the exponentials: two prompts' chunks of 2048 tokens over 16384 rows, 32 heads of 128 on 8
+// key heads (1.01 Tflop) 1.13 ms after a pause and 1.03 in a run of calls, 0.9 to 0.98 Pflop/s (a library product of 8192^3
+// 1.10); the matrix cores are busy 48 % of the cycles at the clock that the power leaves. With 16-row tiles 4.1 ms.
 template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_paged_read_wide(PagedArgs a) {
   using C = WideTile<DH>;
   constexpr int NT = 64 * NW, ROWS = 32 * NW, NL = C::KT * C::VPR / NT;    // 16-byte loads per thread of K and of V
@@ -885,7 +899,8 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
   if (half == 0) a.lse[at] = z == 0.f ? -INF : (ref + __builtin_amdgcn_logf(z)) * LN2;
 }
 
-// The pieces of a query tile, in their order.
+// The pieces of a query tile, in their order: 16 threads a query row. Bound by latency: the plan, the maxima, then eight pieces'
+// columns at a time (one token in 16 pieces 4 us, 64 sequences 6, 8192 query rows of 8 key heads 11).
 template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
   const int c = blockIdx.x % a.h_kv;
   Item it = find_item<ROWS, false>(a, blockIdx.x / a.h_kv);
@@ -934,7 +949,7 @@ template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k
 DM_DEV float lse_of(float lse) { return lse == -INF ? INF : lse * LOG2E; }
 
 // weights[b, c, r] += the sum over the sequence's query rows of exp(score - lse), from scores that the read kept: a thread
-// takes 4 cached rows and goes over the query rows.
+// takes 4 cached rows and goes over the query rows. 32 sequences of 3000 to 16384 rows, 32 heads on 8 key heads: 18.5 us.
 __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
   const int c = uniform(blockIdx.x % a.h_kv);
   Item it = find_item<0, true>(a, blockIdx.x / a.h_kv);
@@ -968,8 +983,9 @@ __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
   }
 }
 
-// The same with the scores computed again: weights[b, c, r] += the sum over the sequence's query rows of exp(score - lse), the scores computed again: a wave holds
-// 32 cached rows as fragments and goes over all query tiles, so each weight has one writer and one order of its sum.
+// The same with the scores computed again: a wave holds 32 cached rows as fragments and goes over all query tiles, so each
+// weight has one writer and one order of its sum. fp32, seven sequences of up to 130 tokens over up to 1501 rows, a window of
+// 256: 15 us, most of it latency.
 template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_weights(PagedArgs a) {
   using C = Tile<T, DH>;
   const int c = uniform(blockIdx.x % a.h_kv), lane = threadIdx.x & 63, grp = lane >> 4, col = lane & 15;
@@ -987,7 +1003,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
   const int in_page = (1 << a.page_shift) - 1;
   float* w = a.weights + ((long)it.b * a.h_kv + c) * ((long)a.cols << a.page_shift);
   // Few query rows: each wave takes cached rows of its own; many: the waves share them and take the query tiles in turn
-  // (window_fp32: 23.2 us without)
+  // (the call above 15 us so, 23 without)
   __shared__ float part[2][4][C::KT];
   const bool shared = rows > 4 * TILE_Q;
   const int step = shared ? C::KT : 4 * C::KT, q_first = shared ? TILE_Q * wave : 0, q_step = shared ? 4 * TILE_Q : TILE_Q;
@@ -1059,7 +1075,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
 
 // The same for many query rows: a block takes 64 cached rows, each wave all of them against 32 query rows at a time (every
 // fragment of Q is used twice), the waves' sums are added through LDS. Bound by the exponentials beside the products: two
-// sequences of 16384 rows, 8192 query rows of 128: 0.6 ms, with 16-row tiles 1.84.
+// prompts' chunks of 2048 tokens over 16384 rows, 32 heads of 128 on 8 key heads: 0.86 ms, with 16-row tiles 1.84.
 template <int DH> __global__ __launch_bounds__(256, 2) void k_paged_weights_wide(PagedArgs a) {
   constexpr int NK = DH / 16;
   __shared__ float part[2][4][TILE_K];
@@ -1305,7 +1321,8 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
   }
 }
 
-// One thread per 16 bytes of a kept row of K and of V.
+// One thread per 16 bytes of a kept row of K and of V. Bound by the rows' bytes: 32 sequences, 4096 kept rows of 128 on 8 heads
+// each (1.08 GB) 222 us, 4.85 TB/s, what a large copy reaches.
 __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a, int row_bytes, int esize) {
   const int c = blockIdx.y, b = blockIdx.z, per = row_bytes / 16;
   const long at = blockIdx.x * 256L + threadIdx.x;
@@ -1345,7 +1362,7 @@ int log2_of(int x) {
 // The plan's numbers: about `blocks` blocks over the key heads.
 long query_tiles(const dm_paged_args* a, int rows) { return (long)a->n_tokens * (a->h / a->h_kv) / rows + a->B; }
 // ... but no more than there can be, by the table's and the window's rows: blocks without a piece cost their look at the plan
-// (one_token 8.2 us with 8 blocks per CU, 7.0 with 5).
+// (one token over 1024 rows: 8.2 us with 8 blocks per CU wanted, 7.0 with 5, 6.0 with those that there can be).
 int wanted(const dm_paged_args* a, int blocks, long tiles, int least) {
   long rows = (long)a->table_cols * a->page;
   if (a->window) rows = std::min(rows, (long)a->window + a->n_tokens);
