@@ -324,19 +324,47 @@ template <typename T> DM_DEV void judge(const VerifyArgs& a, int b, bool writes,
     for (int i = end + 1 + threadIdx.x; i < rows.n; i += 1024) a.tokens[rows.first + i] = -1, a.logp[rows.first + i] = 0.f;
 }
 
+// The sums of r and p over part `part` of the chosen row, by a block, into a.sums.
+template <typename T> DM_DEV void sum_part(const VerifyArgs& a, const Choice& ch, int b, int part, const Roots& roots, double (&sums)[2][16]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Residual<T> v(a, ch, part * PART + threadIdx.x * 4, roots);
+  const double r = wave_sum_double((v.r[0] + v.r[1]) + (v.r[2] + v.r[3])), s = wave_sum_double((v.p[0] + v.p[1]) + (v.p[2] + v.p[3]));
+  if (lane == 0) sums[0][wave] = r, sums[1][wave] = s;
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    double sum = 0.0;
+    for (int w = 0; w < 16; ++w) sum += sums[threadIdx.x][w];
+    a.sums[((long)b * 2 + threadIdx.x) * a.n_parts + part] = sum;
+  }
+}
+
+// A sequence per block. Where no draft distribution is subtracted, the chosen row's sums are those of its parts, but for the
+// part of a draft that counts 0: written here, so that only a call with draft distributions takes a launch for them (48
+// sequences, rows of 100003 in bf16: 6.4 us for 4.8 and 10.3 apart).
 template <typename T> __global__ __launch_bounds__(1024) void k_verify_judge(VerifyArgs a) {
   __shared__ Roots roots;
   __shared__ Judging sh;
+  __shared__ double sums[2][16];
   roots.fill();
   __syncthreads();
-  judge<T>(a, blockIdx.x, true, roots, sh);
+  const int b = blockIdx.x;
+  judge<T>(a, b, true, roots, sh);
+  __syncthreads();
+  const Choice ch = sh.choice;
+  if (ch.token != -2 || ch.zq > 0.0) return;
+  const int own = ch.drop >= 0 && ch.drop < a.V ? ch.drop / PART : -1;
+  const Part* p = a.parts + (long)ch.row * a.n_parts;
+  double* to = a.sums + (long)b * 2 * a.n_parts;
+  for (int i = threadIdx.x; i < a.n_parts; i += 1024)
+    if (i != own) to[i] = to[a.n_parts + i] = p[i].z / ch.zp * prob_of(((double)p[i].m - ch.mp) * ch.scale, roots);
+  if (own >= 0) sum_part<T>(a, ch, b, own, roots, sums);
 }
 
 // The sums of r and p over each part of a sequence's chosen row, as in k_verify_parts bound by the exponentials. JUDGE: each block
-// decides over the sequence by itself, a launch less (one sequence of 4 drafts 8.5 us, 5.5 and 5.1 apart; 64 of 13 parts 26, 6.0
-// and 10 apart).
+// decides over the sequence by itself, a launch less (one sequence of 4 drafts 8.5 us, 5.5 and 5.1 apart; 64 of 13 parts 26, 6.4
+// and 8.4 apart).
 template <typename T, bool JUDGE> __global__ __launch_bounds__(1024) void k_verify_sums(VerifyArgs a) {
-  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.y;
   __shared__ Roots roots;
   __shared__ double sums[2][16];
   __shared__ Judging sh;
@@ -347,16 +375,8 @@ template <typename T, bool JUDGE> __global__ __launch_bounds__(1024) void k_veri
     __syncthreads();
   }
   const Choice ch = JUDGE ? sh.choice : a.choice[b];
-  if (ch.token != -2) return;
-  const Residual<T> v(a, ch, blockIdx.x * PART + threadIdx.x * 4, roots);
-  const double r = wave_sum_double((v.r[0] + v.r[1]) + (v.r[2] + v.r[3])), s = wave_sum_double((v.p[0] + v.p[1]) + (v.p[2] + v.p[3]));
-  if (lane == 0) sums[0][wave] = r, sums[1][wave] = s;
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    double sum = 0.0;
-    for (int w = 0; w < 16; ++w) sum += sums[threadIdx.x][w];
-    a.sums[((long)b * 2 + threadIdx.x) * a.n_parts + blockIdx.x] = sum;
-  }
+  if (ch.token != -2 || (!JUDGE && ch.zq == 0.0)) return;
+  sum_part<T>(a, ch, b, blockIdx.x, roots, sums);
 }
 
 // the sum over the lanes up to this one, by moves inside the rows of 16 lanes and broadcasts of the rows' last lanes
@@ -474,11 +494,11 @@ size_t sums_bytes(const dm_verify_args* a) { return align256((size_t)2 * a->B * 
 
 template <typename T> void run_verify(const VerifyArgs& p, hipStream_t s) {
   hipLaunchKernelGGL(k_verify_parts<T>, dim3(p.n_parts, p.N, p.y ? 2 : 1), dim3(256), 0, s, p);
-  if ((long)p.n_parts * p.B <= 256) {      // a block per CU
+  if (p.y && (long)p.n_parts * p.B <= 256) {      // a block per CU
     hipLaunchKernelGGL((k_verify_sums<T, true>), dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
   } else {
     hipLaunchKernelGGL(k_verify_judge<T>, dim3(p.B), dim3(1024), 0, s, p);
-    hipLaunchKernelGGL((k_verify_sums<T, false>), dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
+    if (p.y) hipLaunchKernelGGL((k_verify_sums<T, false>), dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
   }
   hipLaunchKernelGGL(k_verify_pick<T>, dim3(p.B + cdiv(p.N, 16)), dim3(1024), 0, s, p);
 }
