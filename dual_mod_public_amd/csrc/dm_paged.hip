@@ -1359,15 +1359,16 @@ int log2_of(int x) {
   return -1;
 }
 
-// The plan's numbers: about `blocks` blocks over the key heads.
 long query_tiles(const dm_paged_args* a, int rows) { return (long)a->n_tokens * (a->h / a->h_kv) / rows + a->B; }
-// ... but no more than there can be, by the table's and the window's rows: blocks without a piece cost their look at the plan
-// (one token over 1024 rows: 8.2 us with 8 blocks per CU wanted, 7.0 with 5, 6.0 with those that there can be).
+// the most tiles of cached rows that a query tile can have, by the table's and the window's rows
+long most_tiles(const dm_paged_args* a) {
+  const long rows = (long)a->table_cols * a->page;
+  return (a->window ? std::min(rows, (long)a->window + a->n_tokens + TILE_K) : rows) / TILE_K + 1;
+}
+// The plan's numbers: about `blocks` blocks over the key heads, but no more than there can be: blocks without a piece cost their
+// look at the plan (one token over 1024 rows: 8.2 us with 8 blocks per CU wanted, 7.0 with 5, 6.0 with those that there can be).
 int wanted(const dm_paged_args* a, int blocks, long tiles, int least) {
-  long rows = (long)a->table_cols * a->page;
-  if (a->window) rows = std::min(rows, (long)a->window + a->n_tokens);
-  const long each = (rows / TILE_K + 2 + least - 1) / least;     // pieces of a tile
-  return (int)std::max(1L, std::min((long)cdiv(blocks, a->h_kv), tiles * each));
+  return (int)std::max(1L, std::min((long)cdiv(blocks, a->h_kv), tiles * ((most_tiles(a) + least - 1) / least)));
 }
 constexpr int WEIGHT_BLOCKS = 8 * CUS;
 
@@ -1376,12 +1377,20 @@ constexpr int WEIGHT_BLOCKS = 8 * CUS;
 // 24 rows 60 / 69 / 115 and 60 / 62 / 82, 48 rows 78 / 71 / 115 and 84 / 65 / 86, 256 rows 303 / 123 / 134 and 307 / 117 / 119,
 // 512 rows 572 / 225 / 215 and 596 / 195 / 188; two sequences of 16384 rows, 8192 query rows: 4110 / 1340 / 1150). Pieces:
 // what fills the CUs with the blocks that one holds (at 8192 query rows 1, 2 and 4 times as many: 1150, 1184, 1206 us).
+// In one piece, with no join, while a tile's keys take no more than 128 KiB, or 256 with blocks for half of the CUs (a call / its
+// kernels in a graph, pieces -> whole: one token, 16 heads of 64, 256 rows 17.1 / 8.9 -> 14.2 / 6.4 us, 512 rows 17.3 / 9.2 ->
+// 14.4 / 7.6, 1024 rows 17.2 / 9.1 -> 14.3 / 9.8, 2048 rows 17.0 / 9.5 -> 14.5 / 14.3; 8 tokens over 2048 rows 23.4 / 24.0 ->
+// 20.4 / 21.0; 7 chunks of 65 fp32 tokens, 8 heads of 64 on 4, over 1024 rows 43 -> 34).
+bool in_one_piece(const dm_paged_args* a) {
+  const long bytes = (most_tiles(a) - 1) * TILE_K * a->dh * (long)esz(a->dtype);
+  return bytes <= (query_tiles(a, TILE_Q) * a->h_kv >= CUS / 2 ? 256 << 10 : 128 << 10);
+}
 struct Form {
   int rows, blocks, least;     // query rows of a tile; blocks wanted; least tiles of cached rows in a piece
 };
 Form form_of(const dm_paged_args* a) {
   const int64_t mean = (int64_t)a->n_tokens * (a->h / a->h_kv) / a->B;
-  if (a->dtype != DM_BF16 || mean <= 2 * TILE_Q) return {TILE_Q, 5 * CUS, 2};
+  if (a->dtype != DM_BF16 || mean <= 2 * TILE_Q) return {TILE_Q, 5 * CUS, in_one_piece(a) ? (int)most_tiles(a) : 2};
   return mean <= 512 ? Form{128, 2 * CUS, 2} : Form{256, CUS, 2};
 }
 // The scores of a call with weights are kept where they take no more room than the pages' keys; else they are computed
@@ -1392,9 +1401,10 @@ size_t score_floats(const dm_paged_args* a) {
   return n * 4 <= (double)a->n_pages * a->h_kv * a->page * a->dh * esz(a->dtype) ? (size_t)n : 0;
 }
 int wanted(const dm_paged_args* a, const Form& f) { return wanted(a, f.blocks, query_tiles(a, f.rows), f.least); }
+bool in_pieces(const dm_paged_args* a, const Form& f) { return most_tiles(a) > f.least; }
 size_t part_floats(const dm_paged_args* a) {
   const Form f = form_of(a);
-  return (size_t)2 * wanted(a, f) * a->h_kv * f.rows * (a->dh + 2);
+  return !in_pieces(a, f) ? 0 : (size_t)2 * wanted(a, f) * a->h_kv * f.rows * (a->dh + 2);
 }
 size_t part_bytes(const dm_paged_args* a) { return align256(part_floats(a) * 4); }
 
@@ -1472,8 +1482,7 @@ template <typename T, int DH> int run_attention(const dm_paged_args* a, hipStrea
   if (score_floats(a)) p.scores = (float*)((char*)a->workspace + part_bytes(a));
   const long tiles = query_tiles(a, f.rows);
   const unsigned blocks = (unsigned)((p.want + tiles) * a->h_kv);
-  // pieces there are only where a sequence can have more tiles than the least of one piece
-  const bool join = (int64_t)a->table_cols * a->page > f.least * TILE_K;
+  const bool join = in_pieces(a, f);
   const dim3 joined((unsigned)(tiles * a->h_kv), f.rows / 16);
   if (f.rows == TILE_Q) {
     if (p.scores) hipLaunchKernelGGL((k_paged_read<T, DH, true>), dim3(blocks), dim3(256), 0, s, p);

@@ -179,8 +179,10 @@ def paged_attention(q, K, V, table, lengths, starts=None, k_self=None, v_self=No
                         dh ** -0.5 if scale is None else float(scale), 0, *q_rows, K.data_ptr(), V.data_ptr(), k_page, v_page, table_p,
                         lengths_p, starts_p, *pair, out.data_ptr(), lse.data_ptr(), weights_p)
     args = L.byref(a)
-    ws = torch.empty(L.lib().dm_paged_workspace_bytes(args), dtype=torch.uint8, device=K.device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    nb = L.lib().dm_paged_workspace_bytes(args)
+    if nb:
+        ws = torch.empty(nb, dtype=torch.uint8, device=K.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nb
     if weights is not None:
         torch.autograd.graph.increment_version(weights)
     L.call_on(K.device, L.lib().dm_paged_attention, args)

@@ -28,7 +28,7 @@ PAGES = [(dict(dtype=2), -1), (dict(dh=96), -2), (dict(page=8), -2), (dict(page=
     (dict(q_token=252), -1), (dict(q_head=-64), -1), (dict(window=-1), -1), (dict(scale=float("inf")), -1), (dict(scale=float("nan")), -1),
     (dict(o=None), -1), (dict(o=0x60004), -1), (dict(lse=None), -1), (dict(k_rows=0x80000), -1), (dict(v_rows=0x80000), -1),
     (dict(k_rows=0x80000, v_rows=0x90008, k_token=128, k_head=64, v_token=128, v_head=64), -1),
-    (dict(workspace=None), -3), (dict(workspace=0x100008), -3), (dict(workspace_bytes=16), -3),
+    (dict(workspace=None, table_cols=200), -3), (dict(workspace=0x100008, table_cols=200), -3), (dict(workspace_bytes=16, table_cols=200), -3),
     (dict(starts=0x51000, n_tokens=1 << 26), -1)])
 def test_attention_refuses(kw, rc):
     lib = L.load()
@@ -100,3 +100,11 @@ def test_more_blocks_than_a_launch_has():
     rows = dict(k_rows=0x80000, v_rows=0x90000, k_token=1024 * 64, k_head=64, v_token=1024 * 64, v_head=64)
     assert lib.dm_paged_attention(L.byref(paged_args(**big)), None) == -1 and b"in all" in lib.dm_last_error()
     assert lib.dm_paged_write(L.byref(paged_args(**big, **rows)), None) == -1
+
+
+def test_workspaces():
+    """None where every tile's rows lie in one piece and no scores are kept; else enough for twice the pieces wanted."""
+    size = L.load().dm_paged_workspace_bytes
+    assert size(L.byref(paged_args())) == 0 and size(L.byref(paged_args(table_cols=64))) == 0
+    assert size(L.byref(paged_args(table_cols=200))) > 0 and size(L.byref(paged_args(weights=0x90000, n_pages=4096))) > 0
+    assert size(L.byref(paged_args(table_cols=200, window=64))) == 0
