@@ -338,28 +338,6 @@ template <typename T> DM_DEV void sum_part(const VerifyArgs& a, const Choice& ch
   }
 }
 
-// A sequence per block. Where no draft distribution is subtracted, the chosen row's sums are those of its parts, but for the
-// part of a draft that counts 0: written here, so that only a call with draft distributions takes a launch for them (48
-// sequences, rows of 100003 in bf16: 6.4 us for 4.8 and 10.3 apart).
-template <typename T> __global__ __launch_bounds__(1024) void k_verify_judge(VerifyArgs a) {
-  __shared__ Roots roots;
-  __shared__ Judging sh;
-  __shared__ double sums[2][16];
-  roots.fill();
-  __syncthreads();
-  const int b = blockIdx.x;
-  judge<T>(a, b, true, roots, sh);
-  __syncthreads();
-  const Choice ch = sh.choice;
-  if (ch.token != -2 || ch.zq > 0.0) return;
-  const int own = ch.drop >= 0 && ch.drop < a.V ? ch.drop / PART : -1;
-  const Part* p = a.parts + (long)ch.row * a.n_parts;
-  double* to = a.sums + (long)b * 2 * a.n_parts;
-  for (int i = threadIdx.x; i < a.n_parts; i += 1024)
-    if (i != own) to[i] = to[a.n_parts + i] = p[i].z / ch.zp * prob_of(((double)p[i].m - ch.mp) * ch.scale, roots);
-  if (own >= 0) sum_part<T>(a, ch, b, own, roots, sums);
-}
-
 // The sums of r and p over each part of a sequence's chosen row, as in k_verify_parts bound by the exponentials. JUDGE: each block
 // decides over the sequence by itself, a launch less (one sequence of 4 drafts 8.5 us, 5.5 and 5.1 apart; 64 of 13 parts 26, 6.4
 // and 8.4 apart).
@@ -396,23 +374,14 @@ DM_DEV double wave_upto(double v) {
   return v;
 }
 
-// One block per sequence: the part of the chosen row in which the place lies, then the thread, then the column. Rows of no
-// sequence get token -1. Bound by latency: the sums, then the part's logits, 5 to 7 us at any size.
-template <typename T> __global__ __launch_bounds__(1024) void k_verify_pick(VerifyArgs a) {
-  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (b >= a.B) {
-    const int t = (b - a.B) * 16 + wave;
-    if (t < a.N && sequence_of(a, t) < 0 && lane == 0) a.tokens[t] = -1, a.logp[t] = 0.f;
-    return;
-  }
-  const double* sums_of = a.sums + (long)b * 2 * a.n_parts;
-  const double ahead = wave == 0 && lane < a.n_parts ? sums_of[lane] : 0.0;      // beside the choice
-  const Choice ch = a.choice[b];
-  if (ch.token != -2) return;
-  __shared__ Roots roots;
-  __shared__ double base, place, sums[16];
-  __shared__ int part, plain, hit[16], most[16];
-  roots.fill();
+// A block: the part of the chosen row in which the place lies, then the thread, then the column. ahead: the first wave's sums of r
+// of parts 0 .. 63. Bound by latency: the sums, then the part's logits.
+struct Picking {
+  double base, place, sums[16];
+  int part, plain, hit[16], most[16];
+};
+template <typename T> DM_DEV void pick(const VerifyArgs& a, const Choice& ch, const double* sums_of, double ahead, const Roots& roots, Picking& sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (wave == 0) {
     const double* s = sums_of;
     double total = 0.0;
@@ -421,7 +390,7 @@ template <typename T> __global__ __launch_bounds__(1024) void k_verify_pick(Veri
       total = kind ? (lane < a.n_parts ? s[lane] : 0.0) : ahead;
       for (int i = lane + 64; i < a.n_parts; i += 64) total += s[i];
       total = wave_sum_double(total);
-      if (lane == 0) plain = kind;
+      if (lane == 0) sh.plain = kind;
       if (total > 0.0) break;
     }
     const double to = (double)ch.u * total;
@@ -444,48 +413,99 @@ template <typename T> __global__ __launch_bounds__(1024) void k_verify_pick(Veri
       before = __shfl(upto, 63, 64);
     }
     if (lane == 0) {
-      part = found < 0 ? any : found;
-      base = found < 0 ? any_base : found_base;
-      place = to;
+      sh.part = found < 0 ? any : found;
+      sh.base = found < 0 ? any_base : found_base;
+      sh.place = to;
     }
   }
   __syncthreads();
-  const int c0 = part * PART + threadIdx.x * 4;
+  const int c0 = sh.part * PART + threadIdx.x * 4;
   const Residual<T> v(a, ch, c0, roots);
   double r[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = plain ? v.p[i] : v.r[i];
+  for (int i = 0; i < 4; ++i) r[i] = sh.plain ? v.p[i] : v.r[i];
   const double mine = (r[0] + r[1]) + (r[2] + r[3]), upto = wave_upto(mine);
-  if (lane == 63) sums[wave] = upto;
+  if (lane == 63) sh.sums[wave] = upto;
   __syncthreads();
-  double before = base;
-  for (int w = 0; w < wave; ++w) before += sums[w];
+  double before = sh.base;
+  for (int w = 0; w < wave; ++w) before += sh.sums[w];
   before += upto - mine;
   int first = 0x7fffffff, last = -1;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     before += r[i];
     if (r[i] > 0.0) last = c0 + i;
-    if (before > place && r[i] > 0.0) first = min(first, c0 + i);
+    if (before > sh.place && r[i] > 0.0) first = min(first, c0 + i);
   }
   // columns ascend with the lanes and the waves
   const uint64_t hits = __ballot(first != 0x7fffffff), some = __ballot(last >= 0);
-  if (hits && lane == __ffsll((unsigned long long)hits) - 1) hit[wave] = first;
-  else if (!hits && lane == 0) hit[wave] = -1;
-  if (some && lane == 63 - __clzll((long long)some)) most[wave] = last;
-  else if (!some && lane == 0) most[wave] = -1;
+  if (hits && lane == __ffsll((unsigned long long)hits) - 1) sh.hit[wave] = first;
+  else if (!hits && lane == 0) sh.hit[wave] = -1;
+  if (some && lane == 63 - __clzll((long long)some)) sh.most[wave] = last;
+  else if (!some && lane == 0) sh.most[wave] = -1;
   __syncthreads();
   int token = -1;
 #pragma unroll
   for (int w = 0; w < 16; ++w)
-    if (most[w] >= 0) token = most[w];
+    if (sh.most[w] >= 0) token = sh.most[w];
 #pragma unroll
   for (int w = 15; w >= 0; --w)
-    if (hit[w] >= 0) token = hit[w];
+    if (sh.hit[w] >= 0) token = sh.hit[w];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (c0 + i == token) a.tokens[ch.row] = token, a.logp[ch.row] = (float)(((double)v.x[i] - ch.mp) / ch.T - ch.log_zp);
   if (token < 0 && threadIdx.x == 0) a.tokens[ch.row] = -1, a.logp[ch.row] = NAN_;
+}
+// blocks from the sequences' number on: 16 rows each, of which those of no sequence get token -1
+DM_DEV bool rows_of_none(const VerifyArgs& a) {
+  if ((int)blockIdx.x < a.B) return false;
+  const int t = ((int)blockIdx.x - a.B) * 16 + (threadIdx.x >> 6);
+  if (t < a.N && sequence_of(a, t) < 0 && (threadIdx.x & 63) == 0) a.tokens[t] = -1, a.logp[t] = 0.f;
+  return true;
+}
+
+// A sequence per block, 5 to 7 us at any size.
+template <typename T> __global__ __launch_bounds__(1024) void k_verify_pick(VerifyArgs a) {
+  if (rows_of_none(a)) return;
+  __shared__ Roots roots;
+  __shared__ Picking sh;
+  const double* sums_of = a.sums + (long)blockIdx.x * 2 * a.n_parts;
+  const double ahead = threadIdx.x < 64 && (int)threadIdx.x < a.n_parts ? sums_of[threadIdx.x] : 0.0;      // beside the choice
+  const Choice ch = a.choice[blockIdx.x];
+  if (ch.token != -2) return;
+  roots.fill();
+  __syncthreads();
+  pick<T>(a, ch, sums_of, ahead, roots, sh);
+}
+
+// A sequence per block. Where no draft distribution is subtracted, the chosen row's sums are those of its parts, but for the
+// part of a draft that counts 0: written here, so that only a call with draft distributions takes a launch for them (48
+// sequences, rows of 100003 in bf16: 6.4 us for 4.8 and 10.3 apart). PICK (a call without them): the token too (10.0 us; 6.6 and 5.4
+// apart, and a launch).
+template <typename T, bool PICK> __global__ __launch_bounds__(1024) void k_verify_judge(VerifyArgs a) {
+  if (PICK && rows_of_none(a)) return;
+  __shared__ Roots roots;
+  __shared__ Judging sh;
+  __shared__ Picking picking;
+  __shared__ double sums[2][16];
+  roots.fill();
+  __syncthreads();
+  const int b = blockIdx.x;
+  judge<T>(a, b, true, roots, sh);
+  __syncthreads();
+  const Choice ch = sh.choice;
+  if (ch.token != -2 || ch.zq > 0.0) return;
+  const int own = ch.drop >= 0 && ch.drop < a.V ? ch.drop / PART : -1;
+  const Part* p = a.parts + (long)ch.row * a.n_parts;
+  double* to = a.sums + (long)b * 2 * a.n_parts;
+  for (int i = threadIdx.x; i < a.n_parts; i += 1024)
+    if (i != own) to[i] = to[a.n_parts + i] = p[i].z / ch.zp * prob_of(((double)p[i].m - ch.mp) * ch.scale, roots);
+  if (own >= 0) sum_part<T>(a, ch, b, own, roots, sums);
+  if constexpr (PICK) {
+    __syncthreads();
+    const double ahead = threadIdx.x < 64 && (int)threadIdx.x < a.n_parts ? to[threadIdx.x] : 0.0;
+    pick<T>(a, ch, to, ahead, roots, picking);
+  }
 }
 
 int n_parts(int V) { return cdiv(V, PART); }
@@ -494,13 +514,18 @@ size_t sums_bytes(const dm_verify_args* a) { return align256((size_t)2 * a->B * 
 
 template <typename T> void run_verify(const VerifyArgs& p, hipStream_t s) {
   hipLaunchKernelGGL(k_verify_parts<T>, dim3(p.n_parts, p.N, p.y ? 2 : 1), dim3(256), 0, s, p);
-  if (p.y && (long)p.n_parts * p.B <= 256) {      // a block per CU
+  const dim3 picks(p.B + cdiv(p.N, 16));
+  if (!p.y) {
+    hipLaunchKernelGGL((k_verify_judge<T, true>), picks, dim3(1024), 0, s, p);
+    return;
+  }
+  if ((long)p.n_parts * p.B <= 256) {      // a block per CU
     hipLaunchKernelGGL((k_verify_sums<T, true>), dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
   } else {
-    hipLaunchKernelGGL(k_verify_judge<T>, dim3(p.B), dim3(1024), 0, s, p);
-    if (p.y) hipLaunchKernelGGL((k_verify_sums<T, false>), dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((k_verify_judge<T, false>), dim3(p.B), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((k_verify_sums<T, false>), dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
   }
-  hipLaunchKernelGGL(k_verify_pick<T>, dim3(p.B + cdiv(p.N, 16)), dim3(1024), 0, s, p);
+  hipLaunchKernelGGL(k_verify_pick<T>, picks, dim3(1024), 0, s, p);
 }
 
 }  // namespace

@@ -304,8 +304,8 @@ DM_DEV long scores_at(const PagedArgs& a, const Seq& s, int c) {
 // exchanges, and the probabilities are already the operand of the product with V, whose columns come from LDS transposed. K goes
 // to the matrix cores straight from memory. The next step's rows of K and V are on their way in registers meanwhile.
 // Bound by the rows' bytes: 64 sequences of 100 to 8192 rows of 64 on 16 key heads (484 MB) 90 us, 5.4 TB/s, of random pages of
-// 64 rows; more blocks per CU or more rows on their way bring nothing. One token over 1024 rows 6 us, most of it latency: the
-// plan, the table, the rows.
+// 64 rows; more blocks per CU or more rows on their way bring nothing. One token over 1024 rows 10 us in one piece per head, 6 in
+// eight, most of it latency: the plan, the table, the rows.
 // KEEP: the scores are kept for the weights (of the lanes behind the last query row too, which work on that one again: a store
 // that some lanes skip would have the next rows' loads wait for it, 276 instead of 273 us). 32 sequences of 3000 to 16384 rows of
 // 128 on 8 key heads, 1.28 GB: 229 us without, 273 with; computing the scores again costs 172.
@@ -900,7 +900,7 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
 }
 
 // The pieces of a query tile, in their order: 16 threads a query row. Bound by latency: the plan, the maxima, then eight pieces'
-// columns at a time (one token in 16 pieces 4 us, 64 sequences 6, 8192 query rows of 8 key heads 11).
+// columns at a time (one token in eight pieces 4 us, 64 sequences 6, 8192 query rows of 8 key heads 11).
 template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
   const int c = blockIdx.x % a.h_kv;
   Item it = find_item<ROWS, false>(a, blockIdx.x / a.h_kv);
@@ -1366,7 +1366,7 @@ long most_tiles(const dm_paged_args* a) {
   return (a->window ? std::min(rows, (long)a->window + a->n_tokens + TILE_K) : rows) / TILE_K + 1;
 }
 // The plan's numbers: about `blocks` blocks over the key heads, but no more than there can be: blocks without a piece cost their
-// look at the plan (one token over 1024 rows: 8.2 us with 8 blocks per CU wanted, 7.0 with 5, 6.0 with those that there can be).
+// look at the plan (one token over 1024 rows in pieces: 8.2 us with 8 blocks per CU wanted, 7.0 with 5, 6.0 with those that there can be).
 int wanted(const dm_paged_args* a, int blocks, long tiles, int least) {
   return (int)std::max(1L, std::min((long)cdiv(blocks, a->h_kv), tiles * ((most_tiles(a) + least - 1) / least)));
 }
