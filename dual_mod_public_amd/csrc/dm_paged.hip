@@ -22,6 +22,7 @@ namespace {
 constexpr float INF = __builtin_inff(), NAN_ = __builtin_nanf("");
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int CUS = 256;
+constexpr float LAST_CACHE = 1 << 28;      // bytes
 constexpr int TILE_Q = 16;      // query rows of a tile
 constexpr int TILE_K = 64;      // cached rows that the plan counts in
 
@@ -67,6 +68,7 @@ struct Item {
   int b = -1;      // -1: there is none
   Seq s;
   int tile, piece, pieces, slot;   // slot of the query tile's piece 0 in the workspace, where pieces > 1
+  float tiles_k;                   // tiles of cached rows of all sequences
 };
 
 // The sum over the lanes up to this one, by moves inside the rows of 16 lanes and broadcasts of the rows' last lanes.
@@ -88,14 +90,16 @@ template <int ROWS, bool PIECES> DM_DEV Item find_item(const PagedArgs& a, int a
   const int lane = threadIdx.x & 63;
   auto tiles_q = [&](const Seq& s) { return ROWS ? (s.n * a.g + ROWS - 1) / (ROWS ? ROWS : 1) : (s.n > 0); };
   Seq s;
-  float cost = 0.f;
+  Item it;
+  float cost = 0.f, tiles_k = 0.f;
   for (int b = lane; b < a.B; b += 64) {
     s = Seq(a, b);
+    tiles_k += (float)s.tiles_k(a);
     cost += (float)tiles_q(s) * (float)s.tiles_k(a);
   }
+  it.tiles_k = wave_sum(tiles_k);
   cost = wave_sum(cost) * (1.f + 1e-4f);                   // 1024 + 6 additions of half a step, 2^-24, each
   const int each = max(a.least, (int)fminf(ceilf(cost / (float)a.want), 1e9f));   // tiles of cached rows per piece
-  Item it;
   int done = 0, slots = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
@@ -303,12 +307,13 @@ DM_DEV long scores_at(const PagedArgs& a, const Seq& s, int c) {
 // joined through LDS. S^T = K Q^T rather than S = Q K^T: a lane then holds scores of one query row only, the maximum needs two
 // exchanges, and the probabilities are already the operand of the product with V, whose columns come from LDS transposed. K goes
 // to the matrix cores straight from memory. The next step's rows of K and V are on their way in registers meanwhile.
-// Bound by the rows' bytes: 64 sequences of 100 to 8192 rows of 64 on 16 key heads (484 MB) 90 us, 5.4 TB/s, of random pages of
+// Bound by the rows' bytes: 64 sequences of 100 to 8192 rows of 64 on 16 key heads (484 MB) 82.5 us, 5.9 TB/s, of random pages of
 // 64 rows; more blocks per CU or more rows on their way bring nothing. One token over 1024 rows 10 us in one piece per head, 6 in
 // eight, most of it latency: the plan, the table, the rows.
 // KEEP: the scores are kept for the weights (of the lanes behind the last query row too, which work on that one again: a store
 // that some lanes skip would have the next rows' loads wait for it, 276 instead of 273 us). 32 sequences of 3000 to 16384 rows of
-// 128 on 8 key heads, 1.28 GB: 229 us without, 273 with; computing the scores again costs 172.
+// 128 on 8 key heads, 1.28 GB: 229 us without, 273 with (267 past the last cache): their 40 MB are written at the memory's
+// pace between reads, 234 where they stay in L2. Computing the scores again costs 172.
 template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile<T, DH>::WAVES)) void k_paged_read(PagedArgs a) {
   using C = Tile<T, DH>;
   constexpr int VBYTES = C::KT * C::LDV * (int)sizeof(T), OBYTES = TILE_Q * DH * 4;
@@ -379,7 +384,16 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
 #pragma unroll
     for (int t = 0; t < 2; ++t) pages[t] = page_of(a, table, r0 + 16 * t, r0 + 16 * t < t_high && r0 + 16 * t + 16 > t_low, bad);
   };
-  auto load = [&](int r0) {
+  // Rows that one tile reads pass the last cache by where the call's are more than it holds: 64 sequences of 2048 rows of 64 on 16
+  // key heads (512 MiB) 81 us, 6.6 TB/s, instead of 92.6; 32 of 8192 rows of 128 on 8 (1 GiB) 168 instead of 197. Fewer rows find
+  // themselves there where they were read before (24 sequences of 50 to 4001 rows 21 us, past it 25.8), those of two tiles are
+  // read by the second one there or in L2 (32 sequences of 4096 rows, two tiles, 121 us, past it 154).
+  const bool stream = rows <= TILE_Q && uniform(it.tiles_k * (2.f * TILE_K * DH * sizeof(T)) * a.h_kv > LAST_CACHE);
+  auto load_rows = [&](int r0, auto passing) {
+    auto ld = [&](const T* p) {
+      if constexpr (passing) return __builtin_nontemporal_load((const __attribute__((address_space(1))) u32x4*)p);
+      else return ld_global<u32x4>(p);
+    };
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int r = r0 + 16 * t;
@@ -388,12 +402,23 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
       const T* K = (const T*)a.K + page * a.k_page + off;
       const T* Vp = (const T*)a.V + page * a.v_page + off;
 #pragma unroll
-      for (int i = 0; i < C::NF; ++i) kf[t][i] = ld_global<u32x4>(K + col * DH + i * 4 * C::V + grp * C::V);
+      for (int i = 0; i < C::NF; ++i) kf[t][i] = ld(K + col * DH + i * 4 * C::V + grp * C::V);
 #pragma unroll
       for (int i = 0; i < C::NV / 2; ++i) {
         const int v = i * 64 + lane;
-        vf[t * (C::NV / 2) + i] = ld_global<u32x4>(Vp + v * C::V);
+        vf[t * (C::NV / 2) + i] = ld(Vp + v * C::V);
       }
+    }
+  };
+  auto load = [&](int r0) {
+    if (stream) {      // (the compiler would make one of both sides but for what differs before and behind the loads)
+      asm volatile("; rows pass the last cache by");
+      load_rows(r0, std::true_type());
+      asm volatile("; passed");
+    } else {
+      asm volatile("; rows may stay in the last cache");
+      load_rows(r0, std::false_type());
+      asm volatile("; stayed");
     }
   };
   int r0 = k0 + C::KT * wave;

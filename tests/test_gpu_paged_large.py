@@ -122,6 +122,20 @@ def test_a_sequence_of_millions_of_rows():
     near(w, add, bw + 2.0 ** -24 * add, "weights")
 
 
+@pytest.mark.parametrize("dh,dtype", [(128, torch.bfloat16), (64, torch.float32), (128, torch.float32)])
+def test_more_rows_than_the_last_cache_holds(dh, dtype):
+    lengths, counts = [600001, 450000, 77], [1, 2, 3]
+    s = make(lengths, counts, 2, 1, dh, 1024, dtype, seed=26)
+    assert s["K"].numel() * s["K"].element_size() * 2 > 1 << 28
+    d = {m: t.to(DEV) for m, t in s.items()}
+    w = torch.zeros(3, 1, s["table"].shape[1] * 1024, device=DEV)
+    r = paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], d["starts"], weights=w)
+    o, lse, add, bo, bl, bw = ref.attention(s["q"], s["K"], s["V"], s["table"], lengths, counts)
+    near(r.o, o, bo, "o")
+    near(r.lse, lse, bl, "lse")
+    near(w, add, bw + 2.0 ** -24 * add, "weights")
+
+
 def test_rows_of_logits_far_apart():
     """A row stride of 2^27 elements: rows past 2^32 elements."""
     counts, V = [20, 3, 17], 5000
