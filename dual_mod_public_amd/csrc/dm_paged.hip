@@ -380,7 +380,7 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
   bool bad = s.bad, odd = false;
   u32x4 kf[2][C::NF], vf[C::NV];
   int pages[2];
-  auto look_up = [&](int r0) {
+  auto look_up = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) pages[t] = page_of(a, table, r0 + 16 * t, r0 + 16 * t < t_high && r0 + 16 * t + 16 > t_low, bad);
   };
@@ -389,7 +389,7 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
   // themselves there where they were read before (24 sequences of 50 to 4001 rows 21 us, past it 25.8), those of two tiles are
   // read by the second one there or in L2 (32 sequences of 4096 rows, two tiles, 121 us, past it 154).
   const bool stream = rows <= TILE_Q && uniform(it.tiles_k * (2.f * TILE_K * DH * sizeof(T)) * a.h_kv > LAST_CACHE);
-  auto load_rows = [&](int r0, auto passing) {
+  auto load_rows = [&](int r0, auto passing) __attribute__((always_inline)) {
     auto ld = [&](const T* p) {
       if constexpr (passing) return __builtin_nontemporal_load((const __attribute__((address_space(1))) u32x4*)p);
       else return ld_global<u32x4>(p);
@@ -410,7 +410,7 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
       }
     }
   };
-  auto load = [&](int r0) {
+  auto load = [&](int r0) __attribute__((always_inline)) {
     if (stream) {      // (the compiler would make one of both sides but for what differs before and behind the loads)
       asm volatile("; rows pass the last cache by");
       load_rows(r0, std::true_type());
