@@ -176,7 +176,10 @@ template <typename T> __global__ __launch_bounds__(256) void k_paged_write(Paged
 
 // ---- the read ----------------------------------------------------------------------------------
 template <typename T, int DH> struct Tile {
-  static constexpr int KT = 32;                                   // cached rows of a wave's step
+  // tiles of 16 cached rows in a wave's step (fp32 rows of 128 two at a time leave room for one wave per SIMD: 16 tokens over 4096
+  // rows on 8 key heads 129 us instead of 96, 512 tokens over 8192 rows 418 instead of 343)
+  static constexpr int NT = sizeof(T) == 4 && DH == 128 ? 1 : 2;
+  static constexpr int KT = 16 * NT;
   static constexpr int V = 16 / (int)sizeof(T);
   static constexpr int LDV = DH + (sizeof(T) == 2 ? 16 : 4);      // 8 rows (fp32: 4 groups) fill the banks once
   static constexpr int NF = DH * (int)sizeof(T) / 64;             // 16-byte loads of a lane for 16 rows in fragments
@@ -185,7 +188,7 @@ template <typename T, int DH> struct Tile {
   static constexpr int NDT = DH / 16;
   // per SIMD at least: what the registers of rows on their way leave (bf16 rows of 64: 105 registers, 4 waves fit; asked for 4 the
   // compiler keeps fewer loads on their way: 64 sequences of 100 to 8192 rows 97 us instead of 92)
-  static constexpr int WAVES = sizeof(T) == 2 ? 3 : 3 - DH / 64;
+  static constexpr int WAVES = sizeof(T) == 2 || DH == 128 ? 3 : 2;
 };
 
 // S^T[16 cached rows][16 query rows] += K Q^T for one 16-byte chunk per lane of each: bf16 lane l holds columns
@@ -268,13 +271,13 @@ template <int N> DM_DEV bf16x8 to_bf16x8(const float (&p)[N], int at) {
   for (int i = 0; i < 8; ++i) r[i] = (bf16)p[at + i];
   return r;
 }
-template <typename T, int LDV> DM_DEV floatx4 mma_values(const T* Vs, const float (&p)[8], floatx4 acc) {
+template <typename T, int LDV, int N> DM_DEV floatx4 mma_values(const T* Vs, const float (&p)[N], floatx4 acc) {
   if constexpr (sizeof(T) == 2) {
     return Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, values_fragment((const bf16*)Vs, LDV)), to_bf16x8(p, 0), acc);
   } else {
     const int lane = threadIdx.x & 63, grp = lane >> 4, s = lane & 15;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc = Mfma<float>::mma(to_f(Vs[(16 * (i >> 2) + 4 * grp + (i & 3)) * LDV + s]), p[i], acc);
+    for (int i = 0; i < N; ++i) acc = Mfma<float>::mma(to_f(Vs[(16 * (i >> 2) + 4 * grp + (i & 3)) * LDV + s]), p[i], acc);
     return acc;
   }
 }
@@ -316,6 +319,7 @@ DM_DEV long scores_at(const PagedArgs& a, const Seq& s, int c) {
 // pace between reads, 234 where they stay in L2. Computing the scores again costs 172.
 template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile<T, DH>::WAVES)) void k_paged_read(PagedArgs a) {
   using C = Tile<T, DH>;
+  constexpr int NP = 4 * C::NT;      // scores of a lane in a step
   constexpr int VBYTES = C::KT * C::LDV * (int)sizeof(T), OBYTES = TILE_Q * DH * 4;
   __shared__ __attribute__((aligned(16))) char smem[4 * (VBYTES > OBYTES ? VBYTES : OBYTES)];
   __shared__ float sm[4][TILE_Q], sz[4][TILE_Q];
@@ -378,11 +382,11 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
   const int in_page = (1 << a.page_shift) - 1;
   T* Vs = reinterpret_cast<T*>(smem) + wave * C::KT * C::LDV;
   bool bad = s.bad, odd = false;
-  u32x4 kf[2][C::NF], vf[C::NV];
-  int pages[2];
+  u32x4 kf[C::NT][C::NF], vf[C::NV];
+  int pages[C::NT];
   auto look_up = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) pages[t] = page_of(a, table, r0 + 16 * t, r0 + 16 * t < t_high && r0 + 16 * t + 16 > t_low, bad);
+    for (int t = 0; t < C::NT; ++t) pages[t] = page_of(a, table, r0 + 16 * t, r0 + 16 * t < t_high && r0 + 16 * t + 16 > t_low, bad);
   };
   // Rows that one tile reads pass the last cache by where the call's are more than it holds: 64 sequences of 2048 rows of 64 on 16
   // key heads (512 MiB) 81 us, 6.6 TB/s, instead of 92.6; 32 of 8192 rows of 128 on 8 (1 GiB) 168 instead of 197. Fewer rows find
@@ -395,7 +399,7 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
       else return ld_global<u32x4>(p);
     };
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < C::NT; ++t) {
       const int r = r0 + 16 * t;
       const long page = pages[t];
       const long off = (((long)c << a.page_shift) + (r & in_page)) * DH;
@@ -404,9 +408,9 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
 #pragma unroll
       for (int i = 0; i < C::NF; ++i) kf[t][i] = ld(K + col * DH + i * 4 * C::V + grp * C::V);
 #pragma unroll
-      for (int i = 0; i < C::NV / 2; ++i) {
+      for (int i = 0; i < C::NV / C::NT; ++i) {
         const int v = i * 64 + lane;
-        vf[t * (C::NV / 2) + i] = ld(Vp + v * C::V);
+        vf[t * (C::NV / C::NT) + i] = ld(Vp + v * C::V);
       }
     }
   };
@@ -438,26 +442,29 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
       const int v = i * 64 + lane;
       *reinterpret_cast<u32x4*>(Vs + v / C::VPR * C::LDV + (v % C::VPR) * C::V) = vf[i];
     }
-    float p[8];      // of rows r0 + 16 (i / 4) + 4 grp + i % 4
+    float p[NP];      // of rows r0 + 16 (i / 4) + 4 grp + i % 4
     floatx4 acc[2] = {zero4(), zero4()};
 #pragma unroll
-    for (int i = 0; i < C::NF; ++i) mma_chunks<T>(kf[0][i], kf[1][i], qf[i], acc);
+    for (int i = 0; i < C::NF; ++i) {
+      if constexpr (C::NT == 2) mma_chunks<T>(kf[0][i], kf[1][i], qf[i], acc);
+      else acc[0] = mma_chunk<T>(kf[0][i], qf[i], acc[0]);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = acc[i >> 2][i & 3] * a.scale2;
+    for (int i = 0; i < NP; ++i) p[i] = acc[i >> 2][i & 3] * a.scale2;
     if (masked) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < NP; ++i) {
         const int r = r0 + 16 * (i >> 2) + 4 * grp + (i & 3);
         if (r < low || r >= high) p[i] = -INF;
       }
     }
     float top = p[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, p[i]);
+    for (int i = 1; i < NP; ++i) top = fmaxf(top, p[i]);
     if constexpr (KEEP) {
       float* x = scores + (long)(r0 >> 2) * (4 * rows);
       *reinterpret_cast<floatx4*>(x) = floatx4{p[0], p[1], p[2], p[3]};
-      *reinterpret_cast<floatx4*>(x + 16 * rows) = floatx4{p[4], p[5], p[6], p[7]};
+      if constexpr (C::NT == 2) *reinterpret_cast<floatx4*>(x + 16 * rows) = floatx4{p[4], p[5], p[6], p[7]};
     }
     if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT), look_up(min(r0 + 8 * C::KT, k1));
     top = xor_max<32>(xor_max<16>(top));
@@ -472,7 +479,7 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
     }
     const float ref = m == -INF ? 0.f : m;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < NP; ++i) {
       p[i] = __builtin_amdgcn_exp2f(p[i] - ref);
       z += p[i];
     }
@@ -484,26 +491,26 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
   if (__ballot(odd)) {      // see split_nonfinite
     for (r0 = k0 + C::KT * wave; r0 < k1; r0 += 4 * C::KT) {
       if (r0 >= all_low && r0 + C::KT <= all_high) continue;
-      float read[8];
-      const T* v[8];
+      float read[NP];
+      const T* v[NP];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < NP; ++i) {
         const int r = r0 + 16 * (i >> 2) + 4 * grp + (i & 3);
         read[i] = r < low || r >= high ? 0.f : 1.f;
         v[i] = value_row<T>(a, table, c, r, t_low, t_high, DH);
       }
       for (int d = 0; d < C::NDT; ++d) {
-        float x[8];
+        float x[NP];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = v[i] ? to_f(v[i][16 * d + col]) : 0.f;
+        for (int i = 0; i < NP; ++i) x[i] = v[i] ? to_f(v[i][16 * d + col]) : 0.f;
         floatx4 said = zero4();
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = split_nonfinite(x[i]);
+          for (int i = 0; i < NP; ++i) x[i] = split_nonfinite(x[i]);
           said = Mfma<bf16>::mma(to_bf16x8(x, 0), to_bf16x8(read, 0), said);
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) said = Mfma<float>::mma(split_nonfinite(x[i]), read[i], said);
+          for (int i = 0; i < NP; ++i) said = Mfma<float>::mma(split_nonfinite(x[i]), read[i], said);
         }
 #pragma unroll
         for (int dd = 0; dd < C::NDT; ++dd)
@@ -1013,6 +1020,7 @@ __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
 // 256: 15 us, most of it latency.
 template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_weights(PagedArgs a) {
   using C = Tile<T, DH>;
+  constexpr int KT = 32;      // cached rows of a step
   const int c = uniform(blockIdx.x % a.h_kv), lane = threadIdx.x & 63, grp = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Item it = find_item<0, true>(a, blockIdx.x / a.h_kv);
@@ -1029,11 +1037,11 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
   float* w = a.weights + ((long)it.b * a.h_kv + c) * ((long)a.cols << a.page_shift);
   // Few query rows: each wave takes cached rows of its own; many: the waves share them and take the query tiles in turn
   // (the call above 15 us so, 23 without)
-  __shared__ float part[2][4][C::KT];
+  __shared__ float part[2][4][KT];
   const bool shared = rows > 4 * TILE_Q;
-  const int step = shared ? C::KT : 4 * C::KT, q_first = shared ? TILE_Q * wave : 0, q_step = shared ? 4 * TILE_Q : TILE_Q;
+  const int step = shared ? KT : 4 * KT, q_first = shared ? TILE_Q * wave : 0, q_step = shared ? 4 * TILE_Q : TILE_Q;
   int buf = 0;
-  for (int r0 = k0 + (shared ? 0 : C::KT * wave); r0 < k1; r0 += step, buf ^= 1) {
+  for (int r0 = k0 + (shared ? 0 : KT * wave); r0 < k1; r0 += step, buf ^= 1) {
     u32x4 kf[2][C::NF];
     bool bad = false;
 #pragma unroll
@@ -1047,7 +1055,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
     float sum[2][4] = {};
     // the tokens that read one of these rows; a tile of their query rows is on its way while the one before is used
     const int past = s.len - s.n;
-    const int j0 = max(0, r0 - past + (a.k_rows ? 1 : 0)), j1 = a.window ? min((long)s.n, (long)r0 - past + C::KT - 1 + a.window) : s.n;
+    const int j0 = max(0, r0 - past + (a.k_rows ? 1 : 0)), j1 = a.window ? min((long)s.n, (long)r0 - past + KT - 1 + a.window) : s.n;
     u32x4 qf[C::NF];
     float lse2 = 0.f;
     auto fetch = [&](int rho0) {
@@ -1092,7 +1100,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
     if (shared) {     // (the other buffer's sums are read before the next barrier)
       __syncthreads();
       const int r = r0 + threadIdx.x;
-      if (threadIdx.x < C::KT && r >= t_low && r < t_high)
+      if (threadIdx.x < KT && r >= t_low && r < t_high)
         w[r] += (part[buf][0][threadIdx.x] + part[buf][1][threadIdx.x]) + (part[buf][2][threadIdx.x] + part[buf][3][threadIdx.x]);
     }
   }
