@@ -315,8 +315,8 @@ DM_DEV long scores_at(const PagedArgs& a, const Seq& s, int c) {
 // eight, most of it latency: the plan, the table, the rows.
 // KEEP: the scores are kept for the weights (of the lanes behind the last query row too, which work on that one again: a store
 // that some lanes skip would have the next rows' loads wait for it, 276 instead of 273 us). 32 sequences of 3000 to 16384 rows of
-// 128 on 8 key heads, 1.28 GB: 229 us without, 273 with (267 past the last cache): their 40 MB are written at the memory's
-// pace between reads, 234 where they stay in L2. Computing the scores again costs 172.
+// 128 on 8 key heads, 1.28 GB: 229 us without, 273 with; past the last cache 204 and 266 (of which 5 where they stay in L2,
+// 55 for the 40 MB in memory). Computing the scores again costs 172.
 template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile<T, DH>::WAVES)) void k_paged_read(PagedArgs a) {
   using C = Tile<T, DH>;
   constexpr int NP = 4 * C::NT;      // scores of a lane in a step
