@@ -352,3 +352,65 @@ def test_outputs_in_the_place_of_inputs():
             verify_drafts(kw.pop("logits"), *rest, **kw)
     with torch.no_grad():
         verify_drafts(y, *rest)
+
+
+@pytest.mark.parametrize("h", [4, 16])
+def test_captured_prompts_lookups_and_eviction(h):
+    """Tiles of 128 and of 256 query rows, drafts looked up and an eviction in one graph, replayed with other lengths and starts; two
+    graphs of the same calls in turn, each with workspaces of its own."""
+    B, N, h_kv, dh, page, cols, V, keep = 3, 210, 2, 64, 32, 24, 9000, 100
+    K, Vp = (torch.randn(B * cols + 12 + 4, h_kv, page, dh, device=DEV).bfloat16() for _ in range(2))
+    new_table = torch.arange(B * cols + 4, B * cols + 16, device=DEV, dtype=torch.int32).view(3, 4)
+    s = dict(q=torch.randn(N, h, dh, device=DEV).bfloat16(), table=torch.zeros(B, cols, dtype=torch.int32, device=DEV),
+             lengths=i32(70, 70, 70), starts=i32(0, 70, 140, 210), weights=torch.zeros(B, h_kv, cols * page, device=DEV),
+             x=torch.randn(N, V, device=DEV).bfloat16(), ids=torch.zeros(N, dtype=torch.int64, device=DEV), u=torch.rand(N, 2, device=DEV))
+
+    def run():
+        r = paged.paged_attention(s["q"], K, Vp, s["table"], s["lengths"], s["starts"], window=0, weights=s["weights"], out=out)
+        e = paged.evict_rows(K, Vp, s["weights"], s["table"], s["lengths"], keep, new_table, sinks=2, recent=9)
+        v = verify_drafts(s["x"], s["ids"], s["u"], s["starts"], temperature=0.7)
+        return r.o, r.lse, *e, *v
+
+    def fill(seed):
+        c = torch.Generator().manual_seed(seed)
+        s["table"].copy_(torch.randperm(B * cols + 4, generator=c)[:B * cols].view(B, cols))
+        cuts = sorted(torch.randint(0, N + 1, (B,), generator=c).tolist())
+        s["starts"].copy_(torch.tensor([0] + cuts))
+        s["lengths"].copy_(torch.tensor([max(1, b - a) + int(torch.randint(0, 500, (), generator=c)) for a, b in zip([0] + cuts, cuts)]))
+        s["ids"].copy_(torch.randint(0, V, (N,), generator=c))
+        s["u"].copy_(torch.rand(N, 2, generator=c) * torch.tensor([1e-4, 1.0]))
+        s["weights"].copy_(torch.rand(B, h_kv, cols * page, generator=c))
+        out.fill_(3.0)
+
+    out = torch.empty(N, h, dh, device=DEV, dtype=torch.bfloat16)
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = run()
+        graphs.append((graph, held))
+    for seed in range(1, 7):
+        fill(seed)
+        want = [t.clone() for t in (*run(), s["weights"], K[-12:], Vp[-12:])]
+        n = int(s["starts"][-1])
+        fill(seed)
+        K[-12:], Vp[-12:] = 0, 0
+        graph, held = graphs[seed % 2]
+        graph.replay()
+        torch.cuda.synchronize()
+        rows = torch.arange(4 * page, device=DEV)
+        for i, (a, b) in enumerate(zip((*held, s["weights"]), want)):
+            if i == 1:
+                a, b = a[:n], b[:n]
+            assert torch.equal(a, b), (seed, i)
+        for pool, w in zip((K[-12:], Vp[-12:]), want[-2:]):     # the kept rows; what lies behind them stays
+            for b in range(B):
+                left = int(held[3][b])
+                got, exp = (t[4 * b:4 * b + 4].transpose(0, 1).reshape(h_kv, -1, dh)[:, rows < left] for t in (pool, w))
+                assert torch.equal(got, exp)
