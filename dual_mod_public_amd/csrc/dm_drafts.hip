@@ -247,14 +247,14 @@ template <typename T> struct Residual {
   }
 };
 
-struct Judging {
+struct Deciding {
   Part p[16], q[16];
   bool refused[16];
   Choice choice;
 };
 
 // A block decides over a sequence's rows (a wave each, 16 at a time); writes: and writes what is decided.
-template <typename T> DM_DEV void judge(const VerifyArgs& a, int b, bool writes, const Roots& roots, Judging& sh) {
+template <typename T> DM_DEV void decide(const VerifyArgs& a, int b, bool writes, const Roots& roots, Deciding& sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float temperature = a.temperature[b];
   const Rows rows(a, b);
@@ -338,22 +338,22 @@ template <typename T> DM_DEV void sum_part(const VerifyArgs& a, const Choice& ch
   }
 }
 
-// The sums of r and p over each part of a sequence's chosen row, as in k_verify_parts bound by the exponentials. JUDGE: each block
+// The sums of r and p over each part of a sequence's chosen row, as in k_verify_parts bound by the exponentials. DECIDE: each block
 // decides over the sequence by itself, a launch less (one sequence of 4 drafts 8.5 us, 5.5 and 5.1 apart; 64 of 13 parts 26, 6.4
 // and 8.4 apart).
-template <typename T, bool JUDGE> __global__ __launch_bounds__(1024) void k_verify_sums(VerifyArgs a) {
+template <typename T, bool DECIDE> __global__ __launch_bounds__(1024) void k_verify_sums(VerifyArgs a) {
   const int b = blockIdx.y;
   __shared__ Roots roots;
   __shared__ double sums[2][16];
-  __shared__ Judging sh;
+  __shared__ Deciding sh;
   roots.fill();
   __syncthreads();
-  if constexpr (JUDGE) {
-    judge<T>(a, b, blockIdx.x == 0, roots, sh);
+  if constexpr (DECIDE) {
+    decide<T>(a, b, blockIdx.x == 0, roots, sh);
     __syncthreads();
   }
-  const Choice ch = JUDGE ? sh.choice : a.choice[b];
-  if (ch.token != -2 || (!JUDGE && ch.zq == 0.0)) return;
+  const Choice ch = DECIDE ? sh.choice : a.choice[b];
+  if (ch.token != -2 || (!DECIDE && ch.zq == 0.0)) return;
   sum_part<T>(a, ch, b, blockIdx.x, roots, sums);
 }
 
@@ -482,16 +482,16 @@ template <typename T> __global__ __launch_bounds__(1024) void k_verify_pick(Veri
 // part of a draft that counts 0: written here, so that only a call with draft distributions takes a launch for them (48
 // sequences, rows of 100003 in bf16: 6.4 us for 4.8 and 10.3 apart). PICK (a call without them): the token too (10.0 us; 6.6 and 5.4
 // apart, and a launch).
-template <typename T, bool PICK> __global__ __launch_bounds__(1024) void k_verify_judge(VerifyArgs a) {
+template <typename T, bool PICK> __global__ __launch_bounds__(1024) void k_verify_decide(VerifyArgs a) {
   if (PICK && rows_of_none(a)) return;
   __shared__ Roots roots;
-  __shared__ Judging sh;
+  __shared__ Deciding sh;
   __shared__ Picking picking;
   __shared__ double sums[2][16];
   roots.fill();
   __syncthreads();
   const int b = blockIdx.x;
-  judge<T>(a, b, true, roots, sh);
+  decide<T>(a, b, true, roots, sh);
   __syncthreads();
   const Choice ch = sh.choice;
   if (ch.token != -2 || ch.zq > 0.0) return;
@@ -516,13 +516,13 @@ template <typename T> void run_verify(const VerifyArgs& p, hipStream_t s) {
   hipLaunchKernelGGL(k_verify_parts<T>, dim3(p.n_parts, p.N, p.y ? 2 : 1), dim3(256), 0, s, p);
   const dim3 picks(p.B + cdiv(p.N, 16));
   if (!p.y) {
-    hipLaunchKernelGGL((k_verify_judge<T, true>), picks, dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((k_verify_decide<T, true>), picks, dim3(1024), 0, s, p);
     return;
   }
   if ((long)p.n_parts * p.B <= 256) {      // a block per CU
     hipLaunchKernelGGL((k_verify_sums<T, true>), dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
   } else {
-    hipLaunchKernelGGL((k_verify_judge<T, false>), dim3(p.B), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((k_verify_decide<T, false>), dim3(p.B), dim3(1024), 0, s, p);
     hipLaunchKernelGGL((k_verify_sums<T, false>), dim3(p.n_parts, p.B), dim3(1024), 0, s, p);
   }
   hipLaunchKernelGGL(k_verify_pick<T>, picks, dim3(1024), 0, s, p);

@@ -1,7 +1,7 @@
 """Drafted tokens against the target's probabilities, from given random numbers (dm_verify_drafts).
 
 A speculative step gives the model a chunk of input tokens per sequence: its last token and the drafts after it. Row t of
-the chunk's ``logits`` is the target's distribution after ``ids[t]``, and ``ids[t + 1]`` the draft it judges. With
+the chunk's ``logits`` is the target's distribution after ``ids[t]``, and ``ids[t + 1]`` the draft that it answers. With
 p = softmax(logits / T), q = softmax(draft_logits / T) (or 1 at the draft, where it was looked up rather than drawn), a draft d is accepted
 where ``uniforms[t, 0] q(d) < p(d)``; the first row without an accepted draft gives a token drawn from max(p - q, 0)
 (the last row: from p) by ``uniforms[t, 1]``. The tokens are then distributed as if drawn from p one by one. T = 0 is greedy.

@@ -149,7 +149,7 @@ def test_drafts_decode_what_the_graph_decoder_does():
         pos = torch.cat([torch.arange(c, c + n) for c, n in zip(cached, counts)]).to(DEV)
         starts = i32(0, counts[0], sum(counts))
         logits = dec.extend(ids, pos, pool.table(lengths, 6), i32(*lengths), starts, n_sweeps=max(counts))
-        # judged from each text's last token on; the prompt's rows before it are of no sequence
+        # verified from each text's last token on; the prompt's rows before it are of no sequence
         first = [len(t) - c - 1 for t, c in zip(texts, cached)]
         for b in range(2):
             lo, hi = (first[0], counts[0]) if b == 0 else (counts[0] + first[1], sum(counts))
