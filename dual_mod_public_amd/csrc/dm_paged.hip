@@ -142,35 +142,52 @@ DM_DEV void make_uniform(Item& it) {
 }
 
 // ---- rows into the pages ---------------------------------------------------------------------
-// One thread per 16 bytes of a new token's key or value row (in turns where there are more of them than a launch has
-// threads). Bound by latency at ordinary sizes: 4 us for 200 tokens, 12 for 4096 tokens of 8 key heads of 128 (34 MB moved).
-template <typename T> __global__ __launch_bounds__(256) void k_paged_write(PagedArgs a, int dh) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const int per = dh / V;
-  const long each = (long)a.h_kv * per * 2, all = a.N * each;
-  for (long at = blockIdx.x * 256L + threadIdx.x; at < all; at += gridDim.x * 256L) {
-    const int t = (int)(at / each), rest = (int)(at % each);
-    const bool value = rest >= a.h_kv * per;
-    const int c = (rest / per) % a.h_kv, v = rest % per;
+// A wave per token and 256 of its 16-byte pieces of key and value rows (tokens in turn where there are more of them than a launch
+// has threads). The token's sequence is searched for by all lanes, a 64th at a time. Bound by latency for few tokens (4 us for 200),
+// by the bytes for many: 10000 tokens of 16 key heads of 64 in fp32 (168 MB moved) 30 us, 5.6 TB/s (62 with a thread per 16 bytes,
+// its quotients and a binary search), 4096 tokens of 8 key heads of 128 in bf16 9.7.
+template <typename T> __global__ __launch_bounds__(256) void k_paged_write(PagedArgs a, int dh_shift) {
+  constexpr int V = 16 / (int)sizeof(T), SHIFT = sizeof(T) == 2 ? 3 : 2, EACH = 4;
+  const int lane = threadIdx.x & 63, per_shift = dh_shift - SHIFT, half = a.h_kv << per_shift;
+  const int in_page = (1 << a.page_shift) - 1;
+  for (long at = blockIdx.x * 4L + (threadIdx.x >> 6); at < a.N; at += gridDim.x * 4L) {
+    const int t = uniform((int)at);
     int b = t;
     if (a.starts) {   // the last sequence that starts at t or before
-      int lo = 0, hi = a.B;
-      while (lo + 1 < hi) {
-        const int mid = (lo + hi) / 2;
-        if (a.starts[mid] <= t) lo = mid;
-        else hi = mid;
+      b = 0;
+      for (int n = a.B; n > 1;) {
+        const int step = (n + 63) >> 6, i = lane * step;
+        const uint64_t before = __ballot(i < n && a.starts[b + min(i, n - 1)] <= t);
+        const int k = max(0, (int)__popcll(before) - 1) * step;
+        b += k;
+        n = min(step, n - k);
       }
-      b = lo;
+      b = uniform(b);
     }
     const Seq s(a, b);
     if (s.bad || t < s.first || t >= s.first + s.n) continue;
     const int row = s.len - s.n + (t - s.first);
     const int page = a.table[(long)b * a.cols + (row >> a.page_shift)];
     if (page < 0 || page >= a.n_pages) continue;
-    const T* src = value ? (const T*)a.v_rows + t * a.vr_token + c * a.vr_head : (const T*)a.k_rows + t * a.kr_token + c * a.kr_head;
-    T* dst = value ? (T*)a.V + page * a.v_page : (T*)a.K + page * a.k_page;
-    dst += ((long)c << a.page_shift) * dh + (long)(row & ((1 << a.page_shift) - 1)) * dh;
-    *reinterpret_cast<u32x4*>(dst + v * V) = *reinterpret_cast<const u32x4*>(src + v * V);
+    const T* k = (const T*)a.k_rows + t * a.kr_token;
+    const T* v = (const T*)a.v_rows + t * a.vr_token;
+    T* const K = (T*)a.K + page * a.k_page + ((long)(row & in_page) << dh_shift);
+    T* const Vp = (T*)a.V + page * a.v_page + ((long)(row & in_page) << dh_shift);
+    u32x4 x[EACH];
+    T* to[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = ((int)blockIdx.y * EACH + e) * 64 + lane;
+      const bool value = i >= half;
+      const int j = value ? i - half : i, c = j >> per_shift, at_v = (j & ((1 << per_shift) - 1)) * V;
+      to[e] = nullptr;
+      if (j >= half) continue;
+      x[e] = ld_global<u32x4>((value ? v + c * a.vr_head : k + c * a.kr_head) + at_v);
+      to[e] = (value ? Vp : K) + ((long)c << (a.page_shift + dh_shift)) + at_v;
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+      if (to[e]) *reinterpret_cast<u32x4*>(to[e]) = x[e];
   }
 }
 
@@ -376,8 +393,8 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
     }
   }
 
-  // kept scores of the lane's query row: [cached rows / 4][query rows][4] for each sequence and key head
-  float* scores = a.scores + scores_at(a, s, c) + 4 * rho + grp * (4 * rows);
+  // kept scores of the lane's query row: [cached rows / 32][query rows][32] for each sequence and key head
+  float* scores = a.scores + scores_at(a, s, c) + 32L * rho + 4 * grp;
   const int32_t* table = a.table + (long)it.b * a.cols;
   const int in_page = (1 << a.page_shift) - 1;
   T* Vs = reinterpret_cast<T*>(smem) + wave * C::KT * C::LDV;
@@ -462,9 +479,9 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
 #pragma unroll
     for (int i = 1; i < NP; ++i) top = fmaxf(top, p[i]);
     if constexpr (KEEP) {
-      float* x = scores + (long)(r0 >> 2) * (4 * rows);
+      float* x = scores + (long)(r0 >> 5) * (32L * rows) + (r0 & 31);
       *reinterpret_cast<floatx4*>(x) = floatx4{p[0], p[1], p[2], p[3]};
-      if constexpr (C::NT == 2) *reinterpret_cast<floatx4*>(x + 16 * rows) = floatx4{p[4], p[5], p[6], p[7]};
+      if constexpr (C::NT == 2) *reinterpret_cast<floatx4*>(x + 16) = floatx4{p[4], p[5], p[6], p[7]};
     }
     if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT), look_up(min(r0 + 8 * C::KT, k1));
     top = xor_max<32>(xor_max<16>(top));
@@ -981,9 +998,10 @@ template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k
 DM_DEV float lse_of(float lse) { return lse == -INF ? INF : lse * LOG2E; }
 
 // weights[b, c, r] += the sum over the sequence's query rows of exp(score - lse), from scores that the read kept: a thread
-// takes 4 cached rows and goes over the query rows. 32 sequences of 3000 to 16384 rows, 32 heads on 8 key heads: 15.4 us;
-// 24 chunks of up to 8 tokens over 50 to 4001 rows on 16 heads 6.2 (8.0 without the loads of four query rows at a time, 6.6 and the
-// first call 19.3 with eight).
+// takes 4 cached rows and goes over the query rows; 32 cached rows of one query row lie together, a cache line for both sides (12 chunks
+// of 13 fp32 tokens over 1824 to 6130 rows, 32 heads on 16: 18.8 us, with 4 rows of all query rows together 45.5). 32 sequences of 3000 to 16384 rows, 32 heads on 8 key heads: 14.5 us;
+// 24 chunks of up to 8 tokens over 50 to 4001 rows on 16 heads 5.8 (four query rows on their way; with one 1.8 more, with eight the
+// first call 4 more).
 __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
   constexpr int AT_ONCE = 4;      // query rows on their way
   const int c = uniform(blockIdx.x % a.h_kv);
@@ -1001,7 +1019,7 @@ __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
   for (int r = k0 + 4 * threadIdx.x; r < k1; r += 1024) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     const int rows = s.n * a.g;
-    const float* x = a.scores + scores_at(a, s, c) + (long)r * rows;
+    const float* x = a.scores + scores_at(a, s, c) + (long)(r >> 5) * (32L * rows) + (r & 31);
     const float* lse = a.lse + (long)s.first * a.h + c * a.g;
     int j = 0, i = 0;      // the query row's token and head
     for (int rho = 0; rho < rows; rho += AT_ONCE) {
@@ -1010,7 +1028,7 @@ __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
       int token[AT_ONCE];
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
-        v[u] = *reinterpret_cast<const floatx4*>(x + 4 * min(rho + u, rows - 1));
+        v[u] = *reinterpret_cast<const floatx4*>(x + 32L * min(rho + u, rows - 1));
         lse2[u] = lse[(long)min(j, s.n - 1) * a.h + i];
         token[u] = j;
         if (++i == a.g) i = 0, ++j;
@@ -1574,10 +1592,10 @@ int dm_paged_write(const dm_paged_args* a, void* stream) {
   const int rc = check_paged(a, true);
   if (rc || a->n_tokens == 0) return rc;
   const PagedArgs p = paged(a);
-  const long n = (long)a->n_tokens * a->h_kv * 2 * (a->dh * (long)esz(a->dtype) / 16);
-  const dim3 grid((unsigned)std::min((n + 255) / 256, 1L << 20));
-  if (a->dtype == DM_BF16) hipLaunchKernelGGL(k_paged_write<bf16>, grid, dim3(256), 0, S(stream), p, a->dh);
-  else hipLaunchKernelGGL(k_paged_write<float>, grid, dim3(256), 0, S(stream), p, a->dh);
+  const int pieces = a->h_kv * 2 * (a->dh * (int)esz(a->dtype) / 16);      // 16 bytes each, of a token
+  const dim3 grid((unsigned)std::min(cdiv(a->n_tokens, 4), 1 << 20), cdiv(pieces, 256));
+  if (a->dtype == DM_BF16) hipLaunchKernelGGL(k_paged_write<bf16>, grid, dim3(256), 0, S(stream), p, log2_of(a->dh));
+  else hipLaunchKernelGGL(k_paged_write<float>, grid, dim3(256), 0, S(stream), p, log2_of(a->dh));
   DM_HIP(hipGetLastError());
   return DM_OK;
 }
