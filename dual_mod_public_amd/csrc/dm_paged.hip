@@ -998,10 +998,10 @@ template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k
 DM_DEV float lse_of(float lse) { return lse == -INF ? INF : lse * LOG2E; }
 
 // weights[b, c, r] += the sum over the sequence's query rows of exp(score - lse), from scores that the read kept: a thread
-// takes 4 cached rows and goes over the query rows; 32 cached rows of one query row lie together, a cache line for both sides (12 chunks
-// of 13 fp32 tokens over 1824 to 6130 rows, 32 heads on 16: 18.8 us, with 4 rows of all query rows together 45.5). 32 sequences of 3000 to 16384 rows, 32 heads on 8 key heads: 14.5 us;
-// 24 chunks of up to 8 tokens over 50 to 4001 rows on 16 heads 5.8 (four query rows on their way; with one 1.8 more, with eight the
-// first call 4 more).
+// takes 4 cached rows and goes over the query rows; 32 cached rows of one query row lie together, a cache line for both sides (12
+// chunks of 13 fp32 tokens over 1824 to 6130 rows, 32 heads on 16: 18.8 us, with 4 rows of all query rows together 45.5). 32
+// sequences of 3000 to 16384 rows, 32 heads on 8 key heads: 14.5 us; 24 chunks of up to 8 tokens over 50 to 4001 rows on 16
+// heads 5.8 (four query rows on their way; with one 1.8 more, with eight the other call 4 more).
 __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
   constexpr int AT_ONCE = 4;      // query rows on their way
   const int c = uniform(blockIdx.x % a.h_kv);
@@ -1444,7 +1444,9 @@ constexpr int WEIGHT_BLOCKS = 8 * CUS;
 // In one piece, with no join, while a tile's keys take no more than 128 KiB, or 256 with blocks for half of the CUs (a call / its
 // kernels in a graph, pieces -> whole: one token, 16 heads of 64, 256 rows 17.1 / 8.9 -> 14.2 / 6.4 us, 512 rows 17.3 / 9.2 ->
 // 14.4 / 7.6, 1024 rows 17.2 / 9.1 -> 14.3 / 9.8, 2048 rows 17.0 / 9.5 -> 14.5 / 14.3; 8 tokens over 2048 rows 23.4 / 24.0 ->
-// 20.4 / 21.0; 7 chunks of 65 fp32 tokens, 8 heads of 64 on 4, over 1024 rows 43 -> 34).
+// 20.4 / 21.0; 7 chunks of 65 fp32 tokens, 8 heads of 64 on 4, over 1024 rows 43 -> 34). The larger tiles: up to 512 rows with
+// blocks for half of the CUs (16 chunks of 64 tokens, 8 heads of 64, over 128, 512 and 1024 rows 21.9 -> 17.6, 21.6 -> 16.8 and
+// 22.3 -> 24.9; 33 of 100 tokens, 16 heads of 128, 43 -> 33, 63 -> 54.5 and 106 -> 92; one of 1024 rows among 16 of 70 21 -> 33.6).
 bool in_one_piece(const dm_paged_args* a) {
   const long bytes = (most_tiles(a) - 1) * TILE_K * a->dh * (long)esz(a->dtype);
   return bytes <= (query_tiles(a, TILE_Q) * a->h_kv >= CUS / 2 ? 256 << 10 : 128 << 10);
@@ -1455,7 +1457,9 @@ struct Form {
 Form form_of(const dm_paged_args* a) {
   const int64_t mean = (int64_t)a->n_tokens * (a->h / a->h_kv) / a->B;
   if (a->dtype != DM_BF16 || mean <= 2 * TILE_Q) return {TILE_Q, 5 * CUS, in_one_piece(a) ? (int)most_tiles(a) : 2};
-  return mean <= 512 ? Form{128, 2 * CUS, 2} : Form{256, CUS, 2};
+  Form f = mean <= 512 ? Form{128, 2 * CUS, 2} : Form{256, CUS, 2};
+  if (most_tiles(a) <= 9 && query_tiles(a, f.rows) * a->h_kv >= CUS / 2) f.least = (int)most_tiles(a);
+  return f;
 }
 // The scores of a call with weights are kept where they take no more room than the pages' keys; else they are computed
 // again from the keys.

@@ -370,3 +370,13 @@ def test_many_sequences_and_key_heads():
         o, lse, _, bo, bl, _ = ref.attention(part["q"], part["K"], part["V"], part["table"], [3], [1])
         near(r.o[b:b + 1, i.to(DEV)], o, bo, "o")
         near(r.lse[b:b + 1, i.to(DEV)], lse, bl, "lse")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("dh,page,h,h_kv", [(64, 64, 2, 2), (128, 16, 4, 1)])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1], [6, 3, 0, 9], [150, 2, 90, 40]])
+@pytest.mark.parametrize("with_self,window", [(False, 0), (True, 0), (True, 1301), (False, 700)])
+def test_sequences_in_pieces(dtype, dh, page, h, h_kv, counts, with_self, window):
+    """Tables of more rows than a tile reads in one piece."""
+    s = make([1500, 3, 701, 2303], counts, h, h_kv, dh, page, DT[dtype], seed=sum(counts) + window, cols=-(-4096 // page))
+    check(s, counts, with_self, window)
