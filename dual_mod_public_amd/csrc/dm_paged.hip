@@ -6,8 +6,8 @@
 // the g = h / h_kv heads that share the key head, token by token, in tiles of TILE_Q.
 //
 // How the work is split is decided on the device, from the lengths (a captured call is replayed with other ones): every
-// kernel derives the same plan from them (Plan), in which a sequence's rows are cut into as many pieces as bring the
-// whole call to about `want` pieces. Partial results of a query tile (unnormalised sums with their maximum) wait in the
+// kernel derives the same plan from them (find_item), in which a sequence's rows are cut into as many pieces as bring the
+// whole call to about `want` pieces (one each where they are few). Partial results of a query tile (unnormalised sums with their maximum) wait in the
 // workspace and k_paged_join adds them in the order of the pieces, so a call's results repeat bit for bit.
 #include "dm_common.h"
 #include "dm_error.h"
@@ -1258,8 +1258,8 @@ DM_DEV uint32_t weight_order(float x) {
 // (a histogram over the rows that agree so far), then the rows in order: those above it, and of those equal to it the first.
 // A thread takes 4 rows in turn; the first KEYS * 4096 rows' weights stay in registers. Eight histograms, by lane, since weights
 // share their first bits; one set for each pass, cleared before the first. Bound by its passes'
-// latencies (one sequence of 2304 rows and 16 heads 8.4 us, 32 of 3000 to 16384 rows and 8 heads 15.3; with scans by shuffles, one set of histograms and a sum over
-// the waves' totals in each thread 15.7 and 22.4).
+// latencies (one sequence of 2304 rows and 16 heads 8.4 us, 32 of 3000 to 16384 rows and 8 heads 15.3; with scans by shuffles,
+// one set of histograms and a sum over the waves' totals in each thread 15.7 and 22.4).
 constexpr int KEYS = 4, COPIES = 8, COPY = 256 + 8;      // a copy's first banks lie 8 behind the one's before
 struct Selection {
   int hist[4][COPIES * COPY];

@@ -623,9 +623,9 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
  * v_page elements apart, 16-byte aligned; page a power of two, 16..DM_PAGE_MAX); row r of sequence b lies in page
  * table[b, r / page] (int32 [B, table_cols], unused entries anything). lengths [B]: cached rows, the new tokens' among
  * them; starts [B + 1]: the new tokens starts[b] .. starts[b + 1] - 1 (0 or more) of sequence b, whose token j has row
- * lengths[b] - n + j; NULL: one token per sequence, none where lengths[b] is 0. All three lie on the device and may change between replays of a
- * captured call. Tokens of no sequence (behind starts[B]) are neither read nor written,
- * nor are their rows of o and lse.
+ * lengths[b] - n + j; NULL: one token per sequence, none where lengths[b] is 0. All three lie on the device and may change
+ * between replays of a captured call. Tokens of no sequence (behind starts[B]) are neither read nor written, nor are their
+ * rows of o and lse.
  * starts do not descend. A sequence that its table does not hold (lengths[b] > table_cols * page, or less than its new tokens),
  * or one that reads a page outside [0, n_pages), gets NaN; what such a page would be written is left out. weights of the first
  * kind of sequence stay as they are, of the second they become NaN.
@@ -639,7 +639,8 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
  *   storage dtype, lse [n_tokens, h] fp32, both contiguous.
  *   weights (fp32 [B, h_kv, table_cols * page], may be NULL): weights[b, c, r] += the sum over b's new tokens and the heads
  *   of c of e^(s_r - lse), for the rows that are read. One writer per weight, in a fixed order.
- * Workspace: dm_paged_workspace_bytes(a) (from the sizes and whether there are weights), 16-byte aligned, not shared by calls that may overlap.
+ * Workspace: dm_paged_workspace_bytes(a) (from the sizes and whether there are weights; none where rows are few), 16-byte
+ * aligned, not shared by calls that may overlap.
  * At most DM_PAGED_ROWS rows per sequence, n_tokens * h at most DM_PAGED_TOKENS, B * h_kv at most DM_PAGED_HEADS. */
 #define DM_PAGE_MAX 1024
 #define DM_PAGED_ROWS (1 << 26)
@@ -690,8 +691,8 @@ int dm_paged_evict(const dm_evict_args* a, void* stream);
  *   temperature[b] = 0: accepted where the draft is the first of the largest logits, which is the token otherwise.
  * tokens [rows]: the accepted drafts and the new token, each at the row it was predicted by; -1 behind them, in rows of no
  * sequence and where the row that ends the sequence is no distribution (a NaN, +inf, nothing but -inf; greedy: a NaN, nothing but
- * -inf; a temperature that is negative or not finite). accepted [B]: drafts accepted. logp [rows]: the tokens' target log probabilities (at T = 1 where T is 0), 0 where there is
- * none, NaN where there is no distribution. A draft outside [0, cols) is not accepted. Probabilities, sums and places in 64 bits.
+ * -inf; a temperature that is negative or not finite). accepted [B]: drafts accepted. logp [rows]: the tokens' target log
+ * probabilities (at T = 1 where T is 0), 0 where there is none, NaN where there is no distribution. A draft outside [0, cols) is not accepted. Probabilities, sums and places in 64 bits.
  * At most 65535 rows and sequences. */
 typedef struct dm_verify_args {
   int32_t dtype, rows, cols, B;
