@@ -77,7 +77,7 @@ class PagedTape:
         K, V = (torch.empty(h, N, dh, device=self.device, dtype=self.dtype) for _ in range(2))
         nb = L.lib().dm_refine_kv_workspace_bytes(conf, N)
         ws = torch.empty(nb, device=self.device, dtype=torch.uint8)
-        if n_sweeps > 1:     # the first sweep reads the chunk's raw rows
+        if cache[-1] is not None:     # chunks: the first sweep, which may be the only one, reads their raw rows
             paged_write(k_self, v_self, *cache)
         for i in range(n_sweeps):
             o = paged_attention(q, *cache, k_self=k_self, v_self=v_self, window=self.window,
