@@ -633,7 +633,8 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
  * dm_paged_write: the tokens' rows k_rows, v_rows [n_tokens, h_kv, dh] (any token and head strides) into the pages.
  * dm_paged_attention: for query head a of key head a / (h / h_kv) and a token with row p, over the rows r <= p with
  *   r > p - window (window 0: all),   s_r = scale q . K[r],  lse = log sum e^s,  o = sum e^(s - lse) V[r]
- *   (fp32; bf16: the probabilities rounded to bf16 before the product with V). With k_rows, v_rows: r < p, and the token's own
+ *   (fp32; bf16: before the product with V the probabilities keep 2^-15 of themselves, in a call whose sequences have more than
+ *   32 query rows per key head, n_tokens h / (B h_kv), 2^-8: rounded to bf16). With k_rows, v_rows: r < p, and the token's own
  *   pair takes the place of row p (the raw self pair of dm_attend_one; row p itself is not read). Rows that a token does
  *   not read do not reach its result, whatever they hold; a token that reads nothing: o 0, lse -inf. o [n_tokens, h, dh]
  *   storage dtype, lse [n_tokens, h] fp32, both contiguous.

@@ -1,0 +1,66 @@
+"""The paged operators' results in bits and at odd values, against their definitions in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from dual_mod_public_amd import _lib as L
+from dual_mod_public_amd import paged
+from tests import paged_reference as ref
+from tests.hip_helpers import DEV
+from tests.test_gpu_paged import dev, make, near
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    L.load()
+
+
+def bounds_without_rounded_probabilities(s, lengths, counts, pair):
+    """(o, its bound) where probabilities keep 16 bits. One of two bf16 parts: the first is p cut to 8 bits, what is left is below
+    2^-7 p and rounded by at most 2^-8 of that, or 2^-24 p where it is less. (ref.attention counts 2^-8 for a probability; the share
+    that it multiplies is what the magnitudes of the values give.)"""
+    k, v = (s["k"], s["v"]) if pair else (None, None)
+    o, _, _, bo, _, _ = ref.attention(s["q"], s["K"], s["V"], s["table"], lengths, counts, k, v)
+    share = ref.attention(s["q"], s["K"], s["V"].abs(), s["table"], lengths, counts, k, None if v is None else v.abs())[0]
+    return o, bo + share * (2.0 ** -15 + 2.0 ** -24 - 2.0 ** -8)
+
+
+@pytest.mark.parametrize("dh,page,h,h_kv", [(64, 64, 4, 4), (128, 16, 4, 1), (64, 16, 8, 2)])
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("cols", [None, 1024])
+def test_probabilities_of_few_query_rows_keep_16_bits(dh, page, h, h_kv, new, pair, cols):
+    """Outputs whose terms cancel show a probability's rounding: it is relative to the terms. In one piece and in several."""
+    lengths = [5, 17, 40, 64, 100, 300, 1100]
+    counts = [new] * len(lengths)
+    s = make(lengths, counts, h, h_kv, dh, page, torch.bfloat16, seed=dh + h, cols=cols)
+    s["q"] *= 0.25
+    o, bound = bounds_without_rounded_probabilities(s, lengths, counts, pair)
+    d = dev(s)
+    kw = dict(k_self=d["k"], v_self=d["v"]) if pair else {}
+    near(paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], d["starts"], **kw).o, o, bound, "o")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("new", [1, 3, 90, 600])
+def test_infinite_values_that_are_read(dtype, dh, new):
+    """An infinite value of a row that all tokens read makes its column infinite, in steps without a mask too, and no other one."""
+    lengths, counts = [700 + new], [new]
+    s = make(lengths, counts, 2, 1, dh, 16, dtype, seed=new)
+    s["q"] *= 0.25
+    o, _, _, bo, _, _ = ref.attention(s["q"], s["K"], s["V"], s["table"], lengths, counts)
+    for r, c, x in ((3, 1, math.inf), (70, 9, -math.inf), (400, 33, math.inf), (401, 33, math.inf), (699, 40, -math.inf),
+                    (130, 50, math.nan), (200, 60, math.inf), (201, 60, -math.inf)):
+        s["V"][s["table"][0, r // 16], :, r % 16, c] = x
+    d = dev(s)
+    got = paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], d["starts"]).o.cpu()
+    assert (got[..., [1, 33]] == math.inf).all() and (got[..., [9, 40]] == -math.inf).all() and got[..., [50, 60]].isnan().all()
+    rest = [c for c in range(dh) if c not in (1, 9, 33, 40, 50, 60)]
+    near(got[..., rest], o[..., rest], bo[..., rest], "o")
