@@ -64,3 +64,12 @@ def test_infinite_values_that_are_read(dtype, dh, new):
     assert (got[..., [1, 33]] == math.inf).all() and (got[..., [9, 40]] == -math.inf).all() and got[..., [50, 60]].isnan().all()
     rest = [c for c in range(dh) if c not in (1, 9, 33, 40, 50, 60)]
     near(got[..., rest], o[..., rest], bo[..., rest], "o")
+
+
+@pytest.mark.parametrize("keep", [L.DM_PAGED_ROWS + 1, 2 ** 31 - 1, 2 ** 32 + 5])
+def test_more_kept_rows_than_a_table_has(keep):
+    """Refused before the rows are allocated; past 32 bits too, of which the call would take the lower ones."""
+    K, V = paged.new_pages(4, 2, 16, 64)
+    table, w = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.zeros(1, 2, 32, device=DEV)
+    with pytest.raises(ValueError, match="keep="):
+        paged.evict_rows(K, V, w, table, torch.ones(1, dtype=torch.int32, device=DEV), keep, table + 2)
