@@ -112,6 +112,8 @@ def _sequences(table, lengths, starts, n_tokens, device):
     if table.dim() != 2:
         raise ValueError(f"table: {tuple(table.shape)}; [B, cols] is needed")
     B, cols = table.shape
+    if n_tokens > 0x7fffffff or B > 0x7fffffff or cols > 0x7fffffff:     # (the library's counts; it refuses most of these too)
+        raise ValueError(f"{n_tokens} tokens of sequences of a table {tuple(table.shape)}: too many")
     if starts is None and n_tokens != B:
         raise ValueError(f"{n_tokens} tokens of {B} sequences without starts")
     return (B, cols, _index(table, "table", table.shape, device), _index(lengths, "lengths", (B,), device),

@@ -73,3 +73,13 @@ def test_more_kept_rows_than_a_table_has(keep):
     table, w = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.zeros(1, 2, 32, device=DEV)
     with pytest.raises(ValueError, match="keep="):
         paged.evict_rows(K, V, w, table, torch.ones(1, dtype=torch.int32, device=DEV), keep, table + 2)
+
+
+def test_more_tokens_than_32_bits_count():
+    """Refused, where the library would see the lower 32 bits of their number (here 2 tokens)."""
+    K, V = paged.new_pages(4, 2, 16, 64)
+    table, lengths = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.full((1,), 2, dtype=torch.int32, device=DEV)
+    k = torch.ones(1, 2, 64, device=DEV, dtype=torch.bfloat16).expand(2 ** 32 + 2, 2, 64)
+    with pytest.raises(ValueError, match="too many"):
+        paged.paged_write(k, k, K, V, table, lengths, torch.tensor([0, 2], dtype=torch.int32, device=DEV))
+    assert not K.any()
