@@ -1490,12 +1490,15 @@ Form form_of(const dm_paged_args* a) {
   if (most_tiles(a) <= 9 && query_tiles(a, f.rows) * a->h_kv >= CUS / 2) f.least = (int)most_tiles(a);
   return f;
 }
-// The scores of a call with weights are kept where they take no more room than the pages' keys; else they are computed
-// again from the keys.
+// The scores of a call with weights are kept where they take no more room than the pages' keys, and 1 GiB: they lie under the table's
+// whole width, which may be far more than the sequences' rows, and a pool may leave little memory beside it. Else they are computed
+// again from the keys (us a call, kept / again: 64 tokens over 32768 rows, 32 heads of 128 on 8 key heads, 256 MiB of scores 1832 /
+// 2354; 16 chunks of 8, 512 MiB, 791 / 848; fp32, 8 chunks of 32 over 16384 rows, 512 MiB, 981 / 1408).
+constexpr double SCORE_BYTES = 1 << 30;
 size_t score_floats(const dm_paged_args* a) {
   if (!a->weights || form_of(a).rows != TILE_Q) return 0;
   const double n = (double)a->n_tokens * a->h * (((int64_t)a->table_cols * a->page + 31) & -32);
-  return n * 4 <= (double)a->n_pages * a->h_kv * a->page * a->dh * esz(a->dtype) ? (size_t)n : 0;
+  return n * 4 <= std::min(SCORE_BYTES, (double)a->n_pages * a->h_kv * a->page * a->dh * esz(a->dtype)) ? (size_t)n : 0;
 }
 int wanted(const dm_paged_args* a, const Form& f) { return wanted(a, f.blocks, query_tiles(a, f.rows), f.least); }
 bool in_pieces(const dm_paged_args* a, const Form& f) { return most_tiles(a) > f.least; }

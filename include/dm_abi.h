@@ -640,8 +640,8 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
  *   storage dtype, lse [n_tokens, h] fp32, both contiguous.
  *   weights (fp32 [B, h_kv, table_cols * page], may be NULL): weights[b, c, r] += the sum over b's new tokens and the heads
  *   of c of e^(s_r - lse), for the rows that are read. One writer per weight, in a fixed order.
- * Workspace: dm_paged_workspace_bytes(a) (from the sizes and whether there are weights; none where rows are few), 16-byte
- * aligned, not shared by calls that may overlap.
+ * Workspace: dm_paged_workspace_bytes(a) (from the sizes and whether there are weights, whose scores take 1 GiB at most; none where
+ * rows are few), 16-byte aligned, not shared by calls that may overlap.
  * At most DM_PAGED_ROWS rows per sequence, n_tokens * h at most DM_PAGED_TOKENS, B * h_kv at most DM_PAGED_HEADS. */
 #define DM_PAGE_MAX 1024
 #define DM_PAGED_ROWS (1 << 26)
