@@ -13,6 +13,7 @@ import torch
 
 from . import _lib as L
 from .logprobs import _rows
+from .paged import _no_graph
 
 
 class Verified(NamedTuple):
@@ -33,9 +34,8 @@ def verify_drafts(logits, ids, uniforms, starts, draft_logits=None, temperature=
     distribution that ids[t + 1] was drawn from in row t (a sequence's last row is not read); None: the drafts are certain.
     temperature: one number, or [B] fp32. Returns Verified; no gradients. A row without a distribution (a NaN, +inf, nothing
     but -inf; a temperature that is negative or not finite) ends its sequence with token -1."""
-    for t in (logits, draft_logits):
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise NotImplementedError("verify_drafts keeps no autograd graph; call it under torch.no_grad() or on detached tensors")
+    for t in (logits, draft_logits, temperature if torch.is_tensor(temperature) else None):
+        _no_graph(t, "verify_drafts")
     if not logits.is_cuda or logits.dim() != 2:
         raise ValueError(f"logits: shape {tuple(logits.shape)} on {logits.device}; rows [N, V] on a GPU are needed")
     dev = logits.get_device()

@@ -22,6 +22,7 @@ results of tokens of no sequence (behind ``starts[B]``) are left as they are.
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -43,9 +44,14 @@ def new_pages(n_pages, h_kv, page, dh, device="cuda", dtype=torch.bfloat16):
     return torch.zeros(shape, device=device, dtype=dtype), torch.zeros(shape, device=device, dtype=dtype)
 
 
-def _no_graph(t):
-    if t is not None and t.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("the paged cache keeps no autograd graph; call it under torch.no_grad() or on detached tensors")
+def _no_graph(t, what="the paged cache"):
+    if t is None:
+        return
+    if t.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{what} keeps no autograd graph; call it under torch.no_grad() or on detached tensors")
+    # (the level first: unpacking costs more than the rest of a check, and outside of one there are no tangents)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{what} carries no tangent; call it on detached tensors")
 
 
 def _extent(t):
@@ -102,6 +108,7 @@ def _tokens(t, name, shape, like):
 
 
 def _weights(t, shape, device):
+    _no_graph(t)
     if t.dtype != torch.float32 or t.shape != shape or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"weights: {t.dtype} {tuple(t.shape)} on {t.device}; contiguous fp32 {shape} on cuda:{device} is needed")
     return t.data_ptr()
@@ -170,10 +177,8 @@ def paged_attention(q, K, V, table, lengths, starts=None, k_self=None, v_self=No
         _no_graph(out)
         _apart("out", out, q, K, V, k_self, v_self, weights)
         torch.autograd.graph.increment_version(out)
-    if weights is not None:
-        _no_graph(weights)
-        if K.dtype == torch.float32:
-            _apart("weights", weights, q, K, V, k_self, v_self)
+    if weights is not None and K.dtype == torch.float32:
+        _apart("weights", weights, q, K, V, k_self, v_self)
     lse = torch.empty((N, h), dtype=torch.float32, device=K.device)
     if N == 0 or B == 0:
         return PagedAttention(out, lse)

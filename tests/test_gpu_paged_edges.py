@@ -4,9 +4,11 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from dual_mod_public_amd import _lib as L
 from dual_mod_public_amd import paged
+from dual_mod_public_amd.drafts import verify_drafts
 from tests import paged_reference as ref
 from tests.hip_helpers import DEV
 from tests.test_gpu_paged import dev, make, near
@@ -83,3 +85,36 @@ def test_more_tokens_than_32_bits_count():
     with pytest.raises(ValueError, match="too many"):
         paged.paged_write(k, k, K, V, table, lengths, torch.tensor([0, 2], dtype=torch.int32, device=DEV))
     assert not K.any()
+
+
+def test_tangents_and_graphs_are_refused():
+    """Tensors with a forward-mode tangent have no requires_grad; the calls would drop the tangent. Weights and temperatures with
+    a graph."""
+    K, V = paged.new_pages(4, 2, 16, 64, dtype=torch.float32)
+    table, lengths = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    q, pair, w = torch.zeros(1, 4, 64, device=DEV), torch.zeros(1, 2, 64, device=DEV), torch.zeros(1, 2, 32, device=DEV)
+    x, ids, u = torch.zeros(2, 9, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV), torch.zeros(2, 2, device=DEV)
+    starts, T = torch.tensor([0, 2], dtype=torch.int32, device=DEV), torch.ones(1, device=DEV)
+    calls = {
+        "attend": (lambda **kw: paged.paged_attention(**dict(dict(q=q, K=K, V=V, table=table, lengths=lengths, k_self=pair, v_self=pair,
+                                                                  weights=w), **kw)), dict(q=q, K=K, V=V, k_self=pair, v_self=pair, weights=w)),
+        "write": (lambda **kw: paged.paged_write(**dict(dict(k=pair, v=pair, K=K, V=V, table=table, lengths=lengths), **kw)),
+                  dict(k=pair, v=pair, K=K, V=V)),
+        "evict": (lambda **kw: paged.evict_rows(**dict(dict(K=K, V=V, weights=w, table=table, lengths=lengths, keep=8, new_table=table + 2),
+                                                       **kw)), dict(K=K, V=V, weights=w)),
+        "verify": (lambda **kw: verify_drafts(**dict(dict(logits=x, ids=ids, uniforms=u, starts=starts, draft_logits=x, temperature=T), **kw)),
+                   dict(logits=x, draft_logits=x, temperature=T)),
+    }
+    for name, (call, tensors) in calls.items():
+        call()
+        for n, t in tensors.items():
+            with forward_ad.dual_level():
+                call()
+                with pytest.raises(NotImplementedError, match="tangent"):
+                    call(**{n: forward_ad.make_dual(t.clone(), torch.ones_like(t))})
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
+                    call(**{n: forward_ad.make_dual(t.clone(), torch.ones_like(t))})
+            with pytest.raises(NotImplementedError, match="graph"):
+                call(**{n: t.clone().requires_grad_()})
+            with torch.no_grad():
+                call(**{n: t.clone().requires_grad_()})
