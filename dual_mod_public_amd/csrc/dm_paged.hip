@@ -13,6 +13,7 @@
 #include "dm_error.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 using namespace dm;
@@ -1546,8 +1547,7 @@ int check_paged(const dm_paged_args* a, bool write) {
   }
   if (write) return DM_OK;
   DM_REQUIRE(a->h > 0 && a->h % a->h_kv == 0 && a->h / a->h_kv <= 1024, DM_ERR_INVALID, "h=%d h_kv=%d", a->h, a->h_kv);
-  DM_REQUIRE(a->window >= 0 && a->scale == a->scale && a->scale > -INF && a->scale < INF, DM_ERR_INVALID, "window=%d scale=%g", a->window,
-             a->scale);
+  DM_REQUIRE(a->window >= 0 && std::fabs(a->scale * LOG2E) < INF, DM_ERR_INVALID, "window=%d scale=%g (below 2.3e38)", a->window, a->scale);
   if (const int rc = check_rows("q", a->q, a->q_token, a->q_head, a->dtype)) return rc;
   DM_REQUIRE(a->o && aligned16(a->o) && a->lse, DM_ERR_INVALID, "null or unaligned o, null lse");
   const size_t need = dm_paged_workspace_bytes(a);

@@ -45,3 +45,11 @@ def test_scores_are_kept_within_the_bound():
     size = L.load().dm_paged_workspace_bytes
     kept = size(L.byref(attention_args())) - size(L.byref(attention_args(weights=None)))
     assert kept == 64 * 32 * (1 << 17) * 4 == 1 << 30
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38])
+def test_scales_whose_product_with_log2_e_is_infinite(scale):
+    """Scores are held in units of ln 2: the scale times log2 e has to be a number, or scores of 0 become NaN."""
+    lib = L.load()
+    a = attention_args(weights=None, scale=scale, workspace=0x100000, workspace_bytes=1 << 40)
+    assert lib.dm_paged_attention(L.byref(a), None) == -1 and b"scale" in lib.dm_last_error()
