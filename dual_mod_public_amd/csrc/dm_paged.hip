@@ -621,6 +621,11 @@ DM_DEV i16x8 values_fragment32(const bf16* v, int ldv) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Two bf16 numbers times 0: NaN where one is not finite.
+DM_DEV uint32_t times_zero(uint32_t x) {
+  return ((x & 0x7f80u) == 0x7f80u ? 0x7fc0u : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0x7fc00000u : 0u);
+}
+
 template <int DH> struct WideTile {
   static constexpr int KT = 64;            // cached rows of a step
   static constexpr int LDK = DH + 8;       // 16 rows' 16-byte pieces fill the banks once
@@ -675,7 +680,7 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
     for (int i = 0; i < C::NK; ++i) {
       qf[i] = live ? ld_global<u32x4>(q + 16 * i + 8 * half) : u32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) qf[i][e] = a.scale2 == 0.f ? 0u : qf[i][e] ^ flip;
+      for (int e = 0; e < 4; ++e) qf[i][e] = a.scale2 == 0.f ? times_zero(qf[i][e]) : qf[i][e] ^ flip;
     }
   }
   const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);

@@ -118,3 +118,20 @@ def test_tangents_and_graphs_are_refused():
                 call(**{n: t.clone().requires_grad_()})
             with torch.no_grad():
                 call(**{n: t.clone().requires_grad_()})
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 90, 600])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_scale_of_zero_times_queries_that_are_not_finite(dtype, new, value):
+    """0 times NaN or infinity is NaN, whichever read a call takes; the other query rows are means of the rows read."""
+    lengths, counts = [40 + new], [new]
+    s = make(lengths, counts, 2, 1, 64, 16, dtype, seed=new)
+    o, _, _, bo, _, _ = ref.attention(s["q"], s["K"], s["V"], s["table"], lengths, counts, scale=0.0)
+    s["q"][new // 2, 1, 7] = value
+    d = dev(s)
+    r = paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], d["starts"], scale=0.0)
+    nan = torch.zeros(new, 2, dtype=torch.bool)
+    nan[new // 2, 1] = True
+    assert torch.equal(r.lse.isnan().cpu(), nan) and torch.equal(r.o.isnan().all(-1).cpu(), nan)
+    near(r.o.cpu()[~nan], o[~nan], bo[~nan], "o")
