@@ -326,7 +326,7 @@ template <int LDV, int N> DM_DEV floatx4 mma_values(const float* Vs, const Proba
 }
 
 // The page of rows r .. that lie in one (pages hold 16 rows or more and begin at a multiple of 16). needed: some query of
-// the tile reads some of them. A page outside the pool is read as page 0 and marks the sequence. The table is read through
+// the tile reads some of them. A page outside the pool is read as page 0 and marks the tile's results. The table is read through
 // the scalar cache: a vector load of it would be waited for together with all rows that are on their way (two prompts' chunks
 // of 2048 tokens over 16384 rows 2.50 ms so, 1.66 with scalar loads), and pages are looked up a step ahead of their rows.
 DM_DEV int page_of(const PagedArgs& a, const int32_t* table, int r, bool needed, bool& bad) {

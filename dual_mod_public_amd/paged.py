@@ -11,8 +11,8 @@ its rows lie in pages of a common pool, so requests come and go, and a pass take
             none where the length is 0
 
 All of them lie on the device and are read there: a captured pass is replayed with other lengths, tables and starts. The host
-does not look at them. A sequence that its table does not hold, or one that reads a page outside the pool, gets NaN; the
-results of tokens of no sequence (behind ``starts[B]``) are left as they are.
+does not look at them. A sequence that its table does not hold gets NaN, and so does a token that reads a row of a page outside the
+pool (and others of its sequence may); the results of tokens of no sequence (behind ``starts[B]``) are left as they are.
 
   paged_write       the new tokens' rows into the pages
   paged_attention   the new tokens' attention over their sequences' rows

@@ -626,9 +626,9 @@ int dm_adamw_values(const uint8_t* codes, const uint8_t* exponents, int64_t n_bl
  * lengths[b] - n + j; NULL: one token per sequence, none where lengths[b] is 0. All three lie on the device and may change
  * between replays of a captured call. Tokens of no sequence (behind starts[B]) are neither read nor written, nor are their
  * rows of o and lse.
- * starts do not descend. A sequence that its table does not hold (lengths[b] > table_cols * page, or less than its new tokens),
- * or one that reads a page outside [0, n_pages), gets NaN; what such a page would be written is left out. weights of the first
- * kind of sequence stay as they are, of the second they become NaN.
+ * starts do not descend. A sequence that its table does not hold (lengths[b] > table_cols * page, or less than its new tokens)
+ * gets NaN, and its weights stay as they are. A token that reads a row of a page outside [0, n_pages) gets NaN, and so do the weights
+ * of the rows that it reads; the sequence's other tokens may too. What such a page would be written is left out.
  *
  * dm_paged_write: the tokens' rows k_rows, v_rows [n_tokens, h_kv, dh] (any token and head strides) into the pages.
  * dm_paged_attention: for query head a of key head a / (h / h_kv) and a token with row p, over the rows r <= p with

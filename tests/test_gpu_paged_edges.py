@@ -135,3 +135,34 @@ def test_a_scale_of_zero_times_queries_that_are_not_finite(dtype, new, value):
     nan[new // 2, 1] = True
     assert torch.equal(r.lse.isnan().cpu(), nan) and torch.equal(r.o.isnan().all(-1).cpu(), nan)
     near(r.o.cpu()[~nan], o[~nan], bo[~nan], "o")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new,g", [(3, 1), (60, 2), (300, 4)])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("bad", [0, 7, -1])
+def test_chunks_with_a_page_outside_the_pool(dtype, new, g, window, bad):
+    """The tokens that read a row of it get NaN, the others NaN or what they get without it; and so do the weights of the rows
+    that those read. The other sequence is as ever."""
+    lengths, counts, page = [200 + new, 90], [new, 2], 16
+    s = make(lengths, counts, g, 1, 64, page, dtype, seed=new)
+    d = dev(s)
+    cap = s["table"].shape[1] * page
+    w, v = torch.zeros(2, 1, cap, device=DEV), torch.zeros(2, 1, cap, device=DEV)
+    want = paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], d["starts"], window=window, weights=w)
+    at = bad if bad >= 0 else (lengths[0] - 1) // page
+    d["table"][0, at] = s["K"].shape[0]
+    r = paged.paged_attention(d["q"], d["K"], d["V"], d["table"], d["lengths"], d["starts"], window=window, weights=v)
+    reads_it = torch.zeros(new + 2, dtype=torch.bool)
+    read_by_it = torch.zeros(cap, dtype=torch.bool)
+    for j in range(new):
+        p = 200 + j
+        low = max(0, p - window + 1) if window else 0
+        reads_it[j] = p >= page * at and low < page * (at + 1)
+        if reads_it[j]:
+            read_by_it[low:p + 1] = True
+    nan = r.o.isnan().flatten(1).all(1).cpu()
+    assert nan[reads_it].all() and not nan[new:].any() and torch.equal(r.lse.isnan().all(1).cpu(), nan)
+    assert torch.equal(r.o[~nan], want.o[~nan]) and torch.equal(r.lse[~nan], want.lse[~nan])
+    v, w = v.cpu(), w.cpu()
+    assert v[0, 0, read_by_it].isnan().all() and torch.equal(v[1], w[1]) and not v[0, 0, lengths[0]:].any()
