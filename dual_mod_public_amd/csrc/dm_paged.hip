@@ -668,9 +668,9 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
   const int base = t_low & -TILE_K, tiles = max(0, (t_high - base + TILE_K - 1) / TILE_K);
   const int each = uniform((tiles + it.pieces - 1) / it.pieces);
   const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
-  // rows that all, and that any, of the wave's live query rows read
-  const int w_first = uniform(min(rho0 + 32 * wave, rows - 1) / a.g), w_last = uniform(min(rho0 + 32 * wave + 31, rows - 1) / a.g);
-  const int all_low = s.low(a, w_last), all_high = s.high(a, w_first), any_low = s.low(a, w_first), any_high = s.high(a, w_last);
+  // rows from this on and below that are read by all of the wave's live query rows
+  const int all_low = s.low(a, uniform(min(rho0 + 32 * wave + 31, rows - 1) / a.g));
+  const int all_high = s.high(a, uniform(min(rho0 + 32 * wave, rows - 1) / a.g));
 
   u32x4 qf[C::NK];
   {
