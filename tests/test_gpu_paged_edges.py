@@ -166,3 +166,56 @@ def test_chunks_with_a_page_outside_the_pool(dtype, new, g, window, bad):
     assert torch.equal(r.o[~nan], want.o[~nan]) and torch.equal(r.lse[~nan], want.lse[~nan])
     v, w = v.cpu(), w.cpu()
     assert v[0, 0, read_by_it].isnan().all() and torch.equal(v[1], w[1]) and not v[0, 0, lengths[0]:].any()
+
+
+def guarded(n_bytes, fill=0xa5):
+    """n_bytes in the middle of a buffer of a pattern: (the buffer, their address)."""
+    t = torch.full((n_bytes + 2 * GUARD,), fill, dtype=torch.uint8, device=DEV)
+    return t, t.data_ptr() + GUARD
+
+
+GUARD = 1 << 16
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,N,g", [(200, 200, 2), (5, 150, 4), (3, 400, 4)])
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("starts", ["ascending", "turning", "negative"])
+def test_nothing_around_the_outputs_is_written(dtype, B, N, g, weights, starts):
+    """Outputs, weights and workspace inside buffers of a pattern, which stays, also where starts descend: sequences then share
+    tokens, and no result is defined."""
+    h_kv, dh, page, cols = 2, 64, 16, 200
+    lengths = [(37 * b) % 3000 + N for b in range(B)]
+    rng = torch.Generator().manual_seed(B)
+    table = torch.randint(0, 64, (B, cols), generator=rng, dtype=torch.int32).to(DEV)
+    K, V = (torch.randn(64, h_kv, page, dh, generator=rng).to(dtype).to(DEV) for _ in range(2))
+    q = torch.randn(N, h_kv * g, dh, generator=rng).to(dtype).to(DEV)
+    cut = {"ascending": [N * b // B for b in range(B + 1)], "turning": ([0, N] * B)[:B + 1],
+           "negative": [N - 2 * b for b in range(B)] + [-7]}[starts]
+    cut = torch.tensor(cut, dtype=torch.int32, device=DEV)
+    length = torch.tensor([min(n, cols * page) for n in lengths], dtype=torch.int32, device=DEV)
+    sizes = dict(o=N * h_kv * g * dh * q.element_size(), lse=N * h_kv * g * 4)
+    if weights:
+        sizes["weights"] = B * h_kv * cols * page * 4
+    a = L.dm_paged_args(L.dtype_code(dtype), B, h_kv * g, h_kv, dh, page, 64, cols, N, 0, 0.125, 0, q.data_ptr(), q.stride(0), q.stride(1),
+                        K.data_ptr(), V.data_ptr(), K.stride(0), V.stride(0), table.data_ptr(), length.data_ptr(), cut.data_ptr())
+    if weights:
+        a.weights = 1
+    sizes["workspace"] = L.lib().dm_paged_workspace_bytes(L.byref(a))
+    buffers = {}
+    for n, size in sizes.items():
+        buffers[n], at = guarded(size)
+        setattr(a, n, at)
+    a.workspace_bytes = sizes["workspace"]
+    if weights:
+        buffers["weights"][GUARD:-GUARD] = 0
+    L.call_on(K.device, L.lib().dm_paged_attention, L.byref(a))
+    torch.cuda.synchronize()
+    for n, t in buffers.items():
+        assert (t[:GUARD] == 0xa5).all() and (t[-GUARD:] == 0xa5).all(), n
+    if starts == "ascending":
+        w = torch.zeros(B, h_kv, cols * page, device=DEV) if weights else None
+        want = paged.paged_attention(q, K, V, table, length, cut, scale=0.125, weights=w)
+        assert torch.equal(buffers["o"][GUARD:-GUARD].view(dtype).view_as(want.o), want.o)
+        assert torch.equal(buffers["lse"][GUARD:-GUARD].view(torch.float32).view_as(want.lse), want.lse)
+        assert not weights or torch.equal(buffers["weights"][GUARD:-GUARD].view(torch.float32).view_as(w), w)
