@@ -9,8 +9,10 @@ import torch
 import oracle as O
 from dual_mod_public_amd import _lib as L
 from dual_mod_public_amd.attention import DualModAttention
-from dual_mod_public_amd.paged_decode import PagedTape
-from dual_mod_public_amd.synthetic import make_input, make_state_dict
+from dual_mod_public_amd.config import DualModConfig
+from dual_mod_public_amd.model import DualModLM
+from dual_mod_public_amd.paged_decode import PagedDecoder, PagedTape
+from dual_mod_public_amd.synthetic import make_input, make_lm_state_dict, make_state_dict
 from tests.hip_helpers import DEV, cfg_of, record, relerr
 
 pytestmark = pytest.mark.gpu
@@ -84,3 +86,69 @@ def test_chunks_with_any_number_of_sweeps(dtype, n_sweeps, knobs):
         t0 += c
     record(f"paged chunks {knobs} {dtype} sweeps {n_sweeps}", errs, TOL[dtype])
     assert all(e < TOL[dtype] for e in errs.values()), errs
+
+
+@pytest.mark.parametrize("with_starts", [False, True])
+@pytest.mark.parametrize("knobs", [dict(ctx_mod="mult_res"), dict(ctx_mod="fusion", local_window=30)])
+@pytest.mark.parametrize("d,h", [(256, 4), (256, 2)])
+def test_single_tokens_in_bf16(with_starts, knobs, d, h):
+    """Three steps of one token per sequence behind pasts of 100, 1 and 0 rows, against the oracle's step in 64 bits."""
+    cfg = cfg_of(d=d, h=h, T=128, **knobs)
+    sd = make_state_dict(cfg, seed=32, with_attn_norm=False)
+    sd = {k: (v.bfloat16() if v.dim() == 2 else v).double() for k, v in sd.items()}
+    cos, sin = O.build_rope_cache(128, cfg.head_dim, cfg.rope_theta, dtype=torch.float64)
+    pasts, page = [100, 1, 0], 16
+    tape = PagedTape(attention(cfg, sd), 12, page)
+    table = i32([7, 2, 9, 4, 11, 0, 5], [1] + [-1] * 6, [8] + [-1] * 6)
+    caches = [dict(zip("KV", kv)) for kv in filled(tape, table, pasts, seed=8)]
+    x = make_input((3, 3, d), seed=9).bfloat16()
+    errs = {}
+    for t in range(3):
+        lengths = [p + t + 1 for p in pasts]
+        y = tape.extend(x[:, t].to(DEV), torch.tensor([n - 1 for n in lengths], device=DEV), cos.to(DEV), sin.to(DEV), table, i32(*lengths),
+                        **(dict(starts=i32(0, 1, 2, 3), n_sweeps=1) if with_starts else {}))
+        for b, n in enumerate(lengths):
+            _, want = O.decode_step(cfg, sd, x[b:b + 1, t:t + 1].double(), n - 1, caches[b], cos, sin)
+            errs[f"y{b}@{t}"] = relerr(y[b], want[0, 0])
+            at = int(table[b, (n - 1) // page])
+            for name, pages in (("K", tape.K), ("V", tape.V)):
+                errs[f"{name}{b}@{t}"] = relerr(pages[at, :, (n - 1) % page], caches[b][name][0, :, n - 1])
+    record(f"paged single tokens {knobs} h={h}", errs, TOL[torch.bfloat16])
+    assert all(e < TOL[torch.bfloat16] for e in errs.values()), errs
+
+
+def test_decoder_in_bf16():
+    """Three texts through a bf16 model in chunks of 0 to 9 tokens, exact sweeps: the oracle's 64-bit model within bf16's tolerance,
+    and the same token wherever its two largest logits lie further apart than twice the largest error."""
+    cfg = DualModConfig(d_model=256, n_heads=4, n_layers=2, vocab_size=512, max_seq_len=64, mlp_hidden_override=512, checkpoint_chunk=0,
+                        ctx_mod="mult_res")
+    sd = make_lm_state_dict(cfg, seed=7, std=0.02)
+    m = DualModLM(cfg, dtype=torch.bfloat16).to(DEV)
+    m.load_state_dict({k: v.to(DEV) for k, v in sd.items()})
+    dec = PagedDecoder(m, 10, 16)
+    for tape in dec.tapes:
+        assert tape.K.dtype == torch.bfloat16
+        tape.K.fill_(math.nan), tape.V.fill_(math.nan)
+    g = torch.Generator().manual_seed(3)
+    texts = [torch.randint(0, 512, (n,), generator=g) for n in (48, 17, 31)]
+    table = i32([9, 0, 4], [2, 7, -1], [5, 3, -1])
+    done, rows = [0, 0, 0], [[], [], []]
+    while done != [48, 17, 31]:
+        n = [min(int(torch.randint(0, 10, (), generator=g)), len(t) - k) for t, k in zip(texts, done)]
+        if not sum(n):
+            continue
+        ids = torch.cat([t[k:k + c] for t, k, c in zip(texts, done, n)]).to(DEV)
+        pos = torch.cat([torch.arange(k, k + c) for k, c in zip(done, n)]).to(DEV)
+        done = [k + c for k, c in zip(done, n)]
+        logits = dec.extend(ids, pos, table, i32(*done), i32(0, n[0], n[0] + n[1], sum(n)), n_sweeps=max(n))
+        for b, part in enumerate(logits.cpu().split(n)):
+            rows[b].append(part)
+    for b, text in enumerate(texts):
+        got = torch.cat(rows[b]).double()
+        cos, sin = O.build_rope_cache(len(text), cfg.head_dim, cfg.rope_theta, dtype=torch.float64)
+        want = O.lm_forward(cfg, {k: v.double() for k, v in sd.items()}, text[None], cos, sin)[0]
+        err, off = relerr(got, want), float((got - want).abs().max())
+        record(f"paged decoder bf16 text {b}", {"logits": err}, TOL[torch.bfloat16])
+        top = want.topk(2, -1).values
+        decided = top[:, 0] - top[:, 1] > 2 * off
+        assert err < TOL[torch.bfloat16] and torch.equal(got.argmax(-1)[decided], want.argmax(-1)[decided])
