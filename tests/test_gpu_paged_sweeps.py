@@ -152,3 +152,104 @@ def test_decoder_in_bf16():
         top = want.topk(2, -1).values
         decided = top[:, 0] - top[:, 1] > 2 * off
         assert err < TOL[torch.bfloat16] and torch.equal(got.argmax(-1)[decided], want.argmax(-1)[decided])
+
+
+def decoder(dtype, n_pages, layers=2):
+    cfg = DualModConfig(d_model=256, n_heads=4, n_layers=layers, vocab_size=512, max_seq_len=128, mlp_hidden_override=512,
+                        checkpoint_chunk=0, ctx_mod="mult_res")
+    m = DualModLM(cfg, dtype=dtype).to(DEV)
+    m.load_state_dict({k: v.to(DEV) for k, v in make_lm_state_dict(cfg, seed=7, std=0.02).items()})
+    return m, PagedDecoder(m, n_pages, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_decoder_with_other_sequences(dtype):
+    """A decoder's pass over ragged chunks, captured once and replayed with other tokens, positions, tables, lengths and starts; eager
+    work and synchronizations between the replays."""
+    B, N, cols = 3, 12, 7
+    m, dec = decoder(dtype, B * cols + 4)
+    s = dict(ids=torch.zeros(N, dtype=torch.int64, device=DEV), pos=torch.zeros(N, dtype=torch.int64, device=DEV),
+             table=torch.zeros(B, cols, dtype=torch.int32, device=DEV), lengths=i32(4, 4, 4), starts=i32(0, 4, 8, 12))
+    w = [torch.zeros(B, 4, cols * 16, device=DEV) for _ in range(2)]
+    before = [[torch.randn(t.K.shape, generator=torch.Generator().manual_seed(i)).to(dtype).to(DEV) for _ in "KV"] for i, t in enumerate(dec.tapes)]
+
+    def fill(seed):
+        c = torch.Generator().manual_seed(seed)
+        s["ids"].copy_(torch.randint(0, 512, (N,), generator=c))
+        s["table"].copy_(torch.randperm(B * cols + 4, generator=c)[:B * cols].view(B, cols))
+        cuts = sorted(torch.randint(0, N + 1, (B - 1,), generator=c).tolist()) + [N]
+        counts = [b - a for a, b in zip([0] + cuts, cuts)]
+        past = [int(torch.randint(0, 100, (), generator=c)) for _ in range(B)]
+        s["starts"].copy_(torch.tensor([0] + cuts))
+        s["lengths"].copy_(torch.tensor([max(1, p + n) for p, n in zip(past, counts)]))
+        s["pos"].copy_(torch.cat([torch.arange(p, p + n) for p, n in zip(past, counts)]))
+        for t, (k, v), x in zip(dec.tapes, before, w):
+            t.K.copy_(k), t.V.copy_(v), x.zero_()
+
+    def run():
+        return dec.extend(s["ids"], s["pos"], s["table"], s["lengths"], s["starts"], n_sweeps=3, weights=w)
+
+    def everything(logits):
+        return [logits.clone(), *(x.clone() for x in w), *(x.clone() for t in dec.tapes for x in (t.K, t.V))]
+
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for seed in range(1, 5):
+        fill(seed)
+        want = everything(run())
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(everything(held), want)), seed
+
+
+def test_parameters_that_change():
+    """A step of an optimizer between two passes: the second one has the new parameters, in every layer and the head."""
+    m, dec = decoder(torch.float32, 4)
+    table, ids, pos = i32([0, 1]), torch.tensor([3, 9, 4], device=DEV), torch.arange(3, device=DEV)
+    dec.extend(ids, pos, table, i32(3), i32(0, 3), n_sweeps=3)
+    g = torch.Generator().manual_seed(2)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_((0.01 * torch.randn(p.shape, generator=g)).to(DEV))
+    got = dec.extend(ids, pos, table, i32(3), i32(0, 3), n_sweeps=3)
+    assert torch.equal(got, PagedDecoder(m, 4, 16).extend(ids, pos, table, i32(3), i32(0, 3), n_sweeps=3))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_tokens_in_one_pass(dtype):
+    """2500 tokens of 70 sequences in one pass, a layer of the larger width, against each sequence's own pass. The products may take
+    other forms at other sizes, so their sums another order: within the tolerance of two computations."""
+    cfg = cfg_of(d=1024, h=16, T=128, ctx_mod="mult_res")
+    sd = {k: v.double() for k, v in make_state_dict(cfg, seed=33, with_attn_norm=False).items()}
+    attn = attention(cfg, sd)
+    cos, sin = (t.to(DEV) for t in O.build_rope_cache(128, cfg.head_dim, cfg.rope_theta, dtype=torch.float64))
+    g = torch.Generator().manual_seed(4)
+    counts = torch.randint(1, 72, (70,), generator=g).tolist()
+    starts = [0]
+    for n in counts:
+        starts.append(starts[-1] + n)
+    x = torch.randn(starts[-1], 1024, generator=g).to(dtype).to(DEV)
+    pos = torch.cat([torch.arange(n) for n in counts]).to(DEV)
+    tape = PagedTape(attn, 70 * 5, 16, dtype)
+    table = torch.arange(350, dtype=torch.int32, device=DEV).view(70, 5)
+    y = tape.extend(x, pos, cos, sin, table, i32(*counts), i32(*starts), n_sweeps=2)
+    own = PagedTape(attn, 70 * 5, 16, dtype)
+    errs = {}
+    for b in (0, 1, 33, 69):
+        rows = slice(starts[b], starts[b + 1])
+        want = own.extend(x[rows], pos[rows], cos, sin, table[b:b + 1], i32(counts[b]), i32(0, counts[b]), n_sweeps=2)
+        at = torch.arange(counts[b], device=DEV)
+        page = table[b].long()[at // 16]
+        errs[f"y{b}"] = relerr(y[rows], want)
+        errs[f"K{b}"] = relerr(tape.K[page, :, at % 16], own.K[page, :, at % 16])
+        errs[f"V{b}"] = relerr(tape.V[page, :, at % 16], own.V[page, :, at % 16])
+    record(f"paged pass of many tokens {dtype}", errs, TOL[dtype])
+    assert all(e < TOL[dtype] for e in errs.values()), errs
