@@ -21,7 +21,7 @@ using namespace dm;
 namespace {
 
 constexpr float INF = __builtin_inff(), NAN_ = __builtin_nanf("");
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr int CUS = 256;
 constexpr float LAST_CACHE = 1 << 28;      // bytes
 constexpr int TILE_Q = 16;      // query rows of a tile
@@ -36,7 +36,7 @@ struct PagedArgs {
   int B, h, h_kv, g, n_pages, cols, page_shift, N, window;
   float scale2;                        // scale log2 e
   int want, least;                     // the plan: pieces wanted, least tiles of cached rows in one
-  float* scores;                       // N h cols * page of them in units of ln 2, for the weights; nullptr: not kept
+  float* scores;                       // N h cols * page of them, before the scale, for the weights; nullptr: not kept
 };
 
 // A sequence as the call gives it. A table that does not hold its rows, or fewer rows than new tokens: bad, NaN results.
@@ -209,32 +209,58 @@ template <typename T, int DH> struct Tile {
   static constexpr int WAVES = sizeof(T) == 2 || DH == 128 ? 3 : 2;
 };
 
-// S^T[16 cached rows][16 query rows] += K Q^T for one 16-byte chunk per lane of each: bf16 lane l holds columns
+// S^T = K Q^T of NT tiles of 16 cached rows and 16 query rows, from a lane's 16-byte chunks of each: bf16 lane l holds columns
 // 8 (l / 16) .. + 7 of a 32-column step, fp32 4 (l / 16) .. + 3 of 16 columns (the same in K and Q, so the order of the
-// columns in an instruction does not matter).
-template <typename T> DM_DEV floatx4 mma_chunk(const u32x4& k, const u32x4& q, floatx4 acc) {
+// columns in an instruction does not matter). In fp32 two chains of sums take turns, of LENGTH chunks (of 16 products) each, whose
+// sums are added to the score: short chains round less. Outputs' errors in the 2-norm and us a call of 16 tokens over 4096 rows of 128,
+// 32 heads on 8, with one chain of 128 products 1.12e-6 and 98, two of 64 6.8e-7 and 100 to 104, four of 32 4.6e-7 and 115, two of 16 four
+// times 4.0e-7 and 101 to 103; 512 tokens over 8192 rows 661, 647, 650 and 604.
+template <typename T, int LENGTH, int NT, int NF> DM_DEV void mma_scores(const u32x4 (&k)[NT][NF], const u32x4 (&q)[NF], floatx4 (&acc)[NT]) {
   if constexpr (sizeof(T) == 2) {
-    return Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q), acc);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = zero4();
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        acc[t] = Mfma<bf16>::mma(__builtin_bit_cast(bf16x8, k[t][i]), __builtin_bit_cast(bf16x8, q[i]), acc[t]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc = Mfma<float>::mma(__uint_as_float(k[j]), __uint_as_float(q[j]), acc);
-    return acc;
-  }
-}
-
-// the same for two tiles, whose chains of sums take turns
-template <typename T> DM_DEV void mma_chunks(const u32x4& k0, const u32x4& k1, const u32x4& q, floatx4 (&acc)[2]) {
-  if constexpr (sizeof(T) == 2) {
-    acc[0] = mma_chunk<T>(k0, q, acc[0]);
-    acc[1] = mma_chunk<T>(k1, q, acc[1]);
-  } else {
+    for (int i0 = 0; i0 < NF; i0 += 2 * LENGTH) {
+      floatx4 part[2][NT];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      acc[0] = Mfma<float>::mma(__uint_as_float(k0[j]), __uint_as_float(q[j]), acc[0]);
-      acc[1] = Mfma<float>::mma(__uint_as_float(k1[j]), __uint_as_float(q[j]), acc[1]);
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) part[c][t] = zero4();
+#pragma unroll
+      for (int i = i0; i < i0 + 2 * LENGTH; i += 2)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              part[c][t] = Mfma<float>::mma(__uint_as_float(k[t][i + c][j]), __uint_as_float(q[i + c][j]), part[c][t]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[t] = i0 ? acc[t] + (part[0][t] + part[1][t]) : part[0][t] + part[1][t];
     }
   }
 }
+
+// Scores are held as they come from the products and scaled where their exponential is taken, in one rounding with the reference that
+// is subtracted. Maxima are taken before the scale, so that is positive there: queries carry its sign, or 0 (and then it is 1).
+DM_DEV float positive_scale(float scale2) { return scale2 == 0.f ? 1.f : fabsf(scale2); }
+template <typename T> DM_DEV void carry_sign(u32x4& q, float scale2) {
+  constexpr uint32_t SIGN = sizeof(T) == 2 ? 0x80008000u : 0x80000000u, LOW = sizeof(T) == 2 ? 0x7f80u : 0u, TOP = 0x7f800000u;
+  const uint32_t flip = scale2 < 0.f ? SIGN : 0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t zero = (LOW && (q[e] & LOW) == LOW ? 0x7fc0u : 0u) | ((q[e] & TOP) == TOP ? 0x7fc00000u : 0u);   // NaN where not finite
+    q[e] = scale2 == 0.f ? zero : q[e] ^ flip;
+  }
+}
+// The logarithm of a sum z relative to a reference in units of ln 2, rounded once.
+DM_DEV float log_of(float ref, float z) { return z == 0.f ? -INF : (float)(((double)ref + __builtin_amdgcn_logf(z)) * 0.6931471805599453); }
 
 template <typename T> DM_DEV bool any_nonfinite(const u32x4& v) {
   bool bad = false;
@@ -389,8 +415,9 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
   {
     const T* q = (const T*)a.q + (long)(s.first + j) * a.q_token + (long)head * a.q_head;
 #pragma unroll
-    for (int i = 0; i < C::NF; ++i) qf[i] = ld_global<u32x4>(q + i * 4 * C::V + grp * C::V);
+    for (int i = 0; i < C::NF; ++i) qf[i] = ld_global<u32x4>(q + i * 4 * C::V + grp * C::V), carry_sign<T>(qf[i], a.scale2);
   }
+  const float scale2 = positive_scale(a.scale2);
   floatx4 O[C::NDT];
 #pragma unroll
   for (int d = 0; d < C::NDT; ++d) O[d] = zero4();
@@ -407,8 +434,9 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
 #pragma unroll
       for (int e = 0; e < C::V; ++e) dot = fmaf(x[e], y[e], dot);
     }
-    m = xor_sum<32>(xor_sum<16>(dot)) * a.scale2;
-    const float p = __builtin_amdgcn_exp2f(m - (m == -INF ? 0.f : m));
+    dot = xor_sum<32>(xor_sum<16>(dot));
+    m = dot * scale2;
+    const float p = __builtin_amdgcn_exp2f(fmaf(dot, scale2, m == -INF ? 0.f : -m));
     z = grp == 0 ? p : 0.f;
 #pragma unroll
     for (int d = 0; d < C::NDT; ++d) {
@@ -486,14 +514,10 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
       *reinterpret_cast<u32x4*>(Vs + v / C::VPR * C::LDV + (v % C::VPR) * C::V) = vf[i];
     }
     float p[NP];      // of rows r0 + 16 (i / 4) + 4 grp + i % 4
-    floatx4 acc[2] = {zero4(), zero4()};
+    floatx4 acc[C::NT];
+    mma_scores<T, 1>(kf, qf, acc);
 #pragma unroll
-    for (int i = 0; i < C::NF; ++i) {
-      if constexpr (C::NT == 2) mma_chunks<T>(kf[0][i], kf[1][i], qf[i], acc);
-      else acc[0] = mma_chunk<T>(kf[0][i], qf[i], acc[0]);
-    }
-#pragma unroll
-    for (int i = 0; i < NP; ++i) p[i] = acc[i >> 2][i & 3] * a.scale2;
+    for (int i = 0; i < NP; ++i) p[i] = acc[i >> 2][i & 3];
     if (masked) {
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
@@ -510,7 +534,7 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
       if constexpr (C::NT == 2) *reinterpret_cast<floatx4*>(x + 16) = floatx4{p[4], p[5], p[6], p[7]};
     }
     if (r0 + 4 * C::KT < k1) load(r0 + 4 * C::KT), look_up(min(r0 + 8 * C::KT, k1));
-    top = xor_max<32>(xor_max<16>(top));
+    top = xor_max<32>(xor_max<16>(top)) * scale2;
     // the reference follows the maximum only where that has risen by 2^8: sums and probabilities are relative to it
     if (__ballot(top > m + 8.f)) {
       const float was = m;
@@ -523,7 +547,7 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
     const float ref = m == -INF ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(p[i] - ref);
+      p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], scale2, -ref));
       z += p[i];
     }
     __builtin_amdgcn_wave_barrier();   // LDS operations of one wave complete in order
@@ -603,7 +627,7 @@ template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile
   for (int e = 0; e < E; ++e) x[e] = Z == 0.f ? 0.f : x[e] * inv;
 #pragma unroll
   for (int e = 0; e < E; e += 4) st4<T>((T*)a.o + at * DH + e0 + e, x + e);
-  if (e0 == 0) a.lse[at] = Z == 0.f ? -INF : (ref + __builtin_amdgcn_logf(Z)) * LN2;
+  if (e0 == 0) a.lse[at] = log_of(ref, Z);
 }
 
 // ---- the read of many query rows -------------------------------------------------------------------
@@ -619,11 +643,6 @@ DM_DEV i16x8 values_fragment32(const bf16* v, int ldv) {
   const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
   const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * ldv));
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-// Two bf16 numbers times 0: NaN where one is not finite.
-DM_DEV uint32_t times_zero(uint32_t x) {
-  return ((x & 0x7f80u) == 0x7f80u ? 0x7fc0u : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0x7fc00000u : 0u);
 }
 
 template <int DH> struct WideTile {
@@ -675,15 +694,13 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
   u32x4 qf[C::NK];
   {
     const bf16* q = (const bf16*)a.q + (long)(s.first + j) * a.q_token + (long)head * a.q_head;
-    const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;    // the maximum is taken before the scale
 #pragma unroll
     for (int i = 0; i < C::NK; ++i) {
       qf[i] = live ? ld_global<u32x4>(q + 16 * i + 8 * half) : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) qf[i][e] = a.scale2 == 0.f ? times_zero(qf[i][e]) : qf[i][e] ^ flip;
+      carry_sign<bf16>(qf[i], a.scale2);
     }
   }
-  const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
+  const float scale2 = positive_scale(a.scale2);
   floatx16 O[C::ND];
 #pragma unroll
   for (int d = 0; d < C::ND; ++d)
@@ -702,8 +719,9 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
 #pragma unroll
       for (int e = 0; e < 8; ++e) dot = fmaf(x[e], y[e], dot);
     }
-    m = xor_sum<32>(dot) * scale2;
-    const float p = __builtin_amdgcn_exp2f(m - (m == -INF ? 0.f : m));
+    dot = xor_sum<32>(dot);
+    m = dot * scale2;
+    const float p = __builtin_amdgcn_exp2f(fmaf(dot, scale2, m == -INF ? 0.f : -m));
     z = half == 0 ? p : 0.f;
 #pragma unroll
     for (int d = 0; d < C::ND; ++d)
@@ -980,7 +998,7 @@ template <int DH, int NW> __global__ __launch_bounds__(64 * NW, 8 / NW) void k_p
       for (int e = 0; e < 4; ++e) x[e] = z == 0.f ? 0.f : O[d][4 * i + e] * inv;
       st4<bf16>((bf16*)a.o + at * DH + 32 * d + 8 * i + 4 * half, x);
     }
-  if (half == 0) a.lse[at] = z == 0.f ? -INF : (ref + __builtin_amdgcn_logf(z)) * LN2;
+  if (half == 0) a.lse[at] = log_of(ref, z);
 }
 
 // The pieces of a query tile, in their order: 16 threads a query row. Bound by latency: the plan, the maxima, then eight pieces'
@@ -1025,7 +1043,7 @@ template <typename T, int DH, int ROWS> __global__ __launch_bounds__(256) void k
   for (int e = 0; e < E; ++e) x[e] = Z == 0.f ? 0.f : x[e] * inv;
 #pragma unroll
   for (int e = 0; e < E; e += 4) st4<T>((T*)a.o + at * DH + e0 + e, x + e);
-  if (e0 == 0) a.lse[at] = Z == 0.f ? -INF : (ref + __builtin_amdgcn_logf(Z)) * LN2;
+  if (e0 == 0) a.lse[at] = log_of(ref, Z);
 }
 
 // ---- the weights -------------------------------------------------------------------------------
@@ -1050,6 +1068,7 @@ __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
   const int each = uniform((tiles + it.pieces - 1) / it.pieces);
   const int k0 = base + it.piece * each * TILE_K, k1 = min(k0 + each * TILE_K, t_high);
   const long cap = (long)a.cols << a.page_shift;
+  const float scale2 = positive_scale(a.scale2);
   float* w = a.weights + ((long)it.b * a.h_kv + c) * cap;
   for (int r = k0 + 4 * threadIdx.x; r < k1; r += 1024) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1072,7 +1091,7 @@ __global__ __launch_bounds__(256) void k_paged_weights_of(PagedArgs a) {
       for (int u = 0; u < AT_ONCE; ++u) {
         const int low = s.low(a, token[u]), high = token[u] < s.n ? s.high(a, token[u]) : 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += r + e >= low && r + e < high ? __builtin_amdgcn_exp2f(v[u][e] - lse_of(lse2[u])) : 0.f;
+        for (int e = 0; e < 4; ++e) sum[e] += r + e >= low && r + e < high ? __builtin_amdgcn_exp2f(fmaf(v[u][e], scale2, -lse_of(lse2[u]))) : 0.f;
       }
     }
 #pragma unroll
@@ -1139,9 +1158,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void k_paged_wei
       const int high = live ? s.high(a, j) : 0, low = live ? s.low(a, j) : 0;
       floatx4 acc[2];
       const float minus = -lse2;
-      acc[0] = acc[1] = zero4();
-#pragma unroll
-      for (int i = 0; i < C::NF; ++i) mma_chunks<T>(kf[0][i], kf[1][i], qf[i], acc);
+      mma_scores<T, C::NF / 2>(kf, qf, acc);    // (two chains: more of them take more registers than leave room for three waves)
       if (rho0 + q_step < j1 * a.g) fetch(rho0 + q_step);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
