@@ -148,9 +148,9 @@ template <typename T, int N> DM_DEV void load_columns(const T* x, int c, int col
   }
 }
 
-// One block per row and part of it, of the target and of the draft (blockIdx.z). Bound by the exponentials in 64 bits (about
-// 20 instructions each; the vector units are busy 85 % of the time): 64 sequences of 1 to 8 rows of 50257 in fp32, target and draft
-// (108 MB), 28.5 us, 3.8 TB/s; 48 of 1 to 6 rows of 100003 in bf16, target alone (35 MB), 20 us.
+// One block per row and part of it, of the target and of the draft (blockIdx.z): 64 sequences of 1 to 8 rows of 50257 in fp32, target
+// and draft (108 MB), 30.6 us, 3.5 TB/s; 48 of 1 to 6 rows of 100003 in bf16, target alone (35 MB), 21. Bound by the rows first, which
+// take 20 and 12 us of that without any exponentials, then by those in 64 bits (21 instructions each).
 template <typename T> __global__ __launch_bounds__(256) void k_verify_parts(VerifyArgs a) {
   constexpr int V = 16 / (int)sizeof(T), EACH = PART / 256;
   __shared__ Roots roots;

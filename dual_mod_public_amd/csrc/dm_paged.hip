@@ -195,7 +195,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_paged_write(Paged
 // ---- the read ----------------------------------------------------------------------------------
 template <typename T, int DH> struct Tile {
   // tiles of 16 cached rows in a wave's step (fp32 rows of 128 two at a time leave room for one wave per SIMD: 16 tokens over 4096
-  // rows on 8 key heads 129 us instead of 96, 512 tokens over 8192 rows 418 instead of 343)
+  // rows on 8 key heads 131 us instead of 99, 512 tokens over 8192 rows, 16 heads on 8, 427 instead of 313)
   static constexpr int NT = sizeof(T) == 4 && DH == 128 ? 1 : 2;
   static constexpr int KT = 16 * NT;
   static constexpr int V = 16 / (int)sizeof(T);
@@ -204,8 +204,8 @@ template <typename T, int DH> struct Tile {
   static constexpr int NV = KT * DH * (int)sizeof(T) / 1024;      // 16-byte loads of a lane for the step's V rows
   static constexpr int VPR = DH / V;
   static constexpr int NDT = DH / 16;
-  // per SIMD at least: what the registers of rows on their way leave (bf16 rows of 64: 105 registers, 4 waves fit; asked for 4 the
-  // compiler keeps fewer loads on their way: 64 sequences of 100 to 8192 rows 97 us instead of 92)
+  // per SIMD at least: what the registers of rows on their way leave (bf16 rows of 64: 115 registers, 4 waves fit; asked for 4 the
+  // compiler keeps fewer loads on their way: 64 sequences of 100 to 8192 rows 97 us instead of 92 through the last cache)
   static constexpr int WAVES = sizeof(T) == 2 || DH == 128 ? 3 : 2;
 };
 
@@ -379,12 +379,12 @@ DM_DEV long scores_at(const PagedArgs& a, const Seq& s, int c) {
 // joined through LDS. S^T = K Q^T rather than S = Q K^T: a lane then holds scores of one query row only, the maximum needs two
 // exchanges, and the probabilities are already the operand of the product with V, whose columns come from LDS transposed. K goes
 // to the matrix cores straight from memory. The next step's rows of K and V are on their way in registers meanwhile.
-// Bound by the rows' bytes: 64 sequences of 100 to 8192 rows of 64 on 16 key heads (484 MB) 82.5 us, 5.9 TB/s, of random pages of
-// 64 rows; more blocks per CU or more rows on their way bring nothing. One token over 1024 rows 10 us in one piece per head, 6 in
-// eight, most of it latency: the plan, the table, the rows.
+// Bound by the rows' bytes: 64 sequences of 100 to 8192 rows of 64 on 16 key heads (484 MB) 83.5 us, 5.8 TB/s, of random pages of
+// 64 rows; more blocks per CU or more rows on their way bring nothing. One token over 1024 rows 11 us in one piece per head, most of
+// it latency: the plan, the table, the rows.
 // KEEP: the scores are kept for the weights (of the lanes behind the last query row too, which work on that one again: a store
 // that some lanes skip would have the next rows' loads wait for it, 276 instead of 273 us). 32 sequences of 3000 to 16384 rows of
-// 128 on 8 key heads, 1.28 GB: 229 us without, 273 with; past the last cache 204 and 266 (of which 5 where they stay in L2,
+// 128 on 8 key heads, 1.28 GB: 229 us without, 273 with; past the last cache 204 and 268 (of which 5 where they stay in L2,
 // 55 for the 40 MB in memory). Computing the scores again costs 172.
 template <typename T, int DH, bool KEEP> __global__ __launch_bounds__(256, (Tile<T, DH>::WAVES)) void k_paged_read(PagedArgs a) {
   using C = Tile<T, DH>;
@@ -1490,12 +1490,12 @@ constexpr int WEIGHT_BLOCKS = 8 * CUS;
 
 // Which read a call takes, by the mean number of query rows of a sequence and key head: tiles of 16 rows while two of them
 // hold those, of 128, or of 256 (us, bf16, 16 sequences of 4096 rows, 16 heads of 64 and 32 of 128 on 8 key heads:
-// 24 rows 60 / 69 / 115 and 60 / 62 / 82, 48 rows 78 / 71 / 115 and 84 / 65 / 86, 256 rows 303 / 123 / 134 and 307 / 117 / 119,
-// 512 rows 572 / 225 / 215 and 596 / 195 / 188; two sequences of 16384 rows, 8192 query rows: 4110 / 1340 / 1150). Pieces:
+// 24 rows 59 / 69 / 115 and 60 / 62 / 82, 48 rows 71 / 66 / 115 and 76 / 62 / 86, 256 rows 297 / 120 / 134 and 302 / 112 / 119,
+// 512 rows 559 / 221 / 215 and 583 / 188 / 188; two sequences of 16384 rows, 8192 query rows: 4206 / 1340 / 1061). Pieces:
 // what fills the CUs with the blocks that one holds (at 8192 query rows 1, 2 and 4 times as many: 1150, 1184, 1206 us).
 // In one piece, with no join, while a tile's keys take no more than 128 KiB, or 256 with blocks for half of the CUs (a call / its
-// kernels in a graph, pieces -> whole: one token, 16 heads of 64, 256 rows 17.1 / 8.9 -> 14.2 / 6.4 us, 512 rows 17.3 / 9.2 ->
-// 14.4 / 7.6, 1024 rows 17.2 / 9.1 -> 14.3 / 9.8, 2048 rows 17.0 / 9.5 -> 14.5 / 14.3; 8 tokens over 2048 rows 23.4 / 24.0 ->
+// kernels in a graph, pieces -> whole: one token, 16 heads of 64, 256 rows 18.1 / 8.9 -> 14.0 / 6.5 us, 512 rows 18.0 / 9.3 ->
+// 13.4 / 7.8, 1024 rows 18.1 / 9.2 -> 13.4 / 10.4, 2048 rows 17.0 / 9.5 -> 14.5 / 14.3; 8 tokens over 2048 rows 23.4 / 24.0 ->
 // 20.4 / 21.0; 7 chunks of 65 fp32 tokens, 8 heads of 64 on 4, over 1024 rows 43 -> 34). The larger tiles: up to 512 rows with
 // blocks for half of the CUs (16 chunks of 64 tokens, 8 heads of 64, over 128, 512 and 1024 rows 21.9 -> 17.6, 21.6 -> 16.8 and
 // 22.3 -> 24.9; 33 of 100 tokens, 16 heads of 128, 43 -> 33, 63 -> 54.5 and 106 -> 92; one of 1024 rows among 16 of 70 21 -> 33.6).
