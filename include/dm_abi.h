@@ -693,7 +693,8 @@ int dm_paged_evict(const dm_evict_args* a, void* stream);
  * tokens [rows]: the accepted drafts and the new token, each at the row it was predicted by; -1 behind them, in rows of no
  * sequence and where the row that ends the sequence is no distribution (a NaN, +inf, nothing but -inf; greedy: a NaN, nothing but
  * -inf; a temperature that is negative or not finite). accepted [B]: drafts accepted. logp [rows]: the tokens' target log
- * probabilities (at T = 1 where T is 0), 0 where there is none, NaN where there is no distribution. A draft outside [0, cols) is not accepted. Probabilities, sums and places in 64 bits.
+ * probabilities (at T = 1 where T is 0), 0 where there is none, NaN where there is no distribution. A draft outside [0, cols) is not accepted. Probabilities,
+ * sums and places in 64 bits; what is below 2^-1000 of a row's largest counts 0.
  * At most 65535 rows and sequences. */
 typedef struct dm_verify_args {
   int32_t dtype, rows, cols, B;
