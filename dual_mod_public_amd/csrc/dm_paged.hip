@@ -1345,7 +1345,7 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictArgs a) {
   const int left = min(len, a.keep);
   int32_t* rows = a.rows + ((long)b * a.h + c) * a.keep;
   if (c == 0 && threadIdx.x == 0) a.lengths_out[b] = left;
-  for (int i = left + threadIdx.x; i < a.keep; i += 1024) rows[i] = -1;
+  for (long i = left + (long)threadIdx.x; i < a.keep; i += 1024) rows[i] = -1;     // (keep may be any more than there are)
   if (len <= a.keep) {
     for (int i = threadIdx.x; i < left; i += 1024) rows[i] = i;
     return;
@@ -1669,8 +1669,8 @@ int dm_paged_evict(const dm_evict_args* a, void* stream) {
   DM_REQUIRE(a != nullptr, DM_ERR_INVALID, "null arguments");
   if (const int rc = check_pages(a->dtype, a->dh, a->page, a->n_pages, a->table_cols, a->B, a->h_kv, a->K, a->V, a->k_page, a->v_page)) return rc;
   const int64_t cap = (int64_t)a->table_cols * a->page, new_cap = (int64_t)a->new_cols * a->page;
-  DM_REQUIRE(a->keep > 0 && a->keep <= DM_PAGED_ROWS && a->sinks >= 0 && a->recent >= 0 && (int64_t)a->sinks + a->recent <= a->keep,
-             DM_ERR_INVALID, "keep=%d sinks=%d recent=%d (at most %d rows)", a->keep, a->sinks, a->recent, DM_PAGED_ROWS);
+  DM_REQUIRE(a->keep > 0 && a->sinks >= 0 && a->recent >= 0 && (int64_t)a->sinks + a->recent <= a->keep, DM_ERR_INVALID,
+             "keep=%d sinks=%d recent=%d", a->keep, a->sinks, a->recent);
   DM_REQUIRE(a->new_cols > 0 && new_cap <= DM_PAGED_ROWS && new_cap >= std::min<int64_t>(a->keep, cap), DM_ERR_INVALID,
              "new_cols=%d pages do not hold %d rows", a->new_cols, a->keep);
   DM_REQUIRE(a->table && a->lengths && a->new_table && a->weights && a->weights_out && a->rows && a->lengths_out, DM_ERR_INVALID,

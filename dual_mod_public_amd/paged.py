@@ -209,8 +209,8 @@ def evict_rows(K, V, weights, table, lengths, keep, new_table, sinks=0, recent=0
     B, cols, table_p, lengths_p, _ = _sequences(table, lengths, None, table.shape[0], dev)
     cap, new_cols = cols * page, new_table.shape[1]
     keep, sinks, recent = int(keep), int(sinks), int(recent)
-    if not 1 <= keep <= L.DM_PAGED_ROWS or sinks < 0 or recent < 0 or sinks + recent > keep:
-        raise ValueError(f"keep={keep} sinks={sinks} recent={recent} (at most {L.DM_PAGED_ROWS} rows)")
+    if not 1 <= keep <= 0x7fffffff or sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise ValueError(f"keep={keep} sinks={sinks} recent={recent} (at most 2^31 - 1)")
     if new_cols * page < min(keep, cap):
         raise ValueError(f"new_table holds {new_cols * page} rows; keep={keep}")
     weights_p = _weights(weights, (B, h_kv, cap), dev)

@@ -670,7 +670,7 @@ int dm_paged_attention(const dm_paged_args* a, void* stream);
  * weights: weights_out [B, h_kv, new_cols * page], 0 behind them. rows [B, h_kv, keep]: the rows kept, -1 behind them;
  * lengths_out [B]. The new pages are none that a table of the call names (pages that sequences share may be read, so a
  * shared prefix stays). A length that the table does not hold counts as 0; rows of a page outside the pool become NaN, and those
- * that a new page outside the pool would be given are left out. B * h_kv at most DM_PAGED_HEADS, keep at most DM_PAGED_ROWS. */
+ * that a new page outside the pool would be given are left out. B * h_kv at most DM_PAGED_HEADS. */
 typedef struct dm_evict_args {
   int32_t dtype, B, h_kv, dh;
   int32_t page, n_pages, table_cols, new_cols;

@@ -68,13 +68,26 @@ def test_infinite_values_that_are_read(dtype, dh, new):
     near(got[..., rest], o[..., rest], bo[..., rest], "o")
 
 
-@pytest.mark.parametrize("keep", [L.DM_PAGED_ROWS + 1, 2 ** 31 - 1, 2 ** 32 + 5])
-def test_more_kept_rows_than_a_table_has(keep):
-    """Refused before the rows are allocated; past 32 bits too, of which the call would take the lower ones."""
+@pytest.mark.parametrize("keep", [2 ** 32 + 5, 2 ** 31])
+def test_keep_past_32_bits(keep):
+    """Refused before the rows are allocated: the call would take the lower bits."""
     K, V = paged.new_pages(4, 2, 16, 64)
     table, w = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.zeros(1, 2, 32, device=DEV)
     with pytest.raises(ValueError, match="keep="):
         paged.evict_rows(K, V, w, table, torch.ones(1, dtype=torch.int32, device=DEV), keep, table + 2)
+
+
+@pytest.mark.parametrize("keep", [2 ** 26 + 1, 2 ** 31 - 1])
+def test_keep_of_more_than_there_is(keep):
+    """All rows stay, and all places behind them hold -1. A block's threads step through the places by 1024: within 1024 of 2^31 a
+    count of 32 bits would wrap, and go on before the buffer."""
+    K, V = paged.new_pages(4, 1, 16, 64)
+    K[1] = torch.randn(1, 16, 64)
+    table, w = torch.tensor([[1]], dtype=torch.int32, device=DEV), torch.rand(1, 1, 16, device=DEV)
+    r = paged.evict_rows(K, V, w, table, torch.tensor([13], dtype=torch.int32, device=DEV), keep, table + 2)
+    assert r.rows.shape == (1, 1, keep) and r.rows[0, 0, :13].tolist() == list(range(13)) and r.lengths.tolist() == [13]
+    assert all((part == -1).all() for part in r.rows[0, 0, 13:].split(1 << 28))
+    assert torch.equal(K[3, 0, :13], K[1, 0, :13]) and torch.equal(r.weights[0, 0, :13], w[0, 0, :13])
 
 
 def test_more_tokens_than_32_bits_count():

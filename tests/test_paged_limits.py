@@ -8,24 +8,6 @@ import pytest
 from dual_mod_public_amd import _lib as L
 
 
-def evict_args(**kw):
-    a = L.dm_evict_args()
-    base = dict(dtype=L.DM_BF16, B=2, h_kv=2, dh=64, page=16, n_pages=5, table_cols=3, new_cols=3, keep=32, sinks=2, recent=4, K=0x20000,
-                V=0x30000, k_page=2048, v_page=2048, table=0x40000, lengths=0x50000, new_table=0x41000, weights=0x60000,
-                weights_out=0x61000, rows=0x62000, lengths_out=0x63000)
-    for k, v in dict(base, **kw).items():
-        setattr(a, k, v)
-    return a
-
-
-@pytest.mark.parametrize("keep", [L.DM_PAGED_ROWS + 1, 2 ** 31 - 1024, 2 ** 31 - 1])
-def test_more_kept_rows_than_a_table_has(keep):
-    """A block's threads step through the keep places of a sequence by 1024: past 2^31 - 1024 their count would leave 32 bits, and the
-    places behind the kept rows be written before the buffer."""
-    lib = L.load()
-    assert lib.dm_paged_evict(L.byref(evict_args(keep=keep)), None) == -1 and b"keep" in lib.dm_last_error()
-
-
 def attention_args(**kw):
     a = L.dm_paged_args()
     base = dict(dtype=L.DM_BF16, B=64, h=32, h_kv=8, dh=128, page=64, n_pages=1 << 20, table_cols=1 << 11, n_tokens=64, scale=0.125,
