@@ -128,7 +128,8 @@ def _sequences(table, lengths, starts, n_tokens, device):
 
 
 def paged_write(k, v, K, V, table, lengths, starts=None):
-    """The rows k, v [N, h_kv, dh] of the new tokens (any strides of tokens and heads) into their places in the pages."""
+    """The rows k, v [N, h_kv, dh] of the new tokens (any strides of tokens and heads; rows of the pool too, but none that the call
+    writes) into their places in the pages."""
     dtype, n_pages, h_kv, page, dh, k_page, v_page = _pages(K, V)
     N = k.shape[0]
     B, cols, table_p, lengths_p, starts_p = _sequences(table, lengths, starts, N, K.get_device())

@@ -47,7 +47,8 @@ class PagedTape:
     def extend(self, xhat, positions, cos, sin, table, lengths, starts=None, n_sweeps=None, weights=None):
         """xhat [N, d] (pre-normed, the tape's dtype) of the new tokens at ``positions`` [N] (int64); cos, sin: RoPE tables.
         Their refined rows are in the pages afterwards. n_sweeps: 1 without starts; with starts the longest chunk's length gives
-        the exact scan. weights: see paged_attention (of the last sweep). Returns W_O o [N, d]."""
+        the exact scan, fewer the chunk cell's Jacobi result. weights: see paged_attention (of the last sweep). Returns W_O o [N, d]; rows of
+        tokens of no sequence hold anything (their positions are looked up all the same)."""
         if n_sweeps is None:
             if starts is not None:
                 raise ValueError("chunks need n_sweeps (the longest one's length: the exact scan)")
